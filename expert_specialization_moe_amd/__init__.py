@@ -21,6 +21,13 @@ from .ops import (  # noqa: F401
     es_mxfp8_quant_weight,
     es_fp8_blockwise_scaled_grouped_mm_swiglu_quant,
     es_mxfp8_blockscaled_grouped_mm_swiglu_quant,
+    es_topk_gating,
+    es_topk_gating_backward,
+    es_combine_rows,
+    es_combine_rows_backward,
+    es_add_rms_norm_quant_1x128,
+    es_mxfp4_grouped_mm,
+    es_mxfp4_grouped_mm_swiglu,
 )
 
 __all__ = [
@@ -36,4 +43,11 @@ __all__ = [
     "es_mxfp8_quant_weight",
     "es_fp8_blockwise_scaled_grouped_mm_swiglu_quant",
     "es_mxfp8_blockscaled_grouped_mm_swiglu_quant",
+    "es_topk_gating",
+    "es_topk_gating_backward",
+    "es_combine_rows",
+    "es_combine_rows_backward",
+    "es_add_rms_norm_quant_1x128",
+    "es_mxfp4_grouped_mm",
+    "es_mxfp4_grouped_mm_swiglu",
 ]

@@ -66,6 +66,20 @@ lib.esmoe_permute_rows.restype = _i
 lib.esmoe_permute_rows.argtypes = [_vp, _vp, ctypes.c_long, _i, ctypes.c_long, _vp, _vp]
 lib.esmoe_swiglu_quant_1x128.restype = _i
 lib.esmoe_swiglu_quant_1x128.argtypes = [_vp, _i, _vp, _vp, ctypes.c_long, _i, _vp]
+_l = ctypes.c_long
+_f = ctypes.c_float
+lib.esmoe_topk_gating.restype = _i
+lib.esmoe_topk_gating.argtypes = [_vp, _i, _l, _vp, _l, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]
+lib.esmoe_topk_gating_backward.restype = _i
+lib.esmoe_topk_gating_backward.argtypes = [_vp, _vp, _i, _l, _vp, _l, _i, _i, _i, _i, _f, _vp, _vp]
+lib.esmoe_combine_rows.restype = _i
+lib.esmoe_combine_rows.argtypes = [_vp, _i, _vp, _vp, _l, _i, _l, _i, _vp, _vp]
+lib.esmoe_combine_rows_backward.restype = _i
+lib.esmoe_combine_rows_backward.argtypes = [_vp, _vp, _i, _vp, _vp, _l, _i, _l, _i, _vp, _vp, _vp]
+lib.esmoe_add_rms_norm_quant_1x128.restype = _i
+lib.esmoe_add_rms_norm_quant_1x128.argtypes = [_vp, _i, _vp, _vp, _f, _l, _i, _vp, _vp, _vp, _vp, _vp]
+lib.esmoe_mxfp4_grouped_mm.restype = _i
+lib.esmoe_mxfp4_grouped_mm.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
 lib.esmoe_last_error.restype = ctypes.c_char_p
 lib.esmoe_last_error.argtypes = []
 lib.esmoe_version.restype = ctypes.c_char_p

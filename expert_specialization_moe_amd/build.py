@@ -24,7 +24,8 @@ OBJ = os.path.join(PKG, "build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["grouped_gemm.hip", "mxfp8_quant.hip", "fp8_quant.hip", "routing.hip", "capi.hip"]
+HIP_SOURCES = ["grouped_gemm.hip", "mxfp8_quant.hip", "fp8_quant.hip", "routing.hip", "gating.hip", "combine.hip",
+               "norm_quant.hip", "mxfp4_gemm.hip", "capi.hip"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-mcode-object-version=5",
     # packed fp32 VALU ops are kept out of the device code

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "esmoe.h"
+#include "gating.h"
 #include "gemm_args.h"
 #include "schedule.h"
 
@@ -36,6 +37,20 @@ extern "C" int esmoe_launch_permute_rows(const void* in, const int* dst_row, lon
 
 extern "C" int esmoe_launch_swiglu_quant(const void* in, int in_dtype, void* q, float* scales, long total_rows, int inter,
                                         hipStream_t stream);
+extern "C" int esmoe_launch_topk_gating(const void* logits, int dtype, long ld, const float* bias, const esmoe::GateArgs* a, int* ids,
+                                        float* weights, hipStream_t stream);
+extern "C" int esmoe_launch_topk_gating_backward(const float* grad, const void* logits, int dtype, long ld, const int* ids,
+                                                 const esmoe::GateArgs* a, void* out, hipStream_t stream);
+extern "C" int esmoe_launch_combine_rows(const void* in, int dtype, const int* dst_row, const float* weights, long tokens, int topk,
+                                         long rows, int hidden, void* out, hipStream_t stream);
+extern "C" int esmoe_launch_combine_rows_backward(const void* grad_out, const void* in, int dtype, const int* dst_row,
+                                                  const float* weights, long tokens, int topk, long rows, int hidden, void* grad_in,
+                                                  float* grad_weights, hipStream_t stream);
+extern "C" int esmoe_launch_add_rms_norm_quant(const void* in, int in_dtype, const void* residual, const void* weight, float eps, long rows,
+                                               int hidden, void* residual_out, void* normed, void* q, float* scales, hipStream_t stream);
+extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const void* b, const uint8_t* sf, const int* problem_sizes,
+                                             const int* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu,
+                                             void* out, hipStream_t stream);
 
 namespace {
 
@@ -542,6 +557,168 @@ int esmoe_permute_rows(const void* in, const int32_t* dst_row, long num_pairs, i
   return 0;
 }
 
+namespace {
+// What both directions of the gating share.
+int gate_args(int dtype, long tokens, int num_experts, long ld, int topk, int scoring, int renormalize, float scale, esmoe::GateArgs* a) {
+  if (dtype != ESMOE_LOGITS_FP32 && dtype != ESMOE_LOGITS_BF16 && dtype != ESMOE_LOGITS_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "logits_dtype must be ESMOE_LOGITS_FP32, ESMOE_LOGITS_BF16 or ESMOE_LOGITS_FP16");
+  if (num_experts < 1 || num_experts > ESMOE_MAX_EXPERTS)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_experts must be in [1, %d], got %d", ESMOE_MAX_EXPERTS, num_experts);
+  if (topk < 1 || topk > ESMOE_MAX_TOPK || topk > num_experts)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "topk must be in [1, %d] and at most num_experts, got %d", ESMOE_MAX_TOPK, topk);
+  if (scoring != ESMOE_SCORING_SOFTMAX && scoring != ESMOE_SCORING_SIGMOID)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "scoring must be ESMOE_SCORING_SOFTMAX or ESMOE_SCORING_SIGMOID");
+  if (tokens < 0 || tokens >= (1L << 31) / topk)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "tokens * topk must be in [0, 2^31), got %ld tokens", tokens);
+  if (ld < 0 || (tokens > 1 && ld > (1L << 40) / tokens)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "row stride out of range: %ld", ld);
+  if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return fail(ESMOE_ERR_INVALID_ARGUMENT, "scale must be finite");
+  *a = esmoe::GateArgs{tokens, num_experts, topk, 1, 1, scoring == ESMOE_SCORING_SIGMOID, renormalize != 0, 0, scale};
+  return 0;
+}
+int gate_dtype(int dtype) {
+  return dtype == ESMOE_LOGITS_FP32 ? esmoe::kGateF32 : dtype == ESMOE_LOGITS_FP16 ? esmoe::kGateF16 : esmoe::kGateBf16;
+}
+}  // namespace
+
+int esmoe_topk_gating(const void* logits, int logits_dtype, long row_stride, const float* bias, long tokens, int num_experts, int topk,
+                      int scoring, int renormalize, float scale, int num_groups, int topk_groups, int32_t* topk_ids, float* topk_weights,
+                      void* stream) {
+  g_err[0] = 0;
+  esmoe::GateArgs a;
+  int rc = gate_args(logits_dtype, tokens, num_experts, row_stride, topk, scoring, renormalize, scale, &a);
+  if (rc) return rc;
+  if (num_groups < 1 || num_groups > esmoe::kGateMaxGroups || num_experts % num_groups)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_groups must be in [1, %d] and divide num_experts, got %d", esmoe::kGateMaxGroups, num_groups);
+  if (topk_groups < 1 || topk_groups > num_groups)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "topk_groups must be in [1, num_groups], got %d", topk_groups);
+  if (topk > num_experts / num_groups * topk_groups)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "topk is more than the experts of topk_groups groups");
+  if (tokens == 0) return 0;
+  if (!logits || !topk_ids || !topk_weights) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  a.groups = topk_groups == num_groups ? 1 : num_groups;   // (all groups stay: no limit)
+  a.topk_groups = topk_groups;
+  a.exact = bias || num_groups > 1;
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_topk_gating(logits, gate_dtype(logits_dtype), row_stride, bias, &a, topk_ids, topk_weights, (hipStream_t)stream);
+  if (rc) return fail(rc, "gating launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_topk_gating_backward(const float* grad_weights, const void* logits, int logits_dtype, long row_stride, const int32_t* topk_ids,
+                               long tokens, int num_experts, int topk, int scoring, int renormalize, float scale, void* grad_logits,
+                               void* stream) {
+  g_err[0] = 0;
+  esmoe::GateArgs a;
+  int rc = gate_args(logits_dtype, tokens, num_experts, row_stride, topk, scoring, renormalize, scale, &a);
+  if (rc) return rc;
+  if (tokens == 0) return 0;
+  if (!grad_weights || !logits || !topk_ids || !grad_logits) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_topk_gating_backward(grad_weights, logits, gate_dtype(logits_dtype), row_stride, topk_ids, &a, grad_logits,
+                                         (hipStream_t)stream);
+  if (rc) return fail(rc, "gating gradient launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+namespace {
+int combine_args(int dtype, long num_pairs, int topk, long rows, int hidden) {
+  if (dtype != ESMOE_IN_BF16 && dtype != ESMOE_IN_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "dtype must be ESMOE_IN_BF16 or ESMOE_IN_FP16");
+  if (topk < 1 || num_pairs < 0 || num_pairs % topk || num_pairs >= (1L << 31))
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_pairs must be tokens * topk in [0, 2^31), got %ld pairs, topk %d", num_pairs, topk);
+  if (rows < 0 || rows >= (1L << 31)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "rows out of range: %ld", rows);
+  if (hidden <= 0 || hidden % 8 || hidden > (1 << 24))
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "hidden must be a multiple of 8 (rows of 16 bytes) up to 2^24, got %d", hidden);
+  return 0;
+}
+}  // namespace
+
+int esmoe_combine_rows(const void* in, int dtype, const int32_t* dst_row, const float* weights, long num_pairs, int topk, long rows,
+                       int hidden, void* out, void* stream) {
+  g_err[0] = 0;
+  int rc = combine_args(dtype, num_pairs, topk, rows, hidden);
+  if (rc) return rc;
+  if (num_pairs == 0) return 0;
+  if ((!in && rows) || !dst_row || !out) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)in % 16 || (uintptr_t)out % 16) return fail(ESMOE_ERR_INVALID_ARGUMENT, "in and out must be 16-byte aligned");
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_combine_rows(in, dtype == ESMOE_IN_FP16, dst_row, weights, num_pairs / topk, topk, rows, hidden, out, (hipStream_t)stream);
+  if (rc) return fail(rc, "combine launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_combine_rows_backward(const void* grad_out, const void* in, int dtype, const int32_t* dst_row, const float* weights,
+                                long num_pairs, int topk, long rows, int hidden, void* grad_in, float* grad_weights, void* stream) {
+  g_err[0] = 0;
+  int rc = combine_args(dtype, num_pairs, topk, rows, hidden);
+  if (rc) return rc;
+  if (num_pairs == 0) return 0;
+  if (!grad_out || ((!in || !grad_in) && rows) || !dst_row || !weights || !grad_weights)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)grad_out % 16 || (uintptr_t)in % 16 || (uintptr_t)grad_in % 16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "grad_out, in and grad_in must be 16-byte aligned");
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_combine_rows_backward(grad_out, in, dtype == ESMOE_IN_FP16, dst_row, weights, num_pairs / topk, topk, rows, hidden, grad_in,
+                                          grad_weights, (hipStream_t)stream);
+  if (rc) return fail(rc, "combine gradient launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_add_rms_norm_quant_1x128(const void* in, int in_dtype, const void* residual, const void* weight, float eps, long total_rows, int k,
+                                   void* residual_out, void* normed, void* q, float* scales, void* stream) {
+  g_err[0] = 0;
+  if (k <= 0 || k % 128 || k > 32768) return fail(ESMOE_ERR_INVALID_ARGUMENT, "k must align to 128 and be at most 32768, got %d", k);
+  if (in_dtype != ESMOE_IN_BF16 && in_dtype != ESMOE_IN_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "in_dtype must be ESMOE_IN_BF16 or ESMOE_IN_FP16");
+  if (total_rows < 0 || total_rows > (1L << 40) / k) return fail(ESMOE_ERR_INVALID_ARGUMENT, "total_rows out of range: %ld", total_rows);
+  if (!(eps >= 0.f && eps < __builtin_inff())) return fail(ESMOE_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (total_rows == 0) return 0;
+  if (!in || !weight || !q || !scales) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!residual != !residual_out) return fail(ESMOE_ERR_INVALID_ARGUMENT, "residual and residual_out go together");
+  if ((uintptr_t)in % 16 || (uintptr_t)residual % 16 || (uintptr_t)weight % 16 || (uintptr_t)residual_out % 16 || (uintptr_t)normed % 16 ||
+      (uintptr_t)q % 8 || (uintptr_t)scales % 4)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "16-bit tensors must be 16-byte aligned, q 8-byte aligned, scales 4-byte aligned");
+  DeviceInfo info;
+  int rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_add_rms_norm_quant(in, in_dtype == ESMOE_IN_FP16, residual, weight, eps, total_rows, k, residual_out, normed, q, scales,
+                                       (hipStream_t)stream);
+  if (rc) return fail(rc, "norm quant launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, const uint8_t* sfb, const int32_t* problem_sizes,
+                           const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream) {
+  g_err[0] = 0;
+  if (dtype != ESMOE_OUT_BF16 && dtype != ESMOE_OUT_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "dtype must be ESMOE_OUT_BF16 or ESMOE_OUT_FP16");
+  if (num_experts < 1 || num_experts > ESMOE_MAX_EXPERTS)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_experts must be in [1, %d], got %d", ESMOE_MAX_EXPERTS, num_experts);
+  if (total_rows < 0) return fail(ESMOE_ERR_INVALID_ARGUMENT, "total_rows must be >= 0");
+  if (k <= 0 || k % 128 || k > 32768) return fail(ESMOE_ERR_INVALID_ARGUMENT, "k must be a multiple of 128 up to 32768, got %d", k);
+  if (n <= 0 || n % (swiglu ? 32 : 16) || n > (1 << 20))
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "n must be a multiple of 16 (of 32 with SwiGLU) up to 2^20, got %d", n);
+  if (total_rows == 0) return 0;
+  if (!out || !a || !b || !sfb || !problem_sizes || !expert_offsets) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)sfb % 4 || (uintptr_t)out % 2)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "a and b must be 16-byte aligned, sfb 4-byte aligned");
+  DeviceInfo info;
+  int rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_mxfp4_grouped_mm(a, dtype == ESMOE_OUT_FP16, b, sfb, problem_sizes, expert_offsets, num_experts, total_rows, n, k,
+                                     swiglu != 0, out, (hipStream_t)stream);
+  if (rc) return fail(rc, "mxfp4 grouped mm launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
 int esmoe_host_schedule(const int32_t* problem_sizes_host, int num_experts, int n, int force_bm, int kind,
                         int32_t* ws_host) {
   g_err[0] = 0;
@@ -651,6 +828,6 @@ int esmoe_host_decode_light(const int32_t* problem_sizes_host, const int32_t* ws
 
 const char* esmoe_last_error(void) { return g_err; }
 
-const char* esmoe_version(void) { return "esmoe 0.3 (gfx950)"; }
+const char* esmoe_version(void) { return "esmoe 0.4 (gfx950)"; }
 
 }  // extern "C"

@@ -1,0 +1,145 @@
+// Residual addition, root-mean-square norm and 1x128 FP8 quantisation in one pass over a row.
+//
+//   h = in + residual (fp32, rounded to the tensors' type: the new residual), or in
+//   y = h * (1 / sqrt(mean(h^2) + eps)) * weight      (fp32)
+//   normed = y rounded to the tensors' type (optional: what a router reads)
+//   per 128 columns: amax = max(|y|, 1e-4), q = e4m3fn(y * (1 / amax * 448)), scale = amax * fl(1 / 448)
+// The quantisation is fp8_quant.hip's, of y as it is: one rounding less than quantising the rounded norm.  A NaN of y is a NaN of its
+// block's scale and bytes.  The reference has no norm; its callers quantise with a torch helper (test/test_es_grouped_gemm.py:36-44).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "wave_scan.h"
+
+namespace esmoe {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+
+constexpr int kNormThreads = 256;
+
+template <bool FP16>
+__device__ __forceinline__ float half_to_f32(uint32_t bits) {
+  if constexpr (FP16) return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  else return __builtin_bit_cast(float, bits << 16);
+}
+template <bool FP16>
+__device__ __forceinline__ uint32_t f32_to_half(float v) {
+  if constexpr (FP16) return __builtin_bit_cast(uint16_t, (_Float16)v);
+  else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// Maximum over sixteen lanes; on bit patterns of non-negative floats, so that a NaN is the largest.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax16(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  return v > o ? v : o;
+}
+
+// One workgroup per row, its values in registers: CHUNKS times eight per thread.
+template <bool FP16, int CHUNKS>
+__global__ void __launch_bounds__(kNormThreads) add_rms_norm_quant_kernel(const uint16_t* in, const uint16_t* residual,
+                                                                          const uint16_t* __restrict__ weight, float eps, int hidden,
+                                                                          uint16_t* residual_out, uint16_t* __restrict__ normed,
+                                                                          uint8_t* __restrict__ q, float* __restrict__ scales) {
+  __shared__ float s_sum[kNormThreads / 64];
+  const int tid = threadIdx.x;
+  const long row = (long)blockIdx.x * hidden;
+  float h[CHUNKS][8];
+  float sum = 0;
+#pragma unroll
+  for (int u = 0; u < CHUNKS; u++) {
+    const int col = (u * kNormThreads + tid) * 8;
+    if (col < hidden) {
+      const v4i a = *(const v4i*)(in + row + col);
+      v4i r = {0, 0, 0, 0};
+      if (residual) r = *(const v4i*)(residual + row + col);
+      v4i o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float lo = half_to_f32<FP16>((uint32_t)a[i] & 0xffffu), hi = half_to_f32<FP16>((uint32_t)a[i] >> 16);
+        if (residual) {
+          const uint32_t l = f32_to_half<FP16>(lo + half_to_f32<FP16>((uint32_t)r[i] & 0xffffu));
+          const uint32_t g = f32_to_half<FP16>(hi + half_to_f32<FP16>((uint32_t)r[i] >> 16));
+          o[i] = (int)(l | g << 16);
+          lo = half_to_f32<FP16>(l);
+          hi = half_to_f32<FP16>(g);
+        }
+        h[u][2 * i] = lo;
+        h[u][2 * i + 1] = hi;
+        sum = __builtin_fmaf(lo, lo, sum);
+        sum = __builtin_fmaf(hi, hi, sum);
+      }
+      if (residual) *(v4i*)(residual_out + row + col) = o;
+    }
+  }
+  sum = wave_sum_last(sum);
+  if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
+  __syncthreads();
+  sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  const float rstd = 1.0f / sqrtf(sum / (float)hidden + eps);
+#pragma unroll
+  for (int u = 0; u < CHUNKS; u++) {
+    const int col = (u * kNormThreads + tid) * 8;   // sixteen lanes hold 128 columns: in or out of the row as one
+    if (col < hidden) {
+      const v4i g = *(const v4i*)(weight + col);
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        h[u][i] = h[u][i] * rstd * half_to_f32<FP16>(i & 1 ? (uint32_t)g[i / 2] >> 16 : (uint32_t)g[i / 2] & 0xffffu);
+        const uint32_t b = __builtin_bit_cast(uint32_t, h[u][i]) & 0x7fffffffu;
+        amax = amax > b ? amax : b;
+      }
+      amax = dpp_umax16<0x140>(dpp_umax16<0x141>(dpp_umax16<0x4E>(dpp_umax16<0xB1>(amax))));
+      const uint32_t least = __builtin_bit_cast(uint32_t, 1e-4f);
+      const float top = __builtin_bit_cast(float, amax > least ? amax : least);
+      const float mult = (1.0f / top) * 448.0f;
+      if (normed) {
+        v4i o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = (int)(f32_to_half<FP16>(h[u][2 * i]) | f32_to_half<FP16>(h[u][2 * i + 1]) << 16);
+        *(v4i*)(normed + row + col) = o;
+      }
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[i] = h[u][i] * mult;   // (at most 448 and an ulp or two, which rounds to 448)
+      int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
+      int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+      w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
+      *(v2i*)(q + row + col) = v2i{w0, w1};
+      if ((tid & 15) == 0) scales[(row + col) >> 7] = top * (1.0f / 448.0f);
+    }
+  }
+}
+
+template <bool FP16>
+static int launch_norm(const void* in, const void* residual, const void* weight, float eps, long rows, int hidden, void* residual_out,
+                       void* normed, void* q, float* scales, hipStream_t stream) {
+  const int chunks = (hidden + kNormThreads * 8 - 1) / (kNormThreads * 8);
+  const long step = 1L << 22;
+  for (long r = 0; r < rows; r += step) {
+    const unsigned n = (unsigned)(rows - r < step ? rows - r : step);
+    const long at = r * hidden;
+#define ESMOE_NORM(C)                                                                                                             \
+  hipLaunchKernelGGL((add_rms_norm_quant_kernel<FP16, C>), dim3(n), dim3(kNormThreads), 0, stream, (const uint16_t*)in + at,       \
+                     residual ? (const uint16_t*)residual + at : nullptr, (const uint16_t*)weight, eps, hidden,                   \
+                     residual ? (uint16_t*)residual_out + at : nullptr, normed ? (uint16_t*)normed + at : nullptr,                \
+                     (uint8_t*)q + at, scales + at / 128)
+    if (chunks <= 1) ESMOE_NORM(1);
+    else if (chunks <= 2) ESMOE_NORM(2);
+    else if (chunks <= 4) ESMOE_NORM(4);
+    else if (chunks <= 8) ESMOE_NORM(8);
+    else ESMOE_NORM(16);
+#undef ESMOE_NORM
+  }
+  return (int)hipGetLastError();
+}
+
+}  // namespace esmoe
+
+extern "C" int esmoe_launch_add_rms_norm_quant(const void* in, int in_dtype, const void* residual, const void* weight, float eps, long rows,
+                                               int hidden, void* residual_out, void* normed, void* q, float* scales, hipStream_t stream) {
+  return in_dtype ? esmoe::launch_norm<true>(in, residual, weight, eps, rows, hidden, residual_out, normed, q, scales, stream)
+                  : esmoe::launch_norm<false>(in, residual, weight, eps, rows, hidden, residual_out, normed, q, scales, stream);
+}

@@ -14,6 +14,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/all.h>
 
+#include <cmath>
+#include <initializer_list>
+
 #include "esmoe.h"
 
 extern "C" {
@@ -508,6 +511,246 @@ void es_mxfp8_quant_weight(const torch::Tensor& input, torch::Tensor& quant_outp
   check_rc(rc, "es_mxfp8_quant_weight");
 }
 
+// ---- the operators around the grouped GEMMs of a mixture-of-experts block (no counterparts in the reference) ----
+namespace {
+
+// These operators are not part of autograd: where a gradient exists it is an operator of its own, and a result that silently had
+// none would train nothing.
+void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), op,
+                ": not differentiable by autograd (call it under torch.no_grad(); gradients are operators of their own)");
+}
+
+void check_device(const torch::Tensor& like, std::initializer_list<const torch::Tensor*> tensors) {
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || t->device() == like.device(), "all tensors must be on the same device");
+}
+
+bool is_half_type(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kHalf; }
+
+int logits_dtype_of(const torch::Tensor& t) {
+  return t.scalar_type() == torch::kFloat32 ? ESMOE_LOGITS_FP32 : t.scalar_type() == torch::kHalf ? ESMOE_LOGITS_FP16 : ESMOE_LOGITS_BF16;
+}
+
+void check_logits(const torch::Tensor& logits, int64_t topk) {
+  TORCH_CHECK(logits.dim() == 2, "logits must be 2D tensor");
+  TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || is_half_type(logits), "logits must be float32, bfloat16 or half");
+  const int64_t experts = logits.size(1);
+  TORCH_CHECK(experts >= 1 && experts <= ESMOE_MAX_EXPERTS, "Number of experts must be in [1, 1024]");
+  TORCH_CHECK(experts == 1 || logits.stride(1) == 1, "logits must be row major");
+  TORCH_CHECK(topk >= 1 && topk <= ESMOE_MAX_TOPK && topk <= experts, "topk must be in [1, 64] and at most the number of experts");
+  TORCH_CHECK(logits.size(0) < (int64_t(1) << 31) / topk, "tensor too large");
+}
+
+const torch::Tensor& tensor_or_none(const c10::optional<torch::Tensor>& t) {
+  static const torch::Tensor none;
+  return t.has_value() ? *t : none;
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, torch::Tensor> es_topk_gating(const torch::Tensor& logits, int64_t topk, const c10::optional<torch::Tensor>& bias_,
+                                                        bool sigmoid, bool renormalize, double scale, int64_t num_groups,
+                                                        int64_t topk_groups) {
+  const torch::Tensor& bias = tensor_or_none(bias_);
+  check_logits(logits, topk);
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == experts && bias.scalar_type() == torch::kFloat32 && bias.is_contiguous()),
+              "bias must be a contiguous float32 tensor with one element per expert");
+  TORCH_CHECK(num_groups >= 1 && num_groups <= 64 && experts % num_groups == 0, "num_groups must be in [1, 64] and divide the number of experts");
+  TORCH_CHECK(topk_groups >= 1 && topk_groups <= num_groups, "topk_groups must be in [1, num_groups]");
+  TORCH_CHECK(topk <= experts / num_groups * topk_groups, "topk is more than the experts of topk_groups groups");
+  TORCH_CHECK(std::isfinite((float)scale), "scale must be finite");
+  check_no_autograd("es_topk_gating", {&logits, &bias});
+  require_device(logits, "es_topk_gating");
+  check_device(logits, {&bias});
+  c10::DeviceGuard guard(logits.device());
+  torch::Tensor ids = torch::empty({tokens, topk}, logits.options().dtype(torch::kInt32)),
+                weights = torch::empty({tokens, topk}, logits.options().dtype(torch::kFloat32));
+  if (tokens == 0) return {ids, weights};
+  int rc = esmoe_topk_gating(logits.data_ptr(), logits_dtype_of(logits), (long)logits.stride(0), bias.defined() ? bias.data_ptr<float>() : nullptr,
+                             (long)tokens, (int)experts, (int)topk, sigmoid ? ESMOE_SCORING_SIGMOID : ESMOE_SCORING_SOFTMAX, renormalize,
+                             (float)scale, (int)num_groups, (int)topk_groups, ids.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                             current_stream(logits));
+  check_rc(rc, "es_topk_gating");
+  return {ids, weights};
+}
+
+torch::Tensor es_topk_gating_backward(const torch::Tensor& grad_weights, const torch::Tensor& logits, const torch::Tensor& topk_ids,
+                                      bool sigmoid, bool renormalize, double scale) {
+  TORCH_CHECK(topk_ids.dim() == 2 && topk_ids.scalar_type() == torch::kInt32 && topk_ids.is_contiguous(),
+              "topk_ids must be a contiguous int32 (tokens, topk) tensor");
+  const int64_t topk = topk_ids.size(1);
+  check_logits(logits, topk);
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  TORCH_CHECK(topk_ids.size(0) == tokens, "topk_ids must have a row per row of logits");
+  TORCH_CHECK(grad_weights.sizes() == topk_ids.sizes() && grad_weights.scalar_type() == torch::kFloat32 && grad_weights.is_contiguous(),
+              "grad_weights must be a contiguous float32 tensor of topk_ids' shape");
+  TORCH_CHECK(std::isfinite((float)scale), "scale must be finite");
+  check_no_autograd("es_topk_gating_backward", {&grad_weights, &logits});
+  require_device(logits, "es_topk_gating_backward");
+  check_device(logits, {&grad_weights, &topk_ids});
+  c10::DeviceGuard guard(logits.device());
+  torch::Tensor grad = torch::empty({tokens, experts}, logits.options());
+  if (tokens == 0) return grad;
+  int rc = esmoe_topk_gating_backward(grad_weights.data_ptr<float>(), logits.data_ptr(), logits_dtype_of(logits), (long)logits.stride(0),
+                                      topk_ids.data_ptr<int32_t>(), (long)tokens, (int)experts, (int)topk,
+                                      sigmoid ? ESMOE_SCORING_SIGMOID : ESMOE_SCORING_SOFTMAX, renormalize, (float)scale, grad.data_ptr(),
+                                      current_stream(logits));
+  check_rc(rc, "es_topk_gating_backward");
+  return grad;
+}
+
+namespace {
+// Checks that both directions of the combine share; returns the tokens.
+int64_t check_combine(const torch::Tensor& rows, const torch::Tensor& dst_row, int64_t topk, const torch::Tensor& weights) {
+  TORCH_CHECK(rows.dim() == 2 && rows.is_contiguous() && is_half_type(rows), "input must be a contiguous 2D bfloat16 or half tensor");
+  TORCH_CHECK(rows.size(1) > 0 && rows.size(1) % 8 == 0, "rows must be a multiple of 16 bytes");
+  TORCH_CHECK(dst_row.scalar_type() == torch::kInt32 && dst_row.is_contiguous(), "dst_row must be contiguous int32");
+  TORCH_CHECK(topk >= 1 && dst_row.numel() % topk == 0, "dst_row must have tokens * topk entries");
+  TORCH_CHECK(!weights.defined() || (weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.numel() == dst_row.numel()),
+              "weights must be a contiguous float32 tensor of dst_row's size");
+  TORCH_CHECK(rows.size(0) < (int64_t(1) << 31) && rows.size(1) <= (int64_t(1) << 24) && dst_row.numel() < (int64_t(1) << 31), "tensor too large");
+  return dst_row.numel() / topk;
+}
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  const char *pa = (const char*)a.data_ptr(), *pb = (const char*)b.data_ptr();
+  return a.numel() && b.numel() && pa < pb + b.nbytes() && pb < pa + a.nbytes();
+}
+}  // namespace
+
+void es_combine_rows(const torch::Tensor& input, const torch::Tensor& dst_row, int64_t topk, const c10::optional<torch::Tensor>& weights_,
+                     torch::Tensor& output) {
+  const torch::Tensor& weights = tensor_or_none(weights_);
+  const int64_t tokens = check_combine(input, dst_row, topk, weights);
+  TORCH_CHECK(output.dim() == 2 && output.is_contiguous() && output.scalar_type() == input.scalar_type() && output.size(0) == tokens &&
+                  output.size(1) == input.size(1),
+              "output must be a contiguous (tokens, row length) tensor of input's dtype");
+  check_no_autograd("es_combine_rows", {&input, &weights});
+  require_device(input, "es_combine_rows");
+  check_device(input, {&dst_row, &weights, &output});
+  TORCH_CHECK(!overlap(input, output), "output may not overlap input");
+  if (tokens == 0) return;
+  c10::DeviceGuard guard(input.device());
+  int rc = esmoe_combine_rows(input.data_ptr(), input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16,
+                              dst_row.data_ptr<int32_t>(), weights.defined() ? weights.data_ptr<float>() : nullptr, (long)dst_row.numel(),
+                              (int)topk, (long)input.size(0), (int)input.size(1), output.data_ptr(), current_stream(input));
+  check_rc(rc, "es_combine_rows");
+}
+
+void es_combine_rows_backward(const torch::Tensor& grad_output, const torch::Tensor& input, const torch::Tensor& dst_row, int64_t topk,
+                              const torch::Tensor& weights, torch::Tensor& grad_input, torch::Tensor& grad_weights) {
+  const int64_t tokens = check_combine(input, dst_row, topk, weights);
+  TORCH_CHECK(grad_output.dim() == 2 && grad_output.is_contiguous() && grad_output.scalar_type() == input.scalar_type() &&
+                  grad_output.size(0) == tokens && grad_output.size(1) == input.size(1),
+              "grad_output must be a contiguous (tokens, row length) tensor of input's dtype");
+  TORCH_CHECK(grad_input.sizes() == input.sizes() && grad_input.is_contiguous() && grad_input.scalar_type() == input.scalar_type(),
+              "grad_input must be a contiguous tensor of input's shape and dtype");
+  TORCH_CHECK(grad_weights.scalar_type() == torch::kFloat32 && grad_weights.is_contiguous() && grad_weights.numel() == dst_row.numel(),
+              "grad_weights must be a contiguous float32 tensor of dst_row's size");
+  check_no_autograd("es_combine_rows_backward", {&grad_output, &input, &weights});
+  require_device(input, "es_combine_rows_backward");
+  check_device(input, {&grad_output, &dst_row, &weights, &grad_input, &grad_weights});
+  TORCH_CHECK(!overlap(grad_input, input) && !overlap(grad_input, grad_output), "grad_input may not overlap input or grad_output");
+  if (tokens == 0) return;
+  c10::DeviceGuard guard(input.device());
+  int rc = esmoe_combine_rows_backward(grad_output.data_ptr(), input.data_ptr(),
+                                       input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16, dst_row.data_ptr<int32_t>(),
+                                       weights.data_ptr<float>(), (long)dst_row.numel(), (int)topk, (long)input.size(0), (int)input.size(1),
+                                       grad_input.data_ptr(), grad_weights.data_ptr<float>(), current_stream(input));
+  check_rc(rc, "es_combine_rows_backward");
+}
+
+void es_add_rms_norm_quant_1x128(const torch::Tensor& input, const torch::Tensor& weight, double eps,
+                                 const c10::optional<torch::Tensor>& residual_, const c10::optional<torch::Tensor>& residual_out_,
+                                 const c10::optional<torch::Tensor>& normed_, torch::Tensor& quant_output, torch::Tensor& scales) {
+  const torch::Tensor &residual = tensor_or_none(residual_), &residual_out = tensor_or_none(residual_out_), &normed = tensor_or_none(normed_);
+  TORCH_CHECK(input.dim() == 2 && input.is_contiguous(), "input must be a contiguous 2D tensor");
+  TORCH_CHECK(is_half_type(input), "dtype must be kFloat16 or kBFloat16");
+  const int64_t rows = input.size(0), k = input.size(1);
+  TORCH_CHECK(k > 0 && k % 128 == 0 && k <= 32768, "k must align to 128 and be at most 32768");
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == k && weight.is_contiguous() && weight.scalar_type() == input.scalar_type(),
+              "weight must be a contiguous tensor of k elements of input's dtype");
+  TORCH_CHECK(eps >= 0 && std::isfinite((float)eps), "eps must be finite and not negative");
+  TORCH_CHECK(residual.defined() == residual_out.defined(), "residual and residual_out go together");
+  for (const torch::Tensor* t : {&residual, &residual_out, &normed})
+    TORCH_CHECK(!t->defined() || (t->sizes() == input.sizes() && t->is_contiguous() && t->scalar_type() == input.scalar_type()),
+                "residual, residual_out and normed must be contiguous tensors of input's shape and dtype");
+  TORCH_CHECK(quant_output.is_contiguous() && quant_output.element_size() == 1 && quant_output.numel() == rows * k,
+              "quant_output must be a contiguous 1-byte tensor of rows * k elements");
+  TORCH_CHECK(scales.is_contiguous() && scales.scalar_type() == torch::kFloat32 && scales.numel() == rows * (k / 128),
+              "scales must be a contiguous float32 tensor of rows * k / 128 elements");
+  check_no_autograd("es_add_rms_norm_quant_1x128", {&input, &weight, &residual});
+  require_device(input, "es_add_rms_norm_quant_1x128");
+  check_device(input, {&weight, &residual, &residual_out, &normed, &quant_output, &scales});
+  if (rows == 0) return;
+  // a row is read before any of its results is written: the new residual may take input's or residual's place, nothing else may overlap
+  for (const torch::Tensor* in : {&input, &residual, &weight}) {
+    if (!in->defined()) continue;
+    for (const torch::Tensor* out : {(const torch::Tensor*)&quant_output, (const torch::Tensor*)&scales, &normed})
+      TORCH_CHECK(!out->defined() || !overlap(*in, *out), "outputs may not overlap inputs");
+    TORCH_CHECK(!residual_out.defined() || !overlap(*in, residual_out) || (in != &weight && in->data_ptr() == residual_out.data_ptr()),
+                "residual_out may be input or residual, not a part of them");
+  }
+  c10::DeviceGuard guard(input.device());
+  int rc = esmoe_add_rms_norm_quant_1x128(
+      input.data_ptr(), input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16, residual.defined() ? residual.data_ptr() : nullptr,
+      weight.data_ptr(), (float)eps, (long)rows, (int)k, residual.defined() ? residual_out.data_ptr() : nullptr,
+      normed.defined() ? normed.data_ptr() : nullptr, quant_output.data_ptr(), scales.data_ptr<float>(), current_stream(input));
+  check_rc(rc, "es_add_rms_norm_quant_1x128");
+}
+
+namespace {
+void mxfp4_grouped_mm(const char* op, bool swiglu, torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b,
+                      const torch::Tensor& sfb, const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets) {
+  TORCH_CHECK(problem_sizes.dim() == 2 && problem_sizes.size(1) == 3, "problem_sizes must have shape (num_experts, 3)");
+  const int64_t num_experts = problem_sizes.size(0);
+  TORCH_CHECK(expert_offsets.dim() == 1 && expert_offsets.size(0) == num_experts, "Number of experts in problem_sizes must match expert_offsets");
+  TORCH_CHECK(problem_sizes.dtype() == torch::kInt32 && expert_offsets.dtype() == torch::kInt32, "problem_sizes and expert_offsets must be int32");
+  TORCH_CHECK(num_experts >= 1 && num_experts <= ESMOE_MAX_EXPERTS, "Number of experts cannot exceed 1024");
+  TORCH_CHECK(is_half_type(a), "a must be bfloat16 or half");
+  TORCH_CHECK(a.dim() == 2 && a.is_contiguous(), "a must be a packed row-major (rows, k) tensor");
+  const int64_t total_rows = a.size(0), k = a.size(1);
+  TORCH_CHECK(k > 0 && k % 128 == 0 && k <= 32768, "k must be a multiple of 128 up to 32768");
+  TORCH_CHECK(b.dim() == 3 && b.size(0) == num_experts && b.element_size() == 1 && b.size(1) == k / 2,
+              "b must be a 1-byte (num_experts, k/2, n) tensor of two 4-bit codes each");
+  const int64_t n = b.size(2);
+  TORCH_CHECK(n > 0 && n % (swiglu ? 32 : 16) == 0 && n <= (int64_t(1) << 20), "n must be a multiple of 16 (of 32 with SwiGLU) up to 2^20");
+  TORCH_CHECK(b.stride(1) == 1 && b.stride(2) == k / 2 && (num_experts == 1 || b.stride(0) == n * (k / 2)),
+              "b must be the column-major (num_experts, k/2, n) view of a packed (num_experts, n, k/2) tensor");
+  TORCH_CHECK(sfb.dim() == 3 && sfb.element_size() == 1 && sfb.size(0) == num_experts && sfb.size(1) == k / 32 && sfb.size(2) == n &&
+                  sfb.stride(1) == 1 && sfb.stride(2) == k / 32 && (num_experts == 1 || sfb.stride(0) == n * (k / 32)),
+              "sfb must be the 1-byte column-major (num_experts, k/32, n) view of a packed (num_experts, n, k/32) tensor");
+  TORCH_CHECK(output.dim() == 2 && output.is_contiguous() && output.scalar_type() == a.scalar_type() && output.size(0) == total_rows &&
+                  output.size(1) == (swiglu ? n / 2 : n),
+              "output must be a contiguous (rows, n) tensor, (rows, n / 2) with SwiGLU, of a's dtype");
+  TORCH_CHECK(total_rows < (int64_t(1) << 31), "tensor too large");
+  check_no_autograd(op, {&a});
+  require_device(a, op);
+  check_device(a, {&output, &b, &sfb, &problem_sizes, &expert_offsets});
+  TORCH_CHECK(problem_sizes.is_contiguous() && expert_offsets.is_contiguous(), "metadata tensors must be contiguous");
+  TORCH_CHECK(!overlap(a, output), "output may not overlap a");
+  if (total_rows == 0) return;
+  c10::DeviceGuard guard(a.device());
+  int rc = esmoe_mxfp4_grouped_mm(output.data_ptr(), out_dtype_of(output), a.data_ptr(), b.data_ptr(), (const uint8_t*)sfb.data_ptr(),
+                                  problem_sizes.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), (int)num_experts, (int)total_rows,
+                                  (int)n, (int)k, swiglu, current_stream(a));
+  check_rc(rc, op);
+}
+}  // namespace
+
+void es_mxfp4_grouped_mm(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& sfb,
+                         const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets) {
+  mxfp4_grouped_mm("es_mxfp4_grouped_mm", false, output, a, b, sfb, problem_sizes, expert_offsets);
+}
+
+void es_mxfp4_grouped_mm_swiglu(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& sfb,
+                                const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets) {
+  mxfp4_grouped_mm("es_mxfp4_grouped_mm_swiglu", true, output, a, b, sfb, problem_sizes, expert_offsets);
+}
+
 TORCH_LIBRARY(expert_specialization, m) {
   m.def(
       "es_fp8_blockwise_scaled_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor scales_a, Tensor scales_b, Tensor "
@@ -534,6 +777,21 @@ TORCH_LIBRARY(expert_specialization, m) {
   m.def("es_mxfp8_quant_weight(Tensor input, Tensor quant_output, Tensor scale_factor) -> ()");
   m.def("es_route_metadata(Tensor topk_ids, int first_expert, int num_experts, int n, int k) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("es_permute_rows(Tensor input, Tensor dst_row, int topk, Tensor output) -> ()");
+  m.def(
+      "es_topk_gating(Tensor logits, int topk, Tensor? bias, bool sigmoid, bool renormalize, float scale, int num_groups, int "
+      "topk_groups) -> (Tensor, Tensor)");
+  m.def(
+      "es_topk_gating_backward(Tensor grad_weights, Tensor logits, Tensor topk_ids, bool sigmoid, bool renormalize, float scale) -> "
+      "Tensor");
+  m.def("es_combine_rows(Tensor input, Tensor dst_row, int topk, Tensor? weights, Tensor output) -> ()");
+  m.def(
+      "es_combine_rows_backward(Tensor grad_output, Tensor input, Tensor dst_row, int topk, Tensor weights, Tensor grad_input, Tensor "
+      "grad_weights) -> ()");
+  m.def(
+      "es_add_rms_norm_quant_1x128(Tensor input, Tensor weight, float eps, Tensor? residual, Tensor? residual_out, Tensor? normed, "
+      "Tensor quant_output, Tensor scales) -> ()");
+  m.def("es_mxfp4_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
+  m.def("es_mxfp4_grouped_mm_swiglu(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(expert_specialization, CUDA, m) {
@@ -549,6 +807,13 @@ TORCH_LIBRARY_IMPL(expert_specialization, CUDA, m) {
   m.impl("es_mxfp8_quant_weight", &es_mxfp8_quant_weight);
   m.impl("es_route_metadata", &es_route_metadata);
   m.impl("es_permute_rows", &es_permute_rows);
+  m.impl("es_topk_gating", &es_topk_gating);
+  m.impl("es_topk_gating_backward", &es_topk_gating_backward);
+  m.impl("es_combine_rows", &es_combine_rows);
+  m.impl("es_combine_rows_backward", &es_combine_rows_backward);
+  m.impl("es_add_rms_norm_quant_1x128", &es_add_rms_norm_quant_1x128);
+  m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
+  m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
 }
 
 // Same functions on the CPU key: the checks run, then require_device() raises.
@@ -565,4 +830,11 @@ TORCH_LIBRARY_IMPL(expert_specialization, CPU, m) {
   m.impl("es_mxfp8_quant_weight", &es_mxfp8_quant_weight);
   m.impl("es_route_metadata", &es_route_metadata);
   m.impl("es_permute_rows", &es_permute_rows);
+  m.impl("es_topk_gating", &es_topk_gating);
+  m.impl("es_topk_gating_backward", &es_topk_gating_backward);
+  m.impl("es_combine_rows", &es_combine_rows);
+  m.impl("es_combine_rows_backward", &es_combine_rows_backward);
+  m.impl("es_add_rms_norm_quant_1x128", &es_add_rms_norm_quant_1x128);
+  m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
+  m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
 }

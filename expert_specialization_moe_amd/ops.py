@@ -130,3 +130,80 @@ def es_mxfp8_blockscaled_grouped_mm_swiglu_quant(quant_output, scale_factor, a, 
     _ns.es_mxfp8_blockscaled_grouped_mm_swiglu_quant.default(quant_output, scale_factor, a, b, sfa, sfb, problem_sizes,
                                                              expert_offsets, blockscale_offsets,
                                                              mid_dtype == torch.bfloat16)
+
+
+_SIGMOID = {"softmax": False, "sigmoid": True}
+
+
+def _is_sigmoid(scoring):
+    if scoring not in _SIGMOID:
+        raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    return _SIGMOID[scoring]
+
+
+def es_topk_gating(logits, topk, bias=None, scoring="softmax", renormalize=True, scale=1.0, num_groups=1, topk_groups=1):
+    """Router logits [T, E] (fp32, bf16 or fp16) -> (topk_ids int32 [T, topk], topk_weights fp32 [T, topk]), the ids for
+    es_route_metadata and the weights for es_combine_rows (no counterpart in the reference).
+
+    Scores s are the softmax or the sigmoid of a token's logits.  Its experts are the topk largest of s + bias (fp32 [E]; of the logits
+    where there is no bias), ties to the lower index, from the topk_groups groups of E / num_groups experts with the largest sum of
+    their two best.  The weights are scale * s, divided by the chosen experts' sum where renormalize is set.  An expert with a logit
+    of -inf is never chosen; a place that none is left for gets id -1 and weight 0."""
+    return _ns.es_topk_gating.default(logits, topk, bias, _is_sigmoid(scoring), renormalize, scale, num_groups, topk_groups)
+
+
+def es_topk_gating_backward(grad_weights, logits, topk_ids, scoring="softmax", renormalize=True, scale=1.0):
+    """Gradient of es_topk_gating's weights with respect to the logits ([T, E], logits' dtype), the ids held fixed; a bias has none."""
+    return _ns.es_topk_gating_backward.default(grad_weights, logits, topk_ids, _is_sigmoid(scoring), renormalize, scale)
+
+
+def es_combine_rows(input, dst_row, topk, weights=None, output=None):
+    """output[t] = sum over j of weights[t, j] * input[dst_row[t * topk + j]] (pairs with dst_row < 0 are left out): the experts' packed
+    rows back at their tokens, summed in fp32.  Without weights it is the gradient of es_permute_rows.  No counterpart in the reference."""
+    if output is None:
+        output = input.new_empty((dst_row.numel() // max(topk, 1), input.size(1)))
+    _ns.es_combine_rows.default(input, dst_row, topk, weights, output)
+    return output
+
+
+def es_combine_rows_backward(grad_output, input, dst_row, topk, weights, grad_input=None, grad_weights=None):
+    """Gradients of es_combine_rows: (grad_input [rows, H], grad_weights fp32 of weights' shape).  Rows of a given grad_input that no
+    pair points to are left as they were; in one that is allocated here they are zero.  No two pairs may share a row (those of
+    es_route_metadata do not)."""
+    if grad_input is None:
+        grad_input = torch.zeros_like(input)
+    if grad_weights is None:
+        grad_weights = torch.empty_like(weights)
+    _ns.es_combine_rows_backward.default(grad_output, input, dst_row, topk, weights, grad_input, grad_weights)
+    return grad_input, grad_weights
+
+
+def es_add_rms_norm_quant_1x128(input, weight, eps=1e-6, residual=None, residual_out=None, normed=None, quant_output=None, scales=None,
+                                return_normed=False):
+    """h = input + residual, y = h / sqrt(mean(h^2) + eps) * weight, y quantised as es_fp8_quant_act_1x128 does, in one pass:
+    (e4m3fn [M, K], fp32 scales [M, K/128], h or None, y or None).  h is the new residual, in input's dtype; it may be written over
+    input or residual (residual_out).  y in input's dtype is given back where `normed` is given or return_normed is set.  Serving
+    only: there is no gradient.  No counterpart in the reference."""
+    m, k = input.shape
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(input)
+    if normed is None and return_normed:
+        normed = torch.empty_like(input)
+    if quant_output is None:
+        quant_output = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=input.device)
+    if scales is None:
+        scales = torch.empty((m, k // 128), dtype=torch.float32, device=input.device)
+    _ns.es_add_rms_norm_quant_1x128.default(input, weight, eps, residual, residual_out, normed, quant_output, scales)
+    return quant_output, scales, residual_out, normed
+
+
+def es_mxfp4_grouped_mm(output, a, b, sfb, problem_sizes, expert_offsets):
+    """Grouped product of bf16/fp16 rows with 4-bit weights, for the few rows per expert of a decode step: ``b`` is the (E, K/2, N) view of
+    e2m1 codes [E, N, K/2] (even column in the low half of a byte), ``sfb`` the (E, K/32, N) view of E8M0 scales [E, N, K/32]
+    (quant.quant_weight_mxfp4 makes both); metadata as es_fp8_blockwise_scaled_grouped_mm.  No counterpart in the reference."""
+    _ns.es_mxfp4_grouped_mm.default(output, a, b, sfb, problem_sizes, expert_offsets)
+
+
+def es_mxfp4_grouped_mm_swiglu(output, a, b, sfb, problem_sizes, expert_offsets):
+    """es_mxfp4_grouped_mm of a gate_up projection (N = 2 * I, gate rows first) with output = silu(gate) * up of its fp32 sums, [M, I]."""
+    _ns.es_mxfp4_grouped_mm_swiglu.default(output, a, b, sfb, problem_sizes, expert_offsets)

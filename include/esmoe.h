@@ -35,11 +35,19 @@ extern "C" {
 
 #define ESMOE_MAX_EXPERTS 1024 /* same limit as the reference, es_fp8_blockwise_launcher.cuh:53 */
 
+#define ESMOE_LOGITS_BF16 0
+#define ESMOE_LOGITS_FP16 1
+#define ESMOE_LOGITS_FP32 2
+#define ESMOE_SCORING_SOFTMAX 0
+#define ESMOE_SCORING_SIGMOID 1
+#define ESMOE_MAX_TOPK 64
+
 /* ABI revision of this header; esmoe_version() of a matching library reads "esmoe 0.<ESMOE_ABI> (gfx950)".
+ * 4: esmoe_topk_gating, esmoe_combine_rows, their gradients, esmoe_add_rms_norm_quant_1x128 and esmoe_mxfp4_grouped_mm added.
  * 3: a null `workspace` selects the library's own; esmoe_stream_workspace added; the workspace layout gained an exit
  *    counter (same size).  2: the esmoe_host_* mirrors gained `kind` after `force_bm`; esmoe_gemm_workspace_bytes
  *    grew from 16 E + 80 to 16 E + 1296 bytes and the workspace must be 16-byte aligned. */
-#define ESMOE_ABI 3
+#define ESMOE_ABI 4
 
 /* Bytes of device scratch the GEMM entry points need for `num_experts` experts
  * (the device-built tile schedule and its hand-out counters).  The scratch must be 16-byte aligned (device allocations
@@ -272,6 +280,70 @@ int esmoe_route_metadata(const int32_t* topk_ids, long num_pairs, int first_expe
  * (a multiple of 16), `in` and `out` 16-byte aligned.  No counterpart in the reference. */
 int esmoe_permute_rows(const void* in, const int32_t* dst_row, long num_pairs, int topk, long row_bytes, void* out,
                        void* stream);
+
+/*
+ * Router gating: the top-k experts of every token and their weights.  No counterpart in the reference, whose callers draw the
+ * ids at random (benchmark/benchmark_es_fp8_blockwise_moe.py:44-56).
+ *
+ *   logits [tokens, num_experts] of logits_dtype, rows row_stride elements apart;  bias [num_experts] fp32 or NULL
+ *   s = softmax(logits) or sigmoid(logits) (scoring), per token
+ *   choice = fp32(s + bias) from 64-bit arithmetic, or the logits themselves where there is neither a bias nor num_groups > 1
+ *   num_groups groups of consecutive experts: of these the topk_groups with the largest sum of their two largest choices stay
+ *   topk_ids [tokens, topk] int32: the largest choices left, falling, ties to the lower index; NaN above every number.  An expert
+ *     whose logit or choice is -infinity is never taken: a place with no expert left gets id -1 (which esmoe_route_metadata skips)
+ *     and weight 0.
+ *   topk_weights [tokens, topk] fp32: scale * s[id], with renormalize divided by the sum of s over the token's ids.
+ * num_experts <= ESMOE_MAX_EXPERTS, topk <= ESMOE_MAX_TOPK, num_groups <= 64 and a divisor of num_experts.
+ *
+ * esmoe_topk_gating_backward: the gradient of topk_weights with respect to the logits, the ids held fixed (the bias takes part in
+ * the choice alone and has no gradient): grad_logits [tokens, num_experts] of logits_dtype, packed, every element written.  Places
+ * with an id outside [0, num_experts) are left out, an id that stands twice counts twice.
+ */
+int esmoe_topk_gating(const void* logits, int logits_dtype, long row_stride, const float* bias, long tokens, int num_experts, int topk,
+                      int scoring, int renormalize, float scale, int num_groups, int topk_groups, int32_t* topk_ids,
+                      float* topk_weights, void* stream);
+int esmoe_topk_gating_backward(const float* grad_weights, const void* logits, int logits_dtype, long row_stride,
+                               const int32_t* topk_ids, long tokens, int num_experts, int topk, int scoring, int renormalize, float scale,
+                               void* grad_logits, void* stream);
+
+/*
+ * The way back from the experts: out[t] = sum over j < topk of weights[t, j] * in[dst_row[t * topk + j]], in fp32 with j rising and
+ * one rounding; pairs whose dst_row lies outside [0, rows) are left out, and a token without any gets zeros.  dst_row is what
+ * esmoe_route_metadata writes.  weights [num_pairs] fp32, or NULL for ones: the gradient of esmoe_permute_rows.
+ *   in [rows, hidden], out [num_pairs / topk, hidden], both bf16 or fp16 (dtype), 16-byte aligned; hidden % 8 == 0; out may not
+ *   overlap in.
+ * esmoe_combine_rows_backward: grad_in[dst_row[p]] = weights[p] * grad_out[p / topk] (rows that no pair points to are left as they
+ * were) and grad_weights[p] = <grad_out[p / topk], in[dst_row[p]]> (0 for a pair that is left out).  Two pairs may not share a row.
+ * No counterpart in the reference.
+ */
+int esmoe_combine_rows(const void* in, int dtype, const int32_t* dst_row, const float* weights, long num_pairs, int topk, long rows,
+                       int hidden, void* out, void* stream);
+int esmoe_combine_rows_backward(const void* grad_out, const void* in, int dtype, const int32_t* dst_row, const float* weights,
+                                long num_pairs, int topk, long rows, int hidden, void* grad_in, float* grad_weights, void* stream);
+
+/*
+ * Residual addition, root-mean-square norm and 1x128 quantisation in one pass, the step in front of a projection:
+ *   h = in + residual, rounded to in_dtype and written to residual_out (residual NULL: h = in, residual_out NULL too)
+ *   y = h / sqrt(mean(h^2) + eps) * weight in fp32;  normed [total_rows, k] = y rounded to in_dtype, unless NULL
+ *   q, scales: y quantised as esmoe_fp8_quant_act_1x128 quantises (y as it is, not rounded before)
+ * in, residual, weight [k], residual_out, normed of in_dtype (bf16/fp16), 16-byte aligned; k % 128 == 0, k <= 32768.
+ * residual_out may be in or residual itself.  No counterpart in the reference.
+ */
+int esmoe_add_rms_norm_quant_1x128(const void* in, int in_dtype, const void* residual, const void* weight, float eps, long total_rows,
+                                   int k, void* residual_out, void* normed, void* q, float* scales, void* stream);
+
+/*
+ * Grouped product with 4-bit weights for few rows per expert (decode): activations as they are, no quantisation of them.
+ *   out[off_e + m, j] = cast( sum_k a[off_e + m, k] * e2m1(b[e, j, k]) * 2^(sfb[e, j, k / 32] - 127) )
+ *   swiglu != 0, n = 2 * inter, gate rows first: out[off_e + m, i] = cast( silu(gate) * up ) of the two fp32 sums
+ *   out [total_rows, n] ([total_rows, inter] with SwiGLU) and a [total_rows, k], both bf16 or fp16 (dtype)
+ *   b [E, n, k/2] bytes, two e2m1 codes each, the even column in the low half;  sfb [E, n, k/32] E8M0 bytes, row-major (not swizzled)
+ * k % 128 == 0, k <= 32768; n % 16 == 0 (% 32 with SwiGLU); problem_sizes and expert_offsets as above, column 0 is used.  Rows of out
+ * that belong to no expert are not written.  Any number of rows is right; from some dozen per expert on the 8-bit GEMMs are the
+ * faster ones.  No counterpart in the reference.
+ */
+int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, const uint8_t* sfb, const int32_t* problem_sizes,
+                           const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream);
 
 /*
  * Host mirrors of the device-side tile schedule, for inspection and CPU tests; they touch no GPU.
