@@ -50,7 +50,7 @@ extern "C" int esmoe_launch_add_rms_norm_quant(const void* in, int in_dtype, con
                                                int hidden, void* residual_out, void* normed, void* q, float* scales, hipStream_t stream);
 extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const void* b, const uint8_t* sf, const int* problem_sizes,
                                              const int* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu,
-                                             void* out, hipStream_t stream);
+                                             void* out, int cus, hipStream_t stream);
 
 namespace {
 
@@ -714,7 +714,7 @@ int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, c
   int rc = current_device_info(&info);
   if (rc) return rc;
   rc = esmoe_launch_mxfp4_grouped_mm(a, dtype == ESMOE_OUT_FP16, b, sfb, problem_sizes, expert_offsets, num_experts, total_rows, n, k,
-                                     swiglu != 0, out, (hipStream_t)stream);
+                                     swiglu != 0, out, info.cus, (hipStream_t)stream);
   if (rc) return fail(rc, "mxfp4 grouped mm launch failed: %s", hipGetErrorString((hipError_t)rc));
   return 0;
 }

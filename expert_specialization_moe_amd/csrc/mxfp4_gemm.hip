@@ -20,6 +20,7 @@
 namespace esmoe {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v4i_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -30,27 +31,26 @@ constexpr int kFp4Threads = 256, kFp4Waves = 4, kFp4Rows = 16;
 
 // Eight weights of a dword as values of the activations' type.
 template <bool FP16>
-__device__ __forceinline__ v4i fp4_values(uint32_t w) {
+__device__ __forceinline__ v4i fp4_values(uint32_t w, float scale) {
   v4i r;
   if constexpr (FP16) {
-    r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0));
-    r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1));
-    r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2));
-    r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3));
+    r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
+    r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1));
+    r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2));
+    r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
   } else {
-    r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0));
-    r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1));
-    r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2));
-    r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3));
+    r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
   }
   return r;
 }
 
 template <bool FP16>
-__device__ __forceinline__ v4f mfma32(v4i a, v4i b) {
-  const v4f zero = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (FP16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), zero, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), zero, 0, 0, 0);
+__device__ __forceinline__ v4f mfma32(v4i a, v4i b, v4f c) {
+  if constexpr (FP16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
 // 2^(code - 127); NaN for 255.
@@ -76,35 +76,47 @@ __device__ __forceinline__ void transpose_rows(uint32_t* d) {
   swap16(d[2], d[3]);
 }
 
+template <bool FP16>
+__device__ __forceinline__ uint16_t to_half(float v) {
+  if constexpr (FP16) return __builtin_bit_cast(uint16_t, (_Float16)v);
+  else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// A barrier that orders LDS alone: loads from memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 struct Fp4Unit {
   int expert, row0, rows;   // rows 0: no such unit
 };
 
-// Unit u of the launch: experts in order, each in tiles of kFp4Rows rows.  Rows are clamped to the tensor.
-__device__ __forceinline__ Fp4Unit fp4_unit(int u, const int* __restrict__ problem_sizes, const int* __restrict__ expert_offsets,
-                                            int num_experts, int total_rows) {
-  const int lane = threadIdx.x & 63;
-  for (int e0 = 0; e0 < num_experts; e0 += 64) {
-    const int e = e0 + lane;
-    int m = 0, off = 0;
+// The units of a launch: experts in order, each in tiles of ROWS rows; a lane per expert, 64 at a time.  Rows are clamped to the tensor.
+template <int ROWS>
+struct Fp4Units {
+  int m, off, tiles, end;   // of the lane's expert; end: units up to and with it, from the 64's first on
+  __device__ __forceinline__ void read(int e0, const int* __restrict__ problem_sizes, const int* __restrict__ expert_offsets, int num_experts,
+                                       int total_rows) {
+    const int e = e0 + (threadIdx.x & 63);
+    m = off = 0;
     if (e < num_experts) {
       m = problem_sizes[e * 3];
       off = expert_offsets[e];
-      m = off < 0 || off >= total_rows || m < 0 ? 0 : m > total_rows - off ? total_rows - off : m;
     }
-    const int tiles = (m + kFp4Rows - 1) / kFp4Rows;
-    const int end = wave_inclusive_sum(tiles);
-    const unsigned long long behind = __ballot(end > u);
-    if (behind) {
-      const int l = __builtin_ctzll(behind);
-      const int tile = u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(tiles, l));
-      const int rows = __builtin_amdgcn_readlane(m, l) - tile * kFp4Rows;
-      return {e0 + l, __builtin_amdgcn_readlane(off, l) + tile * kFp4Rows, rows < kFp4Rows ? rows : kFp4Rows};
-    }
-    u -= __builtin_amdgcn_readlane(end, 63);
+    m = off < 0 || off >= total_rows || m < 0 ? 0 : m > total_rows - off ? total_rows - off : m;
+    tiles = (m + ROWS - 1) / ROWS;
+    end = wave_inclusive_sum(tiles);
   }
-  return {0, 0, 0};
-}
+  __device__ __forceinline__ int count() const { return __builtin_amdgcn_readlane(end, 63); }
+  __device__ __forceinline__ Fp4Unit unit(int e0, int u) const {   // u < count()
+    const int l = __builtin_ctzll(__ballot(end > u));
+    const int tile = u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(tiles, l));
+    const int rows = __builtin_amdgcn_readlane(m, l) - tile * ROWS;
+    return {e0 + l, __builtin_amdgcn_readlane(off, l) + tile * ROWS, rows < ROWS ? rows : ROWS};
+  }
+};
 
 template <bool FP16, bool SWIGLU>
 __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ b,
@@ -117,7 +129,16 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int l16 = lane & 15, lr = lane >> 4;
   const int unit = blockIdx.x / col_tiles, tile = blockIdx.x - unit * col_tiles;
-  const Fp4Unit g = fp4_unit(unit0 + unit, problem_sizes, expert_offsets, num_experts, total_rows);
+  Fp4Unit g = {0, 0, 0};
+  for (int e0 = 0, u = unit0 + unit; e0 < num_experts; e0 += 64) {
+    Fp4Units<kFp4Rows> some;
+    some.read(e0, problem_sizes, expert_offsets, num_experts, total_rows);
+    if (u < some.count()) {
+      g = some.unit(e0, u);
+      break;
+    }
+    u -= some.count();
+  }
   if (g.rows == 0) return;   // the whole workgroup
   const int wide = n / NT;   // columns of the output
   const long kb = k / 2, ks = k / 32;
@@ -157,7 +178,7 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
       transpose_rows(d[t]);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const v4f p = mfma32<FP16>(x[i], fp4_values<FP16>(d[t][i]));
+        const v4f p = mfma32<FP16>(x[i], fp4_values<FP16>(d[t][i], 1.0f), v4f{0.f, 0.f, 0.f, 0.f});
         const float scale = e8m0(s[t] >> (8 * i) & 0xff);
 #pragma unroll
         for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], scale, acc[t][r]);
@@ -182,15 +203,266 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
   out[(long)(g.row0 + m) * wide + tile * 16 + col] = bits;
 }
 
+// Sixteen rows of `a` stay in registers: wavefront w of a workgroup holds their K range of up to two pairs of chunks (a chunk is 128
+// columns, a pair 128 bytes of weights), and the workgroup streams tiles of sixteen weight rows past them, two tiles a step (SwiGLU: the
+// gate's and the up projection's; otherwise neighbours).  A step's partial sums meet in LDS; a tile's registers are loaded again as soon
+// as it is used up, and the barrier waits for LDS alone.  The tiles' scales come in whole, a dword per thread, a step ahead.  The steps
+// of all units are one line that is cut evenly over the workgroups, as many as are resident at once.
+//
+// A load takes 128 bytes of eight rows (whole cache lines); lanes eight apart then trade halves, so that a lane has one row's chunk.
+// A lane's sixteen bytes are the 32 columns of one scale, which goes into the conversion: the value is exact in bf16 up to a scale of
+// 2^125, in fp16 from 2^-23 to 2^13.  A step that meets other scales is done again by fp4_any_scale.
+constexpr int kFp4MaxWaves = 16, kFp4Chunks = 4;
+
+struct Fp4Args {
+  const uint16_t* a;
+  const uint8_t *b, *sf;
+  const int *problem_sizes, *expert_offsets;
+  int num_experts, total_rows, n, k;
+  uint16_t* out;
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_bytes(const uint8_t* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00027000);
+}
+
+// Lanes with bit 3 clear keep x and get y's place of the lane eight above in y; lanes with it set the other way round.
+__device__ __forceinline__ void trade_halves(v4i& x, v4i& y) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int a = x[i], b = y[i];
+    x[i] = __builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false);   // row_ror:8 into lanes 8 .. 15
+    y[i] = __builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false);   // into lanes 0 .. 7
+  }
+}
+
+// Sums of `count` chunks of sixteen weight rows times sixteen rows of `a`, whatever the scales: a product of 32 columns is multiplied by
+// its scale when it is added up.  src, ssrc, ap: the lane's row (l16) and, of the bytes and columns, its lane row's first.
+template <bool FP16>
+__device__ __forceinline__ v4f fp4_any_scale(const uint8_t* src, const uint8_t* ssrc, const uint16_t* ap, bool has_row, int count) {
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < count; c++) {
+    const v4i raw = *(const v4i*)(src + c * 64);
+    const uint32_t s = *(const uint32_t*)(ssrc + c * 4);
+    v4i x[4];
+    uint32_t d[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[i] = v4i{0, 0, 0, 0};
+      if (has_row) x[i] = *(const v4i*)(ap + c * 128 + i * 32);
+      d[i] = (uint32_t)raw[i];
+    }
+    transpose_rows(d);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const v4f r = mfma32<FP16>(x[i], fp4_values<FP16>(d[i], 1.0f), v4f{0.f, 0.f, 0.f, 0.f});
+      const float scale = e8m0(s >> (8 * i) & 0xff);
+#pragma unroll
+      for (int q = 0; q < 4; q++) acc[q] = __builtin_fmaf(r[q], scale, acc[q]);
+    }
+  }
+  return acc;
+}
+
+template <bool FP16, bool SWIGLU>
+__global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args p) {
+  constexpr uint32_t kLeast = FP16 ? 104 : 0, kSpan = FP16 ? 36 : 252;   // scale codes of exact values
+  extern __shared__ uint32_t s_mem[];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+  const int l16 = lane & 15, lr = lane >> 4;
+  const int chunks = p.k / 128, pairs = (chunks + 1) / 2;
+  float* s_part = (float*)s_mem;                    // [2 steps][2 tiles][wavefronts][256]
+  uint32_t* s_scale = s_mem + 1024 * waves;         // [2 steps][2 tiles][chunks][16 rows]
+  uint32_t* s_far = s_scale + 64 * chunks;          // [2 steps]: whether a wavefront met a scale that needs fp4_any_scale
+  const int inter = p.n / 2;
+  const int steps = SWIGLU ? p.n / 32 : (p.n / 16 + 1) / 2;   // of a unit
+  const long kb = p.k / 2, ks = p.k / 32;
+  const int p0 = pairs * w / waves, c0 = 2 * p0;
+  const int count = 2 * (pairs * (w + 1) / waves) < chunks ? 2 * (pairs * (w + 1) / waves) - c0 : chunks - c0;   // (1 .. kFp4Chunks)
+  Fp4Units<kFp4Rows> some;
+  some.read(0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
+  int units = some.count();
+  for (int e0 = 64; e0 < p.num_experts; e0 += 64) {
+    Fp4Units<kFp4Rows> more;
+    more.read(e0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
+    units += more.count();
+  }
+  // (the launch sees to it that the steps of all units are fewer than 2^31)
+  const uint32_t total = (uint32_t)units * steps, share = total / gridDim.x, rest = total % gridDim.x;
+  uint32_t at = blockIdx.x * share + (blockIdx.x < rest ? blockIdx.x : rest);
+  const uint32_t end = at + share + (blockIdx.x < rest ? 1 : 0);
+  // The lane's place in the wavefront's bytes of eight weight rows: row l16 % 8, half l16 / 8 of a pair's line (a pair that ends a row of
+  // an odd number of chunks has one half: taken twice, times zeros of `a`; so is the last pair of a wavefront that has only one).
+  uint32_t wlane[2];
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int pair = 2 * q < count ? q : 0;
+    wlane[q] = (uint32_t)((l16 & 7) * (int)kb + pair * 128 + (l16 >= 8 && 2 * pair + 1 < count ? 64 : 0) + lr * 16);
+  }
+  const int srow = tid / chunks, splace = (tid - srow * chunks) * 16 + srow;   // the thread's dword of a tile's scales
+  const bool has_scale = tid < 16 * chunks;
+  if (tid < 2) s_far[tid] = 0;   // (before the first step's barrier)
+  int e0 = 0, before = 0;   // `some` holds the experts from e0 on, whose units are those from `before` on
+  int buf = 0;
+  while (at < end) {
+    const uint32_t unit = at / steps;
+    int step = (int)(at - unit * steps);
+    const int last = end - unit * steps < (uint32_t)steps ? (int)(end - unit * steps) : steps;
+    while ((int)unit >= before + some.count()) {
+      before += some.count();
+      e0 += 64;
+      some.read(e0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
+    }
+    const Fp4Unit g = some.unit(e0, (int)unit - before);
+    const uint8_t* bw = p.b + (long)g.expert * p.n * kb + p0 * 128;
+    const uint8_t* sw = p.sf + (long)g.expert * p.n * ks;
+    v4i wt[kFp4Chunks];
+    uint32_t sc[2];
+    auto first_row = [&](int h, int st) {   // of half h of step st; the second half of a last step that has none: the one before
+      const int row = SWIGLU ? h * inter + st * 16 : st * 32 + h * 16;
+      return (long)(!SWIGLU && row >= p.n ? p.n - 16 : row);
+    };
+    // (descriptors of a tile's bytes: a lane's place in them is all that the loads take from vector registers, and a dword past the
+    // tile's scales reads as 0)
+    auto load = [&](int q, int h, int st) {   // pair q of the wavefront's range
+      const auto src = tile_bytes(bw + first_row(h, st) * kb, (int)(16 * kb) - p0 * 128);
+#pragma unroll
+      for (int r = 0; r < 2; r++) wt[2 * q + r] = __builtin_amdgcn_raw_buffer_load_b128(src, wlane[q], r * 8 * (int)kb, 0);
+    };
+    auto load_scales = [&](int st) {
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        sc[h] = __builtin_amdgcn_raw_buffer_load_b32(tile_bytes(sw + first_row(h, st) * ks, 16 * (int)ks), tid * 4, 0, 0);
+    };
+    auto store_scales = [&](int b) {
+      if (has_scale) {
+        s_scale[(b * 2 + 0) * 16 * chunks + splace] = sc[0];
+        s_scale[(b * 2 + 1) * 16 * chunks + splace] = sc[1];
+      }
+    };
+    load_scales(step);
+    load(0, 0, step);
+    load(1, 0, step);
+    __builtin_amdgcn_sched_barrier(0);   // (ahead of the rows of `a`, which come from a cache)
+    v4i x[kFp4Chunks][4];
+    {
+      const bool has_row = l16 < g.rows;
+      const uint16_t* ap = p.a + (long)(g.row0 + (has_row ? l16 : 0)) * p.k + c0 * 128 + lr * 32;
+#pragma unroll
+      for (int j = 0; j < kFp4Chunks; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const v4i v = *(const v4i*)(ap + (j < count ? j : 0) * 128 + i * 8);
+          x[j][i] = has_row && j < count ? v : v4i{0, 0, 0, 0};
+        }
+    }
+    // The outputs of a step from its partial sums: four lanes for a sum, every fourth wavefront's each, then the four in one order.
+    auto finish = [&](int b, int st) {
+      const int outputs = (SWIGLU ? 16 : 32) * g.rows;
+      int t = tid;
+      asm volatile("" : "+v"(t));   // (what follows from it is worked out here, not kept in registers over the steps)
+      for (; t < 4 * outputs; t += blockDim.x) {
+        const int v = t >> 2, col = v & 15, h = SWIGLU ? 0 : v >> 4 & 1, m = SWIGLU ? v >> 4 : v >> 5;
+        auto sum = [&](int half) {
+          const float* part = s_part + (b * 2 + half) * waves * 256 + (m >> 2) * 64 + col * 4 + (m & 3);
+          float f = 0;
+#pragma unroll 4
+          for (int i = t & 3; i < waves; i += 4) f += part[i * 256];
+          f += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0xB1, 0xf, 0xf, true));
+          return f + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0x4E, 0xf, 0xf, true));
+        };
+        float f;
+        if constexpr (SWIGLU) f = swiglu_f32(sum(0), sum(1));
+        else f = sum(h);
+        const int c = SWIGLU ? st * 16 + col : st * 32 + h * 16 + col;
+        if ((t & 3) == 0 && (SWIGLU || c < p.n)) p.out[(long)(g.row0 + m) * (SWIGLU ? inter : p.n) + c] = to_half<FP16>(f);
+      }
+    };
+    store_scales(buf);
+    lds_barrier();
+    for (; step < last; step++) {
+      const int next = step + 1 < last ? step + 1 : step;   // (the last step's loads are its own again: nothing waits for them)
+      load_scales(next);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        int code[kFp4Chunks];
+        uint32_t far = 0;
+#pragma unroll
+        for (int j = 0; j < kFp4Chunks; j++) {
+          const uint32_t four = s_scale[((buf * 2 + h) * chunks + c0 + (j < count ? j : 0)) * 16 + l16];
+          code[j] = (int)__builtin_amdgcn_ubfe(four, lr * 8, 8);
+          const uint32_t d = (uint32_t)code[j] - kLeast;
+          far = far > d ? far : d;
+        }
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        if (far > kSpan) s_far[buf] = 1;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          trade_halves(wt[2 * q], wt[2 * q + 1]);
+#pragma unroll
+          for (int j = 2 * q; j < 2 * q + 2; j++) {
+            __builtin_amdgcn_sched_barrier(0);   // (a chunk's values at a time: more of them do not fit the registers)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              acc = mfma32<FP16>(x[j][i], fp4_values<FP16>((uint32_t)wt[j][i], __builtin_bit_cast(float, code[j] << 23)), acc);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          load(q, h ^ 1, h ? next : step);
+        }
+        *(v4f*)&s_part[((buf * 2 + h) * waves + w) * 256 + lane * 4] = acc;
+      }
+      store_scales(buf ^ 1);
+      lds_barrier();
+      if (__builtin_amdgcn_readfirstlane(s_far[buf]) != 0) {
+        lds_barrier();   // (everyone has seen it)
+        if (tid == 0) s_far[buf] = 0;
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          int place = lane;
+          asm volatile("" : "+v"(place));   // (as in finish)
+          const int row = place & 15, part = place >> 4;
+          const bool has_row = row < g.rows;
+          *(v4f*)&s_part[((buf * 2 + h) * waves + w) * 256 + place * 4] = fp4_any_scale<FP16>(
+              bw + (first_row(h, step) + row) * kb + part * 16, sw + (first_row(h, step) + row) * ks + c0 * 4,
+              p.a + (long)(g.row0 + (has_row ? row : 0)) * p.k + c0 * 128 + part * 8, has_row, count);
+        }
+        lds_barrier();
+        finish(buf, step++);
+        buf ^= 1;
+        break;   // (the registers are loaded again: none are kept across this)
+      }
+      finish(buf, step);
+      buf ^= 1;
+    }
+    at = unit * steps + step;
+  }
+}
+
 }  // namespace esmoe
 
 extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const void* b, const uint8_t* sf, const int* problem_sizes,
                                              const int* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* out,
-                                             hipStream_t stream) {
+                                             int cus, hipStream_t stream) {
   using namespace esmoe;
-  const int col_tiles = n / (swiglu ? 32 : 16);
+  const int steps = swiglu ? n / 32 : (n / 16 + 1) / 2, chunks = k / 128, pairs = (chunks + 1) / 2;
   // units with rows: at most one per expert or row, and one more per full tile
-  const long units = (num_experts < total_rows ? num_experts : total_rows) + (long)total_rows / kFp4Rows;
+  const long experts = num_experts < total_rows ? num_experts : total_rows;
+  const long most = (experts + (long)total_rows / kFp4Rows) * steps;
+  if (chunks <= kFp4Chunks * kFp4MaxWaves && most < 1L << 31) {
+    int waves = (pairs + 1) / 2;
+    const int per_cu = kFp4MaxWaves / waves;
+    waves = kFp4MaxWaves / per_cu < pairs ? kFp4MaxWaves / per_cu : pairs;
+    const int each = (pairs + waves - 1) / waves;
+    waves = (pairs + each - 1) / each;
+    const unsigned grid = (unsigned)(most < (long)cus * per_cu ? most : (long)cus * per_cu);
+    const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint16_t*)out};
+    auto kernel = dtype ? swiglu ? mxfp4_stream_kernel<true, true> : mxfp4_stream_kernel<true, false>
+                        : swiglu ? mxfp4_stream_kernel<false, true> : mxfp4_stream_kernel<false, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 4096 * waves + 256 * chunks + 8, stream, args);
+    return (int)hipGetLastError();
+  }
+  const long units = experts + (long)total_rows / kFp4Rows;
+  const int col_tiles = n / (swiglu ? 32 : 16);
   const long step = (1L << 23) / col_tiles > 1 ? (1L << 23) / col_tiles : 1;   // units of a launch: a grid holds fewer than 2^32 threads
   auto kernel = dtype ? swiglu ? mxfp4_grouped_mm_kernel<true, true> : mxfp4_grouped_mm_kernel<true, false>
                       : swiglu ? mxfp4_grouped_mm_kernel<false, true> : mxfp4_grouped_mm_kernel<false, false>;
