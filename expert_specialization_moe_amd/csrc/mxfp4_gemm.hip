@@ -203,16 +203,16 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
   out[(long)(g.row0 + m) * wide + tile * 16 + col] = bits;
 }
 
-// Sixteen rows of `a` stay in registers: wavefront w of a workgroup holds their K range of up to two pairs of chunks (a chunk is 128
+// Sixteen rows of `a` stay in registers: wavefront w of a workgroup holds their K range of up to four pairs of chunks (a chunk is 128
 // columns, a pair 128 bytes of weights), and the workgroup streams tiles of sixteen weight rows past them, two tiles a step (SwiGLU: the
 // gate's and the up projection's; otherwise neighbours).  A step's partial sums meet in LDS; a tile's registers are loaded again as soon
-// as it is used up, and the barrier waits for LDS alone.  The tiles' scales come in whole, a dword per thread, a step ahead.  The steps
+// as it is used up, and the barrier waits for LDS alone.  The tiles' scales come in whole, two dwords per thread, a step ahead.  The steps
 // of all units are one line that is cut evenly over the workgroups, as many as are resident at once.
 //
 // A load takes 128 bytes of eight rows (whole cache lines); lanes eight apart then trade halves, so that a lane has one row's chunk.
 // A lane's sixteen bytes are the 32 columns of one scale, which goes into the conversion: the value is exact in bf16 up to a scale of
 // 2^125, in fp16 from 2^-23 to 2^13.  A step that meets other scales is done again by fp4_any_scale.
-constexpr int kFp4MaxWaves = 16, kFp4Chunks = 4;
+constexpr int kFp4MaxWaves = 8, kFp4Pairs = 4, kFp4Chunks = 2 * kFp4Pairs;
 
 struct Fp4Args {
   const uint16_t* a;
@@ -293,14 +293,19 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
   const uint32_t end = at + share + (blockIdx.x < rest ? 1 : 0);
   // The lane's place in the wavefront's bytes of eight weight rows: row l16 % 8, half l16 / 8 of a pair's line (a pair that ends a row of
   // an odd number of chunks has one half: taken twice, times zeros of `a`; so is the last pair of a wavefront that has only one).
-  uint32_t wlane[2];
+  uint32_t wlane[kFp4Pairs];
 #pragma unroll
-  for (int q = 0; q < 2; q++) {
+  for (int q = 0; q < kFp4Pairs; q++) {
     const int pair = 2 * q < count ? q : 0;
     wlane[q] = (uint32_t)((l16 & 7) * (int)kb + pair * 128 + (l16 >= 8 && 2 * pair + 1 < count ? 64 : 0) + lr * 16);
   }
-  const int srow = tid / chunks, splace = (tid - srow * chunks) * 16 + srow;   // the thread's dword of a tile's scales
-  const bool has_scale = tid < 16 * chunks;
+  // the thread's two dwords of a tile's scales, [16 rows][chunks] in memory, [chunks][16 rows] in LDS
+  int splace[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int at = tid + i * (int)blockDim.x, row = at / chunks;
+    splace[i] = row < 16 ? (at - row * chunks) * 16 + row : -1;
+  }
   if (tid < 2) s_far[tid] = 0;   // (before the first step's barrier)
   int e0 = 0, before = 0;   // `some` holds the experts from e0 on, whose units are those from `before` on
   int buf = 0;
@@ -316,8 +321,8 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
     const Fp4Unit g = some.unit(e0, (int)unit - before);
     const uint8_t* bw = p.b + (long)g.expert * p.n * kb + p0 * 128;
     const uint8_t* sw = p.sf + (long)g.expert * p.n * ks;
-    v4i wt[kFp4Chunks];
-    uint32_t sc[2];
+    v4i wt[2][kFp4Chunks];
+    uint32_t sc[2][2];
     auto first_row = [&](int h, int st) {   // of half h of step st; the second half of a last step that has none: the one before
       const int row = SWIGLU ? h * inter + st * 16 : st * 32 + h * 16;
       return (long)(!SWIGLU && row >= p.n ? p.n - 16 : row);
@@ -327,22 +332,28 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
     auto load = [&](int q, int h, int st) {   // pair q of the wavefront's range
       const auto src = tile_bytes(bw + first_row(h, st) * kb, (int)(16 * kb) - p0 * 128);
 #pragma unroll
-      for (int r = 0; r < 2; r++) wt[2 * q + r] = __builtin_amdgcn_raw_buffer_load_b128(src, wlane[q], r * 8 * (int)kb, 0);
+      for (int r = 0; r < 2; r++) wt[h][2 * q + r] = __builtin_amdgcn_raw_buffer_load_b128(src, wlane[q], r * 8 * (int)kb, 0);
     };
     auto load_scales = [&](int st) {
 #pragma unroll
       for (int h = 0; h < 2; h++)
-        sc[h] = __builtin_amdgcn_raw_buffer_load_b32(tile_bytes(sw + first_row(h, st) * ks, 16 * (int)ks), tid * 4, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          sc[h][i] = __builtin_amdgcn_raw_buffer_load_b32(tile_bytes(sw + first_row(h, st) * ks, 16 * (int)ks), tid * 4, i * (int)blockDim.x * 4, 0);
     };
     auto store_scales = [&](int b) {
-      if (has_scale) {
-        s_scale[(b * 2 + 0) * 16 * chunks + splace] = sc[0];
-        s_scale[(b * 2 + 1) * 16 * chunks + splace] = sc[1];
-      }
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (splace[i] >= 0) {
+          s_scale[(b * 2 + 0) * 16 * chunks + splace[i]] = sc[0][i];
+          s_scale[(b * 2 + 1) * 16 * chunks + splace[i]] = sc[1][i];
+        }
     };
     load_scales(step);
-    load(0, 0, step);
-    load(1, 0, step);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int q = 0; q < kFp4Pairs; q++) load(q, h, step);
     __builtin_amdgcn_sched_barrier(0);   // (ahead of the rows of `a`, which come from a cache)
     v4i x[kFp4Chunks][4];
     {
@@ -356,26 +367,26 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
           x[j][i] = has_row && j < count ? v : v4i{0, 0, 0, 0};
         }
     }
-    // The outputs of a step from its partial sums: four lanes for a sum, every fourth wavefront's each, then the four in one order.
+    // The outputs of a step from its partial sums, in the wavefronts' order.
     auto finish = [&](int b, int st) {
-      const int outputs = (SWIGLU ? 16 : 32) * g.rows;
       int t = tid;
       asm volatile("" : "+v"(t));   // (what follows from it is worked out here, not kept in registers over the steps)
-      for (; t < 4 * outputs; t += blockDim.x) {
-        const int v = t >> 2, col = v & 15, h = SWIGLU ? 0 : v >> 4 & 1, m = SWIGLU ? v >> 4 : v >> 5;
-        auto sum = [&](int half) {
-          const float* part = s_part + (b * 2 + half) * waves * 256 + (m >> 2) * 64 + col * 4 + (m & 3);
-          float f = 0;
-#pragma unroll 4
-          for (int i = t & 3; i < waves; i += 4) f += part[i * 256];
-          f += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0xB1, 0xf, 0xf, true));
-          return f + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0x4E, 0xf, 0xf, true));
-        };
-        float f;
-        if constexpr (SWIGLU) f = swiglu_f32(sum(0), sum(1));
-        else f = sum(h);
+      for (; t < (SWIGLU ? 16 : 32) * g.rows; t += blockDim.x) {
+        const int col = t & 15, h = SWIGLU ? 0 : t >> 4 & 1, m = SWIGLU ? t >> 4 : t >> 5;
+        const float* part = s_part + b * 2 * waves * 256 + (m >> 2) * 64 + col * 4 + (m & 3);
+        float f[SWIGLU ? 2 : 1][kFp4MaxWaves];
+#pragma unroll
+        for (int u = 0; u < (SWIGLU ? 2 : 1); u++)
+#pragma unroll
+          for (int i = 0; i < kFp4MaxWaves; i++) f[u][i] = part[((SWIGLU ? u : h) * waves + (i < waves ? i : 0)) * 256];
+#pragma unroll
+        for (int u = 0; u < (SWIGLU ? 2 : 1); u++)
+#pragma unroll
+          for (int i = 1; i < kFp4MaxWaves; i++) f[u][0] += i < waves ? f[u][i] : 0.f;
         const int c = SWIGLU ? st * 16 + col : st * 32 + h * 16 + col;
-        if ((t & 3) == 0 && (SWIGLU || c < p.n)) p.out[(long)(g.row0 + m) * (SWIGLU ? inter : p.n) + c] = to_half<FP16>(f);
+        float y = f[0][0];
+        if constexpr (SWIGLU) y = swiglu_f32(y, f[1][0]);
+        if (SWIGLU || c < p.n) p.out[(long)(g.row0 + m) * (SWIGLU ? inter : p.n) + c] = to_half<FP16>(y);
       }
     };
     store_scales(buf);
@@ -394,21 +405,20 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
           const uint32_t d = (uint32_t)code[j] - kLeast;
           far = far > d ? far : d;
         }
-        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        v4f sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // (of even and odd chunks: two chains of matrix instructions)
         if (far > kSpan) s_far[buf] = 1;
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-          trade_halves(wt[2 * q], wt[2 * q + 1]);
+        for (int q = 0; q < kFp4Pairs; q++) {
+          trade_halves(wt[h][2 * q], wt[h][2 * q + 1]);
 #pragma unroll
-          for (int j = 2 * q; j < 2 * q + 2; j++) {
-            __builtin_amdgcn_sched_barrier(0);   // (a chunk's values at a time: more of them do not fit the registers)
+          for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              acc = mfma32<FP16>(x[j][i], fp4_values<FP16>((uint32_t)wt[j][i], __builtin_bit_cast(float, code[j] << 23)), acc);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          load(q, h ^ 1, h ? next : step);
+            for (int j = 2 * q; j < 2 * q + 2; j++)
+              sum[j & 1] = mfma32<FP16>(x[j][i], fp4_values<FP16>((uint32_t)wt[h][j][i], __builtin_bit_cast(float, code[j] << 23)), sum[j & 1]);
+          __builtin_amdgcn_sched_barrier(0);   // (a pair's registers are loaded again as soon as it is used up)
+          load(q, h, next);
         }
+        const v4f acc = sum[0] + sum[1];
         *(v4f*)&s_part[((buf * 2 + h) * waves + w) * 256 + lane * 4] = acc;
       }
       store_scales(buf ^ 1);
@@ -427,14 +437,11 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
               p.a + (long)(g.row0 + (has_row ? row : 0)) * p.k + c0 * 128 + part * 8, has_row, count);
         }
         lds_barrier();
-        finish(buf, step++);
-        buf ^= 1;
-        break;   // (the registers are loaded again: none are kept across this)
       }
       finish(buf, step);
       buf ^= 1;
     }
-    at = unit * steps + step;
+    at = unit * steps + last;
   }
 }
 
@@ -449,7 +456,7 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
   const long experts = num_experts < total_rows ? num_experts : total_rows;
   const long most = (experts + (long)total_rows / kFp4Rows) * steps;
   if (chunks <= kFp4Chunks * kFp4MaxWaves && most < 1L << 31) {
-    int waves = (pairs + 1) / 2;
+    int waves = (pairs + kFp4Pairs - 1) / kFp4Pairs;
     const int per_cu = kFp4MaxWaves / waves;
     waves = kFp4MaxWaves / per_cu < pairs ? kFp4MaxWaves / per_cu : pairs;
     const int each = (pairs + waves - 1) / waves;
