@@ -13,8 +13,8 @@
 //
 // The reference has no router: its callers draw the ids at random (benchmark/benchmark_es_fp8_blockwise_moe.py:44-56).
 //
-// One wavefront per token, every expert's order key (a float mapped to an unsigned integer of the same order) in a register: lane l
-// holds experts l * PER .. l * PER + PER - 1, so that the lowest lane of a ballot holds the lowest index.
+// Two kernels.  Sixteen lanes per token, four tokens per wavefront, for up to 256 experts and 16 places: what a router has.  One
+// wavefront per token for everything else.  Both order experts by unsigned keys that have the floats' order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
@@ -46,45 +46,57 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return b == 0xff800000u ? 0u : k;
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
-  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-  return v > o ? v : o;
+__device__ __forceinline__ float key_value(uint32_t k) {   // the float behind a key other than 0
+  return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
-// Maximum over the wavefront, in every lane.
+
+// A wavefront's reductions run on the vector ALU: row shifts, then row broadcasts; the last lane's value is everybody's.
+template <int CTRL, int ROWS, typename F, typename Op>
+__device__ __forceinline__ F dpp_step(F v, F neutral, Op op) {
+  const int o = __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, neutral), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
+  return op(v, __builtin_bit_cast(F, o));
+}
+template <typename F, typename Op>
+__device__ __forceinline__ F wave_reduce(F v, F neutral, Op op) {
+  v = dpp_step<0x111, 0xf>(v, neutral, op);
+  v = dpp_step<0x112, 0xf>(v, neutral, op);
+  v = dpp_step<0x114, 0xf>(v, neutral, op);
+  v = dpp_step<0x118, 0xf>(v, neutral, op);
+  v = dpp_step<0x142, 0xa>(v, neutral, op);
+  v = dpp_step<0x143, 0xc>(v, neutral, op);
+  return __builtin_bit_cast(F, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-  v = dpp_umax<0x111, 0xf>(v);
-  v = dpp_umax<0x112, 0xf>(v);
-  v = dpp_umax<0x114, 0xf>(v);
-  v = dpp_umax<0x118, 0xf>(v);
-  v = dpp_umax<0x142, 0xa>(v);
-  v = dpp_umax<0x143, 0xc>(v);
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+  return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
-template <typename F>
-__device__ __forceinline__ F wave_sum_all(F v) {
+__device__ __forceinline__ float wave_sum_all(float v) {
+  return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ double wave_sum_all(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
   return v;
 }
 // NaN where any lane holds one (the maximum of a softmax).
 __device__ __forceinline__ float wave_max_nan(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const float o = __shfl_xor(v, d);
-    v = o != o ? o : (v != v ? v : (v > o ? v : o));
-  }
-  return v;
+  const float m = wave_reduce(v, -__builtin_inff(), [](float a, float b) { return __builtin_fmaxf(a, b); });
+  return __ballot(v != v) ? __builtin_nanf("") : m;
 }
 
+// A renormalised weight before the division by the places' sum: the score, scaled by the largest of them (of logit m), so that the sum
+// is never 0 / 0.
+__device__ __forceinline__ float gate_term(float x, float m, int sigmoid) {
+  if (!sigmoid) return expf(x - m);
+  if (x >= 0) return 1.0f / (1.0f + expf(-x));
+  return expf(x - (m < 0 ? m : 0.f)) / (1.0f + expf(x));
+}
+
+// One token by a whole wavefront: the order from 64 bits wherever it hangs on them.  Lane l holds experts l * PER .. l * PER + PER - 1, so
+// that the lowest lane of a ballot holds the lowest index.
 template <typename T, int PER>
-__global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* __restrict__ logits, long ld, const float* __restrict__ bias,
-                                                                      GateArgs a, int* __restrict__ ids, float* __restrict__ weights) {
-  __shared__ uint32_t s_key[kGateWaves][64 * PER];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long t = (long)blockIdx.x * kGateWaves + w;
-  if (t >= a.tokens) return;   // (no barrier below: a wavefront's LDS is its own)
-  const T* row = logits + t * ld;
+__device__ __forceinline__ void gate_token(const T* __restrict__ row, const float* __restrict__ bias, const GateArgs& a, uint32_t* s_key,
+                                           int* __restrict__ ids, float* __restrict__ weights) {
+  const int lane = threadIdx.x & 63;
   float x[PER];
   uint32_t key[PER];
 #pragma unroll
@@ -94,7 +106,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* _
     key[i] = order_key(x[i]);
   }
   float top = 0, sum = 0;   // of the softmax over all experts
-  if (!a.sigmoid) {
+  if (!a.sigmoid && (a.exact || !a.renormalize)) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < PER; i++) m = x[i] != x[i] ? x[i] : (m != m ? m : (m > x[i] ? m : x[i]));
@@ -124,21 +136,19 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* _
   }
   if (a.groups > 1) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) s_key[w][lane * PER + i] = key[i];
+    for (int i = 0; i < PER; i++) s_key[lane * PER + i] = key[i];
     wave_lds_fence();
     const int width = a.experts / a.groups;
     uint32_t first = 0, second = 0;
     if (lane < a.groups)
       for (int i = 0; i < width; i++) {
-        const uint32_t k = s_key[w][lane * width + i];
-        if (k > first) { second = first; first = k; }
-        else if (k > second) second = k;
+        const uint32_t k = s_key[lane * width + i], low = first < k ? first : k;
+        first = first > k ? first : k;
+        second = second > low ? second : low;
       }
-    auto value = [](uint32_t k) {   // the float behind a key; nothing for an expert that is out
-      return k == 0 ? 0.f : __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
-    };
-    uint32_t score = first == 0 ? 0u : order_key(value(first) + value(second));
-    if (first != 0 && score == 0) score = 1;   // two finite choices whose sum is -inf
+    // (1: finite choices whose sum is -inf; 0: no expert left)
+    uint32_t score = first == 0 ? 0u : order_key(key_value(first) + (second ? key_value(second) : 0.f));
+    if (first != 0 && score == 0) score = 1;
     unsigned long long keep = 0;
     for (int j = 0; j < a.topk_groups; j++) {
       const uint32_t best = wave_umax(score);
@@ -150,6 +160,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* _
 #pragma unroll
     for (int i = 0; i < PER; i++)
       if (!((keep >> ((lane * PER + i) / width & 63)) & 1)) key[i] = 0;
+    wave_lds_fence();   // (another token's keys may come next)
   }
   int mine = -1;   // lane j: the j-th expert
   for (int j = 0; j < a.topk; j++) {
@@ -174,18 +185,292 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* _
   if (!a.renormalize) {
     v = a.sigmoid ? 1.0f / (1.0f + expf(-xs)) : expf(xs - top) / sum;
   } else {
-    // scaled by the largest of them, so that the sum is never 0 / 0
-    const float m = wave_max_nan(xs);
-    if (!a.sigmoid) v = expf(xs - m);
-    else if (xs >= 0) v = 1.0f / (1.0f + expf(-xs));
-    else v = expf(xs - (m < 0 ? m : 0.f)) / (1.0f + expf(xs));
+    v = gate_term(xs, wave_max_nan(xs), a.sigmoid);
     v = real ? v : 0.f;
     v /= wave_sum_all(v);
   }
   if (lane < a.topk) {
-    ids[t * a.topk + lane] = mine;
-    weights[t * a.topk + lane] = real ? v * a.scale : 0.f;
+    ids[lane] = mine;
+    weights[lane] = real ? v * a.scale : 0.f;
   }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(64 * kGateWaves) topk_gating_kernel(const T* __restrict__ logits, long ld, const float* __restrict__ bias,
+                                                                      GateArgs a, int* __restrict__ ids, float* __restrict__ weights) {
+  __shared__ uint32_t s_key[kGateWaves][64 * PER];
+  const int w = threadIdx.x >> 6;
+  const long t = (long)blockIdx.x * kGateWaves + w;
+  if (t < a.tokens) gate_token<T, PER>(logits + t * ld, bias, a, s_key[w], ids + t * a.topk, weights + t * a.topk);
+}
+
+// A lane's PER values from `first` on, `none` past the last; VEC: in whole, aligned pieces of sixteen bytes (or all PER).
+template <bool VEC, typename T, int PER>
+__device__ __forceinline__ void load_lane(const T* row, int first, int count, float none, float (&v)[PER]) {
+  if constexpr (VEC) {
+    constexpr int kPiece = PER * sizeof(T) < 16 ? PER : 16 / sizeof(T);
+    struct alignas(sizeof(T) * kPiece) Piece { T v[kPiece]; };
+    Piece c[PER / kPiece];
+#pragma unroll
+    for (int u = 0; u < PER / kPiece; u++) {
+      c[u] = Piece{};
+      if (first + u * kPiece < count) c[u] = *(const Piece*)(row + first + u * kPiece);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = first + i / kPiece * kPiece < count ? gate_load(&c[i / kPiece].v[i % kPiece]) : none;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = first + i < count ? gate_load(row + first + i) : none;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T gate_round(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, _Float16>::value) return (_Float16)v;
+  else return (__bf16)v;
+}
+template <bool VEC, typename T, int PER>
+__device__ __forceinline__ void store_lane(T* row, int first, int count, const float (&v)[PER]) {
+  if constexpr (VEC) {
+    constexpr int kPiece = PER * sizeof(T) < 16 ? PER : 16 / sizeof(T);
+    struct alignas(sizeof(T) * kPiece) Piece { T v[kPiece]; };
+#pragma unroll
+    for (int u = 0; u < PER / kPiece; u++) {
+      Piece c;
+#pragma unroll
+      for (int i = 0; i < kPiece; i++) c.v[i] = gate_round<T>(v[u * kPiece + i]);
+      if (first + u * kPiece < count) *(Piece*)(row + first + u * kPiece) = c;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (first + i < count) row[first + i] = gate_round<T>(v[i]);
+  }
+}
+
+// Sixteen lanes' reductions, to all of them.
+template <typename F, typename Op>
+__device__ __forceinline__ F row_reduce(F v, Op op) {
+  v = dpp_step<0xB1, 0xf>(v, v, op);    // lane ^ 1, ^ 2, then the mirrors of eight and of sixteen lanes
+  v = dpp_step<0x4E, 0xf>(v, v, op);
+  v = dpp_step<0x141, 0xf>(v, v, op);
+  return dpp_step<0x140, 0xf>(v, v, op);
+}
+__device__ __forceinline__ float row_sum(float v) {
+  return row_reduce(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float row_max(float v) {
+  return row_reduce(v, [](float a, float b) { return __builtin_fmaxf(a, b); });
+}
+
+__device__ __forceinline__ float row_max_nan(float v) {
+  return row_reduce(v, [](float a, float b) { return a != a || b != b ? __builtin_nanf("") : __builtin_fmaxf(a, b); });
+}
+
+// Sum of d over the token's later places of the same id, in their order; `first` goes where an earlier place has it.
+template <int R>
+__device__ __forceinline__ float later_terms(int id, float d, int l, bool& first) {
+  if constexpr (R < 16) {
+    // lane l - R of the sixteen (row_ror takes from the lanes below, around the end): a later place where R lanes around is above
+    const int other = __builtin_amdgcn_update_dpp(0, id, 0x120 + R, 0xf, 0xf, false);
+    const float od = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, d), 0x120 + R, 0xf, 0xf, false));
+    if (l >= R && other == id) first = false;
+    const float mine = l < R && other == id ? od : 0.f;
+    return mine + later_terms<R + 1>(id, d, l, first);
+  }
+  return 0.f;
+}
+
+// Counts the groups whose score is ahead of the lane's, and whether one is within `near` of it; R lanes on, and so forth.
+template <int R>
+__device__ __forceinline__ void compare_rotated(float score, float near, int lanes, int& ahead, bool& close) {
+  if constexpr (R < 16) {
+    if (R % lanes == 0) {
+      const float other = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, score), 0x120 + R, 0xf, 0xf, false));
+      ahead += other > score;
+      // (no expert left: -inf on either side says nothing; NaN is close to everything)
+      close |= !(__builtin_fabsf(other - score) > near) && other != -__builtin_inff() && score != -__builtin_inff();
+    }
+    compare_rotated<R + 1>(score, near, lanes, ahead, close);
+  }
+}
+
+// Four tokens per wavefront, a lane l of sixteen holds a token's experts l * PER .. l * PER + PER - 1.
+//
+// Bound by the instructions that find the largest of E keys topk times.  So a key is one register: the upper 24 bits of the choice's order
+// and below them 255 - expert, and a largest one stands for itself and its place.  The largest key below the one before is
+//   before + max over keys of (key - before mod 2^32),
+// a subtraction per key and no removal: what is not below `before` wraps to the small side.
+// 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number between the token's largest and
+// smallest choice, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
+// ones by less than `slack`.  Where two neighbours of the order, or two groups' scores, are too close to tell, the wavefront does the
+// token again by gate_token: of random tokens one in some hundred.
+// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 16.0, one 6.3 / 5.4; softmax over
+// 128 experts, bf16, 16384 tokens 11.2 / 6.2.
+template <typename T, int PER, bool VEC>
+__global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const T* __restrict__ logits, long ld,
+                                                                           const float* __restrict__ bias, GateArgs a, int* __restrict__ ids,
+                                                                           float* __restrict__ weights) {
+  constexpr int kTokenPer = PER / 4;   // experts of a lane where a wavefront takes a token
+  __shared__ uint32_t s_key[kGateWaves][64 * kTokenPer];
+  const int lane = threadIdx.x & 63, l = lane & 15, w = threadIdx.x >> 6;
+  const long t0 = ((long)blockIdx.x * kGateWaves + w) * 4;
+  if (t0 >= a.tokens) return;   // (no barrier below)
+  const long t = t0 + (lane >> 4);
+  const bool in = t < a.tokens;
+  const T* row = logits + (in ? t : t0) * ld;
+  const float ninf = -__builtin_inff();
+  float x[PER], b[PER];
+  load_lane<VEC>(row, l * PER, a.experts, ninf, x);
+  if (bias) {
+    load_lane<VEC>(bias, l * PER, a.experts, 0.f, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i++) b[i] = 0.f;
+  }
+  bool unsure = false;
+  float top = 0, sum = 1;   // of the softmax over all experts
+  if (!a.sigmoid && (a.exact || !a.renormalize)) {
+    top = x[0];
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) {
+      top = __builtin_fmaxf(top, x[i]);
+      nan |= x[i] != x[i];
+    }
+    top = row_max(top);
+    unsure = nan;
+    // e^x by 2^(x log2 e): off by |x - top| 2^-24 of itself, which is below .4 * 2^-24 of 1, and by a unit of the last place
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += __builtin_amdgcn_exp2f((x[i] - top) * 1.44269504088896340736f);
+    sum = row_sum(sum);
+  }
+  uint32_t key[PER];
+  const bool whole = sizeof(T) == 2 && !a.exact;   // the keys hold all of a choice
+  uint32_t near = 0;                               // keys' upper 24 bits no further apart than this may be in either order
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const uint32_t k = order_key(x[i]);
+      key[i] = k ? (k & 0xffffff00u) | (uint32_t)(255 - (l * PER + i)) : 0u;
+    }
+  } else {
+    float choice[PER], slack = 0.f;
+    if (!a.exact) {
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        unsure |= x[i] != x[i];
+        choice[i] = x[i];
+      }
+    } else {
+      const float scale = a.sigmoid ? 1.f : 1.0f / sum;
+      float largest = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const float e = __builtin_amdgcn_exp2f((a.sigmoid ? -x[i] : x[i] - top) * 1.44269504088896340736f);
+        float c = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + e) : e * scale;
+        c += b[i];
+        unsure |= c != c;
+        choice[i] = x[i] == ninf ? ninf : c;
+        largest = __builtin_fmaxf(largest, choice[i] == ninf ? 0.f : __builtin_fabsf(c));
+      }
+      // in units of 2^-24: a sigmoid's error is below 3.8 (|x| s (1 - s) < .23 from the argument's rounding, .5 from 2^x, 1 and 2 from the
+      // sum and its reciprocal), a softmax's below 33 of the largest score (its sum's 20 additions and the mean |x - top| of its terms
+      // among them); and half a unit of the last place for the fp32 sum on either side
+      slack = (a.sigmoid ? 2.5e-7f : 2e-6f * scale) + 1.25e-7f * row_max(largest);
+      if (a.groups > 1) {
+        float first = choice[0], second = ninf;
+#pragma unroll
+        for (int i = 1; i < PER; i++) {
+          const float low = __builtin_fminf(first, choice[i]);
+          first = __builtin_fmaxf(first, choice[i]);
+          second = __builtin_fmaxf(second, low);
+        }
+        const int lanes = a.experts / a.groups / PER;   // of a group: a power of two
+        auto join = [&](float f, float s) {
+          const float low = __builtin_fminf(first, f), high = __builtin_fmaxf(second, s);
+          first = __builtin_fmaxf(first, f);
+          second = __builtin_fmaxf(low, high);
+        };
+        auto other = [](float v, auto ctrl) {
+          return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true));
+        };
+        if (lanes > 1) join(other(first, std::integral_constant<int, 0xB1>()), other(second, std::integral_constant<int, 0xB1>()));
+        if (lanes > 2) join(other(first, std::integral_constant<int, 0x4E>()), other(second, std::integral_constant<int, 0x4E>()));
+        if (lanes > 4) join(other(first, std::integral_constant<int, 0x141>()), other(second, std::integral_constant<int, 0x141>()));
+        const float score = first == ninf ? ninf : first + (second == ninf ? 0.f : second);
+        int ahead = 0;
+        bool close = false;
+        // (a group without an expert left is out: behind all others, and its experts have no key)
+        compare_rotated<1>(score, 4.f * slack, lanes, ahead, close);
+        unsure |= close && l < a.groups * lanes;
+        if (ahead >= a.topk_groups) {
+#pragma unroll
+          for (int i = 0; i < PER; i++) choice[i] = ninf;
+        }
+      }
+    }
+    // fixed point, from the smallest choice on or from so far below the largest that what lies under it is hardly taken (it gets one key,
+    // and is close to its like)
+    float hi = choice[0], lo = __builtin_inff();
+#pragma unroll
+    for (int i = 1; i < PER; i++) hi = __builtin_fmaxf(hi, choice[i]);
+#pragma unroll
+    for (int i = 0; i < PER; i++) lo = __builtin_fminf(lo, choice[i] == ninf ? __builtin_inff() : choice[i]);
+    hi = row_max(hi);
+    lo = -row_max(-lo);
+    lo = __builtin_fmaxf(lo, hi - 64.f);
+    const float units = 16777200.f / (hi > lo ? hi - lo : 1.f);   // (its own rounding and the products' stay below 2^24)
+    // (three units of rounding on either side; where the units are not finite numbers nothing is sure)
+    const float apart = 2.f * slack * units + 6.f;
+    unsure |= !(apart < 16777216.f) && hi != ninf;
+    near = (uint32_t)apart;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const uint32_t q = (uint32_t)__builtin_fmaxf((choice[i] - lo) * units, 0.f) + 1u;   // 1 .. 2^24 - 1
+      key[i] = choice[i] == ninf ? 0u : q << 8 | (uint32_t)(255 - (l * PER + i));
+    }
+  }
+  int mine = -1;   // lane j of a token: the j-th expert
+  uint32_t before = 0;   // (as if 2^32: every key is below)
+  bool left = true;
+  for (int j = 0; j < a.topk + (whole ? 0 : 1); j++) {   // (one more than are taken: how close it came)
+    uint32_t d = key[0] - before;
+#pragma unroll
+    for (int i = 1; i < PER; i++) {
+      const uint32_t o = key[i] - before;
+      d = d > o ? d : o;
+    }
+    d = row_reduce(d, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
+    const uint32_t max = left ? before + d : 0;
+    left = max != 0;
+    if (l == j && j < a.topk && left) mine = 255 - (int)(max & 255u);
+    if (!whole && j > 0) unsure |= left && (before >> 8) - (max >> 8) <= near;
+    before = max;
+  }
+  // the weights, a lane per place
+  const bool real = mine >= 0;
+  const float xs = real ? gate_load(row + mine) : ninf;
+  float v;
+  if (!a.renormalize) {
+    v = a.sigmoid ? 1.0f / (1.0f + expf(-xs)) : expf(xs - top) / sum;
+  } else {
+    unsure |= xs != xs;
+    v = gate_term(xs, row_max(xs), a.sigmoid);
+    v = real ? v : 0.f;
+    v /= row_sum(v);
+  }
+  const unsigned long long again = __ballot(unsure);
+  const bool mine_again = (again >> (lane & 48)) & 0xffff;
+  if (in && l < a.topk && !mine_again) {
+    ids[t * a.topk + l] = mine;
+    weights[t * a.topk + l] = real ? v * a.scale : 0.f;
+  }
+  for (int r = 0; r < 4; r++)
+    if (t0 + r < a.tokens && (again >> (16 * r) & 0xffff))
+      gate_token<T, kTokenPer>(logits + (t0 + r) * ld, bias, a, s_key[w], ids + (t0 + r) * a.topk, weights + (t0 + r) * a.topk);
 }
 
 // One wavefront per token; ids that stand twice in a row add up, ids outside [0, experts) are places without an expert.
@@ -221,12 +506,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_backward_kernel(c
     d = g;
   } else if (a.renormalize) {
     const float m = wave_max_nan(xs);
-    float v = 0;
-    if (real) {
-      if (!a.sigmoid) v = expf(xs - m);
-      else if (xs >= 0) v = 1.0f / (1.0f + expf(-xs));
-      else v = expf(xs - (m < 0 ? m : 0.f)) / (1.0f + expf(xs));
-    }
+    float v = real ? gate_term(xs, m, a.sigmoid) : 0.f;
     const float all = wave_sum_all(v);
     v = real ? v / all : 0.f;
     const float mid = wave_sum_all(g * v);
@@ -247,15 +527,101 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_backward_kernel(c
   for (int e = lane; e < a.experts; e += 64) {
     float v = s_grad[w][e];
     if (dense) v = expf(gate_load(row + e) - top) / sum * (v - mean);
-    T* o = out + t * a.experts + e;
-    if constexpr (sizeof(T) == 4) *o = v;
-    else if constexpr (std::is_same<T, _Float16>::value) *o = (_Float16)v;
-    else *o = (__bf16)v;
+    out[t * a.experts + e] = gate_round<T>(v);
   }
+}
+
+// The same by sixteen lanes per token, under the conditions of topk_gating_rows_kernel: a token's logits are read once, in whole pieces,
+// and its gradient is written so; the places' terms meet their experts in LDS.  A place whose id an earlier one has leaves its term to
+// that one.  us, a wavefront per token / this: BACK_FIGURES
+template <typename T, int PER, bool VEC>
+__global__ void __launch_bounds__(64 * kGateWaves) topk_gating_backward_rows_kernel(const float* __restrict__ grad,
+                                                                                    const T* __restrict__ logits, long ld,
+                                                                                    const int* __restrict__ ids, GateArgs a,
+                                                                                    T* __restrict__ out) {
+  __shared__ float __attribute__((aligned(16))) s_grad[kGateWaves][4][16 * PER];
+  const int lane = threadIdx.x & 63, l = lane & 15, w = threadIdx.x >> 6;
+  const long t0 = ((long)blockIdx.x * kGateWaves + w) * 4;
+  if (t0 >= a.tokens) return;   // (no barrier below)
+  const long t = t0 + (lane >> 4);
+  const bool in = t < a.tokens;
+  const T* row = logits + (in ? t : t0) * ld;
+  const bool dense = !a.sigmoid && !a.renormalize;
+  float x[PER];
+  if (dense) load_lane<VEC>(row, l * PER, a.experts, -__builtin_inff(), x);
+  int id = in && l < a.topk ? ids[t * a.topk + l] : -1;
+  if ((unsigned)id >= (unsigned)a.experts) id = -1;
+  const bool real = id >= 0;
+  const float g = real ? grad[t * a.topk + l] * a.scale : 0.f;
+  const float xs = real ? gate_load(row + id) : -__builtin_inff();
+  float* mine = s_grad[w][lane >> 4];
+#pragma unroll
+  for (int i = 0; i < PER; i++) mine[l * PER + i] = 0.f;
+  float d, mean = 0;
+  if (dense) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) top = __builtin_fmaxf(top, x[i]);
+    top = row_max(top);
+    if (top == -__builtin_inff()) top = 0;   // every expert masked: all terms 0
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      x[i] = expf(x[i] - top);
+      sum += x[i];
+    }
+    sum = row_sum(sum);
+    const float scale = 1.0f / (sum == 0 ? 1.f : sum);
+#pragma unroll
+    for (int i = 0; i < PER; i++) x[i] *= scale;   // the scores
+    const float part = real ? g * (expf(xs - top) * scale) : 0.f;
+    mean = row_sum(part);
+    d = g;
+  } else if (a.renormalize) {
+    const float m = row_max_nan(xs);   // (with every lane)
+    float v = real ? gate_term(xs, m, a.sigmoid) : 0.f;
+    const float all = row_sum(v);
+    v = real ? v / all : 0.f;
+    const float mid = row_sum(g * v);
+    d = real ? v * (g - mid) * (a.sigmoid ? 1.0f / (1.0f + expf(xs)) : 1.0f) : 0.f;
+  } else {
+    d = real ? g / (1.0f + expf(-xs)) / (1.0f + expf(xs)) : 0.f;
+  }
+  bool first = real;
+  const float total = d + later_terms<1>(id, d, l, first);
+  wave_lds_fence();
+  if (first) mine[id] = total;
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const float v = mine[l * PER + i];
+    x[i] = dense ? x[i] * (v - mean) : v;
+  }
+  if (in) store_lane<VEC>(out + t * a.experts, l * PER, a.experts, x);
 }
 
 template <typename T>
 static int launch_gating(const void* logits, long ld, const float* bias, const GateArgs& a, int* ids, float* weights, hipStream_t stream) {
+  const int rows_per = a.experts <= 64 ? 4 : a.experts <= 128 ? 8 : 16;
+  // Whether a group is a power of two of a sixteenth's lanes (1, 2, 4 or 8), or there are none.
+  const int width = a.experts / a.groups, lanes = width / rows_per;
+  const bool groups_fit = a.groups == 1 || (width == lanes * rows_per && lanes >= 1 && lanes <= 8 && (lanes & (lanes - 1)) == 0);
+  if (a.experts <= 256 && a.topk <= 16 && groups_fit) {
+    const unsigned grid = (unsigned)((a.tokens + 4 * kGateWaves - 1) / (4 * kGateWaves));
+#define ESMOE_GATE(P)                                                                                                                \
+  do {                                                                                                                               \
+    constexpr int kPiece = P * sizeof(T) < 16 ? P : 16 / sizeof(T);                                                                  \
+    const bool vec = a.experts % kPiece == 0 && ld % kPiece == 0 && (uintptr_t)logits % (kPiece * sizeof(T)) == 0 &&                  \
+                     a.experts % 4 == 0 && (uintptr_t)bias % 16 == 0;                                                                \
+    hipLaunchKernelGGL((vec ? topk_gating_rows_kernel<T, P, true> : topk_gating_rows_kernel<T, P, false>), dim3(grid),               \
+                       dim3(64 * kGateWaves), 0, stream, (const T*)logits, ld, bias, a, ids, weights);                               \
+  } while (0)
+    if (rows_per == 4) ESMOE_GATE(4);
+    else if (rows_per == 8) ESMOE_GATE(8);
+    else ESMOE_GATE(16);
+#undef ESMOE_GATE
+    return (int)hipGetLastError();
+  }
   const unsigned grid = (unsigned)((a.tokens + kGateWaves - 1) / kGateWaves);
   const int per = (a.experts + 63) / 64;
 #define ESMOE_GATE(P)                                                                                                              \
@@ -272,6 +638,22 @@ static int launch_gating(const void* logits, long ld, const float* bias, const G
 template <typename T>
 static int launch_gating_backward(const float* grad, const void* logits, long ld, const int* ids, const GateArgs& a, void* out,
                                   hipStream_t stream) {
+  if (a.experts <= 256 && a.topk <= 16) {
+    const unsigned grid = (unsigned)((a.tokens + 4 * kGateWaves - 1) / (4 * kGateWaves));
+#define ESMOE_GATE(P)                                                                                                                \
+  do {                                                                                                                               \
+    constexpr int kPiece = P * sizeof(T) < 16 ? P : 16 / sizeof(T);                                                                  \
+    const bool vec = a.experts % kPiece == 0 && ld % kPiece == 0 && (uintptr_t)logits % (kPiece * sizeof(T)) == 0 &&                  \
+                     (uintptr_t)out % (kPiece * sizeof(T)) == 0;                                                                     \
+    hipLaunchKernelGGL((vec ? topk_gating_backward_rows_kernel<T, P, true> : topk_gating_backward_rows_kernel<T, P, false>),         \
+                       dim3(grid), dim3(64 * kGateWaves), 0, stream, grad, (const T*)logits, ld, ids, a, (T*)out);                   \
+  } while (0)
+    if (a.experts <= 64) ESMOE_GATE(4);
+    else if (a.experts <= 128) ESMOE_GATE(8);
+    else ESMOE_GATE(16);
+#undef ESMOE_GATE
+    return (int)hipGetLastError();
+  }
   const unsigned grid = (unsigned)((a.tokens + kGateWaves - 1) / kGateWaves);
   hipLaunchKernelGGL((topk_gating_backward_kernel<T>), dim3(grid), dim3(64 * kGateWaves), 0, stream, grad, (const T*)logits, ld, ids, a,
                      (T*)out);

@@ -107,6 +107,30 @@ def test_masks_ties_and_extremes(esmoe, scoring, bias):
         assert ids[0].tolist() == [3, 0, 1] and ids[1].tolist() == [60, 3, 0]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts", [60, 128, 200, 256, 300])
+def test_order_at_the_ends_of_the_range(esmoe, dtype, experts):
+    """NaN and the largest values at the first and last experts, values that differ in the last place of the type, masks by the type's lowest
+    value beside ordinary logits, one expert far above all others."""
+    info = torch.finfo(dtype)
+    x = _logits(40, experts, dtype, experts)
+    x[0, 0], x[1, -1], x[2, 0], x[2, -1] = float("nan"), float("nan"), float("nan"), float("nan")
+    x[3, 0], x[4, -1], x[5, :] = info.max, info.max, info.min
+    x[6, ::2] = info.min
+    x[7, 1:] = info.min
+    x[8] = 1.0 + info.eps * torch.arange(experts)
+    x[9] = 1.0 + info.eps * torch.arange(experts).flip(0)
+    x[10] = -1.0 - info.eps * torch.arange(experts)
+    x[11] = info.tiny * torch.arange(experts)
+    x[12, experts // 2] = 30000.0
+    x[13:20] = x[13:20].round()
+    bias = 0.1 * torch.randn(experts, generator=torch.Generator().manual_seed(3))
+    groups = 4
+    for scoring in ("softmax", "sigmoid"):
+        for args in ((None, 1, 1), (bias, 1, 1), (None, groups, 2), (bias, groups, 3), (100 * bias, 1, 1), (1e-6 * bias, groups, 1)):
+            _check(esmoe, x, 8, args[0], scoring, True, 1.0, args[1], args[2], grad=False)
+
+
 def test_gradient_of_given_ids(esmoe):
     """Ids that no gating would give: one twice, ids of no expert; NaN gradients at places that do not count."""
     x = _logits(6, 40, torch.float32, 2)
