@@ -640,6 +640,15 @@ void es_combine_rows(const torch::Tensor& input, const torch::Tensor& dst_row, i
   check_rc(rc, "es_combine_rows");
 }
 
+// The same into a new tensor (allocated here: a tensor made in Python costs a call twice as much).
+torch::Tensor es_combine_rows_new(const torch::Tensor& input, const torch::Tensor& dst_row, int64_t topk,
+                                  const c10::optional<torch::Tensor>& weights) {
+  const int64_t tokens = check_combine(input, dst_row, topk, tensor_or_none(weights));
+  torch::Tensor output = torch::empty({tokens, input.size(1)}, input.options().requires_grad(false));
+  es_combine_rows(input, dst_row, topk, weights, output);
+  return output;
+}
+
 void es_combine_rows_backward(const torch::Tensor& grad_output, const torch::Tensor& input, const torch::Tensor& dst_row, int64_t topk,
                               const torch::Tensor& weights, torch::Tensor& grad_input, torch::Tensor& grad_weights) {
   const int64_t tokens = check_combine(input, dst_row, topk, weights);
@@ -700,6 +709,20 @@ void es_add_rms_norm_quant_1x128(const torch::Tensor& input, const torch::Tensor
       weight.data_ptr(), (float)eps, (long)rows, (int)k, residual.defined() ? residual_out.data_ptr() : nullptr,
       normed.defined() ? normed.data_ptr() : nullptr, quant_output.data_ptr(), scales.data_ptr<float>(), current_stream(input));
   check_rc(rc, "es_add_rms_norm_quant_1x128");
+}
+
+// The same into new tensors; those that are not asked for stay undefined (None in Python).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> es_add_rms_norm_quant_1x128_new(
+    const torch::Tensor& input, const torch::Tensor& weight, double eps, const c10::optional<torch::Tensor>& residual, bool return_normed) {
+  TORCH_CHECK(input.dim() == 2, "input must be a contiguous 2D tensor");
+  const auto opts = input.options().requires_grad(false);
+  torch::Tensor q = torch::empty({input.size(0), input.size(1)}, opts.dtype(torch::kFloat8_e4m3fn)),
+                scales = torch::empty({input.size(0), input.size(1) / 128}, opts.dtype(torch::kFloat32)), residual_out, normed;
+  if (residual.has_value() && residual->defined()) residual_out = torch::empty(input.sizes(), opts);
+  if (return_normed) normed = torch::empty(input.sizes(), opts);
+  const auto given = [](const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; };
+  es_add_rms_norm_quant_1x128(input, weight, eps, residual, given(residual_out), given(normed), q, scales);
+  return {q, scales, residual_out, normed};
 }
 
 namespace {
@@ -784,12 +807,16 @@ TORCH_LIBRARY(expert_specialization, m) {
       "es_topk_gating_backward(Tensor grad_weights, Tensor logits, Tensor topk_ids, bool sigmoid, bool renormalize, float scale) -> "
       "Tensor");
   m.def("es_combine_rows(Tensor input, Tensor dst_row, int topk, Tensor? weights, Tensor output) -> ()");
+  m.def("es_combine_rows.new(Tensor input, Tensor dst_row, int topk, Tensor? weights) -> Tensor");
   m.def(
       "es_combine_rows_backward(Tensor grad_output, Tensor input, Tensor dst_row, int topk, Tensor weights, Tensor grad_input, Tensor "
       "grad_weights) -> ()");
   m.def(
       "es_add_rms_norm_quant_1x128(Tensor input, Tensor weight, float eps, Tensor? residual, Tensor? residual_out, Tensor? normed, "
       "Tensor quant_output, Tensor scales) -> ()");
+  m.def(
+      "es_add_rms_norm_quant_1x128.new(Tensor input, Tensor weight, float eps, Tensor? residual, bool return_normed) -> (Tensor, Tensor, "
+      "Tensor, Tensor)");
   m.def("es_mxfp4_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
   m.def("es_mxfp4_grouped_mm_swiglu(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
 }
@@ -810,8 +837,10 @@ TORCH_LIBRARY_IMPL(expert_specialization, CUDA, m) {
   m.impl("es_topk_gating", &es_topk_gating);
   m.impl("es_topk_gating_backward", &es_topk_gating_backward);
   m.impl("es_combine_rows", &es_combine_rows);
+  m.impl("es_combine_rows.new", &es_combine_rows_new);
   m.impl("es_combine_rows_backward", &es_combine_rows_backward);
   m.impl("es_add_rms_norm_quant_1x128", &es_add_rms_norm_quant_1x128);
+  m.impl("es_add_rms_norm_quant_1x128.new", &es_add_rms_norm_quant_1x128_new);
   m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
   m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
 }
@@ -833,8 +862,10 @@ TORCH_LIBRARY_IMPL(expert_specialization, CPU, m) {
   m.impl("es_topk_gating", &es_topk_gating);
   m.impl("es_topk_gating_backward", &es_topk_gating_backward);
   m.impl("es_combine_rows", &es_combine_rows);
+  m.impl("es_combine_rows.new", &es_combine_rows_new);
   m.impl("es_combine_rows_backward", &es_combine_rows_backward);
   m.impl("es_add_rms_norm_quant_1x128", &es_add_rms_norm_quant_1x128);
+  m.impl("es_add_rms_norm_quant_1x128.new", &es_add_rms_norm_quant_1x128_new);
   m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
   m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
 }

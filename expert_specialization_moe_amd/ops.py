@@ -161,7 +161,7 @@ def es_combine_rows(input, dst_row, topk, weights=None, output=None):
     """output[t] = sum over j of weights[t, j] * input[dst_row[t * topk + j]] (pairs with dst_row < 0 are left out): the experts' packed
     rows back at their tokens, summed in fp32.  Without weights it is the gradient of es_permute_rows.  No counterpart in the reference."""
     if output is None:
-        output = input.new_empty((dst_row.numel() // max(topk, 1), input.size(1)))
+        return _ns.es_combine_rows.new(input, dst_row, topk, weights)
     _ns.es_combine_rows.default(input, dst_row, topk, weights, output)
     return output
 
@@ -184,6 +184,8 @@ def es_add_rms_norm_quant_1x128(input, weight, eps=1e-6, residual=None, residual
     (e4m3fn [M, K], fp32 scales [M, K/128], h or None, y or None).  h is the new residual, in input's dtype; it may be written over
     input or residual (residual_out).  y in input's dtype is given back where `normed` is given or return_normed is set.  Serving
     only: there is no gradient.  No counterpart in the reference."""
+    if residual_out is None and normed is None and quant_output is None and scales is None:
+        return _ns.es_add_rms_norm_quant_1x128.new(input, weight, eps, residual, return_normed)
     m, k = input.shape
     if residual is not None and residual_out is None:
         residual_out = torch.empty_like(input)
