@@ -630,6 +630,7 @@ int combine_args(int dtype, long num_pairs, int topk, long rows, int hidden) {
     return fail(ESMOE_ERR_INVALID_ARGUMENT, "dtype must be ESMOE_IN_BF16 or ESMOE_IN_FP16");
   if (topk < 1 || num_pairs < 0 || num_pairs % topk || num_pairs >= (1L << 31))
     return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_pairs must be tokens * topk in [0, 2^31), got %ld pairs, topk %d", num_pairs, topk);
+  if (topk > 65536) return fail(ESMOE_ERR_INVALID_ARGUMENT, "topk must be at most 65536, got %d", topk);
   if (rows < 0 || rows >= (1L << 31)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "rows out of range: %ld", rows);
   if (hidden <= 0 || hidden % 8 || hidden > (1 << 24))
     return fail(ESMOE_ERR_INVALID_ARGUMENT, "hidden must be a multiple of 8 (rows of 16 bytes) up to 2^24, got %d", hidden);

@@ -533,7 +533,8 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_backward_kernel(c
 
 // The same by sixteen lanes per token, under the conditions of topk_gating_rows_kernel: a token's logits are read once, in whole pieces,
 // and its gradient is written so; the places' terms meet their experts in LDS.  A place whose id an earlier one has leaves its term to
-// that one.  us, a wavefront per token / this: BACK_FIGURES
+// that one.  us, a wavefront per token / this: 16384 tokens, softmax over all, 256 experts fp32
+// 16.2 / 11.5, 128 experts bf16 11.5 / 5.0.
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_backward_rows_kernel(const float* __restrict__ grad,
                                                                                     const T* __restrict__ logits, long ld,

@@ -16,8 +16,6 @@ namespace esmoe {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 
-constexpr int kNormThreads = 256;
-
 template <bool FP16>
 __device__ __forceinline__ float half_to_f32(uint32_t bits) {
   if constexpr (FP16) return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
@@ -36,20 +34,22 @@ __device__ __forceinline__ uint32_t dpp_umax16(uint32_t v) {
   return v > o ? v : o;
 }
 
-// One workgroup per row, its values in registers: CHUNKS times eight per thread.
-template <bool FP16, int CHUNKS>
-__global__ void __launch_bounds__(kNormThreads) add_rms_norm_quant_kernel(const uint16_t* in, const uint16_t* residual,
-                                                                          const uint16_t* __restrict__ weight, float eps, int hidden,
+// A row's values stay in registers: CHUNKS times eight per thread, THREADS threads per row; with 64 (a wavefront) four rows per workgroup.
+template <bool FP16, int THREADS, int CHUNKS>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_quant_kernel(const uint16_t* in, const uint16_t* residual,
+                                                                          const uint16_t* __restrict__ weight, float eps, long rows, int hidden,
                                                                           uint16_t* residual_out, uint16_t* __restrict__ normed,
                                                                           uint8_t* __restrict__ q, float* __restrict__ scales) {
-  __shared__ float s_sum[kNormThreads / 64];
-  const int tid = threadIdx.x;
-  const long row = (long)blockIdx.x * hidden;
+  __shared__ float s_sum[THREADS / 64];
+  const int tid = THREADS < 256 ? threadIdx.x % THREADS : threadIdx.x;
+  const long number = THREADS < 256 ? (long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS : blockIdx.x;
+  if (number >= rows) return;   // (a whole wavefront, and no barrier where there are several rows)
+  const long row = number * hidden;
   float h[CHUNKS][8];
   float sum = 0;
 #pragma unroll
   for (int u = 0; u < CHUNKS; u++) {
-    const int col = (u * kNormThreads + tid) * 8;
+    const int col = (u * THREADS + tid) * 8;
     if (col < hidden) {
       const v4i a = *(const v4i*)(in + row + col);
       v4i r = {0, 0, 0, 0};
@@ -74,13 +74,19 @@ __global__ void __launch_bounds__(kNormThreads) add_rms_norm_quant_kernel(const 
     }
   }
   sum = wave_sum_last(sum);
-  if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
-  __syncthreads();
-  sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  if constexpr (THREADS == 64) {
+    sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
+  } else {
+    if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
+    __syncthreads();
+    sum = s_sum[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; i++) sum += s_sum[i];
+  }
   const float rstd = 1.0f / sqrtf(sum / (float)hidden + eps);
 #pragma unroll
   for (int u = 0; u < CHUNKS; u++) {
-    const int col = (u * kNormThreads + tid) * 8;   // sixteen lanes hold 128 columns: in or out of the row as one
+    const int col = (u * THREADS + tid) * 8;   // sixteen lanes hold 128 columns: in or out of the row as one
     if (col < hidden) {
       const v4i g = *(const v4i*)(weight + col);
       uint32_t amax = 0;
@@ -116,21 +122,34 @@ __global__ void __launch_bounds__(kNormThreads) add_rms_norm_quant_kernel(const 
 template <bool FP16>
 static int launch_norm(const void* in, const void* residual, const void* weight, float eps, long rows, int hidden, void* residual_out,
                        void* normed, void* q, float* scales, hipStream_t stream) {
-  const int chunks = (hidden + kNormThreads * 8 - 1) / (kNormThreads * 8);
+  // Threads per row: a wavefront where a row is short enough to be its registers' (no barrier, more rows in flight); sixteen wavefronts
+  // where there is at most a row per CU (what counts is how long one takes); four else.  us, always four / as chosen: 8 rows x 7168 4.5 / 3.45, 256 x 7168
+  // 5.8 / 4.9, 16384 x 256 12.0 / 10.1, 65536 x 512 63.9 / 49.9, 16384 x 1024 24.6 / 23.5.
+  const int threads = rows <= 256 && hidden > 1024 ? 1024 : hidden <= 1024 ? 64 : 256;
+  const int chunks = (hidden + threads * 8 - 1) / (threads * 8);
   const long step = 1L << 22;
   for (long r = 0; r < rows; r += step) {
-    const unsigned n = (unsigned)(rows - r < step ? rows - r : step);
-    const long at = r * hidden;
-#define ESMOE_NORM(C)                                                                                                             \
-  hipLaunchKernelGGL((add_rms_norm_quant_kernel<FP16, C>), dim3(n), dim3(kNormThreads), 0, stream, (const uint16_t*)in + at,       \
-                     residual ? (const uint16_t*)residual + at : nullptr, (const uint16_t*)weight, eps, hidden,                   \
-                     residual ? (uint16_t*)residual_out + at : nullptr, normed ? (uint16_t*)normed + at : nullptr,                \
+    const long n = rows - r < step ? rows - r : step, at = r * hidden;
+    const unsigned grid = (unsigned)(threads == 64 ? (n + 3) / 4 : n);
+#define ESMOE_NORM(T, C)                                                                                                          \
+  hipLaunchKernelGGL((add_rms_norm_quant_kernel<FP16, T, C>), dim3(grid), dim3(T < 256 ? 256 : T), 0, stream,                      \
+                     (const uint16_t*)in + at, residual ? (const uint16_t*)residual + at : nullptr, (const uint16_t*)weight, eps, n, \
+                     hidden, residual ? (uint16_t*)residual_out + at : nullptr, normed ? (uint16_t*)normed + at : nullptr,        \
                      (uint8_t*)q + at, scales + at / 128)
-    if (chunks <= 1) ESMOE_NORM(1);
-    else if (chunks <= 2) ESMOE_NORM(2);
-    else if (chunks <= 4) ESMOE_NORM(4);
-    else if (chunks <= 8) ESMOE_NORM(8);
-    else ESMOE_NORM(16);
+    if (threads == 64) {
+      if (chunks <= 1) ESMOE_NORM(64, 1);
+      else ESMOE_NORM(64, 2);
+    } else if (threads == 1024) {
+      if (chunks <= 1) ESMOE_NORM(1024, 1);
+      else if (chunks <= 2) ESMOE_NORM(1024, 2);
+      else ESMOE_NORM(1024, 4);
+    } else {
+      if (chunks <= 1) ESMOE_NORM(256, 1);
+      else if (chunks <= 2) ESMOE_NORM(256, 2);
+      else if (chunks <= 4) ESMOE_NORM(256, 4);
+      else if (chunks <= 8) ESMOE_NORM(256, 8);
+      else ESMOE_NORM(256, 16);
+    }
 #undef ESMOE_NORM
   }
   return (int)hipGetLastError();
