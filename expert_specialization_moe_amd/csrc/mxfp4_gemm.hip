@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
 // A load takes 128 bytes of eight rows (whole cache lines); lanes eight apart then trade halves, so that a lane has one row's chunk.
 // A lane's sixteen bytes are the 32 columns of one scale, which goes into the conversion: the value is exact in bf16 up to a scale of
 // 2^125, in fp16 from 2^-23 to 2^13.  A step that meets other scales is done again by fp4_any_scale.
-constexpr int kFp4MaxWaves = 8, kFp4Pairs = 4, kFp4Chunks = 2 * kFp4Pairs;
+constexpr int kFp4MaxWaves = 8, kFp4MaxPairs = 4;
+// Wavefronts of a CU, by the pairs of chunks that each holds registers for.
+constexpr int fp4_waves(int pairs) { return pairs == 1 ? 16 : pairs == 2 ? 12 : 8; }
 
 struct Fp4Args {
   const uint16_t* a;
@@ -264,8 +266,10 @@ __device__ __forceinline__ v4f fp4_any_scale(const uint8_t* src, const uint8_t* 
   return acc;
 }
 
-template <bool FP16, bool SWIGLU>
-__global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args p) {
+template <bool FP16, bool SWIGLU, int PAIRS>
+__global__ void __launch_bounds__(64 * kFp4MaxWaves) __attribute__((amdgpu_waves_per_eu(fp4_waves(PAIRS) / 4)))
+mxfp4_stream_kernel(Fp4Args p) {
+  constexpr int kChunks = 2 * PAIRS;
   constexpr uint32_t kLeast = FP16 ? 104 : 0, kSpan = FP16 ? 36 : 252;   // scale codes of exact values
   extern __shared__ uint32_t s_mem[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
   const int steps = SWIGLU ? p.n / 32 : (p.n / 16 + 1) / 2;   // of a unit
   const long kb = p.k / 2, ks = p.k / 32;
   const int p0 = pairs * w / waves, c0 = 2 * p0;
-  const int count = 2 * (pairs * (w + 1) / waves) < chunks ? 2 * (pairs * (w + 1) / waves) - c0 : chunks - c0;   // (1 .. kFp4Chunks)
+  const int count = 2 * (pairs * (w + 1) / waves) < chunks ? 2 * (pairs * (w + 1) / waves) - c0 : chunks - c0;   // (1 .. kChunks)
   Fp4Units<kFp4Rows> some;
   some.read(0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
   int units = some.count();
@@ -293,9 +297,9 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
   const uint32_t end = at + share + (blockIdx.x < rest ? 1 : 0);
   // The lane's place in the wavefront's bytes of eight weight rows: row l16 % 8, half l16 / 8 of a pair's line (a pair that ends a row of
   // an odd number of chunks has one half: taken twice, times zeros of `a`; so is the last pair of a wavefront that has only one).
-  uint32_t wlane[kFp4Pairs];
+  uint32_t wlane[PAIRS];
 #pragma unroll
-  for (int q = 0; q < kFp4Pairs; q++) {
+  for (int q = 0; q < PAIRS; q++) {
     const int pair = 2 * q < count ? q : 0;
     wlane[q] = (uint32_t)((l16 & 7) * (int)kb + pair * 128 + (l16 >= 8 && 2 * pair + 1 < count ? 64 : 0) + lr * 16);
   }
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
     const Fp4Unit g = some.unit(e0, (int)unit - before);
     const uint8_t* bw = p.b + (long)g.expert * p.n * kb + p0 * 128;
     const uint8_t* sw = p.sf + (long)g.expert * p.n * ks;
-    v4i wt[2][kFp4Chunks];
+    v4i wt[2][kChunks];
     uint32_t sc[2][2];
     auto first_row = [&](int h, int st) {   // of half h of step st; the second half of a last step that has none: the one before
       const int row = SWIGLU ? h * inter + st * 16 : st * 32 + h * 16;
@@ -353,14 +357,14 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int q = 0; q < kFp4Pairs; q++) load(q, h, step);
+      for (int q = 0; q < PAIRS; q++) load(q, h, step);
     __builtin_amdgcn_sched_barrier(0);   // (ahead of the rows of `a`, which come from a cache)
-    v4i x[kFp4Chunks][4];
+    v4i x[kChunks][4];
     {
       const bool has_row = l16 < g.rows;
       const uint16_t* ap = p.a + (long)(g.row0 + (has_row ? l16 : 0)) * p.k + c0 * 128 + lr * 32;
 #pragma unroll
-      for (int j = 0; j < kFp4Chunks; j++)
+      for (int j = 0; j < kChunks; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const v4i v = *(const v4i*)(ap + (j < count ? j : 0) * 128 + i * 8);
@@ -369,20 +373,22 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
     }
     // The outputs of a step from its partial sums, in the wavefronts' order.
     auto finish = [&](int b, int st) {
-      int t = tid;
-      asm volatile("" : "+v"(t));   // (what follows from it is worked out here, not kept in registers over the steps)
+      int t = tid, parts = waves;
+      // (what follows from these is worked out here, not kept in registers over the steps; scalar ones are short with SwiGLU alone)
+      if constexpr (SWIGLU) asm volatile("" : "+v"(t), "+s"(parts));
+      else asm volatile("" : "+v"(t));
       for (; t < (SWIGLU ? 16 : 32) * g.rows; t += blockDim.x) {
         const int col = t & 15, h = SWIGLU ? 0 : t >> 4 & 1, m = SWIGLU ? t >> 4 : t >> 5;
-        const float* part = s_part + b * 2 * waves * 256 + (m >> 2) * 64 + col * 4 + (m & 3);
+        const float* part = s_part + b * 2 * parts * 256 + (m >> 2) * 64 + col * 4 + (m & 3);
         float f[SWIGLU ? 2 : 1][kFp4MaxWaves];
 #pragma unroll
         for (int u = 0; u < (SWIGLU ? 2 : 1); u++)
 #pragma unroll
-          for (int i = 0; i < kFp4MaxWaves; i++) f[u][i] = part[((SWIGLU ? u : h) * waves + (i < waves ? i : 0)) * 256];
+          for (int i = 0; i < kFp4MaxWaves; i++) f[u][i] = part[((SWIGLU ? u : h) * parts + (i < parts ? i : 0)) * 256];
 #pragma unroll
         for (int u = 0; u < (SWIGLU ? 2 : 1); u++)
 #pragma unroll
-          for (int i = 1; i < kFp4MaxWaves; i++) f[u][0] += i < waves ? f[u][i] : 0.f;
+          for (int i = 1; i < kFp4MaxWaves; i++) f[u][0] += i < parts ? f[u][i] : 0.f;
         const int c = SWIGLU ? st * 16 + col : st * 32 + h * 16 + col;
         float y = f[0][0];
         if constexpr (SWIGLU) y = swiglu_f32(y, f[1][0]);
@@ -396,10 +402,10 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
       load_scales(next);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        int code[kFp4Chunks];
+        int code[kChunks];
         uint32_t far = 0;
 #pragma unroll
-        for (int j = 0; j < kFp4Chunks; j++) {
+        for (int j = 0; j < kChunks; j++) {
           const uint32_t four = s_scale[((buf * 2 + h) * chunks + c0 + (j < count ? j : 0)) * 16 + l16];
           code[j] = (int)__builtin_amdgcn_ubfe(four, lr * 8, 8);
           const uint32_t d = (uint32_t)code[j] - kLeast;
@@ -408,7 +414,7 @@ __global__ void __launch_bounds__(64 * kFp4MaxWaves) mxfp4_stream_kernel(Fp4Args
         v4f sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // (of even and odd chunks: two chains of matrix instructions)
         if (far > kSpan) s_far[buf] = 1;
 #pragma unroll
-        for (int q = 0; q < kFp4Pairs; q++) {
+        for (int q = 0; q < PAIRS; q++) {
           trade_halves(wt[h][2 * q], wt[h][2 * q + 1]);
 #pragma unroll
           for (int i = 0; i < 4; i++)
@@ -455,17 +461,25 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
   // units with rows: at most one per expert or row, and one more per full tile
   const long experts = num_experts < total_rows ? num_experts : total_rows;
   const long most = (experts + (long)total_rows / kFp4Rows) * steps;
-  if (chunks <= kFp4Chunks * kFp4MaxWaves && most < 1L << 31) {
-    int waves = (pairs + kFp4Pairs - 1) / kFp4Pairs;
-    const int per_cu = kFp4MaxWaves / waves;
-    waves = kFp4MaxWaves / per_cu < pairs ? kFp4MaxWaves / per_cu : pairs;
+  if (pairs <= kFp4MaxPairs * kFp4MaxWaves && most < 1L << 31) {
+    // as few wavefronts as K takes, and as many workgroups as that leaves room for; then K evenly over the wavefronts
+    int waves = (pairs + kFp4MaxPairs - 1) / kFp4MaxPairs;
     const int each = (pairs + waves - 1) / waves;
     waves = (pairs + each - 1) / each;
+    const int per_cu = fp4_waves(each) / waves;
     const unsigned grid = (unsigned)(most < (long)cus * per_cu ? most : (long)cus * per_cu);
     const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint16_t*)out};
-    auto kernel = dtype ? swiglu ? mxfp4_stream_kernel<true, true> : mxfp4_stream_kernel<true, false>
-                        : swiglu ? mxfp4_stream_kernel<false, true> : mxfp4_stream_kernel<false, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 4096 * waves + 256 * chunks + 8, stream, args);
+#define ESMOE_FP4(P)                                                                                                               \
+  do {                                                                                                                             \
+    auto kernel = dtype ? swiglu ? mxfp4_stream_kernel<true, true, P> : mxfp4_stream_kernel<true, false, P>                        \
+                        : swiglu ? mxfp4_stream_kernel<false, true, P> : mxfp4_stream_kernel<false, false, P>;                     \
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 4096 * waves + 256 * chunks + 8, stream, args);                       \
+  } while (0)
+    if (each == 1) ESMOE_FP4(1);
+    else if (each == 2) ESMOE_FP4(2);
+    else if (each == 3) ESMOE_FP4(3);
+    else ESMOE_FP4(4);
+#undef ESMOE_FP4
     return (int)hipGetLastError();
   }
   const long units = experts + (long)total_rows / kFp4Rows;
