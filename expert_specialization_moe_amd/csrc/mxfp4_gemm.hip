@@ -462,11 +462,11 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
   const long experts = num_experts < total_rows ? num_experts : total_rows;
   const long most = (experts + (long)total_rows / kFp4Rows) * steps;
   if (pairs <= kFp4MaxPairs * kFp4MaxWaves && most < 1L << 31) {
-    // as few wavefronts as K takes, and as many workgroups as that leaves room for; then K evenly over the wavefronts
-    int waves = (pairs + kFp4MaxPairs - 1) / kFp4MaxPairs;
-    const int each = (pairs + waves - 1) / waves;
-    waves = (pairs + each - 1) / each;
-    const int per_cu = fp4_waves(each) / waves;
+    // As many wavefronts as a workgroup has, each with as little of K as that takes.  us, as few wavefronts as K takes / this:
+    // 32 experts x 7168 x K 2048, a row each 49.2 / 46.3, eight rows 55.8 / 52.0; 8 experts, 64 rows each 44 / 37; 64 experts x 1536 x
+    // K 4096, eight rows 46.6 / 45.8; (sixteen wavefronts of one workgroup instead of eight: 57.0).
+    const int each = (pairs + kFp4MaxWaves - 1) / kFp4MaxWaves;
+    const int waves = (pairs + each - 1) / each, per_cu = fp4_waves(each) / waves;
     const unsigned grid = (unsigned)(most < (long)cus * per_cu ? most : (long)cus * per_cu);
     const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint16_t*)out};
 #define ESMOE_FP4(P)                                                                                                               \
