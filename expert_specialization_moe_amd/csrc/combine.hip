@@ -53,10 +53,10 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(const uint16_t* __res
                                                            const float* __restrict__ weights, long tokens, int topk, long rows,
                                                            int hidden, uint32_t pieces, uint16_t* __restrict__ out) {
   const int lane = threadIdx.x & 63;
-  const long piece = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const long t = piece / pieces;
+  const uint32_t piece = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long t = pieces == 1 ? piece : piece / pieces;
   if (t >= tokens) return;
-  const int col = (int)(piece - t * pieces) * 512 + lane * 8;
+  const int col = (int)(piece - (uint32_t)t * pieces) * 512 + lane * 8;
   float acc[8] = {};
   for (int j0 = 0; j0 < topk; j0 += 64) {
     const int j = j0 + lane;

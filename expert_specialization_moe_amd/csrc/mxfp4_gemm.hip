@@ -343,7 +343,7 @@ mxfp4_stream_kernel(Fp4Args p) {
       for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int i = 0; i < 2; i++)
-          sc[h][i] = __builtin_amdgcn_raw_buffer_load_b32(tile_bytes(sw + first_row(h, st) * ks, 16 * (int)ks), tid * 4, i * (int)blockDim.x * 4, 0);
+          sc[h][i] = __builtin_amdgcn_raw_buffer_load_b32(tile_bytes(sw + first_row(h, st) * ks, 16 * (int)ks), (tid + i * (int)blockDim.x) * 4, 0, 0);
     };
     auto store_scales = [&](int b) {
 #pragma unroll
