@@ -250,12 +250,16 @@ __device__ __forceinline__ void store_lane(T* row, int first, int count, const f
 }
 
 // Sixteen lanes' reductions, to all of them.
+template <int CTRL, typename F, typename Op>
+__device__ __forceinline__ F row_step(F v, Op op) {   // (every lane has a partner: the move becomes part of the operation)
+  return op(v, __builtin_bit_cast(F, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
+}
 template <typename F, typename Op>
 __device__ __forceinline__ F row_reduce(F v, Op op) {
-  v = dpp_step<0xB1, 0xf>(v, v, op);    // lane ^ 1, ^ 2, then the mirrors of eight and of sixteen lanes
-  v = dpp_step<0x4E, 0xf>(v, v, op);
-  v = dpp_step<0x141, 0xf>(v, v, op);
-  return dpp_step<0x140, 0xf>(v, v, op);
+  v = row_step<0xB1>(v, op);    // lane ^ 1, ^ 2, then the mirrors of eight and of sixteen lanes
+  v = row_step<0x4E>(v, op);
+  v = row_step<0x141>(v, op);
+  return row_step<0x140>(v, op);
 }
 __device__ __forceinline__ float row_sum(float v) {
   return row_reduce(v, [](float a, float b) { return a + b; });
@@ -306,8 +310,8 @@ __device__ __forceinline__ void compare_rotated(float score, float near, int lan
 // smallest choice, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
 // ones by less than `slack`.  Where two neighbours of the order, or two groups' scores, are too close to tell, the wavefront does the
 // token again by gate_token: of random tokens one in some hundred.
-// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 16.0, one 6.3 / 5.4; softmax over
-// 128 experts, bf16, 16384 tokens 11.2 / 6.2.
+// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 15.3, one 6.3 / 5.0; softmax over
+// 128 experts, bf16, 16384 tokens 11.2 / 5.8.
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const T* __restrict__ logits, long ld,
                                                                            const float* __restrict__ bias, GateArgs a, int* __restrict__ ids,
@@ -354,32 +358,46 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const uint32_t k = order_key(x[i]);
-      key[i] = k ? (k & 0xffffff00u) | (uint32_t)(255 - (l * PER + i)) : 0u;
+      key[i] = (k & 0xffffff00u) | (uint32_t)(255 - (l * PER + i));   // (below 256: out)
     }
   } else {
-    float choice[PER], slack = 0.f;
+    float choice[PER], slack = 0.f, lo = __builtin_inff(), any = 0.f;   // (any: NaN where a choice is)
     if (!a.exact) {
+      float hi = x[0];
+#pragma unroll
+      for (int i = 1; i < PER; i++) hi = __builtin_fmaxf(hi, x[i]);
+      lo = row_max(hi) - 64.f;   // (as below)
 #pragma unroll
       for (int i = 0; i < PER; i++) {
-        unsure |= x[i] != x[i];
-        choice[i] = x[i];
+        any += x[i] == ninf ? 0.f : x[i];
+        choice[i] = x[i] == ninf ? ninf : __builtin_fmaxf(x[i], lo);
       }
     } else {
       const float scale = a.sigmoid ? 1.f : 1.0f / sum;
-      float largest = 0.f;
 #pragma unroll
       for (int i = 0; i < PER; i++) {
         const float e = __builtin_amdgcn_exp2f((a.sigmoid ? -x[i] : x[i] - top) * 1.44269504088896340736f);
-        float c = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + e) : e * scale;
-        c += b[i];
-        unsure |= c != c;
+        const float c = (a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + e) : e * scale) + b[i];
+        any += c;
+        lo = __builtin_fminf(lo, c);
         choice[i] = x[i] == ninf ? ninf : c;
-        largest = __builtin_fmaxf(largest, choice[i] == ninf ? 0.f : __builtin_fabsf(c));
+      }
+      float largest = choice[0];
+#pragma unroll
+      for (int i = 1; i < PER; i++) largest = __builtin_fmaxf(largest, choice[i]);
+      largest = row_max(largest);
+      lo = -row_max(-lo);
+      const bool far = lo < largest - 64.f;   // a bias that is -inf or very low
+      if (far) {
+        lo = __builtin_inff();
+#pragma unroll
+        for (int i = 0; i < PER; i++) lo = __builtin_fminf(lo, choice[i] == ninf ? __builtin_inff() : choice[i]);
+        lo = -row_max(-lo);
       }
       // in units of 2^-24: a sigmoid's error is below 3.8 (|x| s (1 - s) < .23 from the argument's rounding, .5 from 2^x, 1 and 2 from the
       // sum and its reciprocal), a softmax's below 33 of the largest score (its sum's 20 additions and the mean |x - top| of its terms
       // among them); and half a unit of the last place for the fp32 sum on either side
-      slack = (a.sigmoid ? 2.5e-7f : 2e-6f * scale) + 1.25e-7f * row_max(largest);
+      const float err = a.sigmoid ? 2.5e-7f : 2e-6f * scale;
       if (a.groups > 1) {
         float first = choice[0], second = ninf;
 #pragma unroll
@@ -404,33 +422,35 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
         int ahead = 0;
         bool close = false;
         // (a group without an expert left is out: behind all others, and its experts have no key)
-        compare_rotated<1>(score, 4.f * slack, lanes, ahead, close);
-        unsure |= close && l < a.groups * lanes;
+        compare_rotated<1>(score, 4.f * (err + 1.25e-7f * __builtin_fmaxf(largest, -lo)), lanes, ahead, close);
+        unsure |= (close || (score == ninf && first != ninf)) && l < a.groups * lanes;   // (the sum's overflow)
         if (ahead >= a.topk_groups) {
 #pragma unroll
           for (int i = 0; i < PER; i++) choice[i] = ninf;
         }
       }
+      if (far) {   // (what lies far below the largest is hardly taken: it gets one key, and is close to its like)
+        lo = __builtin_fmaxf(lo, largest - 64.f);
+#pragma unroll
+        for (int i = 0; i < PER; i++) choice[i] = choice[i] == ninf ? ninf : __builtin_fmaxf(choice[i], lo);
+      }
+      slack = err + 1.25e-7f * __builtin_fmaxf(largest, -lo);
     }
-    // fixed point, from the smallest choice on or from so far below the largest that what lies under it is hardly taken (it gets one key,
-    // and is close to its like)
-    float hi = choice[0], lo = __builtin_inff();
+    float hi = choice[0];
 #pragma unroll
     for (int i = 1; i < PER; i++) hi = __builtin_fmaxf(hi, choice[i]);
-#pragma unroll
-    for (int i = 0; i < PER; i++) lo = __builtin_fminf(lo, choice[i] == ninf ? __builtin_inff() : choice[i]);
     hi = row_max(hi);
-    lo = -row_max(-lo);
-    lo = __builtin_fmaxf(lo, hi - 64.f);
+    // fixed point from 1 on; an expert that is out gets 0
     const float units = 16777200.f / (hi > lo ? hi - lo : 1.f);   // (its own rounding and the products' stay below 2^24)
     // (three units of rounding on either side; where the units are not finite numbers nothing is sure)
     const float apart = 2.f * slack * units + 6.f;
-    unsure |= !(apart < 16777216.f) && hi != ninf;
+    unsure |= any != any || hi == __builtin_inff() || (!(apart < 16777216.f) && hi != ninf);
     near = (uint32_t)apart;
+    const uint32_t place = 255 - l * PER;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const uint32_t q = (uint32_t)__builtin_fmaxf((choice[i] - lo) * units, 0.f) + 1u;   // 1 .. 2^24 - 1
-      key[i] = choice[i] == ninf ? 0u : q << 8 | (uint32_t)(255 - (l * PER + i));
+      const uint32_t q = (uint32_t)__builtin_fmaxf(__builtin_fmaf(choice[i] - lo, units, 1.f), 0.f);   // (the conversion's own clamp)
+      key[i] = (q << 8) + (place - i);
     }
   }
   int mine = -1;   // lane j of a token: the j-th expert
@@ -445,7 +465,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
     }
     d = row_reduce(d, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
     const uint32_t max = left ? before + d : 0;
-    left = max != 0;
+    left = max >= 256u;
     if (l == j && j < a.topk && left) mine = 255 - (int)(max & 255u);
     if (!whole && j > 0) unsure |= left && (before >> 8) - (max >> 8) <= near;
     before = max;

@@ -66,6 +66,24 @@ def test_gating(esmoe, t, e, topk, scoring, renormalize):
         _check(esmoe, _logits(t, e, dtype, t + e), topk, None, scoring, renormalize, 2.5)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (8, 2), (8, 6)])
+def test_low_and_high_biases(esmoe, scoring, groups, kept):
+    """Biases far below the rest decide between groups like any other, and experts that have one are chosen when nothing else is left."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((33, 128), generator=g)
+    x[5, 16:] = float("-inf")
+    for high in (0.0, 1000.0):
+        for low in (float("-inf"), torch.finfo(torch.float32).min, -1e4, -65.0):
+            b = high + torch.rand(128, generator=g) * 0.2
+            b[32:64], b[3], b[127] = low, low, low
+            b[64:68] -= torch.rand(4, generator=g) + 80.0
+            b[66:] -= 0.0 if low < -1e4 else 70 * torch.rand(62, generator=g)
+            for topk in (1, 6, 16):
+                with np.errstate(over="ignore"):
+                    _check(esmoe, x, topk, b, scoring, True, grad=False, groups=groups, topk_groups=kept)
+
+
 @pytest.mark.parametrize("t,e,topk,groups,topk_groups", [(9, 256, 8, 1, 1), (130, 256, 8, 8, 4), (5, 60, 7, 4, 3), (11, 64, 5, 64, 5), (17, 1024, 16, 8, 1),
                                                          (3, 36, 12, 3, 1), (6, 100, 10, 2, 2), (40, 512, 8, 16, 3), (21, 72, 4, 36, 3)])
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
