@@ -47,8 +47,19 @@ __device__ __forceinline__ v4i pack8(const float* x) {
   return r;
 }
 
-// One wavefront per 512 columns of a token.
-template <bool FP16>
+// Each row is read once, and what is written is another kernel's to read: the stores are non-temporal, and where a call's rows are more than
+// the memory-side cache holds (STREAM) the loads are too.  us, plain / stores / both: 4096 tokens x top-8 x 7168 104.3 / 98 / 88, its gradient
+// 204 / 193 / 186; where the rows fit in the cache the loads' hint costs (1024 x top-8 x 7168, gradient, stores / both 39.7 / 45.7).
+constexpr long kCacheBytes = 1L << 28;
+template <bool STREAM>
+__device__ __forceinline__ v4i load8(const uint16_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const v4i*)p);
+  else return *(const v4i*)p;
+}
+
+// One wavefront per 512 columns of a token, eight rows' loads in flight.  Bound by memory: 88 us for 4096 tokens x top-8 x 7168 are 5.9 TB/s.
+// One row after the other was 3.7 us for one token, this is 2.6.
+template <bool FP16, bool STREAM>
 __global__ void __launch_bounds__(256) combine_rows_kernel(const uint16_t* __restrict__ in, const int* __restrict__ dst_row,
                                                            const float* __restrict__ weights, long tokens, int topk, long rows,
                                                            int hidden, uint32_t pieces, uint16_t* __restrict__ out) {
@@ -63,26 +74,38 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(const uint16_t* __res
     int mine = j < topk ? dst_row[t * topk + j] : -1;
     if ((unsigned long)(long)mine >= (unsigned long)rows) mine = -1;
     const float weight = mine < 0 ? 0.f : weights ? weights[t * topk + j] : 1.f;
-    for (unsigned long long todo = __ballot(mine >= 0); todo; todo &= todo - 1) {
-      const int k = __builtin_ctzll(todo);
-      const long row = __builtin_amdgcn_readlane(mine, k);
-      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k));
-      if (col < hidden) {
-        float x[8];
-        unpack8<FP16>(*(const v4i*)(in + row * hidden + col), x);
+    // (a lane beyond the columns loads from the row's start)
+    for (unsigned long long todo = __ballot(mine >= 0); todo;) {
+      v4i raw[8];
+      float w[8];
+      int n = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(w, x[i], acc[i]);
-      }
+      for (int u = 0; u < 8; u++)
+        if (todo) {
+          const int k = __builtin_ctzll(todo);
+          todo &= todo - 1;
+          n = u + 1;
+          w[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k));
+          raw[u] = load8<STREAM>(in + (long)__builtin_amdgcn_readlane(mine, k) * hidden + (col < hidden ? col : 0));
+        }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (u < n) {
+          float x[8];
+          unpack8<FP16>(raw[u], x);
+#pragma unroll
+          for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(w[u], x[i], acc[i]);
+        }
     }
   }
-  if (col < hidden) *(v4i*)(out + t * hidden + col) = pack8<FP16>(acc);
+  if (col < hidden) __builtin_nontemporal_store(pack8<FP16>(acc), (v4i*)(out + t * hidden + col));
 }
 
 // One wavefront per pair; the four of a workgroup are mostly a token's, whose gradient row comes from HBM once and then from a cache.
 // A workgroup per token that took its pairs one after the other was the same speed for many long rows, but three times as long for few
 // tokens (one token x top-8 x 7168: 10.7 us, as it is 4.5; 16384 tokens
 // x top-8 x 512 95 / 51).
-template <bool FP16>
+template <bool FP16, bool STREAM>
 __global__ void __launch_bounds__(256) combine_rows_backward_kernel(const uint16_t* __restrict__ grad_out, const uint16_t* __restrict__ in,
                                                                     const int* __restrict__ dst_row, const float* __restrict__ weights,
                                                                     uint32_t num_pairs, uint32_t topk, long rows, int hidden,
@@ -106,7 +129,7 @@ __global__ void __launch_bounds__(256) combine_rows_backward_kernel(const uint16
     for (int u = 0; u < 4; u++)
       if (col + u * 512 < hidden) {
         g[u] = *(const v4i*)(gp + col + u * 512);
-        x[u] = __builtin_nontemporal_load((const v4i*)(xp + col + u * 512));
+        x[u] = load8<STREAM>(xp + col + u * 512);
       }
 #pragma unroll
     for (int u = 0; u < 4; u++)
@@ -119,7 +142,7 @@ __global__ void __launch_bounds__(256) combine_rows_backward_kernel(const uint16
           dot = __builtin_fmaf(gf[i], xf[i], dot);
           gf[i] *= weight;
         }
-        *(v4i*)(op + col + u * 512) = pack8<FP16>(gf);
+        __builtin_nontemporal_store(pack8<FP16>(gf), (v4i*)(op + col + u * 512));
       }
   }
   dot = wave_sum_last(dot);
@@ -133,7 +156,9 @@ extern "C" int esmoe_launch_combine_rows(const void* in, int dtype, const int* d
   using namespace esmoe;
   const long pieces = (hidden + 511) / 512;
   const long step = (1L << 24) / pieces;   // tokens of a launch: a grid holds fewer than 2^32 threads
-  auto kernel = dtype ? combine_rows_kernel<true> : combine_rows_kernel<false>;
+  const bool stream_in = 2 * (rows < tokens * topk ? rows : tokens * topk) * hidden > kCacheBytes;
+  auto kernel = dtype ? (stream_in ? combine_rows_kernel<true, true> : combine_rows_kernel<true, false>)
+                      : (stream_in ? combine_rows_kernel<false, true> : combine_rows_kernel<false, false>);
   for (long t = 0; t < tokens; t += step) {
     const long n = tokens - t < step ? tokens - t : step;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((n * pieces + 3) / 4)), dim3(256), 0, stream, (const uint16_t*)in, dst_row + t * topk,
@@ -147,7 +172,9 @@ extern "C" int esmoe_launch_combine_rows_backward(const void* grad_out, const vo
                                                   hipStream_t stream) {
   using namespace esmoe;
   const long step = (1L << 25) / topk > 0 ? (1L << 25) / topk : 1;   // tokens of a launch: a grid holds fewer than 2^32 threads
-  auto kernel = dtype ? combine_rows_backward_kernel<true> : combine_rows_backward_kernel<false>;
+  const bool stream_in = 4 * (rows < tokens * topk ? rows : tokens * topk) * hidden > kCacheBytes;   // (with their gradients)
+  auto kernel = dtype ? (stream_in ? combine_rows_backward_kernel<true, true> : combine_rows_backward_kernel<true, false>)
+                      : (stream_in ? combine_rows_backward_kernel<false, true> : combine_rows_backward_kernel<false, false>);
   for (long t = 0; t < tokens; t += step) {
     const long n = tokens - t < step ? tokens - t : step;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((n * topk + 3) / 4)), dim3(256), 0, stream, (const uint16_t*)grad_out + t * hidden,

@@ -116,6 +116,25 @@ def test_offsets_past_32_bits(esmoe):
     assert (np.abs(_np(gw) - want_w) <= (hidden / 64 + 16) * 2.0 ** -24 * mag).all()
 
 
+def test_rows_beyond_the_cache_give_the_bytes_of_small_calls(esmoe):
+    """More than 256 MB of rows and gradients, ragged, some pairs remote, against the same tokens a few at a time."""
+    for tokens, topk, hidden in ((2503, 8, 8184), (40007, 3, 1160)):
+        rows, dst, weights, grad = (t.cuda() for t in _case(tokens, topk, hidden, torch.bfloat16, 8, 0.1))
+        assert rows.numel() * 2 > 2 ** 28 // 2
+        for w in (weights, None):
+            whole = esmoe.es_combine_rows(rows, dst, topk, w)
+            for t in range(0, tokens, 997):
+                part = slice(t, min(t + 997, tokens))
+                assert torch.equal(whole[part], esmoe.es_combine_rows(rows, dst[part.start * topk:part.stop * topk], topk, None if w is None else w[part]))
+        into, small = torch.full_like(rows, 7.0), torch.full_like(rows, 7.0)
+        _, gw = esmoe.es_combine_rows_backward(grad, rows, dst, topk, weights, into)
+        for t in range(0, tokens, 997):
+            part = slice(t, min(t + 997, tokens))
+            _, g = esmoe.es_combine_rows_backward(grad[part], rows, dst[part.start * topk:part.stop * topk], topk, weights[part], small)
+            assert torch.equal(gw[part], g)
+        assert torch.equal(into, small)
+
+
 def test_empty_calls_and_overlaps(esmoe):
     rows = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
     none = torch.zeros(0, dtype=torch.int32, device="cuda")

@@ -115,6 +115,24 @@ def test_bytes_are_the_quantisers(esmoe):
     assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(scales, want_s)
 
 
+@pytest.mark.parametrize("rows,k", [(65537, 512), (9001, 7168), (40001, 1024)])
+def test_rows_beyond_the_cache_give_the_bytes_of_small_calls(esmoe, rows, k):
+    gen = torch.Generator().manual_seed(3)
+    x, r = (torch.randn((rows, k), generator=gen).to(torch.bfloat16).cuda() for _ in range(2))
+    w = torch.randn(k, generator=gen).to(torch.bfloat16).cuda()
+    assert 9 * rows * k > 2 ** 28
+    for residual, normed in ((r, True), (None, False)):
+        whole = esmoe.es_add_rms_norm_quant_1x128(x, w, 1e-6, residual, return_normed=normed)
+        for t in (*range(0, rows - 2999, 2999), rows - 2999):   # (256 rows or fewer are summed in another order)
+            part = esmoe.es_add_rms_norm_quant_1x128(x[t:t + 2999], w, 1e-6, None if residual is None else residual[t:t + 2999],
+                                                     return_normed=normed)
+            for a, b in zip(whole, part):
+                assert (a is None) == (b is None)
+                if a is not None:
+                    a = a[t:t + 2999]
+                    assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
 def test_no_rows_and_offsets_past_32_bits(esmoe):
     w = torch.ones(8192, dtype=torch.bfloat16, device="cuda")
     assert esmoe.es_add_rms_norm_quant_1x128(torch.zeros((0, 8192), dtype=torch.bfloat16, device="cuda"), w)[0].shape == (0, 8192)
