@@ -4,12 +4,12 @@
 //   swiglu form, n = 2 * inter, gate rows first: out[off_e + m, i] = cast( silu(gate) * up ) of the two fp32 sums
 //
 // Decode: every weight of an expert with rows is read once, 17/32 bytes each, and used for a handful of rows; the bound is HBM.
-// The 4-bit codes become bf16/fp16 values exactly (v_cvt_scalef32_pk_*_fp4, scale 1) and go through v_mfma_f32_16x16x32 with up to
-// sixteen rows of `a`; a product of 32 columns belongs to one scale, which its fp32 result is multiplied by as it is added up: no range
-// of scales is lost in a 16-bit format.
+// The 4-bit codes become bf16/fp16 values exactly (v_cvt_scalef32_pk_*_fp4) and go through v_mfma_f32_16x16x32 with up to sixteen rows of
+// `a`.  A product of 32 columns belongs to one scale: where the scaled value is exact in the 16-bit type the conversion takes it in,
+// otherwise the product's fp32 result is multiplied by it as it is added up, so that no range of scales is lost.
 //
-// A workgroup of four wavefronts takes 16 weight rows (16 of the gate and 16 of the up projection) for 16 rows of `a`; the wavefronts
-// split K, their sums are added in LDS in wavefront order.  No counterpart in the reference (its operators are 8-bit).
+// The wavefronts of a workgroup split K; their sums are added in LDS in wavefront order.  No counterpart in the reference (its operators are
+// 8-bit).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
@@ -27,7 +27,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
-constexpr int kFp4Threads = 256, kFp4Waves = 4, kFp4Rows = 16;
+constexpr int kFp4Rows = 16, kLongWaves = 8;
 
 // Eight weights of a dword as values of the activations' type.
 template <bool FP16>
@@ -118,17 +118,20 @@ struct Fp4Units {
   }
 };
 
+// For a K whose sixteen rows of `a` are more than a workgroup's registers: a workgroup takes two tiles of sixteen weight rows (one of the
+// gate's and one of the up projection's) for sixteen rows of `a`, which come from a cache as they are needed; its wavefronts split K.
+// Bound by the loads it has in flight: 16 experts x 2048 x K 12288, a row each 67.6 us (3.1 TB/s), 16 rows 99; with four tiles 71 and 84, but
+// two experts of K 14336 44 instead of 23; non-temporal loads of the weights, half a line each, 72.7.
 template <bool FP16, bool SWIGLU>
-__global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ b,
-                                                                       const uint8_t* __restrict__ sf, const int* __restrict__ problem_sizes,
-                                                                       const int* __restrict__ expert_offsets, int num_experts,
-                                                                       int total_rows, int n, int k, int col_tiles, int unit0,
-                                                                       uint16_t* __restrict__ out) {
-  constexpr int NT = SWIGLU ? 2 : 1;
-  __shared__ float s_sum[kFp4Waves][NT][kFp4Rows][16];
+__global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ b,
+                                                                     const uint8_t* __restrict__ sf, const int* __restrict__ problem_sizes,
+                                                                     const int* __restrict__ expert_offsets, int num_experts, int total_rows,
+                                                                     int n, int k, int col_tiles, int unit0, uint16_t* __restrict__ out) {
+  constexpr int kCols = SWIGLU ? 16 : 32;   // of the output
+  __shared__ float s_sum[kLongWaves][2][kFp4Rows][16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int l16 = lane & 15, lr = lane >> 4;
-  const int unit = blockIdx.x / col_tiles, tile = blockIdx.x - unit * col_tiles;
+  const int unit = blockIdx.x / col_tiles, col0 = (blockIdx.x - unit * col_tiles) * kCols;
   Fp4Unit g = {0, 0, 0};
   for (int e0 = 0, u = unit0 + unit; e0 < num_experts; e0 += 64) {
     Fp4Units<kFp4Rows> some;
@@ -140,30 +143,30 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
     u -= some.count();
   }
   if (g.rows == 0) return;   // the whole workgroup
-  const int wide = n / NT;   // columns of the output
+  const int wide = SWIGLU ? n / 2 : n;   // columns of the output
   const long kb = k / 2, ks = k / 32;
-  const uint8_t* bp[NT];
-  const uint8_t* sp[NT];
+  const uint8_t* bp[2];
+  const uint8_t* sp[2];
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const long row = (long)g.expert * n + t * wide + tile * 16 + l16;
+  for (int t = 0; t < 2; t++) {
+    const int col = SWIGLU ? t * wide + col0 : col0 + t * 16;   // (a tile beyond the last column is the last one again, and not stored)
+    const long row = (long)g.expert * n + (col < n ? col : n - 16) + l16;
     bp[t] = b + row * kb + lr * 16;
     sp[t] = sf + row * ks;
   }
-  const bool has_row = l16 < g.rows;
+  const bool has_row = l16 < g.rows;   // (loads of a row that is not there: 69 us instead of 67.6)
   const uint16_t* ap = a + (long)(g.row0 + (has_row ? l16 : 0)) * k + lr * 8;
-  v4f acc[NT];
+  v4f acc[2];
 #pragma unroll
-  for (int t = 0; t < NT; t++) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-  const int chunks = k / 128, per = (chunks + kFp4Waves - 1) / kFp4Waves;
-  const int end = (w + 1) * per < chunks ? (w + 1) * per : chunks;
+  for (int t = 0; t < 2; t++) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  const int chunks = k / 128, end = (int)((long)chunks * (w + 1) / kLongWaves);
 #pragma unroll 2
-  for (int c = w * per; c < end; c++) {
-    uint32_t d[NT][4], s[NT];
+  for (int c = (int)((long)chunks * w / kLongWaves); c < end; c++) {
+    uint32_t d[2][4], s[2];
     v4i x[4];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      const v4i raw = __builtin_nontemporal_load((const v4i*)(bp[t] + c * 64));
+    for (int t = 0; t < 2; t++) {
+      const v4i raw = *(const v4i*)(bp[t] + c * 64);   // (half a line: the other half is the next chunk's)
 #pragma unroll
       for (int i = 0; i < 4; i++) d[t][i] = (uint32_t)raw[i];
       s[t] = *(const uint32_t*)(sp[t] + c * 4);
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
       if (has_row) x[i] = *(const v4i*)(ap + c * 128 + i * 32);
     }
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
+    for (int t = 0; t < 2; t++) {
       transpose_rows(d[t]);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -186,21 +189,21 @@ __global__ void __launch_bounds__(kFp4Threads) mxfp4_grouped_mm_kernel(const uin
     }
   }
 #pragma unroll
-  for (int t = 0; t < NT; t++)
+  for (int t = 0; t < 2; t++)
 #pragma unroll
     for (int r = 0; r < 4; r++) s_sum[w][t][lr * 4 + r][l16] = acc[t][r];
   __syncthreads();
-  const int m = tid >> 4, col = tid & 15;
-  if (m >= g.rows) return;
-  float v[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) v[t] = (s_sum[0][t][m][col] + s_sum[1][t][m][col]) + (s_sum[2][t][m][col] + s_sum[3][t][m][col]);
-  float y = v[0];
-  if constexpr (SWIGLU) y = swiglu_f32(v[0], v[1]);
-  uint16_t bits;
-  if constexpr (FP16) bits = __builtin_bit_cast(uint16_t, (_Float16)y);
-  else bits = __builtin_bit_cast(uint16_t, (__bf16)y);
-  out[(long)(g.row0 + m) * wide + tile * 16 + col] = bits;
+  for (int i = tid; i < g.rows * kCols; i += 64 * kLongWaves) {
+    const int m = i / kCols, col = i % kCols;
+    if (col0 + col >= wide) continue;
+    float y = 0, up = 0;
+    for (int u = 0; u < kLongWaves; u++) {
+      y += s_sum[u][col >> 4][m][col & 15];
+      if constexpr (SWIGLU) up += s_sum[u][1][m][col];
+    }
+    if constexpr (SWIGLU) y = swiglu_f32(y, up);
+    out[(long)(g.row0 + m) * wide + col0 + col] = to_half<FP16>(y);
+  }
 }
 
 // Sixteen rows of `a` stay in registers: wavefront w of a workgroup holds their K range of up to four pairs of chunks (a chunk is 128
@@ -483,13 +486,13 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
     return (int)hipGetLastError();
   }
   const long units = experts + (long)total_rows / kFp4Rows;
-  const int col_tiles = n / (swiglu ? 32 : 16);
-  const long step = (1L << 23) / col_tiles > 1 ? (1L << 23) / col_tiles : 1;   // units of a launch: a grid holds fewer than 2^32 threads
-  auto kernel = dtype ? swiglu ? mxfp4_grouped_mm_kernel<true, true> : mxfp4_grouped_mm_kernel<true, false>
-                      : swiglu ? mxfp4_grouped_mm_kernel<false, true> : mxfp4_grouped_mm_kernel<false, false>;
+  const int cols = swiglu ? 16 : 32, col_tiles = ((swiglu ? n / 2 : n) + cols - 1) / cols;
+  const long step = (1L << 22) / col_tiles > 1 ? (1L << 22) / col_tiles : 1;   // units of a launch: a grid holds fewer than 2^32 threads
+  auto kernel = dtype ? swiglu ? mxfp4_long_kernel<true, true> : mxfp4_long_kernel<true, false>
+                      : swiglu ? mxfp4_long_kernel<false, true> : mxfp4_long_kernel<false, false>;
   for (long u = 0; u < units; u += step) {
     const long some = units - u < step ? units - u : step;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(some * col_tiles)), dim3(kFp4Threads), 0, stream, (const uint16_t*)a, (const uint8_t*)b, sf,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(some * col_tiles)), dim3(64 * kLongWaves), 0, stream, (const uint16_t*)a, (const uint8_t*)b, sf,
                        problem_sizes, expert_offsets, num_experts, total_rows, n, k, col_tiles, (int)u, (uint16_t*)out);
   }
   return (int)hipGetLastError();

@@ -82,6 +82,22 @@ def test_sixteen_columns_and_odd_tiles(esmoe):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,n,k", [([5, 18], 16, 8320), ([1], 48, 12288), ([3, 0, 33], 80, 14336), ([1] * 70, 32, 8448)])
+def test_long_k(esmoe, rows, n, k, dtype):
+    """Past what a workgroup's registers hold of `a`; an odd number of column tiles, more than 64 experts, scales far apart."""
+    a, b, sf = _operands(rows, n, k, dtype, n + k)
+    sf[:, :, 3], sf[:, :, -1] = 2, 150
+    _check(_run(esmoe, a, b, sf, rows, False), a, b, sf, rows, False)
+    if n % 32 == 0:
+        sf[:, :, -1] = 120
+        _check(_run(esmoe, a, b, sf, rows, True), a, b, sf, rows, True)
+    sf[-1, n // 2, 7] = 255   # NaN: its column, in its expert's rows
+    out = _run(esmoe, a, b, sf, rows, False).cpu()
+    first = sum(rows) - rows[-1]
+    assert out[first:sum(rows), n // 2].isnan().all() and out.isnan().sum() == rows[-1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_every_code_exactly(esmoe, dtype):
     """Integer activations and every 4-bit code with scales 2^-1 .. 2^2: all sums are exact in fp32, the output their rounding."""
     rng = np.random.default_rng(1)
