@@ -306,8 +306,8 @@ __device__ __forceinline__ void compare_rotated(float score, float near, int lan
 // and below them 255 - expert, and a largest one stands for itself and its place.  The largest key below the one before is
 //   before + max over keys of (key - before mod 2^32),
 // a subtraction per key and no removal: what is not below `before` wraps to the small side.
-// 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number between the token's largest and
-// smallest choice, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
+// 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number from the token's smallest choice (or 64 below
+// the largest) on, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
 // ones by less than `slack`.  Where two neighbours of the order, or two groups' scores, are too close to tell, the wavefront does the
 // token again by gate_token: of random tokens one in some hundred.
 // us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 15.3, one 6.3 / 5.0; softmax over
@@ -683,18 +683,34 @@ static int launch_gating_backward(const float* grad, const void* logits, long ld
 
 }  // namespace esmoe
 
+namespace {
+// A launch of some of the tokens, from t on: a grid holds fewer than 2^32 threads.
+constexpr long kGateStep = 1L << 24;
+template <typename Launch>
+int gate_steps(int dtype, const esmoe::GateArgs& a, Launch launch) {
+  int rc = 0;
+  for (long t = 0; t < a.tokens && rc == 0; t += kGateStep) {
+    esmoe::GateArgs some = a;
+    some.tokens = a.tokens - t < kGateStep ? a.tokens - t : kGateStep;
+    rc = dtype == esmoe::kGateF32 ? launch(float(), t, some) : dtype == esmoe::kGateF16 ? launch(_Float16(), t, some) : launch(__bf16(), t, some);
+  }
+  return rc;
+}
+}  // namespace
+
 extern "C" int esmoe_launch_topk_gating(const void* logits, int dtype, long ld, const float* bias, const esmoe::GateArgs* a, int* ids,
                                         float* weights, hipStream_t stream) {
-  using namespace esmoe;
-  if (dtype == kGateF32) return launch_gating<float>(logits, ld, bias, *a, ids, weights, stream);
-  if (dtype == kGateF16) return launch_gating<_Float16>(logits, ld, bias, *a, ids, weights, stream);
-  return launch_gating<__bf16>(logits, ld, bias, *a, ids, weights, stream);
+  return gate_steps(dtype, *a, [=](auto type, long t, const esmoe::GateArgs& some) {
+    using T = decltype(type);
+    return esmoe::launch_gating<T>((const T*)logits + t * ld, ld, bias, some, ids + t * a->topk, weights + t * a->topk, stream);
+  });
 }
 
 extern "C" int esmoe_launch_topk_gating_backward(const float* grad, const void* logits, int dtype, long ld, const int* ids,
                                                  const esmoe::GateArgs* a, void* out, hipStream_t stream) {
-  using namespace esmoe;
-  if (dtype == kGateF32) return launch_gating_backward<float>(grad, logits, ld, ids, *a, out, stream);
-  if (dtype == kGateF16) return launch_gating_backward<_Float16>(grad, logits, ld, ids, *a, out, stream);
-  return launch_gating_backward<__bf16>(grad, logits, ld, ids, *a, out, stream);
+  return gate_steps(dtype, *a, [=](auto type, long t, const esmoe::GateArgs& some) {
+    using T = decltype(type);
+    return esmoe::launch_gating_backward<T>(grad + t * a->topk, (const T*)logits + t * ld, ld, ids + t * a->topk, some,
+                                            (T*)out + t * a->experts, stream);
+  });
 }

@@ -619,6 +619,12 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   const char *pa = (const char*)a.data_ptr(), *pb = (const char*)b.data_ptr();
   return a.numel() && b.numel() && pa < pb + b.nbytes() && pb < pa + a.nbytes();
 }
+// (undefined tensors overlap nothing)
+bool any_overlap(const torch::Tensor& out, std::initializer_list<const torch::Tensor*> others) {
+  for (const torch::Tensor* t : others)
+    if (out.defined() && t->defined() && overlap(out, *t)) return true;
+  return false;
+}
 }  // namespace
 
 void es_combine_rows(const torch::Tensor& input, const torch::Tensor& dst_row, int64_t topk, const c10::optional<torch::Tensor>& weights_,
@@ -631,7 +637,7 @@ void es_combine_rows(const torch::Tensor& input, const torch::Tensor& dst_row, i
   check_no_autograd("es_combine_rows", {&input, &weights});
   require_device(input, "es_combine_rows");
   check_device(input, {&dst_row, &weights, &output});
-  TORCH_CHECK(!overlap(input, output), "output may not overlap input");
+  TORCH_CHECK(!any_overlap(output, {&input, &dst_row, &weights}), "output may not overlap input, dst_row or weights");
   if (tokens == 0) return;
   c10::DeviceGuard guard(input.device());
   int rc = esmoe_combine_rows(input.data_ptr(), input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16,
@@ -662,7 +668,9 @@ void es_combine_rows_backward(const torch::Tensor& grad_output, const torch::Ten
   check_no_autograd("es_combine_rows_backward", {&grad_output, &input, &weights});
   require_device(input, "es_combine_rows_backward");
   check_device(input, {&grad_output, &dst_row, &weights, &grad_input, &grad_weights});
-  TORCH_CHECK(!overlap(grad_input, input) && !overlap(grad_input, grad_output), "grad_input may not overlap input or grad_output");
+  TORCH_CHECK(!any_overlap(grad_input, {&input, &grad_output, &dst_row, &weights, &grad_weights}) &&
+                  !any_overlap(grad_weights, {&input, &grad_output, &dst_row, &weights}),
+              "grad_input and grad_weights may not overlap each other or the inputs");
   if (tokens == 0) return;
   c10::DeviceGuard guard(input.device());
   int rc = esmoe_combine_rows_backward(grad_output.data_ptr(), input.data_ptr(),
@@ -695,14 +703,13 @@ void es_add_rms_norm_quant_1x128(const torch::Tensor& input, const torch::Tensor
   require_device(input, "es_add_rms_norm_quant_1x128");
   check_device(input, {&weight, &residual, &residual_out, &normed, &quant_output, &scales});
   if (rows == 0) return;
-  // a row is read before any of its results is written: the new residual may take input's or residual's place, nothing else may overlap
-  for (const torch::Tensor* in : {&input, &residual, &weight}) {
-    if (!in->defined()) continue;
-    for (const torch::Tensor* out : {(const torch::Tensor*)&quant_output, (const torch::Tensor*)&scales, &normed})
-      TORCH_CHECK(!out->defined() || !overlap(*in, *out), "outputs may not overlap inputs");
-    TORCH_CHECK(!residual_out.defined() || !overlap(*in, residual_out) || (in != &weight && in->data_ptr() == residual_out.data_ptr()),
-                "residual_out may be input or residual, not a part of them");
-  }
+  TORCH_CHECK(!any_overlap(quant_output, {&input, &residual, &weight, &scales, &normed, &residual_out}) &&
+                  !any_overlap(scales, {&input, &residual, &weight, &normed, &residual_out}) &&
+                  !any_overlap(normed, {&input, &residual, &weight, &residual_out}) && !any_overlap(residual_out, {&weight}),
+              "outputs may not overlap inputs or each other");
+  // a row is read before its new residual is written
+  for (const torch::Tensor* in : {&input, &residual})
+    TORCH_CHECK(!any_overlap(residual_out, {in}) || in->data_ptr() == residual_out.data_ptr(), "residual_out may be input or residual, not a part of them");
   c10::DeviceGuard guard(input.device());
   int rc = esmoe_add_rms_norm_quant_1x128(
       input.data_ptr(), input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16, residual.defined() ? residual.data_ptr() : nullptr,
@@ -754,7 +761,7 @@ void mxfp4_grouped_mm(const char* op, bool swiglu, torch::Tensor& output, const 
   require_device(a, op);
   check_device(a, {&output, &b, &sfb, &problem_sizes, &expert_offsets});
   TORCH_CHECK(problem_sizes.is_contiguous() && expert_offsets.is_contiguous(), "metadata tensors must be contiguous");
-  TORCH_CHECK(!overlap(a, output), "output may not overlap a");
+  TORCH_CHECK(!any_overlap(output, {&a, &b, &sfb, &problem_sizes, &expert_offsets}), "output may not overlap an input");
   if (total_rows == 0) return;
   c10::DeviceGuard guard(a.device());
   int rc = esmoe_mxfp4_grouped_mm(output.data_ptr(), out_dtype_of(output), a.data_ptr(), b.data_ptr(), (const uint8_t*)sfb.data_ptr(),

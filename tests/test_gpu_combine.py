@@ -148,6 +148,12 @@ def test_empty_calls_and_overlaps(esmoe):
         esmoe.es_combine_rows(rows, dst, 1, None, rows)
     with pytest.raises(RuntimeError, match="may not overlap"):
         esmoe.es_combine_rows_backward(rows, rows.clone(), dst, 1, torch.ones(4, 1, device="cuda"), rows)
+    w = torch.ones(4, 1, device="cuda")
+    with pytest.raises(RuntimeError, match="may not overlap"):
+        esmoe.es_combine_rows_backward(rows, rows.clone(), dst, 1, w, grad_weights=w)
+    out = torch.zeros_like(rows)
+    with pytest.raises(RuntimeError, match="may not overlap"):
+        esmoe.es_combine_rows(rows, dst, 1, out.view(-1).view(torch.float32)[4:8], out)
 
 
 def test_c_abi(esmoe):

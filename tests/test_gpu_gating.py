@@ -199,3 +199,17 @@ def test_results_are_the_same_every_time(esmoe):
     # a token's result does not hang on its neighbours
     alone = esmoe.es_topk_gating(x[4096:], 8, b, "sigmoid", True, 2.5, 8, 4)
     assert torch.equal(alone[0], first[0][4096:]) and torch.equal(alone[1], first[1][4096:])
+
+
+def test_more_tokens_than_a_launch_takes(esmoe):
+    """Over 2^24 tokens; one expert of four each, the weight an unnormalised sigmoid: values and gradients of a few known logits."""
+    t = (1 << 24) + 37
+    picked = torch.arange(t, device="cuda", dtype=torch.int32) * 7 % 5 % 4
+    x = torch.zeros((t, 4), dtype=torch.bfloat16, device="cuda").scatter_(1, picked.long().unsqueeze(1), 2.0)
+    ids, w = esmoe.es_topk_gating(x, 1, None, "sigmoid", False)
+    p = torch.sigmoid(torch.tensor(2.0, dtype=torch.float64)).item()
+    assert torch.equal(ids[:, 0], picked) and ((w.double() - p).abs() <= 4 * 2.0 ** -24).all()
+    d = esmoe.es_topk_gating_backward(torch.ones_like(w), x, ids, "sigmoid", False)
+    want = torch.tensor(p * (1 - p)).to(torch.bfloat16).item()
+    assert (d.gather(1, picked.long().unsqueeze(1)).float() - want).abs().max() <= want * 2.0 ** -8
+    assert torch.count_nonzero(d) == t

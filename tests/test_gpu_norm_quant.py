@@ -76,6 +76,11 @@ def test_overlaps_are_refused(esmoe):
         esmoe.es_add_rms_norm_quant_1x128(x, w, 1e-6, normed=x)
     with pytest.raises(RuntimeError, match="may not overlap"):
         esmoe.es_add_rms_norm_quant_1x128(x, w, 1e-6, quant_output=buf[:512].view(torch.uint8).view(4, 256))
+    both = torch.zeros_like(x)
+    with pytest.raises(RuntimeError, match="each other"):
+        esmoe.es_add_rms_norm_quant_1x128(x, w, 1e-6, x.clone(), both, both)
+    with pytest.raises(RuntimeError, match="each other"):
+        esmoe.es_add_rms_norm_quant_1x128(x, w, 1e-6, normed=both, quant_output=both.view(-1)[:512].view(torch.uint8).view(4, 256))
 
 
 def test_zero_rows_tiny_rows_and_large_ones(esmoe):
