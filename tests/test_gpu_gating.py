@@ -213,3 +213,17 @@ def test_more_tokens_than_a_launch_takes(esmoe):
     want = torch.tensor(p * (1 - p)).to(torch.bfloat16).item()
     assert (d.gather(1, picked.long().unsqueeze(1)).float() - want).abs().max() <= want * 2.0 ** -8
     assert torch.count_nonzero(d) == t
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 8])
+def test_a_token_is_the_same_in_any_batch(esmoe, scoring, groups):
+    x = _logits(301, 256, torch.float32, 11).cuda()
+    x[40] = x[41].round()   # (ties: decided in 64 bits)
+    b = torch.zeros(256, device="cuda")
+    ids, w = esmoe.es_topk_gating(x, 8, b, scoring, True, 2.5, groups, min(groups, 4))
+    for t in (0, 1, 40, 41, 42, 43, 300):
+        one = esmoe.es_topk_gating(x[t:t + 1], 8, b, scoring, True, 2.5, groups, min(groups, 4))
+        assert torch.equal(one[0][0], ids[t]) and torch.equal(one[1][0], w[t])
+    back = esmoe.es_topk_gating(x.flip(0), 8, b, scoring, True, 2.5, groups, min(groups, 4))
+    assert torch.equal(back[0].flip(0), ids) and torch.equal(back[1].flip(0), w)
