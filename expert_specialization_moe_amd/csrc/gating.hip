@@ -139,13 +139,16 @@ __device__ __forceinline__ void gate_token(const T* __restrict__ row, const floa
     for (int i = 0; i < PER; i++) s_key[lane * PER + i] = key[i];
     wave_lds_fence();
     const int width = a.experts / a.groups;
+    const int log = 31 - __builtin_clz(64 / a.groups), lanes = 1 << log, own = lane >> log;   // lanes of a group, the lane's group
     uint32_t first = 0, second = 0;
-    if (lane < a.groups)
-      for (int i = 0; i < width; i++) {
-        const uint32_t k = s_key[lane * width + i], low = first < k ? first : k;
-        first = first > k ? first : k;
-        second = second > low ? second : low;
-      }
+    auto join = [&](uint32_t f, uint32_t s) {
+      const uint32_t low = first < f ? first : f, high = second > s ? second : s;
+      first = first > f ? first : f;
+      second = high > low ? high : low;
+    };
+    if (own < a.groups)
+      for (int i = lane & (lanes - 1); i < width; i += lanes) join(s_key[own * width + i], 0);
+    for (int d = 1; d < lanes; d <<= 1) join(__shfl_xor(first, d), __shfl_xor(second, d));
     // (1: finite choices whose sum is -inf; 0: no expert left)
     uint32_t score = first == 0 ? 0u : order_key(key_value(first) + (second ? key_value(second) : 0.f));
     if (first != 0 && score == 0) score = 1;
@@ -153,9 +156,9 @@ __device__ __forceinline__ void gate_token(const T* __restrict__ row, const floa
     for (int j = 0; j < a.topk_groups; j++) {
       const uint32_t best = wave_umax(score);
       if (best == 0) break;
-      const int g = __builtin_ctzll(__ballot(score == best));
+      const int g = __builtin_ctzll(__ballot(score == best)) >> log;
       keep |= 1ull << g;
-      if (lane == g) score = 0;
+      if (own == g) score = 0;
     }
 #pragma unroll
     for (int i = 0; i < PER; i++)
@@ -286,18 +289,29 @@ __device__ __forceinline__ float later_terms(int id, float d, int l, bool& first
   return 0.f;
 }
 
-// Counts the groups whose score is ahead of the lane's, and whether one is within `near` of it; R lanes on, and so forth.
+// Counts the groups whose score is ahead of the lane's by more than `near`, and those that are not as far behind; R lanes on, and so forth.
+// (A group without an expert left has -inf: behind all others, and what is said of it does not matter.)
 template <int R>
-__device__ __forceinline__ void compare_rotated(float score, float near, int lanes, int& ahead, bool& close) {
+__device__ __forceinline__ void compare_rotated(float score, float near, int lanes, int& sure, int& maybe) {
   if constexpr (R < 16) {
     if (R % lanes == 0) {
-      const float other = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, score), 0x120 + R, 0xf, 0xf, false));
-      ahead += other > score;
-      // (no expert left: -inf on either side says nothing; NaN is close to everything)
-      close |= !(__builtin_fabsf(other - score) > near) && other != -__builtin_inff() && score != -__builtin_inff();
+      const float d = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, score), 0x120 + R, 0xf, 0xf, false)) - score;
+      sure += d > near;
+      maybe += d >= -near;
     }
-    compare_rotated<R + 1>(score, near, lanes, ahead, close);
+    compare_rotated<R + 1>(score, near, lanes, sure, maybe);
   }
+}
+
+// How many of the sixteen lanes' keys are ahead of the lane's: larger, or as large and of a lower id.
+template <int R>
+__device__ __forceinline__ int order_rotated(uint32_t key, int id) {
+  if constexpr (R < 16) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)key, 0x120 + R, 0xf, 0xf, false);
+    const int oid = __builtin_amdgcn_update_dpp(0, id, 0x120 + R, 0xf, 0xf, false);
+    return (other > key || (other == key && oid < id) ? 1 : 0) + order_rotated<R + 1>(key, id);
+  }
+  return 0;
 }
 
 // Four tokens per wavefront, a lane l of sixteen holds a token's experts l * PER .. l * PER + PER - 1.
@@ -308,10 +322,10 @@ __device__ __forceinline__ void compare_rotated(float score, float near, int lan
 // a subtraction per key and no removal: what is not below `before` wraps to the small side.
 // 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number from the token's smallest choice (or 64 below
 // the largest) on, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
-// ones by less than `slack`.  Where two neighbours of the order, or two groups' scores, are too close to tell, the wavefront does the
-// token again by gate_token: of random tokens one in some hundred.
-// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 15.3, one 6.3 / 5.0; softmax over
-// 128 experts, bf16, 16384 tokens 11.2 / 5.8.
+// ones by less than `slack`.  Where two neighbours of the order are too close to tell, the candidates alone are put in order by their
+// exact choices; where the last of them and the next, or two groups' scores are, the wavefront does the token again by gate_token.
+// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 13.3 (11.6 where none
+// is done again), one 6.3 / 4.6; softmax over 128 experts, bf16, 16384 tokens 11.2 / 4.8.  The code of what is rare stands behind the rest: .5 of these us.
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const T* __restrict__ logits, long ld,
                                                                            const float* __restrict__ bias, GateArgs a, int* __restrict__ ids,
@@ -388,7 +402,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
       largest = row_max(largest);
       lo = -row_max(-lo);
       const bool far = lo < largest - 64.f;   // a bias that is -inf or very low
-      if (far) {
+      if (__builtin_expect(far, 0)) {
         lo = __builtin_inff();
 #pragma unroll
         for (int i = 0; i < PER; i++) lo = __builtin_fminf(lo, choice[i] == ninf ? __builtin_inff() : choice[i]);
@@ -419,17 +433,16 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
         if (lanes > 2) join(other(first, std::integral_constant<int, 0x4E>()), other(second, std::integral_constant<int, 0x4E>()));
         if (lanes > 4) join(other(first, std::integral_constant<int, 0x141>()), other(second, std::integral_constant<int, 0x141>()));
         const float score = first == ninf ? ninf : first + (second == ninf ? 0.f : second);
-        int ahead = 0;
-        bool close = false;
-        // (a group without an expert left is out: behind all others, and its experts have no key)
-        compare_rotated<1>(score, 4.f * (err + 1.25e-7f * __builtin_fmaxf(largest, -lo)), lanes, ahead, close);
-        unsure |= (close || (score == ninf && first != ninf)) && l < a.groups * lanes;   // (the sum's overflow)
-        if (ahead >= a.topk_groups) {
+        int sure = 0, maybe = 0;
+        compare_rotated<1>(score, 4.f * (err + 1.25e-7f * __builtin_fmaxf(largest, -lo)), lanes, sure, maybe);
+        // (a sum that overflowed says nothing)
+        unsure |= (sure < a.topk_groups ? maybe >= a.topk_groups : false) || (score == ninf && first != ninf);
+        if (sure >= a.topk_groups) {
 #pragma unroll
           for (int i = 0; i < PER; i++) choice[i] = ninf;
         }
       }
-      if (far) {   // (what lies far below the largest is hardly taken: it gets one key, and is close to its like)
+      if (__builtin_expect(far, 0)) {   // (what lies far below the largest is hardly taken: it gets one key, and is close to its like)
         lo = __builtin_fmaxf(lo, largest - 64.f);
 #pragma unroll
         for (int i = 0; i < PER; i++) choice[i] = choice[i] == ninf ? ninf : __builtin_fmaxf(choice[i], lo);
@@ -455,8 +468,8 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
   }
   int mine = -1;   // lane j of a token: the j-th expert
   uint32_t before = 0;   // (as if 2^32: every key is below)
-  bool left = true;
-  for (int j = 0; j < a.topk + (whole ? 0 : 1); j++) {   // (one more than are taken: how close it came)
+  bool left = true, close = false;
+  auto next = [&]() {   // the largest key below the last one, if there is one; whether it is close to that
     uint32_t d = key[0] - before;
 #pragma unroll
     for (int i = 1; i < PER; i++) {
@@ -466,10 +479,31 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
     d = row_reduce(d, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
     const uint32_t max = left ? before + d : 0;
     left = max >= 256u;
-    if (l == j && j < a.topk && left) mine = 255 - (int)(max & 255u);
-    if (!whole && j > 0) unsure |= left && (before >> 8) - (max >> 8) <= near;
+    const bool by = left && (before >> 8) - (max >> 8) <= near;
     before = max;
+    return by;
+  };
+  for (int j = 0; j < a.topk + (whole ? 0 : 1); j++) {   // (one more than are taken: how close it came)
+    const bool by = next();
+    if (l == j && left) mine = 255 - (int)(before & 255u);
+    close |= !whole && j > 0 && by;
   }
+  if (__builtin_expect(__ballot(close) != 0, 0)) {
+    // The taken ones and the one behind them in their order, a lane each, if there is no doubt that they are the first (softmax scores hang
+    // on all experts: they are left to gate_token).
+    unsure |= close && (next() || a.topk > 15 || (a.exact && !a.sigmoid));
+    uint32_t exact = 0;
+    int id = 256 + l;
+    if (mine >= 0) {
+      id = mine;
+      const float c = gate_load(row + id);
+      exact = order_key(a.exact ? (float)(1.0 / (1.0 + exp(-(double)c)) + (bias ? (double)bias[id] : 0.0)) : c);
+    }
+    const int to = order_rotated<1>(exact, id);
+    const int sorted = __builtin_amdgcn_ds_permute(((lane & 48) + to) * 4, mine);
+    if (close) mine = sorted;
+  }
+  if (l >= a.topk) mine = -1;
   // the weights, a lane per place
   const bool real = mine >= 0;
   const float xs = real ? gate_load(row + mine) : ninf;
@@ -488,6 +522,7 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
     ids[t * a.topk + l] = mine;
     weights[t * a.topk + l] = real ? v * a.scale : 0.f;
   }
+  if (__builtin_expect(again == 0, 1)) return;
   for (int r = 0; r < 4; r++)
     if (t0 + r < a.tokens && (again >> (16 * r) & 0xffff))
       gate_token<T, kTokenPer>(logits + (t0 + r) * ld, bias, a, s_key[w], ids + (t0 + r) * a.topk, weights + (t0 + r) * a.topk);
