@@ -227,3 +227,29 @@ def test_a_token_is_the_same_in_any_batch(esmoe, scoring, groups):
         assert torch.equal(one[0][0], ids[t]) and torch.equal(one[1][0], w[t])
     back = esmoe.es_topk_gating(x.flip(0), 8, b, scoring, True, 2.5, groups, min(groups, 4))
     assert torch.equal(back[0].flip(0), ids) and torch.equal(back[1].flip(0), w)
+
+
+@pytest.mark.parametrize("scoring,biased", [("softmax", False), ("sigmoid", True), ("softmax", True)])
+@pytest.mark.parametrize("groups,topk", [(1, 8), (8, 8), (1, 16), (4, 3)])
+@pytest.mark.parametrize("experts", [64, 128, 256])
+def test_close_calls(esmoe, scoring, biased, groups, topk, experts):
+    """Logits a few units of the last place apart, in runs of neighbours and between groups: the order is the one of 64 bits."""
+    gen = torch.Generator().manual_seed(experts + topk)
+    t, inf = 4099, float("inf")
+    x = torch.randint(-6, 7, (t, experts), generator=gen) / 2 + torch.randint(-3, 4, (t, experts), generator=gen) * 1.5 * 2.0 ** -22
+    x[::3] = 2 * torch.randn((len(x[::3]), experts), generator=gen)
+    x = x.cuda()
+    b = (torch.randint(0, 2, (experts,), generator=gen) / 4 + torch.randint(0, 3, (experts,), generator=gen) * 2.0 ** -23).cuda() if biased else None
+    keep = max(1, groups // 2)
+    ids, _ = esmoe.es_topk_gating(x, topk, b, scoring, True, 1.0, groups, keep)
+    xd = x.double()
+    s = torch.softmax(xd, 1) if scoring == "softmax" else torch.sigmoid(xd)
+    choice = x if groups == 1 and b is None else (s if b is None else s + b.double()).float()
+    if groups > 1:
+        g = choice.view(t, groups, -1)
+        score = g.topk(2, dim=2).values.sum(2)
+        kept = torch.sort(score, dim=1, descending=True, stable=True).indices[:, :keep]
+        out = torch.ones_like(score, dtype=torch.bool).scatter_(1, kept, False)
+        choice = g.masked_fill(out.unsqueeze(2), -inf).view(t, experts)
+    want = torch.sort(choice, dim=1, descending=True, stable=True).indices[:, :topk]
+    assert torch.equal(ids.long(), want)
