@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
         if (lanes > 4) join(other(first, std::integral_constant<int, 0x141>()), other(second, std::integral_constant<int, 0x141>()));
         const float score = first == ninf ? ninf : first + (second == ninf ? 0.f : second);
         int sure = 0, maybe = 0;
-        compare_rotated<1>(score, 4.f * (err + 1.25e-7f * __builtin_fmaxf(largest, -lo)), lanes, sure, maybe);
+        // (two scores of two choices each; a sum, of up to twice the largest, is rounded on either side too: half of the 2.5e-7)
+        compare_rotated<1>(score, 4.f * (err + 2.5e-7f * __builtin_fmaxf(largest, -lo)), lanes, sure, maybe);
         // (a sum that overflowed says nothing)
         unsure |= (sure < a.topk_groups ? maybe >= a.topk_groups : false) || (score == ninf && first != ninf);
         if (sure >= a.topk_groups) {
