@@ -336,8 +336,8 @@ mxfp4_stream_kernel(Fp4Args p) {
     };
     // (descriptors of a tile's bytes: a lane's place in them is all that the loads take from vector registers, and a dword past the
     // tile's scales reads as 0)
-    auto load = [&](int q, int h, int st) {   // pair q of the wavefront's range
-      const auto src = tile_bytes(bw + first_row(h, st) * kb, (int)(16 * kb) - p0 * 128);
+    auto load = [&](int q, int h, int st, bool some) {   // pair q of the wavefront's range; none: zeros, without a read
+      const auto src = tile_bytes(bw + first_row(h, st) * kb, some ? (int)(16 * kb) - p0 * 128 : 0);
 #pragma unroll
       for (int r = 0; r < 2; r++) wt[h][2 * q + r] = __builtin_amdgcn_raw_buffer_load_b128(src, wlane[q], r * 8 * (int)kb, 0);
     };
@@ -360,7 +360,7 @@ mxfp4_stream_kernel(Fp4Args p) {
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int q = 0; q < PAIRS; q++) load(q, h, step);
+      for (int q = 0; q < PAIRS; q++) load(q, h, step, true);
     __builtin_amdgcn_sched_barrier(0);   // (ahead of the rows of `a`, which come from a cache)
     v4i x[kChunks][4];
     {
@@ -401,7 +401,8 @@ mxfp4_stream_kernel(Fp4Args p) {
     store_scales(buf);
     lds_barrier();
     for (; step < last; step++) {
-      const int next = step + 1 < last ? step + 1 : step;   // (the last step's loads are its own again: nothing waits for them)
+      // (the last step's loads are empty: 3 % where a workgroup has four steps, 8 experts x 4096 x 7168 31.2 / 30.2 us)
+      const int next = step + 1 < last ? step + 1 : step;
       load_scales(next);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -425,7 +426,7 @@ mxfp4_stream_kernel(Fp4Args p) {
             for (int j = 2 * q; j < 2 * q + 2; j++)
               sum[j & 1] = mfma32<FP16>(x[j][i], fp4_values<FP16>((uint32_t)wt[h][j][i], __builtin_bit_cast(float, code[j] << 23)), sum[j & 1]);
           __builtin_amdgcn_sched_barrier(0);   // (a pair's registers are loaded again as soon as it is used up)
-          load(q, h, next);
+          load(q, h, next, step + 1 < last);
         }
         const v4f acc = sum[0] + sum[1];
         *(v4f*)&s_part[((buf * 2 + h) * waves + w) * 256 + lane * 4] = acc;
