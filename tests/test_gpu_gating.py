@@ -253,3 +253,16 @@ def test_close_calls(esmoe, scoring, biased, groups, topk, experts):
         choice = g.masked_fill(out.unsqueeze(2), -inf).view(t, experts)
     want = torch.sort(choice, dim=1, descending=True, stable=True).indices[:, :topk]
     assert torch.equal(ids.long(), want)
+
+
+def test_a_slice_as_bias_and_one_row_for_all(esmoe):
+    x = _logits(9, 256, torch.float32, 3)
+    b = 0.1 * torch.randn(257, generator=torch.Generator().manual_seed(4))
+    _check(esmoe, x, 8, b[1:], "sigmoid", True, groups=8, topk_groups=3)
+    same = x[:1].cuda().expand(6, 256)
+    ids, w = esmoe.es_topk_gating(same, 8, b.cuda()[1:], "sigmoid", True, 1.0, 8, 3)
+    one = esmoe.es_topk_gating(same[:1], 8, b.cuda()[1:], "sigmoid", True, 1.0, 8, 3)
+    assert (ids == one[0]).all() and (w == one[1]).all()
+    g = torch.ones_like(w)
+    d = esmoe.es_topk_gating_backward(g, same, ids, "softmax", False)
+    assert (d == d[:1]).all() and d.shape == (6, 256)
