@@ -103,8 +103,7 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(const uint16_t* __res
 
 // One wavefront per pair; the four of a workgroup are mostly a token's, whose gradient row comes from HBM once and then from a cache.
 // A workgroup per token that took its pairs one after the other was the same speed for many long rows, but three times as long for few
-// tokens (one token x top-8 x 7168: 10.7 us, as it is 4.5; 16384 tokens
-// x top-8 x 512 95 / 51).
+// tokens (one token x top-8 x 7168: 10.7 us, as it is 4.5; 16384 tokens x top-8 x 512 95 / 51).  All of a token's pairs on one XCD: no change.
 template <bool FP16, bool STREAM>
 __global__ void __launch_bounds__(256) combine_rows_backward_kernel(const uint16_t* __restrict__ grad_out, const uint16_t* __restrict__ in,
                                                                     const int* __restrict__ dst_row, const float* __restrict__ weights,

@@ -320,12 +320,13 @@ __device__ __forceinline__ int order_rotated(uint32_t key, int id) {
 // and below them 255 - expert, and a largest one stands for itself and its place.  The largest key below the one before is
 //   before + max over keys of (key - before mod 2^32),
 // a subtraction per key and no removal: what is not below `before` wraps to the small side.
-// 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number from the token's smallest choice (or 64 below
-// the largest) on, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from the 64-bit
-// ones by less than `slack`.  Where two neighbours of the order are too close to tell, the candidates alone are put in order by their
-// exact choices; where the last of them and the next, or two groups' scores are, the wavefront does the token again by gate_token.
-// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 13.3 (11.6 where none
-// is done again), one 6.3 / 4.6; softmax over 128 experts, bf16, 16384 tokens 11.2 / 4.8.  The code of what is rare stands behind the rest: .5 of these us.
+// 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number from the token's smallest choice
+// (or 64 below the largest) on, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from
+// the 64-bit ones by less than `slack`.  Where two neighbours of the order are too close to tell, the candidates alone are put in order by
+// their exact choices; where the last of them and the next, or two groups' scores are, the wavefront does the token again by gate_token.
+// us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 13.3 (11.6 where none is done
+// again), one 6.3 / 4.6; softmax over 128 experts, bf16, 16384 tokens 11.2 / 4.8.  The code of what is rare stands behind the rest: .5 of
+// these us.
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const T* __restrict__ logits, long ld,
                                                                            const float* __restrict__ bias, GateArgs a, int* __restrict__ ids,

@@ -133,8 +133,8 @@ template <bool FP16, bool STREAM>
 static int launch_norm(const void* in, const void* residual, const void* weight, float eps, long rows, int hidden, void* residual_out,
                        void* normed, void* q, float* scales, hipStream_t stream) {
   // Threads per row: a wavefront where a row is short enough to be its registers' (no barrier, more rows in flight); sixteen wavefronts
-  // where there is at most a row per CU (what counts is how long one takes); four else.  us, always four / as chosen: 8 rows x 7168 4.5 / 3.45, 256 x 7168
-  // 5.8 / 4.9, 16384 x 256 12.0 / 10.1, 65536 x 512 63.9 / 49.9, 16384 x 1024 24.6 / 23.5.
+  // where there is at most a row per CU (what counts is how long one takes); four else.  us, always four / as chosen: 8 rows x 7168 4.5 /
+  // 3.45, 256 x 7168 5.8 / 4.9, 16384 x 256 12.0 / 10.1, 65536 x 512 63.9 / 49.9, 16384 x 1024 24.6 / 23.5.
   const int threads = rows <= 256 && hidden > 1024 ? 1024 : hidden <= 1024 ? 64 : 256;
   const int chunks = (hidden + threads * 8 - 1) / (threads * 8);
   const long step = 1L << 22;
