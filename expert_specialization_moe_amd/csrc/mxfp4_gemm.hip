@@ -14,6 +14,7 @@
 #include <stdint.h>
 #include <type_traits>
 
+#include "mxfp4_units.h"
 #include "swiglu.h"
 #include "wave_scan.h"
 
@@ -27,7 +28,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
-constexpr int kFp4Rows = 16, kLongWaves = 8;
+constexpr int kLongWaves = 8;
 
 // Eight weights of a dword as values of the activations' type.
 template <bool FP16>
@@ -89,14 +90,10 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-struct Fp4Unit {
-  int expert, row0, rows;   // rows 0: no such unit
-};
-
-// The units of a launch: experts in order, each in tiles of ROWS rows; a lane per expert, 64 at a time.  Rows are clamped to the tensor.
-template <int ROWS>
+// The units of a launch: experts in order, each in tiles of sixteen rows; a lane per expert, 64 at a time.
 struct Fp4Units {
-  int m, off, tiles, end;   // of the lane's expert; end: units up to and with it, from the 64's first on
+  int m, off;
+  uint32_t end;   // units up to and with the lane's expert, from the 64's first on
   __device__ __forceinline__ void read(int e0, const int* __restrict__ problem_sizes, const int* __restrict__ expert_offsets, int num_experts,
                                        int total_rows) {
     const int e = e0 + (threadIdx.x & 63);
@@ -105,16 +102,14 @@ struct Fp4Units {
       m = problem_sizes[e * 3];
       off = expert_offsets[e];
     }
-    m = off < 0 || off >= total_rows || m < 0 ? 0 : m > total_rows - off ? total_rows - off : m;
-    tiles = (m + ROWS - 1) / ROWS;
-    end = wave_inclusive_sum(tiles);
+    m = fp4_rows(m, off, total_rows);
+    end = wave_inclusive_sum_or_most(fp4_tiles(m));
   }
-  __device__ __forceinline__ int count() const { return __builtin_amdgcn_readlane(end, 63); }
-  __device__ __forceinline__ Fp4Unit unit(int e0, int u) const {   // u < count()
+  __device__ __forceinline__ uint32_t count() const { return (uint32_t)__builtin_amdgcn_readlane((int)end, 63); }
+  __device__ __forceinline__ Fp4Unit unit(int e0, uint32_t u) const {   // u < count()
     const int l = __builtin_ctzll(__ballot(end > u));
-    const int tile = u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(tiles, l));
-    const int rows = __builtin_amdgcn_readlane(m, l) - tile * ROWS;
-    return {e0 + l, __builtin_amdgcn_readlane(off, l) + tile * ROWS, rows < ROWS ? rows : ROWS};
+    const uint32_t start = l ? (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1) : 0u;
+    return fp4_unit(e0 + l, __builtin_amdgcn_readlane(off, l), __builtin_amdgcn_readlane(m, l), u, start);
   }
 };
 
@@ -133,8 +128,9 @@ __global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint1
   const int l16 = lane & 15, lr = lane >> 4;
   const int unit = blockIdx.x / col_tiles, col0 = (blockIdx.x - unit * col_tiles) * kCols;
   Fp4Unit g = {0, 0, 0};
-  for (int e0 = 0, u = unit0 + unit; e0 < num_experts; e0 += 64) {
-    Fp4Units<kFp4Rows> some;
+  uint32_t u = unit0 + unit;
+  for (int e0 = 0; e0 < num_experts; e0 += 64) {
+    Fp4Units some;
     some.read(e0, problem_sizes, expert_offsets, num_experts, total_rows);
     if (u < some.count()) {
       g = some.unit(e0, u);
@@ -224,6 +220,7 @@ struct Fp4Args {
   const uint8_t *b, *sf;
   const int *problem_sizes, *expert_offsets;
   int num_experts, total_rows, n, k;
+  uint32_t most_units;
   uint16_t* out;
 };
 
@@ -286,16 +283,17 @@ mxfp4_stream_kernel(Fp4Args p) {
   const long kb = p.k / 2, ks = p.k / 32;
   const int p0 = pairs * w / waves, c0 = 2 * p0;
   const int count = 2 * (pairs * (w + 1) / waves) < chunks ? 2 * (pairs * (w + 1) / waves) - c0 : chunks - c0;   // (1 .. kChunks)
-  Fp4Units<kFp4Rows> some;
+  Fp4Units some;
   some.read(0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
-  int units = some.count();
+  uint32_t units = some.count();
   for (int e0 = 64; e0 < p.num_experts; e0 += 64) {
-    Fp4Units<kFp4Rows> more;
+    Fp4Units more;
     more.read(e0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
-    units += more.count();
+    units = sum_or_most(units, more.count());
   }
-  // (the launch sees to it that the steps of all units are fewer than 2^31)
-  const uint32_t total = (uint32_t)units * steps, share = total / gridDim.x, rest = total % gridDim.x;
+  // (more where experts claim the same rows; the launch sees to it that the steps of these are fewer than 2^31)
+  units = units < p.most_units ? units : p.most_units;
+  const uint32_t total = units * steps, share = total / gridDim.x, rest = total % gridDim.x;
   uint32_t at = blockIdx.x * share + (blockIdx.x < rest ? blockIdx.x : rest);
   const uint32_t end = at + share + (blockIdx.x < rest ? 1 : 0);
   // The lane's place in the wavefront's bytes of eight weight rows: row l16 % 8, half l16 / 8 of a pair's line (a pair that ends a row of
@@ -314,18 +312,19 @@ mxfp4_stream_kernel(Fp4Args p) {
     splace[i] = row < 16 ? (at - row * chunks) * 16 + row : -1;
   }
   if (tid < 2) s_far[tid] = 0;   // (before the first step's barrier)
-  int e0 = 0, before = 0;   // `some` holds the experts from e0 on, whose units are those from `before` on
+  int e0 = 0;
+  uint32_t before = 0;   // `some` holds the experts from e0 on, whose units are those from `before` on
   int buf = 0;
   while (at < end) {
     const uint32_t unit = at / steps;
     int step = (int)(at - unit * steps);
     const int last = end - unit * steps < (uint32_t)steps ? (int)(end - unit * steps) : steps;
-    while ((int)unit >= before + some.count()) {
+    while (unit >= sum_or_most(before, some.count())) {   // (ends: unit is less than all counts together)
       before += some.count();
       e0 += 64;
       some.read(e0, p.problem_sizes, p.expert_offsets, p.num_experts, p.total_rows);
     }
-    const Fp4Unit g = some.unit(e0, (int)unit - before);
+    const Fp4Unit g = some.unit(e0, unit - before);
     const uint8_t* bw = p.b + (long)g.expert * p.n * kb + p0 * 128;
     const uint8_t* sw = p.sf + (long)g.expert * p.n * ks;
     v4i wt[2][kChunks];
@@ -462,9 +461,7 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
                                              int cus, hipStream_t stream) {
   using namespace esmoe;
   const int steps = swiglu ? n / 32 : (n / 16 + 1) / 2, chunks = k / 128, pairs = (chunks + 1) / 2;
-  // units with rows: at most one per expert or row, and one more per full tile
-  const long experts = num_experts < total_rows ? num_experts : total_rows;
-  const long most = (experts + (long)total_rows / kFp4Rows) * steps;
+  const long units = fp4_most_units(num_experts, total_rows), most = units * steps;
   if (pairs <= kFp4MaxPairs * kFp4MaxWaves && most < 1L << 31) {
     // As many wavefronts as a workgroup has, each with as little of K as that takes.  us, as few wavefronts as K takes / this:
     // 32 experts x 7168 x K 2048, a row each 49.2 / 46.3, eight rows 55.8 / 52.0; 8 experts, 64 rows each 44 / 37; 64 experts x 1536 x
@@ -472,7 +469,7 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
     const int each = (pairs + kFp4MaxWaves - 1) / kFp4MaxWaves;
     const int waves = (pairs + each - 1) / each, per_cu = fp4_waves(each) / waves;
     const unsigned grid = (unsigned)(most < (long)cus * per_cu ? most : (long)cus * per_cu);
-    const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint16_t*)out};
+    const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint32_t)units, (uint16_t*)out};
 #define ESMOE_FP4(P)                                                                                                               \
   do {                                                                                                                             \
     auto kernel = dtype ? swiglu ? mxfp4_stream_kernel<true, true, P> : mxfp4_stream_kernel<true, false, P>                        \
@@ -486,7 +483,6 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
 #undef ESMOE_FP4
     return (int)hipGetLastError();
   }
-  const long units = experts + (long)total_rows / kFp4Rows;
   const int cols = swiglu ? 16 : 32, col_tiles = ((swiglu ? n / 2 : n) + cols - 1) / cols;
   const long step = (1L << 22) / col_tiles > 1 ? (1L << 22) / col_tiles : 1;   // units of a launch: a grid holds fewer than 2^32 threads
   auto kernel = dtype ? swiglu ? mxfp4_long_kernel<true, true> : mxfp4_long_kernel<true, false>

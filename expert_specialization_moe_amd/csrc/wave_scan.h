@@ -1,6 +1,7 @@
 // Prefix sum over a wavefront, on the vector ALU alone.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 namespace esmoe {
 
@@ -13,6 +14,18 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// The same where a sum of more than 32 bits stays at the largest number.
+__device__ __forceinline__ uint32_t wave_inclusive_sum_or_most(uint32_t v) {
+  auto step = [&](int below) { v = __builtin_elementwise_add_sat(v, (uint32_t)below); };
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
   return v;
 }
 

@@ -339,8 +339,9 @@ int esmoe_add_rms_norm_quant_1x128(const void* in, int in_dtype, const void* res
  *   out [total_rows, n] ([total_rows, inter] with SwiGLU) and a [total_rows, k], both bf16 or fp16 (dtype)
  *   b [E, n, k/2] bytes, two e2m1 codes each, the even column in the low half;  sfb [E, n, k/32] E8M0 bytes, row-major (not swizzled)
  * k % 128 == 0, k <= 32768; n % 16 == 0 (% 32 with SwiGLU); problem_sizes and expert_offsets as above, column 0 is used.  Rows of out
- * that belong to no expert are not written.  Any number of rows is right; from some dozen per expert on the 8-bit GEMMs are the
- * faster ones.  No counterpart in the reference.
+ * that belong to no expert are not written.  Counts and offsets are cut at total_rows; where experts claim the same rows, whose
+ * product these get is open, and of more claims than experts and sixteens of rows the last may not be served.  Any number of
+ * rows is right; from some dozen per expert on the 8-bit GEMMs are the faster ones.  No counterpart in the reference.
  */
 int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, const uint8_t* sfb, const int32_t* problem_sizes,
                            const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream);
