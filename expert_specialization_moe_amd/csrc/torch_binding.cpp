@@ -11,6 +11,7 @@
 // machine without a GPU; after the checks pass a CPU call fails loudly, there is
 // no CPU implementation of the ops.
 #include <Python.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/all.h>
 
@@ -515,10 +516,15 @@ void es_mxfp8_quant_weight(const torch::Tensor& input, torch::Tensor& quant_outp
 namespace {
 
 // These operators are not part of autograd: where a gradient exists it is an operator of its own, and a result that silently had
-// none would train nothing.
-void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor*> tensors) {
+// none would train nothing.  In forward mode, which no_grad leaves on, there is none at all: no result has a tangent, and an output
+// would keep one of what it held before.
+void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor*> inputs, std::initializer_list<const torch::Tensor*> outputs = {}) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const auto& tensors : {inputs, outputs})
+      for (const torch::Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, ": not differentiable, a tensor with a tangent is refused");
   if (!at::GradMode::is_enabled()) return;
-  for (const torch::Tensor* t : tensors)
+  for (const torch::Tensor* t : inputs)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), op,
                 ": not differentiable by autograd (call it under torch.no_grad(); gradients are operators of their own)");
 }
@@ -634,7 +640,7 @@ void es_combine_rows(const torch::Tensor& input, const torch::Tensor& dst_row, i
   TORCH_CHECK(output.dim() == 2 && output.is_contiguous() && output.scalar_type() == input.scalar_type() && output.size(0) == tokens &&
                   output.size(1) == input.size(1),
               "output must be a contiguous (tokens, row length) tensor of input's dtype");
-  check_no_autograd("es_combine_rows", {&input, &weights});
+  check_no_autograd("es_combine_rows", {&input, &weights}, {&output});
   require_device(input, "es_combine_rows");
   check_device(input, {&dst_row, &weights, &output});
   TORCH_CHECK(!any_overlap(output, {&input, &dst_row, &weights}), "output may not overlap input, dst_row or weights");
@@ -665,7 +671,7 @@ void es_combine_rows_backward(const torch::Tensor& grad_output, const torch::Ten
               "grad_input must be a contiguous tensor of input's shape and dtype");
   TORCH_CHECK(grad_weights.scalar_type() == torch::kFloat32 && grad_weights.is_contiguous() && grad_weights.numel() == dst_row.numel(),
               "grad_weights must be a contiguous float32 tensor of dst_row's size");
-  check_no_autograd("es_combine_rows_backward", {&grad_output, &input, &weights});
+  check_no_autograd("es_combine_rows_backward", {&grad_output, &input, &weights}, {&grad_input, &grad_weights});
   require_device(input, "es_combine_rows_backward");
   check_device(input, {&grad_output, &dst_row, &weights, &grad_input, &grad_weights});
   TORCH_CHECK(!any_overlap(grad_input, {&input, &grad_output, &dst_row, &weights, &grad_weights}) &&
@@ -699,7 +705,7 @@ void es_add_rms_norm_quant_1x128(const torch::Tensor& input, const torch::Tensor
               "quant_output must be a contiguous 1-byte tensor of rows * k elements");
   TORCH_CHECK(scales.is_contiguous() && scales.scalar_type() == torch::kFloat32 && scales.numel() == rows * (k / 128),
               "scales must be a contiguous float32 tensor of rows * k / 128 elements");
-  check_no_autograd("es_add_rms_norm_quant_1x128", {&input, &weight, &residual});
+  check_no_autograd("es_add_rms_norm_quant_1x128", {&input, &weight, &residual}, {&residual_out, &normed, &quant_output, &scales});
   require_device(input, "es_add_rms_norm_quant_1x128");
   check_device(input, {&weight, &residual, &residual_out, &normed, &quant_output, &scales});
   if (rows == 0) return;
@@ -757,7 +763,7 @@ void mxfp4_grouped_mm(const char* op, bool swiglu, torch::Tensor& output, const 
                   output.size(1) == (swiglu ? n / 2 : n),
               "output must be a contiguous (rows, n) tensor, (rows, n / 2) with SwiGLU, of a's dtype");
   TORCH_CHECK(total_rows < (int64_t(1) << 31), "tensor too large");
-  check_no_autograd(op, {&a});
+  check_no_autograd(op, {&a}, {&output});
   require_device(a, op);
   check_device(a, {&output, &b, &sfb, &problem_sizes, &expert_offsets});
   TORCH_CHECK(problem_sizes.is_contiguous() && expert_offsets.is_contiguous(), "metadata tensors must be contiguous");
