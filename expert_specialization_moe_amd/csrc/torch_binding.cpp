@@ -527,6 +527,8 @@ void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor
   for (const torch::Tensor* t : inputs)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), op,
                 ": not differentiable by autograd (call it under torch.no_grad(); gradients are operators of their own)");
+  for (const torch::Tensor* t : outputs)   // (what a graph has recorded of it would be overwritten)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), op, ": output that requires a gradient (write to it under torch.no_grad())");
 }
 
 void check_device(const torch::Tensor& like, std::initializer_list<const torch::Tensor*> tensors) {

@@ -51,3 +51,18 @@ def test_tangents_are_refused(esmoe, name):
                 call(**args)
             with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
                 call(**args)
+
+
+@pytest.mark.parametrize("name", ["combine", "combine_backward", "norm", "mxfp4", "mxfp4_swiglu"])
+def test_outputs_that_require_a_gradient_are_refused(esmoe, name):
+    """A buffer of a graph that is overwritten would give that graph's backward pass other values, or none."""
+    call, inputs, outputs = _calls(esmoe)[name]
+    for which in outputs:
+        leaf = outputs[which].clone().requires_grad_()
+        for buffer in (leaf, leaf * 2):
+            args = dict(inputs, **outputs)
+            args[which] = buffer
+            with pytest.raises(RuntimeError, match="output that requires a gradient"):
+                call(**args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU implementation"):
+                call(**args)
