@@ -41,6 +41,8 @@ __device__ __forceinline__ uint32_t dpp_umax16(uint32_t v) {
 }
 
 // A row's values stay in registers: CHUNKS times eight per thread, THREADS threads per row; with 64 (a wavefront) four rows per workgroup.
+// The squares of 512 columns, a wavefront's chunk, are summed for themselves and then one after the other by column: the same order for
+// any number of threads, so a row's bytes do not hang on how many rows a call has.
 // Nothing is read twice: all stores are non-temporal, or, where a call's tensors are more than the memory-side cache holds (STREAM), the loads and
 // all stores but the bytes'.  us, no hints / stores / STREAM: 16384 x 7168 179 / 174 / 162, 65536 x 512 54.6 / 51.6 / 48.8, 1024 x 4096
 // 8.2 / 6.9 / 8.1, 16384 x 1024 30.0 / 23.2 / 26.5.
@@ -49,16 +51,17 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_qu
                                                                           const uint16_t* __restrict__ weight, float eps, long rows, int hidden,
                                                                           uint16_t* residual_out, uint16_t* __restrict__ normed,
                                                                           uint8_t* __restrict__ q, float* __restrict__ scales) {
-  __shared__ float s_sum[THREADS / 64];
+  constexpr int kWaves = THREADS / 64;
+  __shared__ float s_sum[kWaves * CHUNKS];   // by column
   const int tid = THREADS < 256 ? threadIdx.x % THREADS : threadIdx.x;
   const long number = THREADS < 256 ? (long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS : blockIdx.x;
   if (number >= rows) return;   // (a whole wavefront, and no barrier where there are several rows)
   const long row = number * hidden;
-  float h[CHUNKS][8];
-  float sum = 0;
+  float h[CHUNKS][8], part[CHUNKS];
 #pragma unroll
   for (int u = 0; u < CHUNKS; u++) {
     const int col = (u * THREADS + tid) * 8;
+    part[u] = 0;
     if (col < hidden) {
       const v4i a = load8<STREAM>(in + row + col);
       v4i r = {0, 0, 0, 0};
@@ -76,21 +79,28 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_qu
         }
         h[u][2 * i] = lo;
         h[u][2 * i + 1] = hi;
-        sum = __builtin_fmaf(lo, lo, sum);
-        sum = __builtin_fmaf(hi, hi, sum);
+        part[u] = __builtin_fmaf(lo, lo, part[u]);
+        part[u] = __builtin_fmaf(hi, hi, part[u]);
       }
       if (residual) __builtin_nontemporal_store(o, (v4i*)(residual_out + row + col));
     }
   }
-  sum = wave_sum_last(sum);
+#pragma unroll
+  for (int u = 0; u < CHUNKS; u++) part[u] = wave_sum_last(part[u]);
+  float sum;
   if constexpr (THREADS == 64) {
-    sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
+    sum = 0;
+#pragma unroll
+    for (int u = 0; u < CHUNKS; u++) sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, part[u]), 63));
   } else {
-    if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
+    if ((tid & 63) == 63) {
+#pragma unroll
+      for (int u = 0; u < CHUNKS; u++) s_sum[u * kWaves + (tid >> 6)] = part[u];
+    }
     __syncthreads();
     sum = s_sum[0];
 #pragma unroll
-    for (int i = 1; i < THREADS / 64; i++) sum += s_sum[i];
+    for (int i = 1; i < kWaves * CHUNKS; i++) sum += s_sum[i];   // (0 past the row's end)
   }
   const float rstd = 1.0f / sqrtf(sum / (float)hidden + eps);
 #pragma unroll
