@@ -323,7 +323,9 @@ __device__ __forceinline__ int order_rotated(uint32_t key, int id) {
 // 24 bits hold the order key of a bf16 or fp16 logit whole.  Anything else becomes a fixed-point number from the token's smallest choice
 // (or 64 below the largest) on, and has a bound on its error: the choices that groups and a bias decide about are formed in fp32, off from
 // the 64-bit ones by less than `slack`.  Where two neighbours of the order are too close to tell, the candidates alone are put in order by
-// their exact choices; where the last of them and the next, or two groups' scores are, the wavefront does the token again by gate_token.
+// their exact choices, unless they are the same logit and bias; where the last of them and the next, or two groups' scores are, the wavefront
+// does the token again by gate_token.  Equal logits are the rule in 16 bits: bf16 softmax, 256 experts, 4 of 8 groups, every near pair to
+// gate_token / this: 16384 tokens 32.5 / 14.9 us, 2048 23.3 / 10.3, 256 19.0 / 5.7.
 // us for 256 experts, top-8, sigmoid and bias, 4 of 8 groups, a wavefront per token / this: 16384 tokens 29.9 / 13.3 (11.6 where none is done
 // again), one 6.3 / 4.6; softmax over 128 experts, bf16, 16384 tokens 11.2 / 4.8.  The code of what is rare stands behind the rest: .5 of
 // these us.
@@ -468,10 +470,10 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
       key[i] = (q << 8) + (place - i);
     }
   }
-  int mine = -1;   // lane j of a token: the j-th expert
+  uint32_t place_key = 0;   // lane j of a token: the key of its place j
   uint32_t before = 0;   // (as if 2^32: every key is below)
   bool left = true, close = false;
-  auto next = [&]() {   // the largest key below the last one, if there is one; whether it is close to that
+  auto next = [&]() {   // the largest key below the last one, if there is one; whether it is near that
     uint32_t d = key[0] - before;
 #pragma unroll
     for (int i = 1; i < PER; i++) {
@@ -482,28 +484,54 @@ __global__ void __launch_bounds__(64 * kGateWaves) topk_gating_rows_kernel(const
     const uint32_t max = left ? before + d : 0;
     left = max >= 256u;
     const bool by = left && (before >> 8) - (max >> 8) <= near;
-    before = max;
+    before = left ? max : 0;
     return by;
   };
   for (int j = 0; j < a.topk + (whole ? 0 : 1); j++) {   // (one more than are taken: how close it came)
     const bool by = next();
-    if (l == j && left) mine = 255 - (int)(before & 255u);
+    if (l == j) place_key = before;
     close |= !whole && j > 0 && by;
   }
+  int mine = place_key ? 255 - (int)(place_key & 255u) : -1;   // lane j: the j-th expert
   if (__builtin_expect(__ballot(close) != 0, 0)) {
-    // The taken ones and the one behind them in their order, a lane each, if there is no doubt that they are the first (softmax scores hang
-    // on all experts: they are left to gate_token).
-    unsure |= close && (next() || a.topk > 15 || (a.exact && !a.sigmoid));
-    uint32_t exact = 0;
-    int id = 256 + l;
-    if (mine >= 0) {
-      id = mine;
-      const float c = gate_load(row + id);
-      exact = order_key(a.exact ? (float)(1.0 / (1.0 + exp(-(double)c)) + (bias ? (double)bias[id] : 0.0)) : c);
+    // Experts of one logit and one bias have one choice and go by their index, as their keys do; other neighbours that are near are in doubt.
+    struct Expert { float x, b; };
+    auto same = [](Expert u, Expert v) { return u.x == v.x && u.b == v.b; };
+    auto expert = [&](bool is, int e) { return is ? Expert{gate_load(row + e), bias ? bias[e] : 0.f} : Expert{ninf, 0.f}; };
+    auto lane_behind = [](auto v) {   // row_shl:1
+      return __builtin_bit_cast(decltype(v), __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x101, 0xf, 0xf, true));
+    };
+    const Expert own = expert(mine >= 0, mine), spare = expert(left, 255 - (int)(before & 255u));   // (spare: the first that is not taken)
+    Expert behind = {lane_behind(own.x), lane_behind(own.b)};
+    uint32_t key_behind = lane_behind(place_key);
+    if (l == a.topk - 1) {
+      behind = spare;
+      key_behind = before;
     }
-    const int to = order_rotated<1>(exact, id);
-    const int sorted = __builtin_amdgcn_ds_permute(((lane & 48) + to) * 4, mine);
-    if (close) mine = sorted;
+    const bool near_next = l < a.topk && key_behind != 0 && (place_key >> 8) - (key_behind >> 8) <= near;
+    const uint32_t doubts = (uint32_t)(__ballot(near_next && !same(own, behind)) >> (lane & 48)) & 0xffffu;
+    const bool cut = (__ballot(near_next) >> (lane & 48)) >> (a.topk - 1) & 1;   // the spare one is near the last place
+    if (__ballot(cut)) {
+      // What is near the spare one has to be the same, and nothing else may be in doubt; of one more nothing is known.
+      const bool second = next();
+      const Expert e = expert(second, 255 - (int)(before & 255u));
+      const bool third = next();
+      unsure |= cut && second && (third || doubts || !same(e, spare));
+      unsure |= cut && doubts && a.topk > 15;   // (no lane for the spare one)
+    }
+    if (__ballot(doubts != 0)) {
+      // The taken ones and the spare one by their exact choices, a lane each (softmax scores hang on all experts: they are left to gate_token).
+      unsure |= doubts && a.exact && !a.sigmoid;
+      uint32_t exact = 0;
+      int id = 256 + l;
+      if (mine >= 0) {
+        id = mine;
+        exact = order_key(a.exact ? (float)(1.0 / (1.0 + exp(-(double)own.x)) + (double)own.b) : own.x);
+      }
+      const int to = order_rotated<1>(exact, id);
+      const int sorted = __builtin_amdgcn_ds_permute(((lane & 48) + to) * 4, mine);
+      if (doubts) mine = sorted;
+    }
   }
   if (l >= a.topk) mine = -1;
   // the weights, a lane per place
