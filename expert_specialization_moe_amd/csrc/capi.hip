@@ -558,6 +558,8 @@ int esmoe_permute_rows(const void* in, const int32_t* dst_row, long num_pairs, i
 }
 
 namespace {
+static_assert(ESMOE_MAX_TOPK <= 64, "the gating kernels have a lane per place");
+static_assert(ESMOE_MAX_EXPERTS <= esmoe::kGateMaxExperts, "the gating kernels hold sixteen experts a lane");
 // What both directions of the gating share.
 int gate_args(int dtype, long tokens, int num_experts, long ld, int topk, int scoring, int renormalize, float scale, esmoe::GateArgs* a) {
   if (dtype != ESMOE_LOGITS_FP32 && dtype != ESMOE_LOGITS_BF16 && dtype != ESMOE_LOGITS_FP16)

@@ -47,9 +47,12 @@ __device__ __forceinline__ v4i pack8(const float* x) {
   return r;
 }
 
-// Each row is read once, and what is written is another kernel's to read: the stores are non-temporal, and where a call's rows are more than
-// the memory-side cache holds (STREAM) the loads are too.  us, plain / stores / both: 4096 tokens x top-8 x 7168 104.3 / 98 / 88, its gradient
-// 204 / 193 / 186; where the rows fit in the cache the loads' hint costs (1024 x top-8 x 7168, gradient, stores / both 39.7 / 45.7).
+// Each row is read once, and what is written is another kernel's to read: the stores are non-temporal, and where a call's tensor of rows is more
+// than the memory-side cache holds (STREAM) the loads are too.  us, plain / stores / both: 4096 tokens x top-8 x 7168 105 / 99.3 / 91.3, its
+// gradient 201 / 203 / 191.  The rule goes by the tensor, not by the rows that the pairs point to, which stand on the device alone: on a
+// share of the experts these may fit in the cache.  Then the hint gains where they come from memory and costs where they are in the cache,
+// us, stores / both, from memory and again: 8003 x top-8 x 4096, a quarter of the pairs 37.1 / 34.9 and 29.6 / 32.8, its gradient
+// 65.5 / 57.9 and 54.1 / 56.1; an eighth or less costs either way (16384 x top-8 x 4096, a sixteenth 31.4 / 39.5 and 29.2 / 40.3).
 constexpr long kCacheBytes = 1L << 28;
 template <bool STREAM>
 __device__ __forceinline__ v4i load8(const uint16_t* p) {
@@ -57,7 +60,7 @@ __device__ __forceinline__ v4i load8(const uint16_t* p) {
   else return *(const v4i*)p;
 }
 
-// One wavefront per 512 columns of a token, eight rows' loads in flight.  Bound by memory: 88 us for 4096 tokens x top-8 x 7168 are 5.9 TB/s.
+// One wavefront per 512 columns of a token, eight rows' loads in flight.  Bound by memory: 90 us for 4096 tokens x top-8 x 7168 are 5.9 TB/s.
 // One row after the other was 3.7 us for one token, this is 2.6.
 template <bool FP16, bool STREAM>
 __global__ void __launch_bounds__(256) combine_rows_kernel(const uint16_t* __restrict__ in, const int* __restrict__ dst_row,

@@ -4,7 +4,6 @@
 namespace esmoe {
 
 constexpr int kGateMaxExperts = 1024;   // sixteen per lane
-constexpr int kGateMaxTopk = 64;        // a lane per place
 constexpr int kGateMaxGroups = 64;      // a lane per group
 constexpr int kGateF32 = 0, kGateF16 = 1, kGateBf16 = 2;
 

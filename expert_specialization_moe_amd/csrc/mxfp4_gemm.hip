@@ -21,12 +21,9 @@
 namespace esmoe {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v4i_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 constexpr int kLongWaves = 8;
 
@@ -115,7 +112,7 @@ struct Fp4Units {
 
 // For a K whose sixteen rows of `a` are more than a workgroup's registers: a workgroup takes two tiles of sixteen weight rows (one of the
 // gate's and one of the up projection's) for sixteen rows of `a`, which come from a cache as they are needed; its wavefronts split K.
-// Bound by the loads it has in flight: 16 experts x 2048 x K 12288, a row each 67.6 us (3.1 TB/s), 16 rows 99; with four tiles 71 and 84, but
+// Bound by the loads it has in flight, a chunk's per wavefront (64 registers, eight wavefronts a SIMD): 16 experts x 2048 x K 12288, a row each 67.6 us (3.1 TB/s), 16 rows 99; with four tiles 71 and 84, but
 // two experts of K 14336 44 instead of 23; non-temporal loads of the weights, half a line each, 72.7.
 template <bool FP16, bool SWIGLU>
 __global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ b,
@@ -156,7 +153,6 @@ __global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint1
 #pragma unroll
   for (int t = 0; t < 2; t++) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
   const int chunks = k / 128, end = (int)((long)chunks * (w + 1) / kLongWaves);
-#pragma unroll 2
   for (int c = (int)((long)chunks * w / kLongWaves); c < end; c++) {
     uint32_t d[2][4], s[2];
     v4i x[4];
@@ -212,7 +208,8 @@ __global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint1
 // A lane's sixteen bytes are the 32 columns of one scale, which goes into the conversion: the value is exact in bf16 up to a scale of
 // 2^125, in fp16 from 2^-23 to 2^13.  A step that meets other scales is done again by fp4_any_scale.
 constexpr int kFp4MaxWaves = 8, kFp4MaxPairs = 4;
-// Wavefronts of a CU, by the pairs of chunks that each holds registers for.
+// Wavefronts of a CU, by the pairs of chunks that each holds registers for (110, 160, 210 and 256 of them; with four pairs none spill, but
+// 18 to 60 scalar ones do, into lanes).
 constexpr int fp4_waves(int pairs) { return pairs == 1 ? 16 : pairs == 2 ? 12 : 8; }
 
 struct Fp4Args {

@@ -43,9 +43,10 @@ __device__ __forceinline__ uint32_t dpp_umax16(uint32_t v) {
 // A row's values stay in registers: CHUNKS times eight per thread, THREADS threads per row; with 64 (a wavefront) four rows per workgroup.
 // The squares of 512 columns, a wavefront's chunk, are summed for themselves and then one after the other by column: the same order for
 // any number of threads, so a row's bytes do not hang on how many rows a call has.
-// Nothing is read twice: all stores are non-temporal, or, where a call's tensors are more than the memory-side cache holds (STREAM), the loads and
-// all stores but the bytes'.  us, no hints / stores / STREAM: 16384 x 7168 179 / 174 / 162, 65536 x 512 54.6 / 51.6 / 48.8, 1024 x 4096
-// 8.2 / 6.9 / 8.1, 16384 x 1024 30.0 / 23.2 / 26.5.
+// Nothing is read twice: the stores of 16-bit values and bytes are non-temporal (a scale is 4 bytes: stored plainly), or, where a call's tensors are
+// more than the memory-side cache holds (STREAM), the loads and the stores of 16-bit values.  us, no hints / stores / STREAM, over three sets of
+// tensors: 16384 x 7168 194 / 189 / 189, 65536 x 512 55.3 / 54.1 / 49.1; below the cache's size 1024 x 4096 8.7 / 7.3 / 8.4, 16384 x 1024
+// 30.6 / 24.4 / 27.1.  (16384 x 7168 with the outputs in one place: 170.)
 template <bool FP16, int THREADS, int CHUNKS, bool STREAM>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_quant_kernel(const uint16_t* in, const uint16_t* residual,
                                                                           const uint16_t* __restrict__ weight, float eps, long rows, int hidden,
