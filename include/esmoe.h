@@ -326,6 +326,8 @@ int esmoe_combine_rows_backward(const void* grad_out, const void* in, int dtype,
  *   h = in + residual, rounded to in_dtype and written to residual_out (residual NULL: h = in, residual_out NULL too)
  *   y = h / sqrt(mean(h^2) + eps) * weight in fp32;  normed [total_rows, k] = y rounded to in_dtype, unless NULL
  *   q, scales: y quantised as esmoe_fp8_quant_act_1x128 quantises (y as it is, not rounded before)
+ *   The squares are summed in fp32, in one order for any number of rows: a row gives the same bytes in any batch; one whose sum
+ *   passes the largest fp32 number comes out as zeros.
  * in, residual, weight [k], residual_out, normed of in_dtype (bf16/fp16), 16-byte aligned; k % 128 == 0, k <= 32768.
  * residual_out may be in or residual itself.  No counterpart in the reference.
  */
