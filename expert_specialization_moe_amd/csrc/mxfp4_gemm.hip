@@ -466,7 +466,8 @@ extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const voi
     const int each = (pairs + kFp4MaxWaves - 1) / kFp4MaxWaves;
     const int waves = (pairs + each - 1) / each, per_cu = fp4_waves(each) / waves;
     const unsigned grid = (unsigned)(most < (long)cus * per_cu ? most : (long)cus * per_cu);
-    const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k, (uint32_t)units, (uint16_t*)out};
+    const Fp4Args args{(const uint16_t*)a, (const uint8_t*)b, sf, problem_sizes, expert_offsets, num_experts, total_rows, n, k,
+                       (uint32_t)units, (uint16_t*)out};
 #define ESMOE_FP4(P)                                                                                                               \
   do {                                                                                                                             \
     auto kernel = dtype ? swiglu ? mxfp4_stream_kernel<true, true, P> : mxfp4_stream_kernel<true, false, P>                        \

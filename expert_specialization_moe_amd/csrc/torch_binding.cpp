@@ -518,7 +518,8 @@ namespace {
 // These operators are not part of autograd: where a gradient exists it is an operator of its own, and a result that silently had
 // none would train nothing.  In forward mode, which no_grad leaves on, there is none at all: no result has a tangent, and an output
 // would keep one of what it held before.
-void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor*> inputs, std::initializer_list<const torch::Tensor*> outputs = {}) {
+void check_no_autograd(const char* op, std::initializer_list<const torch::Tensor*> inputs,
+                       std::initializer_list<const torch::Tensor*> outputs = {}) {
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
     for (const auto& tensors : {inputs, outputs})
       for (const torch::Tensor* t : tensors)
@@ -707,7 +708,8 @@ void es_add_rms_norm_quant_1x128(const torch::Tensor& input, const torch::Tensor
               "quant_output must be a contiguous 1-byte tensor of rows * k elements");
   TORCH_CHECK(scales.is_contiguous() && scales.scalar_type() == torch::kFloat32 && scales.numel() == rows * (k / 128),
               "scales must be a contiguous float32 tensor of rows * k / 128 elements");
-  check_no_autograd("es_add_rms_norm_quant_1x128", {&input, &weight, &residual}, {&residual_out, &normed, &quant_output, &scales});
+  check_no_autograd("es_add_rms_norm_quant_1x128", {&input, &weight, &residual},
+                    {&residual_out, &normed, &quant_output, &scales});
   require_device(input, "es_add_rms_norm_quant_1x128");
   check_device(input, {&weight, &residual, &residual_out, &normed, &quant_output, &scales});
   if (rows == 0) return;
