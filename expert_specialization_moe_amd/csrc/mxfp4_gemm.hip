@@ -112,8 +112,9 @@ struct Fp4Units {
 
 // For a K whose sixteen rows of `a` are more than a workgroup's registers: a workgroup takes two tiles of sixteen weight rows (one of the
 // gate's and one of the up projection's) for sixteen rows of `a`, which come from a cache as they are needed; its wavefronts split K.
-// Bound by the loads it has in flight, a chunk's per wavefront (64 registers, eight wavefronts a SIMD): 16 experts x 2048 x K 12288, a row each 67.6 us (3.1 TB/s), 16 rows 99; with four tiles 71 and 84, but
-// two experts of K 14336 44 instead of 23; non-temporal loads of the weights, half a line each, 72.7.
+// Bound by the loads it has in flight, a chunk's per wavefront (64 registers, eight wavefronts a SIMD): 16 experts x 2048 x K 12288, a row
+// each 67.6 us (3.1 TB/s), 16 rows 99; with four tiles 71 and 84, but two experts of K 14336 44 instead of 23; non-temporal loads of the
+// weights, half a line each, 72.7.
 template <bool FP16, bool SWIGLU>
 __global__ void __launch_bounds__(64 * kLongWaves) mxfp4_long_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ b,
                                                                      const uint8_t* __restrict__ sf, const int* __restrict__ problem_sizes,

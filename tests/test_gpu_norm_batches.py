@@ -21,3 +21,15 @@ def test_a_row_is_the_same_in_any_batch(esmoe, k, dtype):
             part = esmoe.es_add_rms_norm_quant_1x128(x[some], w, 1e-6, r[some], return_normed=True)
             for a, b in zip(whole, part):
                 assert torch.equal(a[some].view(torch.uint8), b.view(torch.uint8)), (step, t)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_squares_beyond_fp32_give_zeros(esmoe, rows):
+    """A sum of squares above the largest fp32 number is infinite and its reciprocal root 0; other rows do not notice."""
+    x = torch.ones((rows, 2048), dtype=torch.bfloat16, device="cuda")
+    x[1] = 1e19   # 2048 squares of it: 2e41
+    q, scales, _, normed = esmoe.es_add_rms_norm_quant_1x128(x, torch.ones(2048, dtype=torch.bfloat16, device="cuda"), 0.0, return_normed=True)
+    keep = torch.arange(rows, device="cuda") != 1
+    assert (normed[1] == 0).all() and (q[1].float() == 0).all() and (normed[keep] == 1).all() and (q[keep].float() == 448).all()
+    # (the least scale: 1e-4 / 448 within two roundings)
+    assert ((scales[1].double() * 448 / 1e-4 - 1).abs() <= 2.0 ** -22).all()
