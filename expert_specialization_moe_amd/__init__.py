@@ -28,6 +28,15 @@ from .ops import (  # noqa: F401
     es_add_rms_norm_quant_1x128,
     es_mxfp4_grouped_mm,
     es_mxfp4_grouped_mm_swiglu,
+    es_grouped_mm,
+    es_grouped_mm_backward,
+    es_grouped_mm_swiglu,
+    es_grouped_mm_swiglu_backward,
+    es_int8_quant,
+    es_int8_scaled_grouped_mm,
+    es_int8_scaled_grouped_mm_swiglu,
+    es_grad_norm,
+    es_clip_grad_norm,
 )
 
 __all__ = [
@@ -50,4 +59,13 @@ __all__ = [
     "es_add_rms_norm_quant_1x128",
     "es_mxfp4_grouped_mm",
     "es_mxfp4_grouped_mm_swiglu",
+    "es_grouped_mm",
+    "es_grouped_mm_backward",
+    "es_grouped_mm_swiglu",
+    "es_grouped_mm_swiglu_backward",
+    "es_int8_quant",
+    "es_int8_scaled_grouped_mm",
+    "es_int8_scaled_grouped_mm_swiglu",
+    "es_grad_norm",
+    "es_clip_grad_norm",
 ]

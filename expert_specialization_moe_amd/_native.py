@@ -80,6 +80,22 @@ lib.esmoe_add_rms_norm_quant_1x128.restype = _i
 lib.esmoe_add_rms_norm_quant_1x128.argtypes = [_vp, _i, _vp, _vp, _f, _l, _i, _vp, _vp, _vp, _vp, _vp]
 lib.esmoe_mxfp4_grouped_mm.restype = _i
 lib.esmoe_mxfp4_grouped_mm.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
+lib.esmoe_grouped_mm.restype = _i
+lib.esmoe_grouped_mm.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]
+lib.esmoe_grouped_mm_backward.restype = _i
+lib.esmoe_grouped_mm_backward.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]
+lib.esmoe_swiglu_backward.restype = _i
+lib.esmoe_swiglu_backward.argtypes = [_vp, _vp, _i, _l, _i, _vp, _vp]
+lib.esmoe_int8_grouped_mm.restype = _i
+lib.esmoe_int8_grouped_mm.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
+lib.esmoe_int8_quant.restype = _i
+lib.esmoe_int8_quant.argtypes = [_vp, _i, _vp, _vp, _l, _i, _vp]
+lib.esmoe_grad_norm_workspace_bytes.restype = _sz
+lib.esmoe_grad_norm_workspace_bytes.argtypes = [_i]
+lib.esmoe_grad_norm.restype = _i
+lib.esmoe_grad_norm.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _sz, _vp]
+lib.esmoe_clip_grad_norm.restype = _i
+lib.esmoe_clip_grad_norm.argtypes = [_vp, _vp, _vp, _vp, _i, ctypes.c_double, ctypes.c_double, _vp, _vp, _vp, _sz, _vp]
 lib.esmoe_last_error.restype = ctypes.c_char_p
 lib.esmoe_last_error.argtypes = []
 lib.esmoe_version.restype = ctypes.c_char_p

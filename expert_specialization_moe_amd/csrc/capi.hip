@@ -12,8 +12,10 @@
 #include <vector>
 
 #include "esmoe.h"
+#include "expert_mm.h"
 #include "gating.h"
 #include "gemm_args.h"
+#include "grad_norm.h"
 #include "schedule.h"
 
 extern "C" int esmoe_launch_grouped_gemm(const esmoe::GemmArgs* args, int mx, int grid, hipStream_t stream);
@@ -51,6 +53,13 @@ extern "C" int esmoe_launch_add_rms_norm_quant(const void* in, int in_dtype, con
 extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const void* b, const uint8_t* sf, const int* problem_sizes,
                                              const int* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu,
                                              void* out, int cus, hipStream_t stream);
+extern "C" int esmoe_launch_expert_mm(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
+extern "C" int esmoe_launch_swiglu_grad(const void* grad_h, const void* gate_up, int fp16, long rows, int inter, void* grad, hipStream_t stream);
+extern "C" int esmoe_launch_int8_quant(const void* in, int fp16, long rows, int k, void* q, float* scales, hipStream_t stream);
+extern "C" int esmoe_launch_grad_squares(const esmoe::GradTable* t, int grid, double* partial, hipStream_t stream);
+extern "C" int esmoe_launch_grad_norm(const double* partial, int count, float* norm, hipStream_t stream);
+extern "C" int esmoe_launch_grad_clip(const esmoe::GradTable* t, int grid, const double* partial, int count, const float* given, double max_norm,
+                                      float eps, float* norm_out, hipStream_t stream);
 
 namespace {
 
@@ -256,6 +265,37 @@ int launch_gemm(esmoe::GemmArgs& g, int mx, int force_bm, void* stream, bool own
   return 0;
 }
 
+}  // namespace
+
+namespace {
+// The call's tensors in launches of at most kGradTensors, empty ones left out; f(table, workgroups, partial sums before).
+template <typename F>
+int for_grad_tables(const void* const* grads, void* const* outputs, const int* dtypes, const long* sizes, int count, F&& f) {
+  long all = 0;
+  for (int i = 0; i < count; i++) all += (sizes[i] + esmoe::kGradChunk - 1) / esmoe::kGradChunk;
+  int before = 0;
+  for (int i = 0; i < count;) {
+    esmoe::GradTable t;
+    t.count = 0;
+    long chunks = 0;
+    for (; i < count && t.count < esmoe::kGradTensors; i++) {
+      if (sizes[i] == 0) continue;
+      chunks += (sizes[i] + esmoe::kGradChunk - 1) / esmoe::kGradChunk;
+      t.in[t.count] = grads[i];
+      t.out[t.count] = outputs ? outputs[i] : nullptr;
+      t.size[t.count] = sizes[i];
+      t.end[t.count] = chunks;
+      t.type[t.count++] = (uint8_t)dtypes[i];
+    }
+    if (t.count == 0) break;
+    long grid = all <= esmoe::kGradWorkgroups ? chunks : (long)((double)esmoe::kGradWorkgroups * chunks / all) + 1;
+    if (grid > chunks) grid = chunks;
+    const int rc = f(t, (int)grid, before);
+    if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
+    before += (int)grid;
+  }
+  return 0;
+}
 }  // namespace
 
 extern "C" {
@@ -722,6 +762,189 @@ int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, c
   return 0;
 }
 
+namespace {
+// Checks that the 16-bit and int8 grouped products share.  step: elements of 16 bytes of k, of n where its rows are read too.
+int expert_mm_args(int dtype, int num_experts, int total_rows, int n, int k, int swiglu, int k_step, int most_k) {
+  if (dtype != ESMOE_OUT_BF16 && dtype != ESMOE_OUT_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "dtype must be ESMOE_OUT_BF16 or ESMOE_OUT_FP16");
+  if (num_experts < 1 || num_experts > ESMOE_MAX_EXPERTS)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "num_experts must be in [1, %d], got %d", ESMOE_MAX_EXPERTS, num_experts);
+  if (total_rows < 0) return fail(ESMOE_ERR_INVALID_ARGUMENT, "total_rows must be >= 0");
+  if (k <= 0 || k % k_step || k > most_k) return fail(ESMOE_ERR_INVALID_ARGUMENT, "k must be a multiple of %d up to %d, got %d", k_step, most_k, k);
+  if (n <= 0 || n % (swiglu ? 16 : 8) || n > (1 << 20))
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "n must be a multiple of 8 (of 16 with SwiGLU) up to 2^20, got %d", n);
+  return 0;
+}
+int expert_mm_launch(const esmoe::ExpertMmArgs& args, int kind, void* stream) {
+  DeviceInfo info;
+  int rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_expert_mm(&args, kind, info.cus, (hipStream_t)stream);
+  if (rc) return fail(rc, "grouped mm launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+}  // namespace
+
+int esmoe_grouped_mm(void* out, int dtype, const void* a, const void* b, const int32_t* problem_sizes, const int32_t* expert_offsets,
+                     int num_experts, int total_rows, int n, int k, int swiglu, void* gate_up, void* stream) {
+  g_err[0] = 0;
+  int rc = expert_mm_args(dtype, num_experts, total_rows, n, k, swiglu, 8, 1 << 20);
+  if (rc) return rc;
+  if (gate_up && !swiglu) return fail(ESMOE_ERR_INVALID_ARGUMENT, "gate_up goes with swiglu");
+  if (total_rows == 0) return 0;
+  if (!out || !a || !b || !problem_sizes || !expert_offsets) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)out % 16 || (uintptr_t)gate_up % 16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "a, b, out and gate_up must be 16-byte aligned");
+  const esmoe::ExpertMmArgs args = {a, b, out, gate_up, nullptr, nullptr, problem_sizes, expert_offsets, num_experts, total_rows, n, k,
+                                    dtype == ESMOE_OUT_FP16 ? esmoe::kMmFp16 : esmoe::kMmBf16, 0};
+  return expert_mm_launch(args, swiglu ? 1 : 0, stream);
+}
+
+int esmoe_grouped_mm_backward(const void* grad_out, int dtype, const void* a, const void* b, const int32_t* problem_sizes,
+                              const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, void* grad_a, void* grad_b,
+                              void* stream) {
+  g_err[0] = 0;
+  int rc = expert_mm_args(dtype, num_experts, total_rows, n, k, 0, 8, 1 << 20);
+  if (rc) return rc;
+  if (!problem_sizes || !expert_offsets || ((!grad_out || (grad_a && !b) || (grad_b && !a)) && total_rows))
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)grad_out % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)grad_a % 16 || (uintptr_t)grad_b % 16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "grad_out, a, b, grad_a and grad_b must be 16-byte aligned");
+  esmoe::ExpertMmArgs args = {grad_out, b, grad_a, nullptr, nullptr, nullptr, problem_sizes, expert_offsets, num_experts, total_rows, n, k,
+                              dtype == ESMOE_OUT_FP16 ? esmoe::kMmFp16 : esmoe::kMmBf16, 0};
+  if (grad_a && total_rows) rc = expert_mm_launch(args, 2, stream);
+  if (rc || !grad_b) return rc;
+  args.w = a;
+  args.out = grad_b;
+  return expert_mm_launch(args, 3, stream);
+}
+
+int esmoe_swiglu_backward(const void* grad_out, const void* gate_up, int dtype, long total_rows, int inter, void* grad_gate_up, void* stream) {
+  g_err[0] = 0;
+  if (dtype != ESMOE_IN_BF16 && dtype != ESMOE_IN_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "dtype must be ESMOE_IN_BF16 or ESMOE_IN_FP16");
+  if (inter <= 0 || inter % 8 || inter > (1 << 19)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "inter must be a multiple of 8 up to 2^19, got %d", inter);
+  if (total_rows < 0 || total_rows >= (1L << 31)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "total_rows out of range: %ld", total_rows);
+  if (total_rows == 0) return 0;
+  if (!grad_out || !gate_up || !grad_gate_up) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)grad_out % 16 || (uintptr_t)gate_up % 16 || (uintptr_t)grad_gate_up % 16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "grad_out, gate_up and grad_gate_up must be 16-byte aligned");
+  DeviceInfo info;
+  int rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_swiglu_grad(grad_out, gate_up, dtype == ESMOE_IN_FP16, total_rows, inter, grad_gate_up, (hipStream_t)stream);
+  if (rc) return fail(rc, "swiglu gradient launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_int8_quant(const void* in, int in_dtype, void* q, float* scales, long total_rows, int k, void* stream) {
+  g_err[0] = 0;
+  if (in_dtype != ESMOE_IN_BF16 && in_dtype != ESMOE_IN_FP16)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "in_dtype must be ESMOE_IN_BF16 or ESMOE_IN_FP16");
+  if (k <= 0 || k % 16 || k > 65536) return fail(ESMOE_ERR_INVALID_ARGUMENT, "k must be a multiple of 16 up to 65536, got %d", k);
+  if (total_rows < 0 || total_rows > (1L << 40) / k) return fail(ESMOE_ERR_INVALID_ARGUMENT, "total_rows out of range: %ld", total_rows);
+  if (total_rows == 0) return 0;
+  if (!in || !q || !scales) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)in % 16 || (uintptr_t)q % 16 || (uintptr_t)scales % 4)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "in and q must be 16-byte aligned, scales 4-byte aligned");
+  DeviceInfo info;
+  int rc = current_device_info(&info);
+  if (rc) return rc;
+  rc = esmoe_launch_int8_quant(in, in_dtype == ESMOE_IN_FP16, total_rows, k, q, scales, (hipStream_t)stream);
+  if (rc) return fail(rc, "int8 quant launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_int8_grouped_mm(void* out, int out_dtype, const void* a, const void* b, const float* sa, const float* sb, const int32_t* problem_sizes,
+                          const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream) {
+  g_err[0] = 0;
+  int rc = expert_mm_args(out_dtype, num_experts, total_rows, n, k, swiglu, 16, 65536);
+  if (rc) return rc;
+  if (total_rows == 0) return 0;
+  if (!out || !a || !b || !sa || !sb || !problem_sizes || !expert_offsets) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if ((uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)out % 16 || (uintptr_t)sa % 4 || (uintptr_t)sb % 4)
+    return fail(ESMOE_ERR_INVALID_ARGUMENT, "a, b and out must be 16-byte aligned, scales 4-byte aligned");
+  const esmoe::ExpertMmArgs args = {a, b, out, nullptr, sa, sb, problem_sizes, expert_offsets, num_experts, total_rows, n, k, esmoe::kMmInt8,
+                                    out_dtype == ESMOE_OUT_FP16};
+  return expert_mm_launch(args, swiglu ? 1 : 0, stream);
+}
+
+namespace {
+int grad_args(const void* const* grads, void* const* outputs, const int* dtypes, const long* sizes, int count, const void* workspace,
+              size_t workspace_bytes) {
+  if (count < 0 || count > (1 << 20)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "count must be in [0, 2^20], got %d", count);
+  if (count && (!grads || !dtypes || !sizes)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null array");
+  long all = 0;
+  for (int i = 0; i < count; i++) {
+    if (dtypes[i] != ESMOE_GRAD_BF16 && dtypes[i] != ESMOE_GRAD_FP16 && dtypes[i] != ESMOE_GRAD_FP32)
+      return fail(ESMOE_ERR_INVALID_ARGUMENT, "a gradient's dtype must be one of ESMOE_GRAD_*, got %d", dtypes[i]);
+    if (sizes[i] < 0 || sizes[i] > (1L << 40) || (all += sizes[i]) > (1L << 40))
+      return fail(ESMOE_ERR_INVALID_ARGUMENT, "gradients of more than 2^40 elements, or fewer than none");
+    if (sizes[i] && (!grads[i] || (outputs && !outputs[i]))) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    const uintptr_t at = (uintptr_t)grads[i] | (outputs ? (uintptr_t)outputs[i] : 0);
+    if (at % (dtypes[i] == ESMOE_GRAD_FP32 ? 4 : 2)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "a gradient must be aligned to its elements");
+  }
+  if (workspace_bytes < esmoe_grad_norm_workspace_bytes(count) || !workspace || (uintptr_t)workspace % 8)
+    return fail(ESMOE_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed, 8-byte aligned", workspace_bytes,
+                esmoe_grad_norm_workspace_bytes(count));
+  return 0;
+}
+}  // namespace
+
+size_t esmoe_grad_norm_workspace_bytes(int count) {
+  return 8 * (size_t)(esmoe::kGradWorkgroups + (count > 0 ? count : 0) / esmoe::kGradTensors + 1);
+}
+
+int esmoe_grad_norm(const void* const* grads, const int* dtypes, const long* sizes, int count, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = grad_args(grads, nullptr, dtypes, sizes, count, workspace, workspace_bytes);
+  if (rc) return rc;
+  if (!norm) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  int partials = 0;
+  rc = for_grad_tables(grads, nullptr, dtypes, sizes, count, [&](const esmoe::GradTable& t, int grid, int before) {
+    partials = before + grid;
+    return esmoe_launch_grad_squares(&t, grid, (double*)workspace + before, (hipStream_t)stream);
+  });
+  if (rc) return rc;
+  rc = esmoe_launch_grad_norm((const double*)workspace, partials, norm, (hipStream_t)stream);
+  if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
+  return 0;
+}
+
+int esmoe_clip_grad_norm(const void* const* grads, void* const* outputs, const int* dtypes, const long* sizes, int count, double max_norm,
+                         double eps, const float* given_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  if (count && !outputs) return fail(ESMOE_ERR_INVALID_ARGUMENT, "null array");
+  int rc = grad_args(grads, outputs, dtypes, sizes, count, workspace, workspace_bytes);
+  if (rc) return rc;
+  if (!(max_norm >= 0.0)) return fail(ESMOE_ERR_INVALID_ARGUMENT, "max_norm must not be negative or NaN");
+  if (!(eps >= 0.0 && eps < __builtin_inf())) return fail(ESMOE_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  DeviceInfo info;
+  rc = current_device_info(&info);
+  if (rc) return rc;
+  int partials = 0;
+  if (!given_norm) {
+    rc = for_grad_tables(grads, nullptr, dtypes, sizes, count, [&](const esmoe::GradTable& t, int grid, int before) {
+      partials = before + grid;
+      return esmoe_launch_grad_squares(&t, grid, (double*)workspace + before, (hipStream_t)stream);
+    });
+    if (rc) return rc;
+    if (partials == 0 && norm) {   // no elements at all: the norm is 0
+      rc = esmoe_launch_grad_norm((const double*)workspace, 0, norm, (hipStream_t)stream);
+      if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
+      return 0;
+    }
+  }
+  return for_grad_tables(grads, outputs, dtypes, sizes, count, [&](const esmoe::GradTable& t, int grid, int before) {
+    return esmoe_launch_grad_clip(&t, grid, (const double*)workspace, partials, given_norm, max_norm, eps, before ? nullptr : norm,
+                                  (hipStream_t)stream);
+  });
+}
+
 int esmoe_host_schedule(const int32_t* problem_sizes_host, int num_experts, int n, int force_bm, int kind,
                         int32_t* ws_host) {
   g_err[0] = 0;
@@ -831,6 +1054,6 @@ int esmoe_host_decode_light(const int32_t* problem_sizes_host, const int32_t* ws
 
 const char* esmoe_last_error(void) { return g_err; }
 
-const char* esmoe_version(void) { return "esmoe 0.4 (gfx950)"; }
+const char* esmoe_version(void) { return "esmoe 0.5 (gfx950)"; }
 
 }  // extern "C"

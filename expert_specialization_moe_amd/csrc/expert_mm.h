@@ -1,0 +1,24 @@
+// What the entry points hand to the 16-bit and int8 grouped products (expert_mm.hip).
+#pragma once
+#include <stdint.h>
+
+namespace esmoe {
+
+enum { kMmBf16 = 0, kMmFp16 = 1, kMmInt8 = 2 };
+
+// out[m, j] = sum_c t[m, c] * w_e(j, c) for the rows m of expert e.
+//   forward:        t = a [rows, k], w_e = b[e] [n, k] along its rows, out [rows, n]
+//   rows' gradient: t = grad_out [rows, n], w_e = b[e] [n, k] along its columns, out = grad_a [rows, k]
+// weights' gradient: out[e][i, j] = sum over the rows m of expert e of t[m, i] * w[m, j], t = grad_out [rows, n], w = a [rows, k], out [E, n, k]
+struct ExpertMmArgs {
+  const void *t, *w;
+  void* out;
+  void* gate_up;              // SwiGLU: the two projections as well, or null
+  const float *sa, *sb;       // int8: scales of rows and of weight rows [E, n]
+  const int *problem_sizes, *expert_offsets;
+  int num_experts, total_rows, n, k;
+  int type;                   // of t and w
+  int out_fp16;               // int8: type of out
+};
+
+}  // namespace esmoe

@@ -1,0 +1,22 @@
+// A launch's share of the gradients that a norm is taken over (grad_norm.hip): passed by value, so that a captured graph holds it.
+#pragma once
+#include <stdint.h>
+
+namespace esmoe {
+
+enum { kGradBf16 = 0, kGradFp16 = 1, kGradFp32 = 2 };
+constexpr int kGradTensors = 96;       // of a launch: the table has to fit in a kernel's arguments (4 KB)
+constexpr long kGradChunk = 8192;      // elements
+constexpr int kGradWorkgroups = 2048;  // that a call's chunks are dealt to, and one more per launch at most
+
+struct GradTable {
+  const void* in[kGradTensors];
+  void* out[kGradTensors];             // clipping alone
+  long size[kGradTensors];             // elements
+  long end[kGradTensors];              // chunks up to and with the tensor's
+  uint8_t type[kGradTensors];
+  int count;
+};
+static_assert(sizeof(GradTable) <= 3600, "kernel arguments");
+
+}  // namespace esmoe

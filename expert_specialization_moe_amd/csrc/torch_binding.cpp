@@ -15,8 +15,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/all.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <vector>
 
 #include "esmoe.h"
 
@@ -791,6 +793,277 @@ void es_mxfp4_grouped_mm_swiglu(torch::Tensor& output, const torch::Tensor& a, c
   mxfp4_grouped_mm("es_mxfp4_grouped_mm_swiglu", true, output, a, b, sfb, problem_sizes, expert_offsets);
 }
 
+// ---- the experts' products in 16 bits with their gradients, and in 8-bit integers ----
+namespace {
+// A (num_experts, k, n) view of packed rows of k, and the metadata that go with it.
+void check_experts(const char* op, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& problem_sizes,
+                   const torch::Tensor& expert_offsets, int64_t k_step, int64_t most_k, bool swiglu) {
+  TORCH_CHECK(problem_sizes.dim() == 2 && problem_sizes.size(1) == 3, "problem_sizes must have shape (num_experts, 3)");
+  const int64_t num_experts = problem_sizes.size(0);
+  TORCH_CHECK(expert_offsets.dim() == 1 && expert_offsets.size(0) == num_experts, "Number of experts in problem_sizes must match expert_offsets");
+  TORCH_CHECK(problem_sizes.dtype() == torch::kInt32 && expert_offsets.dtype() == torch::kInt32, "problem_sizes and expert_offsets must be int32");
+  TORCH_CHECK(num_experts >= 1 && num_experts <= ESMOE_MAX_EXPERTS, "Number of experts cannot exceed 1024");
+  TORCH_CHECK(a.dim() == 2 && a.is_contiguous(), "a must be a packed row-major (rows, k) tensor");
+  const int64_t k = a.size(1);
+  TORCH_CHECK(k > 0 && k % k_step == 0 && k <= most_k, "k must be a multiple of ", k_step, " up to ", most_k);
+  TORCH_CHECK(b.dim() == 3 && b.size(0) == num_experts && b.size(1) == k && b.scalar_type() == a.scalar_type(),
+              "b must be a (num_experts, k, n) tensor of a's dtype");
+  const int64_t n = b.size(2);
+  TORCH_CHECK(n > 0 && n % (swiglu ? 16 : 8) == 0 && n <= (int64_t(1) << 20), "n must be a multiple of 8 (of 16 with SwiGLU) up to 2^20");
+  TORCH_CHECK(b.stride(1) == 1 && b.stride(2) == k && (num_experts == 1 || b.stride(0) == n * k),
+              "b must be the column-major (num_experts, k, n) view of a packed (num_experts, n, k) tensor");
+  TORCH_CHECK(a.size(0) < (int64_t(1) << 31), "tensor too large");
+  TORCH_CHECK(problem_sizes.is_contiguous() && expert_offsets.is_contiguous(), "metadata tensors must be contiguous");
+}
+
+void check_rows(const torch::Tensor& t, const char* name, int64_t rows, int64_t cols, const torch::Tensor& like) {
+  TORCH_CHECK(t.dim() == 2 && t.is_contiguous() && t.size(0) == rows && t.size(1) == cols && t.scalar_type() == like.scalar_type(), name,
+              " must be a contiguous (", rows, ", ", cols, ") tensor of a's dtype");
+}
+
+// The binding's workspaces are the allocator's, on the current stream: no call waits for the device.
+void grouped_mm(const char* op, bool swiglu, torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b,
+                const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets, const torch::Tensor& gate_up) {
+  TORCH_CHECK(is_half_type(a), "a must be bfloat16 or half");
+  check_experts(op, a, b, problem_sizes, expert_offsets, 8, int64_t(1) << 20, swiglu);
+  const int64_t rows = a.size(0), k = a.size(1), n = b.size(2);
+  check_rows(output, "output", rows, swiglu ? n / 2 : n, a);
+  if (gate_up.defined()) check_rows(gate_up, "gate_up", rows, n, a);
+  check_no_autograd(op, {&a, &b}, {&output, &gate_up});
+  require_device(a, op);
+  check_device(a, {&output, &b, &gate_up, &problem_sizes, &expert_offsets});
+  TORCH_CHECK(!any_overlap(output, {&a, &b, &gate_up, &problem_sizes, &expert_offsets}) &&
+                  !any_overlap(gate_up, {&a, &b, &problem_sizes, &expert_offsets}),
+              "output and gate_up may not overlap each other or an input");
+  if (rows == 0) return;
+  c10::DeviceGuard guard(a.device());
+  int rc = esmoe_grouped_mm(output.data_ptr(), out_dtype_of(a), a.data_ptr(), b.data_ptr(), problem_sizes.data_ptr<int32_t>(),
+                            expert_offsets.data_ptr<int32_t>(), (int)problem_sizes.size(0), (int)rows, (int)n, (int)k, swiglu,
+                            gate_up.defined() ? gate_up.data_ptr() : nullptr, current_stream(a));
+  check_rc(rc, op);
+}
+
+void grouped_mm_backward(const char* op, const torch::Tensor* gate_up, const torch::Tensor& grad_output, const torch::Tensor& a,
+                         const torch::Tensor& b, const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets,
+                         const torch::Tensor& grad_a, const torch::Tensor& grad_b) {
+  TORCH_CHECK(is_half_type(a), "a must be bfloat16 or half");
+  check_experts(op, a, b, problem_sizes, expert_offsets, 8, int64_t(1) << 20, gate_up != nullptr);
+  const int64_t rows = a.size(0), k = a.size(1), n = b.size(2), experts = b.size(0);
+  static const torch::Tensor none;
+  const torch::Tensor& saved = gate_up ? *gate_up : none;
+  check_rows(grad_output, "grad_output", rows, gate_up ? n / 2 : n, a);
+  if (gate_up) check_rows(saved, "gate_up", rows, n, a);
+  if (grad_a.defined()) check_rows(grad_a, "grad_a", rows, k, a);
+  TORCH_CHECK(!grad_b.defined() || (grad_b.sizes() == b.sizes() && grad_b.scalar_type() == b.scalar_type() && grad_b.stride(1) == 1 &&
+                                    grad_b.stride(2) == k && (experts == 1 || grad_b.stride(0) == n * k)),
+              "grad_b must be the column-major (num_experts, k, n) view of a packed (num_experts, n, k) tensor of b's dtype");
+  check_no_autograd(op, {&grad_output, &a, &b, &saved}, {&grad_a, &grad_b});
+  require_device(a, op);
+  check_device(a, {&grad_output, &b, &saved, &problem_sizes, &expert_offsets, &grad_a, &grad_b});
+  TORCH_CHECK(!any_overlap(grad_a, {&grad_output, &a, &b, &saved, &problem_sizes, &expert_offsets, &grad_b}) &&
+                  !any_overlap(grad_b, {&grad_output, &a, &b, &saved, &problem_sizes, &expert_offsets}),
+              "grad_a and grad_b may not overlap each other or the inputs");
+  c10::DeviceGuard guard(a.device());
+  const int dtype = out_dtype_of(a);
+  torch::Tensor grad = grad_output;
+  if (gate_up && rows && (grad_a.defined() || grad_b.defined())) {
+    grad = torch::empty({rows, n}, a.options().requires_grad(false));
+    check_rc(esmoe_swiglu_backward(grad_output.data_ptr(), saved.data_ptr(), dtype, (long)rows, (int)(n / 2), grad.data_ptr(), current_stream(a)), op);
+  }
+  int rc = esmoe_grouped_mm_backward(rows ? grad.data_ptr() : nullptr, dtype, rows ? a.data_ptr() : nullptr, b.data_ptr(),
+                                     problem_sizes.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), (int)experts, (int)rows, (int)n,
+                                     (int)k, grad_a.defined() && rows ? grad_a.data_ptr() : nullptr, grad_b.defined() ? grad_b.data_ptr() : nullptr,
+                                     current_stream(a));
+  check_rc(rc, op);
+}
+}  // namespace
+
+void es_grouped_mm(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& problem_sizes,
+                   const torch::Tensor& expert_offsets) {
+  grouped_mm("es_grouped_mm", false, output, a, b, problem_sizes, expert_offsets, torch::Tensor());
+}
+
+void es_grouped_mm_swiglu(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& problem_sizes,
+                          const torch::Tensor& expert_offsets, const c10::optional<torch::Tensor>& gate_up) {
+  grouped_mm("es_grouped_mm_swiglu", true, output, a, b, problem_sizes, expert_offsets, tensor_or_none(gate_up));
+}
+
+void es_grouped_mm_backward(const torch::Tensor& grad_output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& problem_sizes,
+                            const torch::Tensor& expert_offsets, const c10::optional<torch::Tensor>& grad_a,
+                            const c10::optional<torch::Tensor>& grad_b) {
+  grouped_mm_backward("es_grouped_mm_backward", nullptr, grad_output, a, b, problem_sizes, expert_offsets, tensor_or_none(grad_a),
+                      tensor_or_none(grad_b));
+}
+
+void es_grouped_mm_swiglu_backward(const torch::Tensor& grad_output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& gate_up,
+                                   const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets,
+                                   const c10::optional<torch::Tensor>& grad_a, const c10::optional<torch::Tensor>& grad_b) {
+  grouped_mm_backward("es_grouped_mm_swiglu_backward", &gate_up, grad_output, a, b, problem_sizes, expert_offsets, tensor_or_none(grad_a),
+                      tensor_or_none(grad_b));
+}
+
+void es_int8_quant(const torch::Tensor& input, torch::Tensor& quant_output, torch::Tensor& scales) {
+  TORCH_CHECK(input.dim() >= 1 && input.is_contiguous(), "input must be contiguous with at least 1 dimension");
+  TORCH_CHECK(is_half_type(input), "dtype must be kFloat16 or kBFloat16");
+  const int64_t k = input.size(-1);
+  TORCH_CHECK(k > 0 && k % 16 == 0 && k <= 65536, "k must be a multiple of 16 up to 65536");
+  const int64_t rows = input.numel() / k;
+  TORCH_CHECK(quant_output.is_contiguous() && quant_output.scalar_type() == torch::kInt8 && quant_output.numel() == rows * k,
+              "quant_output must be a contiguous int8 tensor of input's number of elements");
+  TORCH_CHECK(scales.is_contiguous() && scales.scalar_type() == torch::kFloat32 && scales.numel() == rows,
+              "scales must be a contiguous float32 tensor with one element per row");
+  check_no_autograd("es_int8_quant", {&input}, {&scales});
+  require_device(input, "es_int8_quant");
+  check_device(input, {&quant_output, &scales});
+  TORCH_CHECK(!any_overlap(quant_output, {&input, &scales}) && !any_overlap(scales, {&input}), "outputs may not overlap input or each other");
+  if (rows == 0) return;
+  c10::DeviceGuard guard(input.device());
+  int rc = esmoe_int8_quant(input.data_ptr(), input.scalar_type() == torch::kBFloat16 ? ESMOE_IN_BF16 : ESMOE_IN_FP16, quant_output.data_ptr(),
+                            scales.data_ptr<float>(), (long)rows, (int)k, current_stream(input));
+  check_rc(rc, "es_int8_quant");
+}
+
+// The same into new tensors.
+std::tuple<torch::Tensor, torch::Tensor> es_int8_quant_new(const torch::Tensor& input) {
+  TORCH_CHECK(input.dim() >= 1, "input must be contiguous with at least 1 dimension");
+  const auto opts = input.options().requires_grad(false);
+  torch::Tensor q = torch::empty(input.sizes(), opts.dtype(torch::kInt8)),
+                scales = torch::empty(input.sizes().slice(0, input.dim() - 1), opts.dtype(torch::kFloat32));
+  es_int8_quant(input, q, scales);
+  return {q, scales};
+}
+
+namespace {
+void int8_scaled_grouped_mm(const char* op, bool swiglu, torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b,
+                            const torch::Tensor& scales_a, const torch::Tensor& scales_b, const torch::Tensor& problem_sizes,
+                            const torch::Tensor& expert_offsets) {
+  TORCH_CHECK(a.scalar_type() == torch::kInt8, "a must be int8");
+  check_experts(op, a, b, problem_sizes, expert_offsets, 16, 65536, swiglu);
+  const int64_t rows = a.size(0), k = a.size(1), n = b.size(2), experts = b.size(0);
+  TORCH_CHECK(is_half_type(output) && output.dim() == 2 && output.is_contiguous() && output.size(0) == rows && output.size(1) == (swiglu ? n / 2 : n),
+              "output must be a contiguous bfloat16 or half (rows, n) tensor, (rows, n / 2) with SwiGLU");
+  TORCH_CHECK(scales_a.scalar_type() == torch::kFloat32 && scales_a.is_contiguous() && scales_a.numel() == rows,
+              "scales_a must be a contiguous float32 tensor with one element per row");
+  TORCH_CHECK(scales_b.scalar_type() == torch::kFloat32 && scales_b.is_contiguous() && scales_b.dim() == 2 && scales_b.size(0) == experts &&
+                  scales_b.size(1) == n,
+              "scales_b must be a contiguous float32 (num_experts, n) tensor");
+  check_no_autograd(op, {&scales_a, &scales_b}, {&output});
+  require_device(a, op);
+  check_device(a, {&output, &b, &scales_a, &scales_b, &problem_sizes, &expert_offsets});
+  TORCH_CHECK(!any_overlap(output, {&a, &b, &scales_a, &scales_b, &problem_sizes, &expert_offsets}), "output may not overlap an input");
+  if (rows == 0) return;
+  c10::DeviceGuard guard(a.device());
+  int rc = esmoe_int8_grouped_mm(output.data_ptr(), out_dtype_of(output), a.data_ptr(), b.data_ptr(), scales_a.data_ptr<float>(),
+                                 scales_b.data_ptr<float>(), problem_sizes.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), (int)experts,
+                                 (int)rows, (int)n, (int)k, swiglu, current_stream(a));
+  check_rc(rc, op);
+}
+}  // namespace
+
+void es_int8_scaled_grouped_mm(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& scales_a,
+                               const torch::Tensor& scales_b, const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets) {
+  int8_scaled_grouped_mm("es_int8_scaled_grouped_mm", false, output, a, b, scales_a, scales_b, problem_sizes, expert_offsets);
+}
+
+void es_int8_scaled_grouped_mm_swiglu(torch::Tensor& output, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& scales_a,
+                                      const torch::Tensor& scales_b, const torch::Tensor& problem_sizes, const torch::Tensor& expert_offsets) {
+  int8_scaled_grouped_mm("es_int8_scaled_grouped_mm_swiglu", true, output, a, b, scales_a, scales_b, problem_sizes, expert_offsets);
+}
+
+// ---- the norm of gradients and their clipping ----
+namespace {
+struct GradList {
+  std::vector<const void*> in;
+  std::vector<void*> out;
+  std::vector<int> dtypes;
+  std::vector<long> sizes;
+  torch::Tensor workspace;
+};
+
+GradList grad_list(const char* op, at::TensorList grads) {
+  TORCH_CHECK(!grads.empty(), op, ": no gradients given");
+  GradList l;
+  for (const torch::Tensor& g : grads) {
+    TORCH_CHECK(g.defined() && g.layout() == torch::kStrided, op, ": gradients must be dense tensors");
+    TORCH_CHECK(is_half_type(g) || g.scalar_type() == torch::kFloat32, op, ": gradients must be float32, bfloat16 or half");
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), op, ": gradients must be dense in memory (their elements in any order, without gaps)");
+    TORCH_CHECK(g.device() == grads[0].device(), "all tensors must be on the same device");
+    check_no_autograd(op, {&g});
+    l.dtypes.push_back(g.scalar_type() == torch::kFloat32 ? ESMOE_GRAD_FP32 : g.scalar_type() == torch::kHalf ? ESMOE_GRAD_FP16 : ESMOE_GRAD_BF16);
+    l.sizes.push_back((long)g.numel());
+  }
+  return l;
+}
+
+// Whether a range that is written overlaps any other.
+bool written_overlaps(at::TensorList grads, at::TensorList outputs, const torch::Tensor& norm) {
+  struct Range { const char *from, *to; bool written; };
+  std::vector<Range> ranges;
+  const auto add = [&](const torch::Tensor& t, bool written) {
+    if (t.defined() && t.numel()) ranges.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes(), written});
+  };
+  for (size_t i = 0; i < grads.size(); i++) {
+    add(outputs[i], true);
+    if (outputs[i].data_ptr() != grads[i].data_ptr()) add(grads[i], false);
+  }
+  add(norm, false);
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+  const char *any = nullptr, *written = nullptr;   // ends of those before
+  for (const Range& r : ranges) {
+    if (r.from < written || (r.written && r.from < any)) return true;
+    any = std::max(any, r.to);
+    if (r.written) written = std::max(written, r.to);
+  }
+  return false;
+}
+
+void grad_pointers(GradList& l, at::TensorList grads) {
+  for (const torch::Tensor& g : grads) l.in.push_back(g.data_ptr());
+  l.workspace = torch::empty({(int64_t)esmoe_grad_norm_workspace_bytes((int)grads.size())}, grads[0].options().dtype(torch::kUInt8).requires_grad(false));
+}
+}  // namespace
+
+torch::Tensor es_grad_norm(at::TensorList grads) {
+  GradList l = grad_list("es_grad_norm", grads);
+  require_device(grads[0], "es_grad_norm");
+  c10::DeviceGuard guard(grads[0].device());
+  grad_pointers(l, grads);
+  torch::Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32).requires_grad(false));
+  int rc = esmoe_grad_norm(l.in.data(), l.dtypes.data(), l.sizes.data(), (int)l.in.size(), norm.data_ptr<float>(), l.workspace.data_ptr(),
+                           l.workspace.nbytes(), current_stream(grads[0]));
+  check_rc(rc, "es_grad_norm");
+  return norm;
+}
+
+torch::Tensor es_clip_grad_norm(at::TensorList grads, double max_norm, double eps, const c10::optional<torch::Tensor>& norm_, at::TensorList outputs) {
+  const char* op = "es_clip_grad_norm";
+  const torch::Tensor& given = tensor_or_none(norm_);
+  GradList l = grad_list(op, grads);
+  TORCH_CHECK(max_norm >= 0, "max_norm must not be negative or NaN");
+  TORCH_CHECK(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative");
+  TORCH_CHECK(!given.defined() || (given.scalar_type() == torch::kFloat32 && given.numel() == 1), "norm must be a float32 scalar");
+  TORCH_CHECK(outputs.size() == grads.size(), "outputs must have a tensor per gradient");
+  for (size_t i = 0; i < grads.size(); i++) {
+    TORCH_CHECK(outputs[i].defined() && outputs[i].sizes() == grads[i].sizes() && outputs[i].strides() == grads[i].strides() &&
+                    outputs[i].scalar_type() == grads[i].scalar_type(),
+                "outputs must have their gradients' shapes, strides and dtypes");
+    check_no_autograd(op, {&given}, {&outputs[i]});
+  }
+  require_device(grads[0], op);
+  check_device(grads[0], {&given});
+  for (const torch::Tensor& o : outputs) check_device(grads[0], {&o});
+  TORCH_CHECK(!written_overlaps(grads, outputs, given), "outputs may not overlap other gradients, each other or norm");
+  c10::DeviceGuard guard(grads[0].device());
+  grad_pointers(l, grads);
+  for (const torch::Tensor& o : outputs) l.out.push_back(o.data_ptr());
+  torch::Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32).requires_grad(false));
+  int rc = esmoe_clip_grad_norm(l.in.data(), l.out.data(), l.dtypes.data(), l.sizes.data(), (int)l.in.size(), max_norm, eps,
+                                given.defined() ? given.data_ptr<float>() : nullptr, norm.data_ptr<float>(), l.workspace.data_ptr(),
+                                l.workspace.nbytes(), current_stream(grads[0]));
+  check_rc(rc, op);
+  return norm;
+}
+
 TORCH_LIBRARY(expert_specialization, m) {
   m.def(
       "es_fp8_blockwise_scaled_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor scales_a, Tensor scales_b, Tensor "
@@ -836,6 +1109,24 @@ TORCH_LIBRARY(expert_specialization, m) {
       "Tensor, Tensor)");
   m.def("es_mxfp4_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
   m.def("es_mxfp4_grouped_mm_swiglu(Tensor output, Tensor a, Tensor b, Tensor sfb, Tensor problem_sizes, Tensor expert_offsets) -> ()");
+  m.def("es_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor problem_sizes, Tensor expert_offsets) -> ()");
+  m.def("es_grouped_mm_swiglu(Tensor output, Tensor a, Tensor b, Tensor problem_sizes, Tensor expert_offsets, Tensor? gate_up) -> ()");
+  m.def(
+      "es_grouped_mm_backward(Tensor grad_output, Tensor a, Tensor b, Tensor problem_sizes, Tensor expert_offsets, Tensor? grad_a, Tensor? "
+      "grad_b) -> ()");
+  m.def(
+      "es_grouped_mm_swiglu_backward(Tensor grad_output, Tensor a, Tensor b, Tensor gate_up, Tensor problem_sizes, Tensor expert_offsets, "
+      "Tensor? grad_a, Tensor? grad_b) -> ()");
+  m.def("es_int8_quant(Tensor input, Tensor quant_output, Tensor scales) -> ()");
+  m.def("es_int8_quant.new(Tensor input) -> (Tensor, Tensor)");
+  m.def(
+      "es_int8_scaled_grouped_mm(Tensor output, Tensor a, Tensor b, Tensor scales_a, Tensor scales_b, Tensor problem_sizes, Tensor "
+      "expert_offsets) -> ()");
+  m.def(
+      "es_int8_scaled_grouped_mm_swiglu(Tensor output, Tensor a, Tensor b, Tensor scales_a, Tensor scales_b, Tensor problem_sizes, Tensor "
+      "expert_offsets) -> ()");
+  m.def("es_grad_norm(Tensor[] grads) -> Tensor");
+  m.def("es_clip_grad_norm(Tensor[] grads, float max_norm, float eps, Tensor? norm, Tensor[] outputs) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(expert_specialization, CUDA, m) {
@@ -860,6 +1151,16 @@ TORCH_LIBRARY_IMPL(expert_specialization, CUDA, m) {
   m.impl("es_add_rms_norm_quant_1x128.new", &es_add_rms_norm_quant_1x128_new);
   m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
   m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
+  m.impl("es_grouped_mm", &es_grouped_mm);
+  m.impl("es_grouped_mm_swiglu", &es_grouped_mm_swiglu);
+  m.impl("es_grouped_mm_backward", &es_grouped_mm_backward);
+  m.impl("es_grouped_mm_swiglu_backward", &es_grouped_mm_swiglu_backward);
+  m.impl("es_int8_quant", &es_int8_quant);
+  m.impl("es_int8_quant.new", &es_int8_quant_new);
+  m.impl("es_int8_scaled_grouped_mm", &es_int8_scaled_grouped_mm);
+  m.impl("es_int8_scaled_grouped_mm_swiglu", &es_int8_scaled_grouped_mm_swiglu);
+  m.impl("es_grad_norm", &es_grad_norm);
+  m.impl("es_clip_grad_norm", &es_clip_grad_norm);
 }
 
 // Same functions on the CPU key: the checks run, then require_device() raises.
@@ -885,4 +1186,14 @@ TORCH_LIBRARY_IMPL(expert_specialization, CPU, m) {
   m.impl("es_add_rms_norm_quant_1x128.new", &es_add_rms_norm_quant_1x128_new);
   m.impl("es_mxfp4_grouped_mm", &es_mxfp4_grouped_mm);
   m.impl("es_mxfp4_grouped_mm_swiglu", &es_mxfp4_grouped_mm_swiglu);
+  m.impl("es_grouped_mm", &es_grouped_mm);
+  m.impl("es_grouped_mm_swiglu", &es_grouped_mm_swiglu);
+  m.impl("es_grouped_mm_backward", &es_grouped_mm_backward);
+  m.impl("es_grouped_mm_swiglu_backward", &es_grouped_mm_swiglu_backward);
+  m.impl("es_int8_quant", &es_int8_quant);
+  m.impl("es_int8_quant.new", &es_int8_quant_new);
+  m.impl("es_int8_scaled_grouped_mm", &es_int8_scaled_grouped_mm);
+  m.impl("es_int8_scaled_grouped_mm_swiglu", &es_int8_scaled_grouped_mm_swiglu);
+  m.impl("es_grad_norm", &es_grad_norm);
+  m.impl("es_clip_grad_norm", &es_clip_grad_norm);
 }

@@ -209,3 +209,83 @@ def es_mxfp4_grouped_mm(output, a, b, sfb, problem_sizes, expert_offsets):
 def es_mxfp4_grouped_mm_swiglu(output, a, b, sfb, problem_sizes, expert_offsets):
     """es_mxfp4_grouped_mm of a gate_up projection (N = 2 * I, gate rows first) with output = silu(gate) * up of its fp32 sums, [M, I]."""
     _ns.es_mxfp4_grouped_mm_swiglu.default(output, a, b, sfb, problem_sizes, expert_offsets)
+
+
+def es_grouped_mm(output, a, b, problem_sizes, expert_offsets):
+    """Grouped product in 16 bits: output[off_e:off_e+M_e] = a[rows of e] @ b[e] with ``a`` bf16/fp16 [M, K] and ``b`` the (E, K, N) view of
+    weights [E, N, K], sums in fp32; metadata as es_fp8_blockwise_scaled_grouped_mm, N and K multiples of 8.  Rows of no expert are
+    left as they were.  No counterpart in the reference."""
+    _ns.es_grouped_mm.default(output, a, b, problem_sizes, expert_offsets)
+
+
+def es_grouped_mm_swiglu(output, a, b, problem_sizes, expert_offsets, gate_up=None):
+    """es_grouped_mm of a gate_up projection (N = 2 * I, gate rows first) with output = silu(gate) * up of its fp32 sums, [M, I].  gate_up:
+    a tensor [M, 2 * I] that receives the projections as well, which es_grouped_mm_swiglu_backward needs."""
+    _ns.es_grouped_mm_swiglu.default(output, a, b, problem_sizes, expert_offsets, gate_up)
+
+
+def _product_grads(a, b, grad_a, grad_b, need_grad_a, need_grad_b):
+    """Buffers for the gradients that are asked for."""
+    if need_grad_a and grad_a is None:
+        grad_a = torch.zeros_like(a)
+    if need_grad_b and grad_b is None and b.dim() == 3:   # (any other is refused by the operator)
+        e, k, n = b.shape
+        grad_b = torch.empty((e, n, k), dtype=b.dtype, device=b.device).transpose(1, 2)
+    return grad_a if need_grad_a else None, grad_b if need_grad_b else None
+
+
+def es_grouped_mm_backward(grad_output, a, b, problem_sizes, expert_offsets, grad_a=None, grad_b=None, need_grad_a=True, need_grad_b=True):
+    """Gradients of es_grouped_mm from grad_output [M, N]: (grad_a [M, K], grad_b, a (E, K, N) view as b is one).  Rows of a given grad_a that
+    belong to no expert are left as they were; in one that is allocated here they are zero.  grad_b is written whole, zero for an
+    expert without rows.  A gradient that is not needed is not computed, and None."""
+    grad_a, grad_b = _product_grads(a, b, grad_a, grad_b, need_grad_a, need_grad_b)
+    _ns.es_grouped_mm_backward.default(grad_output, a, b, problem_sizes, expert_offsets, grad_a, grad_b)
+    return grad_a, grad_b
+
+
+def es_grouped_mm_swiglu_backward(grad_output, a, b, gate_up, problem_sizes, expert_offsets, grad_a=None, grad_b=None, need_grad_a=True,
+                                  need_grad_b=True):
+    """Gradients of es_grouped_mm_swiglu from grad_output [M, I] and the gate_up that it wrote: (grad_a, grad_b) as es_grouped_mm_backward's.
+    The gradient of gate_up is rounded to its type on the way, into a buffer of the call's own."""
+    grad_a, grad_b = _product_grads(a, b, grad_a, grad_b, need_grad_a, need_grad_b)
+    _ns.es_grouped_mm_swiglu_backward.default(grad_output, a, b, gate_up, problem_sizes, expert_offsets, grad_a, grad_b)
+    return grad_a, grad_b
+
+
+def es_int8_quant(input, quant_output=None, scales=None):
+    """bf16/fp16 rows [..., K] -> (int8 [..., K], fp32 scales [...]): scale = max |x| / 127 of a row, q = x * 127 / max |x| to the nearest
+    integer, ties to even.  A row of zeros has scale 0, one with an infinity or a NaN the scale NaN, both with q = 0.  For activations
+    [M, K] and, a scale per output channel, for weights [E, N, K].  No counterpart in the reference."""
+    if quant_output is None and scales is None:
+        return _ns.es_int8_quant.new(input)
+    if quant_output is None:
+        quant_output = torch.empty(input.shape, dtype=torch.int8, device=input.device)
+    if scales is None:
+        scales = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
+    _ns.es_int8_quant.default(input, quant_output, scales)
+    return quant_output, scales
+
+
+def es_int8_scaled_grouped_mm(output, a, b, scales_a, scales_b, problem_sizes, expert_offsets):
+    """Grouped product in 8-bit integers: output = scales_a[row] * scales_b[e, column] * (a @ b[e]), the sum exact in int32; ``a`` int8 [M, K],
+    ``b`` the (E, K, N) view of int8 weights [E, N, K], scales_a fp32 [M], scales_b fp32 [E, N], output bf16/fp16 [M, N]; metadata as
+    es_fp8_blockwise_scaled_grouped_mm, N a multiple of 8, K of 16.  No counterpart in the reference."""
+    _ns.es_int8_scaled_grouped_mm.default(output, a, b, scales_a, scales_b, problem_sizes, expert_offsets)
+
+
+def es_int8_scaled_grouped_mm_swiglu(output, a, b, scales_a, scales_b, problem_sizes, expert_offsets):
+    """es_int8_scaled_grouped_mm of a gate_up projection (N = 2 * I, gate rows first) with output = silu(gate) * up of its scaled sums, [M, I]."""
+    _ns.es_int8_scaled_grouped_mm_swiglu.default(output, a, b, scales_a, scales_b, problem_sizes, expert_offsets)
+
+
+def es_grad_norm(grads):
+    """The norm over all elements of a list of gradients (fp32, bf16, fp16, mixed), as an fp32 scalar on their device; squares and sums in
+    64 bits.  No counterpart in the reference."""
+    return _ns.es_grad_norm.default(grads)
+
+
+def es_clip_grad_norm(grads, max_norm, eps=1e-6, norm=None, outputs=None):
+    """Scales a list of gradients down to max_norm: coef = max_norm / (norm + eps); each is multiplied by coef where that is less than 1 (or
+    NaN), in place or into `outputs`.  norm: a scalar on the device to go by instead of the gradients' own (the norm over several ranks).
+    Gives back the norm that was used.  Neither waits for the device.  No counterpart in the reference."""
+    return _ns.es_clip_grad_norm.default(grads, max_norm, eps, norm, grads if outputs is None else outputs)

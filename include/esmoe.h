@@ -41,13 +41,17 @@ extern "C" {
 #define ESMOE_SCORING_SOFTMAX 0
 #define ESMOE_SCORING_SIGMOID 1
 #define ESMOE_MAX_TOPK 64
+#define ESMOE_GRAD_BF16 0
+#define ESMOE_GRAD_FP16 1
+#define ESMOE_GRAD_FP32 2
 
 /* ABI revision of this header; esmoe_version() of a matching library reads "esmoe 0.<ESMOE_ABI> (gfx950)".
+ * 5: esmoe_grouped_mm, esmoe_swiglu_backward, esmoe_int8_grouped_mm, esmoe_int8_quant, the norm of gradients and their clipping added.
  * 4: esmoe_topk_gating, esmoe_combine_rows, their gradients, esmoe_add_rms_norm_quant_1x128 and esmoe_mxfp4_grouped_mm added.
  * 3: a null `workspace` selects the library's own; esmoe_stream_workspace added; the workspace layout gained an exit
  *    counter (same size).  2: the esmoe_host_* mirrors gained `kind` after `force_bm`; esmoe_gemm_workspace_bytes
  *    grew from 16 E + 80 to 16 E + 1296 bytes and the workspace must be 16-byte aligned. */
-#define ESMOE_ABI 4
+#define ESMOE_ABI 5
 
 /* Bytes of device scratch the GEMM entry points need for `num_experts` experts
  * (the device-built tile schedule and its hand-out counters).  The scratch must be 16-byte aligned (device allocations
@@ -347,6 +351,64 @@ int esmoe_add_rms_norm_quant_1x128(const void* in, int in_dtype, const void* res
  */
 int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, const uint8_t* sfb, const int32_t* problem_sizes,
                            const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream);
+
+/*
+ * Grouped product of the experts in 16 bits, and its gradients: what trains them, and serves them unquantised.
+ *   out[off_e + m, j] = cast( sum_c a[off_e + m, c] * b[e, j, c] )
+ *   swiglu != 0, n = 2 * inter, gate rows first: out[off_e + m, i] = cast( silu(gate) * up ) of the two fp32 sums, [total_rows, inter];
+ *     gate_up [total_rows, n] = cast(sums) as well, unless NULL: what the gradient needs
+ *   a [total_rows, k], b [E, n, k], out: bf16 or fp16 (dtype), 16-byte aligned, sums in fp32.
+ * n % 8 == 0 (% 16 with SwiGLU), k % 8 == 0, both up to 2^20; problem_sizes and expert_offsets as above, column 0 is used.  Rows of out
+ * that belong to no expert are not written.  Counts and offsets are cut at total_rows; where experts claim the same rows, whose product
+ * these get is open, and of more claims than an honest call can hold the last may not be served.
+ *
+ * esmoe_grouped_mm_backward, from grad_out [total_rows, n]:
+ *   grad_a[off_e + m, c] = cast( sum_j grad_out[off_e + m, j] * b[e, j, c] )    (rows that belong to no expert are not written)
+ *   grad_b[e, j, c] = cast( sum_m grad_out[off_e + m, j] * a[off_e + m, c] )    (every element is written; 0 for an expert without rows)
+ * grad_a or grad_b may be NULL: that one is not computed, and b or a may be NULL with it.
+ *
+ * esmoe_swiglu_backward: from grad_out [total_rows, inter] of silu(gate) * up and gate_up [total_rows, 2 * inter] the gradient
+ *   grad_gate_up = cast( grad_out * up * s * (1 + gate * (1 - s)) | grad_out * gate * s ), s = sigmoid(gate), in fp32; inter % 8 == 0.
+ *   grad_gate_up may be gate_up itself.  It is the grad_out that esmoe_grouped_mm_backward takes for a product with swiglu.
+ * No counterpart in the reference, which is forward only and 8-bit.
+ */
+int esmoe_grouped_mm(void* out, int dtype, const void* a, const void* b, const int32_t* problem_sizes, const int32_t* expert_offsets,
+                     int num_experts, int total_rows, int n, int k, int swiglu, void* gate_up, void* stream);
+int esmoe_grouped_mm_backward(const void* grad_out, int dtype, const void* a, const void* b, const int32_t* problem_sizes,
+                              const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, void* grad_a, void* grad_b,
+                              void* stream);
+int esmoe_swiglu_backward(const void* grad_out, const void* gate_up, int dtype, long total_rows, int inter, void* grad_gate_up, void* stream);
+
+/*
+ * Grouped product in 8-bit integers, a scale per row of a (token) and per row of b (channel):
+ *   out[off_e + m, j] = cast( sa[off_e + m] * sb[e, j] * sum_c a[off_e + m, c] * b[e, j, c] ), the sum in int32 and exact
+ *   swiglu != 0, n = 2 * inter, gate rows first: out[off_e + m, i] = cast( silu(gate) * up ) of the two scaled sums
+ *   a [total_rows, k], b [E, n, k] int8; sa [total_rows], sb [E, n] fp32; out bf16 or fp16 (out_dtype)
+ * k % 16 == 0 up to 65536; the rest as esmoe_grouped_mm.  esmoe_int8_quant makes rows (of a, or of weights) so:
+ *   scales[m] = max |in[m]| / 127, q[m, c] = in[m, c] * 127 / max |in[m]| rounded to nearest, ties to even (of the exact quotient); a row of
+ *   zeros gets scale 0 and zeros, one with an infinity or a NaN the scale NaN and zeros.  in bf16 or fp16, k % 16 == 0 up to 65536.
+ * No counterpart in the reference.
+ */
+int esmoe_int8_grouped_mm(void* out, int out_dtype, const void* a, const void* b, const float* sa, const float* sb, const int32_t* problem_sizes,
+                          const int32_t* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu, void* stream);
+int esmoe_int8_quant(const void* in, int in_dtype, void* q, float* scales, long total_rows, int k, void* stream);
+
+/*
+ * The norm over many gradients, and their clipping to a largest norm, between the backward pass and the optimizer's step.
+ *   norm = sqrt( sum of the squares of all elements ), squares and sums in 64 bits, rounded to fp32
+ *   coef = max_norm / (norm + eps); outputs[i] = grads[i] * coef (fp32, rounded once) where coef < 1 or NaN, else grads[i]
+ * grads, outputs (clipping), dtypes (ESMOE_GRAD_*) and sizes (elements) are HOST arrays of `count` entries, read before the call returns;
+ * the tensors they point to are device memory, dense, aligned to their elements.  outputs[i] may be grads[i] (in place; not written where
+ * coef >= 1), else it may overlap no gradient and no other output.  given_norm: a norm on the device to go by (of several ranks, say), NULL:
+ * that of the gradients.  norm: where it is written, on the device (clipping: NULL if it is not wanted).  max_norm may be infinite: outputs
+ * are then the gradients.  workspace: esmoe_grad_norm_workspace_bytes(count) bytes on the device, any contents, not shared by calls that may overlap.
+ * A call gives the same bytes every time.  No counterpart in the reference.
+ */
+size_t esmoe_grad_norm_workspace_bytes(int count);
+int esmoe_grad_norm(const void* const* grads, const int* dtypes, const long* sizes, int count, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int esmoe_clip_grad_norm(const void* const* grads, void* const* outputs, const int* dtypes, const long* sizes, int count, double max_norm,
+                         double eps, const float* given_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Host mirrors of the device-side tile schedule, for inspection and CPU tests; they touch no GPU.
