@@ -4,6 +4,7 @@
 
 namespace esmoe {
 
+constexpr int kMmExperts = 1024;   // at most (ESMOE_MAX_EXPERTS)
 enum { kMmBf16 = 0, kMmFp16 = 1, kMmInt8 = 2 };
 
 // out[m, j] = sum_c t[m, c] * w_e(j, c) for the rows m of expert e.

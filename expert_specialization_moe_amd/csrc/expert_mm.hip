@@ -6,122 +6,610 @@
 //   weights'        grad_b[e, j, c] = cast( sum_m grad_out[off_e + m, j] * a[off_e + m, c] ), 0 for an expert without rows
 //   int8            sums in int32 (exact), out = cast( sum * sa[off_e + m] * sb[e, j] )
 // The reference has 8-bit floating point products alone and no gradients.
+//
+// One persistent workgroup of eight wavefronts per CU; a tile is 256 output rows ("T" operand) x 256 output columns ("W" operand; with
+// SwiGLU 128 gate columns and the matching 128 up columns), the sum goes in steps of 128 bytes (64 16-bit elements).  A step's operands are
+// copied from memory straight into LDS, in four parts of 16 KB (W0, T0, W1, T1: the halves of each operand), two steps deep.
+//
+// The step is four phases, a quarter of the tile each: (T0, W0), (T0, W1), (T1, W0), (T1, W1).  A phase is a memory half (fragments LDS ->
+// registers, one part of a coming step memory -> LDS), a barrier, and a matrix half (16 MFMAs a wavefront), and a barrier.  The wavefronts
+// form two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the matrix cores the
+// other moves data.  What is read when, in phases since the step's first (the first quarter's W0 is read a phase early, so that every memory half has
+// four or eight fragment reads):
+//     phase            0           1           2           3
+//     fragments read   T0          W1          T1          W0 of the next step
+//     copy issued      T1 of +1    W0 of +2    T0 of +2    W1 of +2
+// Every part is copied into the place it had two steps before, at the earliest two phases after that was read: then both groups have
+// passed a barrier behind their waits for those reads.  It is read six phases after its copy was issued.  The memory half before, every
+// wavefront waits until its own share of it has arrived (ten younger copies may be in flight) and the two barriers up to the read tell
+// all others.
+//
+// The copies run on across tiles: their state is ahead of the one that multiplies, so that a tile begins with its first steps in LDS.
+// They go through buffer descriptors: what lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "expert_mm.h"
+#include "mxfp4_units.h"
 #include "swiglu.h"
+#include "wave_scan.h"
 
 namespace esmoe {
 
-template <int TYPE> struct MmType;
-template <> struct MmType<kMmBf16> { typedef __bf16 T; typedef float Acc; };
-template <> struct MmType<kMmFp16> { typedef _Float16 T; typedef float Acc; };
-template <> struct MmType<kMmInt8> { typedef int8_t T; typedef int Acc; };
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64, kDeep = 16;
+enum { kForward = 0, kSwiglu = 1, kSwigluSave = 2, kRowsGrad = 3, kWeightsGrad = 4 };
 
-__device__ __forceinline__ int rows_in_tensor(int m, int off, int total_rows) {
-  return off < 0 || off >= total_rows || m < 0 ? 0 : m > total_rows - off ? total_rows - off : m;
+constexpr int kMmThreads = 512;
+constexpr int kPart = 16384, kMmStage = 4 * kPart;   // a half of an operand's step in LDS; a step
+constexpr int kW0 = 0, kT0 = kPart, kW1 = 2 * kPart, kT1 = 3 * kPart;
+constexpr uint32_t kNowhere = 0x80000000u;           // an offset beyond every descriptor
+constexpr int kBias = 1024;                          // of descriptors: a copy's second half is 1024 bytes on in LDS and, by the same field, in memory
+
+template <int TYPE> struct MmAcc { typedef v4f T; };
+template <> struct MmAcc<kMmInt8> { typedef v4i T; };
+
+// A quarter of a step: acc[i][j] += rows of t[i] x columns of w[j], i < 4, j < 2, both halves of the step, at a wave priority above that of the memory
+// halves.  pairs: 2, or 1 for the first two i alone, or 0.  One statement with its branches inside: around the compiler's own matrix instructions a
+// condition makes it copy the accumulators.  Between two products of one accumulator stand three others; whoever reads it next has to
+// wait (mm_results).
+#define ESMOE_MMA(op, i, j, ks) op " %[c" #i #j "], %[w" #j #ks "], %[t" #i #ks "], %[c" #i #j "]\n\t"
+#define ESMOE_MMA8(op, i0, i1)                                                                                                          \
+  ESMOE_MMA(op, i0, 0, 0) ESMOE_MMA(op, i0, 1, 0) ESMOE_MMA(op, i1, 0, 0) ESMOE_MMA(op, i1, 1, 0)                                        \
+  ESMOE_MMA(op, i0, 0, 1) ESMOE_MMA(op, i0, 1, 1) ESMOE_MMA(op, i1, 0, 1) ESMOE_MMA(op, i1, 1, 1)
+#define ESMOE_QUARTER(op)                                                                                                              \
+  asm volatile("s_cmp_eq_u32 %[pairs], 0\n\ts_cbranch_scc1 .Lesmoe_mma%=\n\ts_setprio 1\n\t" ESMOE_MMA8(op, 0, 1)                       \
+               "s_cmp_eq_u32 %[pairs], 1\n\ts_cbranch_scc1 .Lesmoe_mma%=\n\t" ESMOE_MMA8(op, 2, 3) ".Lesmoe_mma%=:\n\ts_setprio 0"      \
+               : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]), [c20] "+v"(c[2][0]),               \
+                 [c21] "+v"(c[2][1]), [c30] "+v"(c[3][0]), [c31] "+v"(c[3][1])                                                         \
+               : [w00] "v"(w[0][0]), [w01] "v"(w[0][1]), [w10] "v"(w[1][0]), [w11] "v"(w[1][1]), [t00] "v"(t[0][0]), [t01] "v"(t[0][1]), \
+                 [t10] "v"(t[1][0]), [t11] "v"(t[1][1]), [t20] "v"(t[2][0]), [t21] "v"(t[2][1]), [t30] "v"(t[3][0]), [t31] "v"(t[3][1]), \
+                 [pairs] "s"(pairs)                                                                                                    \
+               : "scc")
+template <int TYPE>
+__device__ __forceinline__ void quarter(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int pairs) {
+  if constexpr (TYPE == kMmInt8) ESMOE_QUARTER("v_mfma_i32_16x16x64_i8");
+  else if constexpr (TYPE == kMmFp16) ESMOE_QUARTER("v_mfma_f32_16x16x32_f16");
+  else ESMOE_QUARTER("v_mfma_f32_16x16x32_bf16");
+}
+// In front of the first vector instruction that reads or writes an accumulator: the last product's result is there 7 issue slots on.
+__device__ __forceinline__ void mm_results() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// One element of the output per thread and quarter; both operands staged through LDS, kDeep of the sum at a time.
-template <int TYPE, typename FT, typename FW>
-__device__ __forceinline__ void tile_product(int depth, FT&& t_at, FW&& w_at, typename MmType<TYPE>::Acc (&acc)[4][4]) {
-  typedef typename MmType<TYPE>::Acc Acc;
-  __shared__ Acc s_t[kDeep][kTile + 1], s_w[kDeep][kTile + 1];
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) acc[i][j] = 0;
-  for (int c0 = 0; c0 < depth; c0 += kDeep) {
-    for (int u = tid; u < kTile * kDeep; u += 256) {
-      const int i = u / kDeep, c = u % kDeep;
-      s_t[c][i] = c0 + c < depth ? t_at(i, c0 + c) : (Acc)0;
-      s_w[c][i] = c0 + c < depth ? w_at(i, c0 + c) : (Acc)0;
-    }
-    __syncthreads();
-    for (int c = 0; c < kDeep; c++)
-      for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) acc[i][j] += s_t[c][ty * 4 + i] * s_w[c][tx + 16 * j];
-    __syncthreads();
-  }
+struct MmShared {
+  uint8_t ring[2 * kMmStage];
+  int rows[kMmExperts], off[kMmExperts];
+  uint32_t full_end[kMmExperts], rest_end[kMmExperts];   // weights' gradient: full_end is the experts by falling rows
+  uint32_t full, rest;
+};
+static_assert(sizeof(MmShared) <= 160 * 1024, "LDS");
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <int N>
+__device__ __forceinline__ void mm_wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0) ; explicit" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mm_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// WT: the sum runs along w's columns (the rows' gradient).  SWIGLU: 32 gate columns and the matching 32 up columns a tile.
-template <int TYPE, bool WT, bool SWIGLU>
-__global__ void __launch_bounds__(256) expert_rows_kernel(ExpertMmArgs g) {
-  typedef typename MmType<TYPE>::T T;
-  typedef typename MmType<TYPE>::Acc Acc;
-  const int depth = WT ? g.n : g.k, cols = WT ? g.k : g.n, wide = SWIGLU ? cols / 2 : cols;
-  int unit = blockIdx.y, expert = -1, row0 = 0, rows = 0;
-  for (int e = 0; e < g.num_experts; e++) {
-    const int off = g.expert_offsets[e], m = rows_in_tensor(g.problem_sizes[e * 3], off, g.total_rows), tiles = (m + kTile - 1) / kTile;
-    if (unit < tiles) {
-      expert = e;
-      row0 = off + unit * kTile;
-      rows = m - unit * kTile;
-      break;
+// Two copies of 64 x 16 bytes into LDS, at lds and 1024 behind it.
+__device__ __forceinline__ void mm_copy2(uint32_t lds, v4i rsrc, uint32_t v0, uint32_t v1) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\tbuffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
+               ::"s"(lds), "v"(v0), "v"(v1), "s"(rsrc) : "memory");   // (the compiler keeps nothing in m0)
+}
+
+struct MmTile {
+  int expert;
+  int row0, rows;   // of the tensor of rows (weights' gradient: of an expert's weights)
+  int col0;         // of the output
+  int steps;
+};
+
+// Where a launch's tiles lie.  Full tiles (more than 128 rows) first, then the experts' short ends; the weights' gradient: by falling
+// number of rows.  Position p of the order belongs to round p / grid; odd rounds are dealt backwards, so that what a round is uneven in evens out.
+template <int TYPE, int KIND>
+struct MmTiles {
+  const MmShared& s;
+  const ExpertMmArgs& g;
+  int cols, col_tiles, row_tiles;
+  uint32_t total, full_tiles;
+
+  static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
+  static constexpr int kWide = kSw ? 128 : 256;
+
+  __device__ __forceinline__ MmTiles(const MmShared& s_, const ExpertMmArgs& g_) : s(s_), g(g_) {
+    cols = kSw ? g.n / 2 : KIND >= kRowsGrad ? g.k : g.n;
+    col_tiles = (cols + kWide - 1) / kWide;
+    row_tiles = (g.n + 255) / 256;
+    if constexpr (KIND == kWeightsGrad) {
+      total = (uint32_t)g.num_experts * row_tiles * col_tiles;
+      full_tiles = 0;
+    } else {
+      full_tiles = (uint32_t)uniform((int)s.full) * col_tiles;
+      total = full_tiles + (uint32_t)uniform((int)s.rest) * col_tiles;
     }
-    unit -= tiles;
   }
-  if (expert < 0) return;
-  const int col0 = blockIdx.x * (SWIGLU ? kTile / 2 : kTile);
-  const T* t = (const T*)g.t + (long)row0 * depth;
-  const T* w = (const T*)g.w + (long)expert * g.n * g.k;
-  auto col_of = [&](int j) { return SWIGLU ? (j & 31) + col0 + (j >> 5) * wide : j + col0; };
-  Acc acc[4][4];
-  tile_product<TYPE>(depth, [&](int i, int c) { return i < rows ? (Acc)t[(long)i * depth + c] : (Acc)0; },
-                     [&](int j, int c) {
-                       if ((SWIGLU ? (j & 31) : j) + col0 >= wide) return (Acc)0;
-                       return (Acc)w[WT ? (long)c * cols + col_of(j) : (long)col_of(j) * depth + c];
-                     }, acc);
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  for (int i = 0; i < 4; i++) {
-    const int m = ty * 4 + i;
-    if (m >= rows) continue;
-    const long row = row0 + m;
-    float v[4];
-    for (int j = 0; j < 4; j++) {
-      v[j] = (float)acc[i][j];
-      if constexpr (TYPE == kMmInt8) {
-        const int c = col_of(tx + 16 * j);
-        v[j] = v[j] * g.sa[row] * (c < cols ? g.sb[(long)expert * g.n + c] : 0.f);
+
+  __device__ __forceinline__ uint32_t position(uint32_t round) const {
+    const uint32_t w = blockIdx.x, n = gridDim.x;
+    // (workgroups go to the eight XCDs in turn: a round's neighbours are dealt to one)
+    const uint32_t i = n % 8 ? w : (w & 7) * (n / 8) + (w >> 3);
+    return round * n + (round & 1 ? n - 1 - i : i);
+  }
+
+  __device__ __forceinline__ MmTile at(uint32_t p) const {
+    MmTile t;
+    if constexpr (KIND == kWeightsGrad) {
+      const uint32_t per = (uint32_t)row_tiles * col_tiles, rank = p / per, i = p - rank * per;
+      t.expert = uniform((int)s.full_end[rank]);
+      const int r = i / col_tiles;
+      t.row0 = r * 256;
+      t.rows = g.n - t.row0 < 256 ? g.n - t.row0 : 256;
+      t.col0 = ((int)i - r * col_tiles) * 256;
+      t.steps = (uniform(s.rows[t.expert]) + 63) >> 6;
+      return t;
+    } else {
+      const bool full = p < full_tiles;
+      uint32_t unit, col;
+      if (full) {   // four units a group, a column's tiles together
+        const uint32_t group = p / (4 * col_tiles), i = p - group * 4 * col_tiles, have = full_tiles / col_tiles - 4 * group,
+                       wide = have < 4 ? have : 4;
+        col = i / wide;
+        unit = 4 * group + i - col * wide;
+      } else {
+        const uint32_t i = p - full_tiles;
+        unit = i / col_tiles;
+        col = i - unit * col_tiles;
+      }
+      const uint32_t* ends = full ? s.full_end : s.rest_end;
+      const int lane = threadIdx.x & 63;
+      int e = 0;
+      uint32_t before = 0;
+      for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+        const uint32_t end = e0 + lane < g.num_experts ? ends[e0 + lane] : 0xffffffffu;
+        const unsigned long long past = __ballot(end > unit);
+        if (past) {
+          const int l = __builtin_ctzll(past);
+          e = e0 + l;
+          if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
+          break;
+        }
+        before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+      }
+      e = e < g.num_experts ? e : g.num_experts - 1;
+      const int m = uniform(s.rows[e]), first = full ? (int)(unit - before) * 256 : m & ~255;
+      t.expert = e;
+      t.row0 = uniform(s.off[e]) + first;
+      t.rows = m - first < 256 ? m - first : 256;
+      t.col0 = (int)col * kWide;
+      t.steps = KIND == kRowsGrad ? (g.n + 63) >> 6 : TYPE == kMmInt8 ? (g.k + 127) >> 7 : (g.k + 63) >> 6;
+      return t;
+    }
+  }
+};
+
+// Reads the experts' rows and offsets, cut at the tensor's, and puts the tiles in order.
+template <int KIND>
+__device__ __forceinline__ void mm_schedule(MmShared& s, const ExpertMmArgs& g) {
+  const int tid = threadIdx.x;
+  for (int e = tid; e < g.num_experts; e += kMmThreads) {
+    const int off = g.expert_offsets[e];
+    s.rows[e] = fp4_rows(g.problem_sizes[e * 3], off, g.total_rows);
+    s.off[e] = off;
+  }
+  __syncthreads();
+  if constexpr (KIND == kWeightsGrad) {
+    for (int e = tid; e < g.num_experts; e += kMmThreads) {
+      const int m = s.rows[e];
+      int rank = 0;
+      for (int j = 0; j < g.num_experts; j++) rank += s.rows[j] > m || (s.rows[j] == m && j < e);
+      s.full_end[rank] = (uint32_t)e;
+    }
+  } else if (tid < 64) {
+    uint32_t full = 0, rest = 0;
+    for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+      const int e = e0 + tid, m = e < g.num_experts ? s.rows[e] : 0, end = m & 255;
+      const uint32_t f = sum_or_most(full, wave_inclusive_sum_or_most((uint32_t)(m >> 8) + (end > 128 ? 1u : 0u)));
+      const uint32_t r = sum_or_most(rest, wave_inclusive_sum_or_most(end && end <= 128 ? 1u : 0u));
+      if (e < g.num_experts) {
+        s.full_end[e] = f;
+        s.rest_end[e] = r;
+      }
+      full = (uint32_t)__builtin_amdgcn_readlane((int)f, 63);
+      rest = (uint32_t)__builtin_amdgcn_readlane((int)r, 63);
+    }
+    if (tid == 0) {   // no more than experts with rows of their own can have
+      const uint32_t most_full = (uint32_t)(g.total_rows / 129), most_rest = (uint32_t)(g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+      s.full = full < most_full ? full : most_full;
+      s.rest = rest < most_rest ? rest : most_rest;
+    }
+  }
+  __syncthreads();
+}
+
+// The copies' state: the tile and the step that they are at, as buffer descriptors and lane offsets.
+template <int TYPE, int KIND>
+struct MmCopies {
+  static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
+  static constexpr bool kTT = KIND == kWeightsGrad, kWT = KIND >= kRowsGrad;   // the operand's rows run along the sum
+  static constexpr int kSize = TYPE == kMmInt8 ? 1 : 2;
+  const MmTiles<TYPE, KIND>& tiles;
+  uint32_t round, lds;
+  int left, depth_left;        // steps; of the sum, rows of a transposed operand
+  uint64_t t_base, w_base;
+  uint64_t w1_base;            // SwiGLU: the up rows
+  int t_len, w_len, w1_len, t_pitch, w_pitch, t_col, w_col;
+  uint32_t vt[2][2], vw[2][2];   // lane offsets of [half][copy]
+  uint32_t tail[2], edge_t[2], edge_w[2];   // kNowhere where a lane's columns lie beyond the sum (last step) or the tensor
+  uint32_t mt[2][2], mw[2][2];
+
+  __device__ __forceinline__ MmCopies(const MmTiles<TYPE, KIND>& tiles_, uint32_t ring) : tiles(tiles_) {
+    const ExpertMmArgs& g = tiles.g;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    lds = ring + wave * 2048;
+    t_pitch = (KIND >= kRowsGrad ? g.n : g.k) * kSize;
+    w_pitch = g.k * kSize;
+    const int depth_bytes = (KIND == kRowsGrad ? g.n : g.k) * kSize;   // of rows along which the sum runs
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      // 128-byte rows, eight a copy: lane l fetches what belongs in slot l % 8 of row l / 8 (the slot of chunk x of row r is x ^ (r / 2 % 8):
+      // sixteen rows' reads of one chunk fall on different banks)
+      const int row = wave * 16 + c * 8 + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+      // 256-byte rows, four a copy: pairs of 16-byte chunks change places by the row's bits 0, 1 and 3
+      const int trow = wave * 8 + c * 4 + (lane >> 4), tchunk = (lane & 15) ^ (((trow & 3) | (trow >> 1 & 4)) << 1);
+      tail[c] = (depth_bytes & 127) && chunk * 16 >= (depth_bytes & 127) ? kNowhere : 0;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        vt[h][c] = (kTT ? trow * t_pitch + h * 256 + tchunk * 16 : (h * 128 + row) * t_pitch + chunk * 16) + (c ? 0 : kBias);
+        vw[h][c] = (kWT ? trow * w_pitch + h * 256 + tchunk * 16 : (h * 128 * !kSw + row) * w_pitch + chunk * 16) + (c ? 0 : kBias);
       }
     }
-    auto put = [&](void* p, long at, float x) {
-      if (TYPE == kMmFp16 || (TYPE == kMmInt8 && g.out_fp16)) ((_Float16*)p)[at] = (_Float16)x;
-      else ((__bf16*)p)[at] = (__bf16)x;
-    };
-    for (int j = 0; j < (SWIGLU ? 2 : 4); j++) {
-      const int c = col0 + tx + 16 * j;
-      if (c >= wide) continue;
-      if constexpr (SWIGLU) {
-        if (g.gate_up) {
-          put(g.gate_up, row * cols + c, v[j]);
-          put(g.gate_up, row * cols + wide + c, v[j + 2]);
+    round = 0;
+    left = 0;
+    next_tile();
+  }
+
+  __device__ __forceinline__ void next_tile() {
+    const ExpertMmArgs& g = tiles.g;
+    MmTile t;
+    do {   // (tiles without rows have nothing to copy; the weights' gradient alone has them, behind all others)
+      const uint32_t p = tiles.position(round++);
+      if (round > (tiles.total + gridDim.x - 1) / gridDim.x) {
+        left = 1 << 30;
+        t_len = w_len = w1_len = 0;
+        depth_left = 0;
+        t_pitch = w_pitch = 0;
+        masks(false);
+        return;
+      }
+      if (p >= tiles.total) {
+        t.steps = 0;
+        continue;
+      }
+      t = tiles.at(p);
+    } while (t.steps == 0);
+    left = t.steps;
+    const long w_expert = (long)t.expert * g.n * g.k * kSize;
+    if constexpr (KIND == kWeightsGrad) {
+      depth_left = uniform(tiles.s.rows[t.expert]);
+      const long first = uniform(tiles.s.off[t.expert]);
+      t_col = t.row0 * 2;
+      w_col = t.col0 * 2;
+      t_base = (uint64_t)g.t + first * t_pitch + t_col - kBias;
+      w_base = (uint64_t)g.w + first * w_pitch + w_col - kBias;
+    } else {
+      t_base = (uint64_t)g.t + (long)t.row0 * t_pitch - kBias;
+      t_len = t.rows * t_pitch + kBias;
+      if constexpr (KIND == kRowsGrad) {
+        depth_left = g.n;
+        w_col = t.col0 * 2;
+        w_base = (uint64_t)g.w + w_expert + w_col - kBias;
+      } else {
+        const int left_rows = tiles.cols - t.col0, n = left_rows < (kSw ? 128 : 256) ? left_rows : (kSw ? 128 : 256);
+        w_base = (uint64_t)g.w + w_expert + (long)t.col0 * w_pitch - kBias;
+        w_len = n * w_pitch + kBias;
+        if constexpr (kSw) {
+          w1_base = w_base + (long)tiles.cols * w_pitch;
+          w1_len = w_len;
         }
-        put(g.out, row * wide + c, swiglu_f32(v[j], v[j + 2]));
-      } else put(g.out, row * wide + c, v[j]);
+      }
+    }
+    if constexpr (kTT || kWT) {
+      const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+      const int trow = wave * 8 + (lane >> 4), tchunk = (lane & 15) ^ (((trow & 3) | (trow >> 1 & 4)) << 1);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int at = h * 128 + tchunk * 8;   // the lane's first column in the tile
+        if constexpr (kTT) edge_t[h] = t.row0 + at >= g.n ? kNowhere : 0;
+        edge_w[h] = t.col0 + at >= g.k ? kNowhere : 0;
+      }
+      lengths();
+    }
+    masks(left == 1);
+  }
+
+  // Descriptors' lengths of transposed operands: the rows of this step that the sum has.
+  __device__ __forceinline__ void lengths() {
+    const int n = depth_left < 64 ? depth_left : 64;
+    if constexpr (kTT) t_len = n * t_pitch - t_col + kBias;
+    if constexpr (kWT) w_len = n * w_pitch - w_col + kBias;
+  }
+
+  __device__ __forceinline__ void masks(bool last) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        mt[h][c] = kTT ? edge_t[h] : last ? tail[c] : 0;
+        mw[h][c] = kWT ? edge_w[h] : last ? tail[c] : 0;
+      }
+  }
+
+  __device__ __forceinline__ void advance() {
+    if (--left == 0) {
+      next_tile();
+      return;
+    }
+    if constexpr (kTT) t_base += 64 * (long)t_pitch;
+    else {
+      t_base += 128;
+      t_len -= t_len ? 128 : 0;
+    }
+    if constexpr (kWT) {
+      w_base += 64 * (long)w_pitch;
+      depth_left -= 64;
+      if (depth_left > 0) lengths();
+    } else {
+      w_base += 128;
+      w_len -= w_len ? 128 : 0;
+      if constexpr (kSw) {
+        w1_base += 128;
+        w1_len -= w1_len ? 128 : 0;
+      }
+    }
+    if constexpr (!kTT || !kWT) masks(left == 1);
+  }
+
+  __device__ __forceinline__ static v4i descriptor(uint64_t base, int len) {
+    return v4i{uniform((int)base), uniform((int)(base >> 32) & 0xffff), uniform(len), 0x00020000};
+  }
+  template <int H>
+  __device__ __forceinline__ void issue_t(uint32_t stage) const {
+    mm_copy2(uniform(lds + stage + (H ? kT1 : kT0)), descriptor(t_base, t_len), vt[H][0] | mt[H][0], vt[H][1] | mt[H][1]);
+  }
+  template <int H>
+  __device__ __forceinline__ void issue_w(uint32_t stage) const {
+    const v4i rsrc = kSw && H ? descriptor(w1_base, w1_len) : descriptor(w_base, w_len);
+    mm_copy2(uniform(lds + stage + (H ? kW1 : kW0)), rsrc, vw[H][0] | mw[H][0], vw[H][1] | mw[H][1]);
+  }
+};
+
+// Lane addresses of fragments in a part: sixteen rows (or columns) each, a lane has 16 bytes along the sum for each half of the step.
+template <bool TRANSPOSED, int COUNT, int EVERY>
+struct MmFragments {
+  uint32_t at[TRANSPOSED ? COUNT : 1];
+  // first: the wavefront's first sixteen; the next ones are EVERY sixteens on
+  __device__ __forceinline__ MmFragments(uint32_t ring, int first) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    if constexpr (TRANSPOSED) {
+      // rows of 256 bytes along the sum; four lanes read 16 columns of a row, sixteen lanes of four rows, and the hardware hands lane i column i
+      const int f = (l16 >> 2) | (g & 1) << 2;
+#pragma unroll
+      for (int i = 0; i < COUNT; i++) at[i] = ring + (8 * g + (l16 >> 2)) * 256 + (((first + i * EVERY) ^ f) * 32) + (l16 & 3) * 8;
+    } else {
+      at[0] = ring + first * 2048 + l16 * 128 + ((g ^ (l16 >> 1)) * 16);
     }
   }
+  __device__ __forceinline__ void read(uint32_t part, v4i (&f)[COUNT][2]) const {
+#pragma unroll
+    for (int i = 0; i < COUNT; i++)
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        if constexpr (TRANSPOSED) {
+          typedef v4s __attribute__((address_space(3))) * Lds;
+          const uint32_t p = at[i] + part + ks * 8192;
+          const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)p)),
+                    hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(p + 1024)));
+          f[i][ks] = v4i{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+          typedef const v4i __attribute__((address_space(3))) * Lds;
+          f[i][ks] = *(Lds)(uintptr_t)((ks ? at[0] ^ 64 : at[0]) + part + i * EVERY * 2048);
+        }
+      }
+  }
+};
+
+__device__ __forceinline__ v2i mm_half4(v4f v, bool fp16) {
+  return fp16 ? __builtin_bit_cast(v2i, __builtin_convertvector(v, v4h)) : __builtin_bit_cast(v2i, __builtin_convertvector(v, v4bf));
+}
+// A lane of group gq = lane / 16 holds columns 4 gq .. + 4 of one row in each of two tiles of 16 columns.  Odd groups give their part of x for
+// the even neighbour's of y: groups 0 and 2 end with columns 0 .. 8 and 8 .. 16 of the first tile, groups 1 and 3 with those of the second.
+__device__ __forceinline__ v4i mm_pair(v2i x, v2i y) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
+  return v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) expert_weights_kernel(ExpertMmArgs g) {
-  typedef typename MmType<TYPE>::T T;
-  const int tiles_k = (g.k + kTile - 1) / kTile, expert = blockIdx.y;
-  const int n0 = blockIdx.x / tiles_k * kTile, k0 = blockIdx.x % tiles_k * kTile;
-  const int off = g.expert_offsets[expert], rows = rows_in_tensor(g.problem_sizes[expert * 3], off, g.total_rows);
-  const T *t = (const T*)g.t + (long)off * g.n, *w = (const T*)g.w + (long)off * g.k;
-  float acc[4][4];
-  tile_product<TYPE>(rows, [&](int i, int c) { return n0 + i < g.n ? (float)t[(long)c * g.n + n0 + i] : 0.f; },
-                     [&](int j, int c) { return k0 + j < g.k ? (float)w[(long)c * g.k + k0 + j] : 0.f; }, acc);
-  T* out = (T*)g.out + (long)expert * g.n * g.k;
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int r = n0 + threadIdx.x / 16 * 4 + i, c = k0 + threadIdx.x % 16 + 16 * j;
-      if (r < g.n && c < g.k) out[(long)r * g.k + c] = (T)acc[i][j];
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mm_buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+}
+
+// Stores of 16 bytes of a tile's outputs, always all of them: a lane whose row or columns lie beyond goes nowhere.
+struct MmOut {
+  __amdgpu_buffer_rsrc_t rsrc;
+  int pitch;
+  __device__ __forceinline__ MmOut(void* out, long row0, int rows, int col0, int cols) {
+    pitch = cols * 2;
+    rsrc = mm_buffer((char*)out + row0 * pitch + (long)col0 * 2, rows * pitch - col0 * 2);
+  }
+  // col: of the tile; room: columns that the output has from the tile's first on
+  __device__ __forceinline__ void put(v4i v, int row, int col, int room) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, col < room ? row * pitch + col * 2 : (int)kNowhere, 0, 0);
+  }
+};
+
+template <int TYPE, int KIND>
+__global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMmArgs g) {
+  typedef typename MmAcc<TYPE>::T Acc;
+  constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
+  constexpr int kStores = KIND == kSwiglu ? 8 : KIND == kSwigluSave ? 24 : 16;   // of a tile's epilogue, per wavefront
+  __shared__ MmShared s;
+  mm_schedule<KIND>(s, g);
+  const MmTiles<TYPE, KIND> tiles(s, g);
+  if (tiles.total == 0) return;   // (the whole launch)
+  const int wave = uniform(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, gq = lane >> 4;
+  const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s.ring;
+  MmCopies<TYPE, KIND> copies(tiles, ring);
+  const MmFragments<KIND == kWeightsGrad, 4, 2> t_at(ring, wm);         // sixteens 0, 2, 4, 6 of a half's 128 rows, or 1, 3, 5, 7
+  const MmFragments<(KIND >= kRowsGrad), 2, 1> w_at(ring, wn * 2);
+  v4i tf[4][2], wf0[2][2], wf1[2][2];
+  Acc acc[2][2][4][2];
+
+  copies.template issue_w<0>(0);
+  copies.template issue_t<0>(0);
+  copies.template issue_w<1>(0);
+  copies.template issue_t<1>(0);
+  copies.advance();
+  copies.template issue_w<0>(kMmStage);
+  copies.template issue_t<0>(kMmStage);
+  copies.template issue_w<1>(kMmStage);
+  mm_wait_copies<10>();
+  mm_barrier();
+  w_at.read(kW0, wf0);
+  if (wm) mm_barrier();   // this group runs a barrier behind from here on
+
+  uint32_t stage = 0;
+  bool stored = false;   // a tile's stores are younger than the copies that this step's waits are for
+  for (uint32_t round = 0, rounds = (tiles.total + gridDim.x - 1) / gridDim.x; round < rounds; round++) {
+    const uint32_t p = tiles.position(round);
+    if (p >= tiles.total) continue;
+    const MmTile t = tiles.at(p);
+    // pairs of sixteen rows that this group has in the upper and in the lower half
+    auto pairs_of = [&](int rows) { return uniform(rows <= wm * 16 ? 0 : rows <= 64 ? 1 : 2); };
+    const int upper = pairs_of(t.rows), lower = pairs_of(t.rows - 128);
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) acc[a][b][i][j] = Acc{0, 0, 0, 0};
+    auto arrived = [&] {
+      if (stored) mm_wait_copies<10 + kStores>();
+      else mm_wait_copies<10>();
+      mm_barrier();
+    };
+    for (int step = 0; step < t.steps; step++) {
+      t_at.read(stage + kT0, tf);
+      copies.template issue_t<1>(stage ^ kMmStage);
+      copies.advance();
+      arrived();
+      quarter<TYPE>(acc[0][0], wf0, tf, upper);
+      mm_barrier();
+
+      w_at.read(stage + kW1, wf1);
+      copies.template issue_w<0>(stage);
+      arrived();
+      quarter<TYPE>(acc[0][1], wf1, tf, upper);
+      mm_barrier();
+
+      t_at.read(stage + kT1, tf);
+      copies.template issue_t<0>(stage);
+      arrived();
+      quarter<TYPE>(acc[1][0], wf0, tf, lower);
+      mm_barrier();
+
+      w_at.read((stage ^ kMmStage) + kW0, wf0);
+      copies.template issue_w<1>(stage);
+      arrived();
+      quarter<TYPE>(acc[1][1], wf1, tf, lower);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (wf0: its place is copied into two phases on)
+      mm_barrier();
+      stage ^= kMmStage;
+      stored = false;
     }
+
+    mm_results();
+    // a lane holds, of rows a * 128 + (2 i + wm) * 16 + l16, columns b * 128 + wn * 32 + j * 16 + 4 gq .. + 4
+    const int room = tiles.cols - t.col0, col = wn * 32 + (gq & 1) * 16 + (gq >> 1) * 8;
+    const long out_row0 = KIND == kWeightsGrad ? (long)t.expert * g.n + t.row0 : (long)t.row0;
+    const MmOut out(g.out, out_row0, t.rows, t.col0, tiles.cols);
+    const bool fp16 = TYPE == kMmFp16 || (TYPE == kMmInt8 && g.out_fp16);
+    v4f sb[2][2];
+    if constexpr (TYPE == kMmInt8) {
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int first = kSw ? b * tiles.cols + t.col0 : t.col0 + b * 128;
+        const auto rsrc = mm_buffer(g.sb + (long)t.expert * g.n, g.n * 4);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          sb[b][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (first + wn * 32 + j * 16 + gq * 4) * 4, 0, 0));
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        __builtin_amdgcn_sched_barrier(0);   // (a row's values at a time: all at once are more than the registers)
+        const int row = a * 128 + (2 * i + wm) * 16 + l16;
+        float sa = 1.0f;
+        if constexpr (TYPE == kMmInt8)
+          sa = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mm_buffer(g.sa + t.row0, t.rows * 4), row * 4, 0, 0));
+        auto value = [&](int b, int j) {
+          const Acc sum = acc[a][b][i][j];
+          if constexpr (TYPE == kMmInt8) {
+            v4f v;
+#pragma unroll
+            for (int x = 0; x < 4; x++) v[x] = (float)sum[x] * sa * sb[b][j][x];
+            return v;
+          } else return sum;
+        };
+        if constexpr (kSw) {
+          v2i h[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const v4f gate = value(0, j), up = value(1, j);
+            v4f y;
+#pragma unroll
+            for (int x = 0; x < 4; x++) y[x] = swiglu_f32(gate[x], up[x]);
+            h[j] = mm_half4(y, fp16);
+          }
+          out.put(mm_pair(h[0], h[1]), row, col, room);
+          if constexpr (KIND == kSwigluSave) {
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+              const MmOut both(g.gate_up, t.row0, t.rows, b * tiles.cols + t.col0, g.n);
+              both.put(mm_pair(mm_half4(value(b, 0), fp16), mm_half4(value(b, 1), fp16)), row, col, room);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < 2; b++) out.put(mm_pair(mm_half4(value(b, 0), fp16), mm_half4(value(b, 1), fp16)), row, b * 128 + col, room);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    stored = true;
+  }
+  if (!wm) mm_barrier();
+  mm_wait_copies<0>();   // (nothing may arrive in LDS that is another workgroup's by then)
 }
 
 }  // namespace esmoe
@@ -131,19 +619,27 @@ using namespace esmoe;
 // kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 gradient of the weights
 extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cus, hipStream_t stream) {
   const ExpertMmArgs& g = *args;
-  const int cols = kind == 2 ? g.k : kind == 1 ? g.n / 2 : g.n, tile = kind == 1 ? kTile / 2 : kTile;
-  const dim3 grid((cols + tile - 1) / tile, g.num_experts + g.total_rows / kTile);
-#define ESMOE_MM(T)                                                                                             \
-  switch (kind) {                                                                                               \
-    case 0: hipLaunchKernelGGL((expert_rows_kernel<T, false, false>), grid, dim3(256), 0, stream, g); break;    \
-    case 1: hipLaunchKernelGGL((expert_rows_kernel<T, false, true>), grid, dim3(256), 0, stream, g); break;     \
-    case 2: hipLaunchKernelGGL((expert_rows_kernel<T, true, false>), grid, dim3(256), 0, stream, g); break;     \
-    default: hipLaunchKernelGGL((expert_weights_kernel<T>), dim3(((g.n + 63) / 64) * ((g.k + 63) / 64), g.num_experts), dim3(256), 0, stream, g); \
+  const long cols = kind >= 2 ? g.k : kind == 1 ? g.n / 2 : g.n, wide = kind == 1 ? 128 : 256, col_tiles = (cols + wide - 1) / wide;
+  const long units = kind == 3 ? (long)g.num_experts * ((g.n + 255) / 256)
+                               : g.total_rows / 129 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+  const long tiles = units * col_tiles, grid = tiles < cus ? tiles : cus;
+  if (grid == 0) return 0;
+#define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
+#define ESMOE_MM16(T)                                  \
+  switch (kind) {                                      \
+    case 0: ESMOE_MM(T, kForward); break;              \
+    case 1:                                            \
+      if (g.gate_up) ESMOE_MM(T, kSwigluSave);         \
+      else ESMOE_MM(T, kSwiglu);                       \
+      break;                                           \
+    case 2: ESMOE_MM(T, kRowsGrad); break;             \
+    default: ESMOE_MM(T, kWeightsGrad);                \
   }
-  if (g.type == kMmBf16) { ESMOE_MM(kMmBf16) }
-  else if (g.type == kMmFp16) { ESMOE_MM(kMmFp16) }
-  else if (kind == 0) hipLaunchKernelGGL((expert_rows_kernel<kMmInt8, false, false>), grid, dim3(256), 0, stream, g);
-  else hipLaunchKernelGGL((expert_rows_kernel<kMmInt8, false, true>), grid, dim3(256), 0, stream, g);
+  if (g.type == kMmBf16) { ESMOE_MM16(kMmBf16) }
+  else if (g.type == kMmFp16) { ESMOE_MM16(kMmFp16) }
+  else if (kind == 0) ESMOE_MM(kMmInt8, kForward);
+  else ESMOE_MM(kMmInt8, kSwiglu);
+#undef ESMOE_MM16
 #undef ESMOE_MM
   return (int)hipGetLastError();
 }
