@@ -96,9 +96,11 @@ static_assert(sizeof(MmShared) <= 160 * 1024, "LDS");
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Until the wavefront's fragments are there and at most N of its copies and stores are not.
 template <int N>
 __device__ __forceinline__ void mm_wait_copies() {
-  asm volatile("s_waitcnt vmcnt(%0) ; explicit" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0) ; explicit" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void mm_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -256,8 +258,8 @@ struct MmCopies {
   uint64_t w1_base;            // SwiGLU: the up rows
   int t_len, w_len, w1_len, t_pitch, w_pitch, t_col, w_col;
   uint32_t vt[2][2], vw[2][2];   // lane offsets of [half][copy]
-  uint32_t tail[2], edge_t[2], edge_w[2];   // kNowhere where a lane's columns lie beyond the sum (last step) or the tensor
-  uint32_t mt[2][2], mw[2][2];
+  // kNowhere where a lane's columns lie beyond the sum (in its last step) or, by half, beyond a transposed operand's columns
+  uint32_t tail[2], now[2], edge_t[2], edge_w[2];
 
   __device__ __forceinline__ MmCopies(const MmTiles<TYPE, KIND>& tiles_, uint32_t ring) : tiles(tiles_) {
     const ExpertMmArgs& g = tiles.g;
@@ -353,12 +355,7 @@ struct MmCopies {
 
   __device__ __forceinline__ void masks(bool last) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        mt[h][c] = kTT ? edge_t[h] : last ? tail[c] : 0;
-        mw[h][c] = kWT ? edge_w[h] : last ? tail[c] : 0;
-      }
+    for (int c = 0; c < 2; c++) now[c] = last ? tail[c] : 0;
   }
 
   __device__ __forceinline__ void advance() {
@@ -391,12 +388,12 @@ struct MmCopies {
   }
   template <int H>
   __device__ __forceinline__ void issue_t(uint32_t stage) const {
-    mm_copy2(uniform(lds + stage + (H ? kT1 : kT0)), descriptor(t_base, t_len), vt[H][0] | mt[H][0], vt[H][1] | mt[H][1]);
+    mm_copy2(uniform(lds + stage + (H ? kT1 : kT0)), descriptor(t_base, t_len), vt[H][0] | (kTT ? edge_t[H] : now[0]), vt[H][1] | (kTT ? edge_t[H] : now[1]));
   }
   template <int H>
   __device__ __forceinline__ void issue_w(uint32_t stage) const {
     const v4i rsrc = kSw && H ? descriptor(w1_base, w1_len) : descriptor(w_base, w_len);
-    mm_copy2(uniform(lds + stage + (H ? kW1 : kW0)), rsrc, vw[H][0] | mw[H][0], vw[H][1] | mw[H][1]);
+    mm_copy2(uniform(lds + stage + (H ? kW1 : kW0)), rsrc, vw[H][0] | (kWT ? edge_w[H] : now[0]), vw[H][1] | (kWT ? edge_w[H] : now[1]));
   }
 };
 
@@ -416,20 +413,24 @@ struct MmFragments {
       at[0] = ring + first * 2048 + l16 * 128 + ((g ^ (l16 >> 1)) * 16);
     }
   }
-  __device__ __forceinline__ void read(uint32_t part, v4i (&f)[COUNT][2]) const {
+  // PART: which of a step's parts
+  template <int PART>
+  __device__ __forceinline__ void read(uint32_t stage, v4i (&f)[COUNT][2]) const {
 #pragma unroll
     for (int i = 0; i < COUNT; i++)
 #pragma unroll
       for (int ks = 0; ks < 2; ks++) {
         if constexpr (TRANSPOSED) {
-          typedef v4s __attribute__((address_space(3))) * Lds;
-          const uint32_t p = at[i] + part + ks * 8192;
-          const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)p)),
-                    hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(p + 1024)));
+          typedef __attribute__((address_space(3))) char* Lds;
+          typedef v4s __attribute__((address_space(3))) * Lds4;
+          const Lds p = (Lds)(uintptr_t)(at[i] + stage) + PART + ks * 8192;
+          const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)p)),
+                    hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(p + 1024)));
           f[i][ks] = v4i{lo[0], lo[1], hi[0], hi[1]};
         } else {
-          typedef const v4i __attribute__((address_space(3))) * Lds;
-          f[i][ks] = *(Lds)(uintptr_t)((ks ? at[0] ^ 64 : at[0]) + part + i * EVERY * 2048);
+          typedef const __attribute__((address_space(3))) char* Lds;
+          typedef const v4i __attribute__((address_space(3))) * Lds16;
+          f[i][ks] = *(Lds16)((Lds)(uintptr_t)((ks ? at[0] ^ 64 : at[0]) + stage) + PART + i * EVERY * 2048);
         }
       }
   }
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   copies.template issue_w<1>(kMmStage);
   mm_wait_copies<10>();
   mm_barrier();
-  w_at.read(kW0, wf0);
+  w_at.template read<kW0>(0, wf0);
   if (wm) mm_barrier();   // this group runs a barrier behind from here on
 
   uint32_t stage = 0;
@@ -518,30 +519,29 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
       mm_barrier();
     };
     for (int step = 0; step < t.steps; step++) {
-      t_at.read(stage + kT0, tf);
+      t_at.template read<kT0>(stage, tf);
       copies.template issue_t<1>(stage ^ kMmStage);
       copies.advance();
       arrived();
       quarter<TYPE>(acc[0][0], wf0, tf, upper);
       mm_barrier();
 
-      w_at.read(stage + kW1, wf1);
+      w_at.template read<kW1>(stage, wf1);
       copies.template issue_w<0>(stage);
       arrived();
       quarter<TYPE>(acc[0][1], wf1, tf, upper);
       mm_barrier();
 
-      t_at.read(stage + kT1, tf);
+      t_at.template read<kT1>(stage, tf);
       copies.template issue_t<0>(stage);
       arrived();
       quarter<TYPE>(acc[1][0], wf0, tf, lower);
       mm_barrier();
 
-      w_at.read((stage ^ kMmStage) + kW0, wf0);
+      w_at.template read<kW0>(stage ^ kMmStage, wf0);
       copies.template issue_w<1>(stage);
       arrived();
       quarter<TYPE>(acc[1][1], wf1, tf, lower);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (wf0: its place is copied into two phases on)
       mm_barrier();
       stage ^= kMmStage;
       stored = false;
