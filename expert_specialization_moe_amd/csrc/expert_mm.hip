@@ -12,22 +12,25 @@
 // copied from memory straight into LDS, in four parts of 16 KB (W0, T0, W1, T1: the halves of each operand), two steps deep.
 //
 // The step is four phases, a quarter of the tile each: (T0, W0), (T0, W1), (T1, W0), (T1, W1).  A phase is a memory half (fragments LDS ->
-// registers, one part of a coming step memory -> LDS), a barrier, and a matrix half (16 MFMAs a wavefront), and a barrier.  The wavefronts
-// form two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the matrix cores the
-// other moves data.  What is read when, in phases since the step's first (the first quarter's W0 is read a phase early, so that every memory half has
-// four or eight fragment reads):
-//     phase            0           1           2           3
-//     fragments read   T0          W1          T1          W0 of the next step
-//     copy issued      T1 of +1    W0 of +2    T0 of +2    W1 of +2
-// Every part is copied into the place it had two steps before, at the earliest two phases after that was read: then both groups have
-// passed a barrier behind their waits for those reads.  It is read six phases after its copy was issued.  The memory half before, every
-// wavefront waits until its own share of it has arrived (ten younger copies may be in flight) and the two barriers up to the read tell
-// all others.
+// registers), a barrier, a matrix half (16 MFMAs a wavefront, a copy of one part of the step after next among them), and a barrier.  The
+// wavefronts form two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the
+// matrix cores the other moves data.  A phase's T fragments take the registers of those before as these are done with, so that every
+// memory half has four fragment reads (of sixteen rows x 64 bytes) a wavefront:
+//     phase                    0               1               2               3
+//     memory half reads        T0, 2nd half    W1              T1, 2nd half    W0 of the next step
+//     matrix half reads                        T1, 1st half                    T0 of the next step, 1st half
+//     matrix half copies       W0 of +2        T0 of +2        W1 of +2        T1 of +2
+// A part is copied into the place it had two steps before.  Its last reads were waited for in front of the barrier that ends a memory half, one
+// phase before the copy; the group behind has passed that barrier as well by then.  It is read again seven or eight phases on: in the memory
+// halves of phases 0 and 2 every wavefront waits until its own shares of what the next two phases read have arrived (the four younger copies
+// may be in flight), and the barriers between tell all others.
 //
 // The copies run on across tiles: their state is ahead of the one that multiplies, so that a tile begins with its first steps in LDS.
 // They go through buffer descriptors: what lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "expert_mm.h"
 #include "mxfp4_units.h"
@@ -56,28 +59,46 @@ constexpr int kBias = 1024;                          // of descriptors: a copy's
 template <int TYPE> struct MmAcc { typedef v4f T; };
 template <> struct MmAcc<kMmInt8> { typedef v4i T; };
 
-// A quarter of a step: acc[i][j] += rows of t[i] x columns of w[j], i < 4, j < 2, both halves of the step, at a wave priority above that of the memory
-// halves.  pairs: 2, or 1 for the first two i alone, or 0.  One statement with its branches inside: around the compiler's own matrix instructions a
-// condition makes it copy the accumulators.  Between two products of one accumulator stand three others; whoever reads it next has to
-// wait (mm_results).
+// What a copy of two times 64 x 16 bytes into LDS needs: lds and 1024 bytes behind it, a descriptor, the lanes' offsets.
+struct MmCopy {
+  uint32_t lds;
+  v4i rsrc;
+  uint32_t v0, v1;
+};
+#define ESMOE_COPY0 "buffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
+#define ESMOE_COPY1 "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024 lds\n\t"
+__device__ __forceinline__ void mm_copy(const MmCopy& p) {
+  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 0\n\t" ESMOE_COPY0 ESMOE_COPY1
+               ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory");   // (the compiler keeps nothing in m0)
+}
+
+// An eighth of a step: c[i][j] += rows of t[i] x columns of w[j], i < 2, j < 2, both halves of the step, at a wave priority above that of the
+// memory halves; COPY: behind the first products a copy.  Where `rows` is at most LIMIT: the copy alone.  One statement with its branches inside: around the
+// compiler's own matrix instructions a condition makes it copy the accumulators.  Between two products of one accumulator stand three
+// others; whoever reads it next has to wait (mm_results).
 #define ESMOE_MMA(op, i, j, ks) op " %[c" #i #j "], %[w" #j #ks "], %[t" #i #ks "], %[c" #i #j "]\n\t"
-#define ESMOE_MMA8(op, i0, i1)                                                                                                          \
-  ESMOE_MMA(op, i0, 0, 0) ESMOE_MMA(op, i0, 1, 0) ESMOE_MMA(op, i1, 0, 0) ESMOE_MMA(op, i1, 1, 0)                                        \
-  ESMOE_MMA(op, i0, 0, 1) ESMOE_MMA(op, i0, 1, 1) ESMOE_MMA(op, i1, 0, 1) ESMOE_MMA(op, i1, 1, 1)
-#define ESMOE_QUARTER(op)                                                                                                              \
-  asm volatile("s_cmp_eq_u32 %[pairs], 0\n\ts_cbranch_scc1 .Lesmoe_mma%=\n\ts_setprio 1\n\t" ESMOE_MMA8(op, 0, 1)                       \
-               "s_cmp_eq_u32 %[pairs], 1\n\ts_cbranch_scc1 .Lesmoe_mma%=\n\t" ESMOE_MMA8(op, 2, 3) ".Lesmoe_mma%=:\n\ts_setprio 0"      \
-               : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]), [c20] "+v"(c[2][0]),               \
-                 [c21] "+v"(c[2][1]), [c30] "+v"(c[3][0]), [c31] "+v"(c[3][1])                                                         \
-               : [w00] "v"(w[0][0]), [w01] "v"(w[0][1]), [w10] "v"(w[1][0]), [w11] "v"(w[1][1]), [t00] "v"(t[0][0]), [t01] "v"(t[0][1]), \
-                 [t10] "v"(t[1][0]), [t11] "v"(t[1][1]), [t20] "v"(t[2][0]), [t21] "v"(t[2][1]), [t30] "v"(t[3][0]), [t31] "v"(t[3][1]), \
-                 [pairs] "s"(pairs)                                                                                                    \
-               : "scc")
-template <int TYPE>
-__device__ __forceinline__ void quarter(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int pairs) {
-  if constexpr (TYPE == kMmInt8) ESMOE_QUARTER("v_mfma_i32_16x16x64_i8");
-  else if constexpr (TYPE == kMmFp16) ESMOE_QUARTER("v_mfma_f32_16x16x32_f16");
-  else ESMOE_QUARTER("v_mfma_f32_16x16x32_bf16");
+#define ESMOE_MMA_LOW(op) ESMOE_MMA(op, 0, 0, 0) ESMOE_MMA(op, 0, 1, 0)
+#define ESMOE_MMA_REST(op) ESMOE_MMA(op, 0, 0, 1) ESMOE_MMA(op, 0, 1, 1) ESMOE_MMA(op, 1, 0, 1) ESMOE_MMA(op, 1, 1, 1)
+#define ESMOE_MMA_IO                                                                                                                 \
+  [c00] "+v"(c[I][0]), [c01] "+v"(c[I][1]), [c10] "+v"(c[I + 1][0]), [c11] "+v"(c[I + 1][1])                                         \
+      : [w00] "v"(w[0][0]), [w01] "v"(w[0][1]), [w10] "v"(w[1][0]), [w11] "v"(w[1][1]), [t00] "v"(t[I][0]), [t01] "v"(t[I][1]),       \
+        [t10] "v"(t[I + 1][0]), [t11] "v"(t[I + 1][1])
+#define ESMOE_COPY_IN [lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc)
+#define ESMOE_EIGHTH(op)                                                                                                              \
+  if constexpr (COPY)                                                                                                                 \
+    asm volatile("s_mov_b32 m0, %[lds]\n\ts_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_copy%=\n\ts_setprio 1\n\t"          \
+                 ESMOE_MMA_LOW(op) ESMOE_COPY0 ESMOE_MMA(op, 1, 0, 0) ESMOE_MMA(op, 1, 1, 0) ESMOE_COPY1 ESMOE_MMA_REST(op)           \
+                 "s_branch .Lesmoe_end%=\n.Lesmoe_copy%=:\n\t" ESMOE_COPY0 ESMOE_COPY1 ".Lesmoe_end%=:"                               \
+                 : ESMOE_MMA_IO, ESMOE_COPY_IN, [rows] "s"(rows), [limit] "n"(LIMIT) : "scc", "memory");                              \
+  else                                                                                                                                \
+    asm volatile("s_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t"                                                 \
+                 ESMOE_MMA_LOW(op) ESMOE_MMA(op, 1, 0, 0) ESMOE_MMA(op, 1, 1, 0) ESMOE_MMA_REST(op)                                   \
+                 ".Lesmoe_end%=:\n\ts_setprio 0" : ESMOE_MMA_IO, [rows] "s"(rows), [limit] "n"(LIMIT) : "scc")
+template <int TYPE, int I, bool COPY, int LIMIT>
+__device__ __forceinline__ void eighth(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows, const MmCopy& p) {
+  if constexpr (TYPE == kMmInt8) { ESMOE_EIGHTH("v_mfma_i32_16x16x64_i8"); }
+  else if constexpr (TYPE == kMmFp16) { ESMOE_EIGHTH("v_mfma_f32_16x16x32_f16"); }
+  else { ESMOE_EIGHTH("v_mfma_f32_16x16x32_bf16"); }
 }
 // In front of the first vector instruction that reads or writes an accumulator: the last product's result is there 7 issue slots on.
 __device__ __forceinline__ void mm_results() {
@@ -102,18 +123,16 @@ __device__ __forceinline__ void mm_wait_copies() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0) ; explicit" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void mm_wait_fragments() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 __device__ __forceinline__ void mm_barrier() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
-}
-
-// Two copies of 64 x 16 bytes into LDS, at lds and 1024 behind it.
-__device__ __forceinline__ void mm_copy2(uint32_t lds, v4i rsrc, uint32_t v0, uint32_t v1) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\tbuffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
-               ::"s"(lds), "v"(v0), "v"(v1), "s"(rsrc) : "memory");   // (the compiler keeps nothing in m0)
 }
 
 struct MmTile {
@@ -253,13 +272,13 @@ struct MmCopies {
   static constexpr int kSize = TYPE == kMmInt8 ? 1 : 2;
   const MmTiles<TYPE, KIND>& tiles;
   uint32_t round, lds;
-  int left, depth_left;        // steps; of the sum, rows of a transposed operand
+  int left, depth_left, along;   // steps; of the sum, rows of a transposed operand; bytes of a step along rows
   uint64_t t_base, w_base;
   uint64_t w1_base;            // SwiGLU: the up rows
   int t_len, w_len, w1_len, t_pitch, w_pitch, t_col, w_col;
   uint32_t vt[2][2], vw[2][2];   // lane offsets of [half][copy]
   // kNowhere where a lane's columns lie beyond the sum (in its last step) or, by half, beyond a transposed operand's columns
-  uint32_t tail[2], now[2], edge_t[2], edge_w[2];
+  uint32_t tail[2], now[2], edge_t0, edge_t1, edge_w0, edge_w1;
 
   __device__ __forceinline__ MmCopies(const MmTiles<TYPE, KIND>& tiles_, uint32_t ring) : tiles(tiles_) {
     const ExpertMmArgs& g = tiles.g;
@@ -284,6 +303,7 @@ struct MmCopies {
     }
     round = 0;
     left = 0;
+    along = 128;
     next_tile();
   }
 
@@ -293,11 +313,9 @@ struct MmCopies {
     do {   // (tiles without rows have nothing to copy; the weights' gradient alone has them, behind all others)
       const uint32_t p = tiles.position(round++);
       if (round > (tiles.total + gridDim.x - 1) / gridDim.x) {
-        left = 1 << 30;
-        t_len = w_len = w1_len = 0;
+        left = 1 << 30;   // no more tiles: descriptors of nothing from here on
+        t_len = w_len = w1_len = along = 0;
         depth_left = 0;
-        t_pitch = w_pitch = 0;
-        masks(false);
         return;
       }
       if (p >= tiles.total) {
@@ -317,7 +335,7 @@ struct MmCopies {
       w_base = (uint64_t)g.w + first * w_pitch + w_col - kBias;
     } else {
       t_base = (uint64_t)g.t + (long)t.row0 * t_pitch - kBias;
-      t_len = t.rows * t_pitch + kBias;
+      t_len = uniform(t.rows * t_pitch + kBias);
       if constexpr (KIND == kRowsGrad) {
         depth_left = g.n;
         w_col = t.col0 * 2;
@@ -325,7 +343,7 @@ struct MmCopies {
       } else {
         const int left_rows = tiles.cols - t.col0, n = left_rows < (kSw ? 128 : 256) ? left_rows : (kSw ? 128 : 256);
         w_base = (uint64_t)g.w + w_expert + (long)t.col0 * w_pitch - kBias;
-        w_len = n * w_pitch + kBias;
+        w_len = uniform(n * w_pitch + kBias);
         if constexpr (kSw) {
           w1_base = w_base + (long)tiles.cols * w_pitch;
           w1_len = w_len;
@@ -335,12 +353,13 @@ struct MmCopies {
     if constexpr (kTT || kWT) {
       const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
       const int trow = wave * 8 + (lane >> 4), tchunk = (lane & 15) ^ (((trow & 3) | (trow >> 1 & 4)) << 1);
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int at = h * 128 + tchunk * 8;   // the lane's first column in the tile
-        if constexpr (kTT) edge_t[h] = t.row0 + at >= g.n ? kNowhere : 0;
-        edge_w[h] = t.col0 + at >= g.k ? kNowhere : 0;
+      const int at = tchunk * 8;   // the lane's first column in a half
+      if constexpr (kTT) {
+        edge_t0 = t.row0 + at >= g.n ? kNowhere : 0;
+        edge_t1 = t.row0 + at + 128 >= g.n ? kNowhere : 0;
       }
+      edge_w0 = t.col0 + at >= g.k ? kNowhere : 0;
+      edge_w1 = t.col0 + at + 128 >= g.k ? kNowhere : 0;
       lengths();
     }
     masks(left == 1);
@@ -354,8 +373,8 @@ struct MmCopies {
   }
 
   __device__ __forceinline__ void masks(bool last) {
-#pragma unroll
-    for (int c = 0; c < 2; c++) now[c] = last ? tail[c] : 0;
+    now[0] = last ? tail[0] : 0;
+    now[1] = last ? tail[1] : 0;
   }
 
   __device__ __forceinline__ void advance() {
@@ -366,7 +385,7 @@ struct MmCopies {
     if constexpr (kTT) t_base += 64 * (long)t_pitch;
     else {
       t_base += 128;
-      t_len -= t_len ? 128 : 0;
+      t_len -= along;
     }
     if constexpr (kWT) {
       w_base += 64 * (long)w_pitch;
@@ -374,26 +393,27 @@ struct MmCopies {
       if (depth_left > 0) lengths();
     } else {
       w_base += 128;
-      w_len -= w_len ? 128 : 0;
+      w_len -= along;
       if constexpr (kSw) {
         w1_base += 128;
-        w1_len -= w1_len ? 128 : 0;
+        w1_len -= along;
       }
     }
     if constexpr (!kTT || !kWT) masks(left == 1);
   }
 
   __device__ __forceinline__ static v4i descriptor(uint64_t base, int len) {
-    return v4i{uniform((int)base), uniform((int)(base >> 32) & 0xffff), uniform(len), 0x00020000};
+    return v4i{uniform((int)base), uniform((int)(base >> 32)), uniform(len), 0x00020000};
   }
   template <int H>
-  __device__ __forceinline__ void issue_t(uint32_t stage) const {
-    mm_copy2(uniform(lds + stage + (H ? kT1 : kT0)), descriptor(t_base, t_len), vt[H][0] | (kTT ? edge_t[H] : now[0]), vt[H][1] | (kTT ? edge_t[H] : now[1]));
+  __device__ __forceinline__ MmCopy t_part(uint32_t stage) const {
+    return {(uint32_t)uniform(lds + stage + (H ? kT1 : kT0)), descriptor(t_base, t_len), vt[H][0] | (kTT ? (H ? edge_t1 : edge_t0) : now[0]),
+            vt[H][1] | (kTT ? (H ? edge_t1 : edge_t0) : now[1])};
   }
   template <int H>
-  __device__ __forceinline__ void issue_w(uint32_t stage) const {
-    const v4i rsrc = kSw && H ? descriptor(w1_base, w1_len) : descriptor(w_base, w_len);
-    mm_copy2(uniform(lds + stage + (H ? kW1 : kW0)), rsrc, vw[H][0] | (kWT ? edge_w[H] : now[0]), vw[H][1] | (kWT ? edge_w[H] : now[1]));
+  __device__ __forceinline__ MmCopy w_part(uint32_t stage) const {
+    return {(uint32_t)uniform(lds + stage + (H ? kW1 : kW0)), kSw && H ? descriptor(w1_base, w1_len) : descriptor(w_base, w_len),
+            vw[H][0] | (kWT ? (H ? edge_w1 : edge_w0) : now[0]), vw[H][1] | (kWT ? (H ? edge_w1 : edge_w0) : now[1])};
   }
 };
 
@@ -413,11 +433,11 @@ struct MmFragments {
       at[0] = ring + first * 2048 + l16 * 128 + ((g ^ (l16 >> 1)) * 16);
     }
   }
-  // PART: which of a step's parts
-  template <int PART>
+  // PART: which of a step's parts; the sixteens FROM .. TO
+  template <int PART, int FROM = 0, int TO = COUNT>
   __device__ __forceinline__ void read(uint32_t stage, v4i (&f)[COUNT][2]) const {
 #pragma unroll
-    for (int i = 0; i < COUNT; i++)
+    for (int i = FROM; i < TO; i++)
 #pragma unroll
       for (int ks = 0; ks < 2; ks++) {
         if constexpr (TRANSPOSED) {
@@ -483,17 +503,17 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   v4i tf[4][2], wf0[2][2], wf1[2][2];
   Acc acc[2][2][4][2];
 
-  copies.template issue_w<0>(0);
-  copies.template issue_t<0>(0);
-  copies.template issue_w<1>(0);
-  copies.template issue_t<1>(0);
-  copies.advance();
-  copies.template issue_w<0>(kMmStage);
-  copies.template issue_t<0>(kMmStage);
-  copies.template issue_w<1>(kMmStage);
-  mm_wait_copies<10>();
+  for (int i = 0; i < 2; i++) {
+    if (i) copies.advance();
+    mm_copy(copies.template w_part<0>(i * kMmStage));
+    mm_copy(copies.template t_part<0>(i * kMmStage));
+    mm_copy(copies.template w_part<1>(i * kMmStage));
+    mm_copy(copies.template t_part<1>(i * kMmStage));
+  }
+  mm_wait_copies<12>();
   mm_barrier();
   w_at.template read<kW0>(0, wf0);
+  t_at.template read<kT0, 0, 2>(0, tf);
   if (wm) mm_barrier();   // this group runs a barrier behind from here on
 
   uint32_t stage = 0;
@@ -502,9 +522,6 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
     const uint32_t p = tiles.position(round);
     if (p >= tiles.total) continue;
     const MmTile t = tiles.at(p);
-    // pairs of sixteen rows that this group has in the upper and in the lower half
-    auto pairs_of = [&](int rows) { return uniform(rows <= wm * 16 ? 0 : rows <= 64 ? 1 : 2); };
-    const int upper = pairs_of(t.rows), lower = pairs_of(t.rows - 128);
 #pragma unroll
     for (int a = 0; a < 2; a++)
 #pragma unroll
@@ -514,35 +531,49 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
 #pragma unroll
           for (int j = 0; j < 2; j++) acc[a][b][i][j] = Acc{0, 0, 0, 0};
     auto arrived = [&] {
-      if (stored) mm_wait_copies<10 + kStores>();
-      else mm_wait_copies<10>();
+      if (stored) mm_wait_copies<8 + kStores>();
+      else mm_wait_copies<8>();
       mm_barrier();
     };
-    for (int step = 0; step < t.steps; step++) {
-      t_at.template read<kT0>(stage, tf);
-      copies.template issue_t<1>(stage ^ kMmStage);
-      copies.advance();
-      arrived();
-      quarter<TYPE>(acc[0][0], wf0, tf, upper);
+    auto read = [&] {
+      mm_wait_fragments();
       mm_barrier();
+    };
+    // A phase's matrix half, of the tile's upper or lower half of rows; behind its first products the first half of the next fragments of T, into
+    // the registers that these leave.  A group whose sixteens have no rows has nothing to multiply.
+    const int rows = t.rows - wm * 16;
+    auto multiply = [&](auto lower, Acc (&c)[4][2], const v4i (&w)[2][2], const MmCopy& copy, auto&& early) {
+      constexpr int kFirst = decltype(lower)::value * 128;
+      eighth<TYPE, 0, true, kFirst>(c, w, tf, rows, copy);
+      __builtin_amdgcn_sched_barrier(0);
+      early();
+      __builtin_amdgcn_sched_barrier(0);
+      eighth<TYPE, 2, false, kFirst + 64>(c, w, tf, rows, copy);
+      mm_barrier();
+    };
+    constexpr std::integral_constant<int, 0> upper;
+    constexpr std::integral_constant<int, 1> lower;
+    for (int step = 0; step < t.steps; step++) {
+      t_at.template read<kT0, 2, 4>(stage, tf);
+      copies.advance();
+      const MmCopy w0 = copies.template w_part<0>(stage);
+      arrived();
+      multiply(upper, acc[0][0], wf0, w0, [] {});
 
       w_at.template read<kW1>(stage, wf1);
-      copies.template issue_w<0>(stage);
-      arrived();
-      quarter<TYPE>(acc[0][1], wf1, tf, upper);
-      mm_barrier();
+      const MmCopy t0 = copies.template t_part<0>(stage);
+      read();
+      multiply(upper, acc[0][1], wf1, t0, [&] { t_at.template read<kT1, 0, 2>(stage, tf); });
 
-      t_at.template read<kT1>(stage, tf);
-      copies.template issue_t<0>(stage);
+      t_at.template read<kT1, 2, 4>(stage, tf);
+      const MmCopy w1 = copies.template w_part<1>(stage);
       arrived();
-      quarter<TYPE>(acc[1][0], wf0, tf, lower);
-      mm_barrier();
+      multiply(lower, acc[1][0], wf0, w1, [] {});
 
       w_at.template read<kW0>(stage ^ kMmStage, wf0);
-      copies.template issue_w<1>(stage);
-      arrived();
-      quarter<TYPE>(acc[1][1], wf1, tf, lower);
-      mm_barrier();
+      const MmCopy t1 = copies.template t_part<1>(stage);
+      read();
+      multiply(lower, acc[1][1], wf1, t1, [&] { t_at.template read<kT0, 0, 2>(stage ^ kMmStage, tf); });
       stage ^= kMmStage;
       stored = false;
     }
