@@ -65,37 +65,34 @@ struct MmCopy {
   v4i rsrc;
   uint32_t v0, v1;
 };
-#define ESMOE_COPY0 "buffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
-#define ESMOE_COPY1 "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024 lds\n\t"
 __device__ __forceinline__ void mm_copy(const MmCopy& p) {
-  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 0\n\t" ESMOE_COPY0 ESMOE_COPY1
+  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 0\n\tbuffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
+               "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024 lds"
                ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory");   // (the compiler keeps nothing in m0)
 }
 
-// An eighth of a step: c[i][j] += rows of t[i] x columns of w[j], i < 2, j < 2, both halves of the step, at a wave priority above that of the
-// memory halves; COPY: behind the first products a copy.  Where `rows` is at most LIMIT: the copy alone.  One statement with its branches inside: around the
-// compiler's own matrix instructions a condition makes it copy the accumulators.  Between two products of one accumulator stand three
-// others; whoever reads it next has to wait (mm_results).
+// An eighth of a step: c[i][j] += rows of t[i] x columns of w[j], i < 2, j < 2, both halves of the step; not where `rows` is at most LIMIT.  One
+// statement with its branches inside: around the compiler's own matrix instructions a condition makes it copy the accumulators.  Between
+// two products of one accumulator stand three others; whoever reads it next has to wait (mm_results).
+// The first eighth of a matrix half raises the wave's priority.  The second has the barrier that ends the matrix half, four products before its end:
+// the other group's first products queue up behind them (without: the matrix cores idle for some 60 cycles a half).
 #define ESMOE_MMA(op, i, j, ks) op " %[c" #i #j "], %[w" #j #ks "], %[t" #i #ks "], %[c" #i #j "]\n\t"
-#define ESMOE_MMA_LOW(op) ESMOE_MMA(op, 0, 0, 0) ESMOE_MMA(op, 0, 1, 0)
-#define ESMOE_MMA_REST(op) ESMOE_MMA(op, 0, 0, 1) ESMOE_MMA(op, 0, 1, 1) ESMOE_MMA(op, 1, 0, 1) ESMOE_MMA(op, 1, 1, 1)
+#define ESMOE_MMA4(op, ks) ESMOE_MMA(op, 0, 0, ks) ESMOE_MMA(op, 0, 1, ks) ESMOE_MMA(op, 1, 0, ks) ESMOE_MMA(op, 1, 1, ks)
 #define ESMOE_MMA_IO                                                                                                                 \
   [c00] "+v"(c[I][0]), [c01] "+v"(c[I][1]), [c10] "+v"(c[I + 1][0]), [c11] "+v"(c[I + 1][1])                                         \
       : [w00] "v"(w[0][0]), [w01] "v"(w[0][1]), [w10] "v"(w[1][0]), [w11] "v"(w[1][1]), [t00] "v"(t[I][0]), [t01] "v"(t[I][1]),       \
-        [t10] "v"(t[I + 1][0]), [t11] "v"(t[I + 1][1])
-#define ESMOE_COPY_IN [lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc)
+        [t10] "v"(t[I + 1][0]), [t11] "v"(t[I + 1][1]), [rows] "s"(rows), [limit] "n"(LIMIT)                                        \
+      : "scc", "memory"
 #define ESMOE_EIGHTH(op)                                                                                                              \
-  if constexpr (COPY)                                                                                                                 \
-    asm volatile("s_mov_b32 m0, %[lds]\n\ts_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_copy%=\n\ts_setprio 1\n\t"          \
-                 ESMOE_MMA_LOW(op) ESMOE_COPY0 ESMOE_MMA(op, 1, 0, 0) ESMOE_MMA(op, 1, 1, 0) ESMOE_COPY1 ESMOE_MMA_REST(op)           \
-                 "s_branch .Lesmoe_end%=\n.Lesmoe_copy%=:\n\t" ESMOE_COPY0 ESMOE_COPY1 ".Lesmoe_end%=:"                               \
-                 : ESMOE_MMA_IO, ESMOE_COPY_IN, [rows] "s"(rows), [limit] "n"(LIMIT) : "scc", "memory");                              \
+  if constexpr (I == 0)                                                                                                               \
+    asm volatile("s_setprio 1\n\ts_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t" ESMOE_MMA4(op, 0) ESMOE_MMA4(op, 1) \
+                 ".Lesmoe_end%=:" : ESMOE_MMA_IO);                                                                                    \
   else                                                                                                                                \
-    asm volatile("s_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t"                                                 \
-                 ESMOE_MMA_LOW(op) ESMOE_MMA(op, 1, 0, 0) ESMOE_MMA(op, 1, 1, 0) ESMOE_MMA_REST(op)                                   \
-                 ".Lesmoe_end%=:\n\ts_setprio 0" : ESMOE_MMA_IO, [rows] "s"(rows), [limit] "n"(LIMIT) : "scc")
-template <int TYPE, int I, bool COPY, int LIMIT>
-__device__ __forceinline__ void eighth(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows, const MmCopy& p) {
+    asm volatile("s_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_mid%=\n\t" ESMOE_MMA4(op, 0)                               \
+                 ".Lesmoe_mid%=:\n\ts_barrier\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t" ESMOE_MMA4(op, 1) ".Lesmoe_end%=:\n\ts_setprio 0"   \
+                 : ESMOE_MMA_IO)
+template <int TYPE, int I, int LIMIT>
+__device__ __forceinline__ void eighth(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows) {
   if constexpr (TYPE == kMmInt8) { ESMOE_EIGHTH("v_mfma_i32_16x16x64_i8"); }
   else if constexpr (TYPE == kMmFp16) { ESMOE_EIGHTH("v_mfma_f32_16x16x32_f16"); }
   else { ESMOE_EIGHTH("v_mfma_f32_16x16x32_bf16"); }
@@ -122,6 +119,12 @@ template <int N>
 __device__ __forceinline__ void mm_wait_copies() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0) ; explicit" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void mm_wait_copies_unless(int already) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_cmp_lg_u32 %1, 0\n\ts_cbranch_scc1 .Lesmoe_wait%=\n\ts_waitcnt vmcnt(%0) ; explicit\n.Lesmoe_wait%=:\n\ts_waitcnt lgkmcnt(0)"
+               ::"n"(N), "s"(uniform(already)) : "memory", "scc");
 }
 __device__ __forceinline__ void mm_wait_fragments() {
   __builtin_amdgcn_sched_barrier(0);
@@ -272,7 +275,7 @@ struct MmCopies {
   static constexpr int kSize = TYPE == kMmInt8 ? 1 : 2;
   const MmTiles<TYPE, KIND>& tiles;
   uint32_t round, lds;
-  int left, depth_left, along;   // steps; of the sum, rows of a transposed operand; bytes of a step along rows
+  int left, end_rows, along;   // steps; rows of a transposed operand in the last one; bytes of a step along rows
   uint64_t t_base, w_base;
   uint64_t w1_base;            // SwiGLU: the up rows
   int t_len, w_len, w1_len, t_pitch, w_pitch, t_col, w_col;
@@ -315,7 +318,6 @@ struct MmCopies {
       if (round > (tiles.total + gridDim.x - 1) / gridDim.x) {
         left = 1 << 30;   // no more tiles: descriptors of nothing from here on
         t_len = w_len = w1_len = along = 0;
-        depth_left = 0;
         return;
       }
       if (p >= tiles.total) {
@@ -327,7 +329,7 @@ struct MmCopies {
     left = t.steps;
     const long w_expert = (long)t.expert * g.n * g.k * kSize;
     if constexpr (KIND == kWeightsGrad) {
-      depth_left = uniform(tiles.s.rows[t.expert]);
+      end_rows = uniform(tiles.s.rows[t.expert]) - (t.steps - 1) * 64;
       const long first = uniform(tiles.s.off[t.expert]);
       t_col = t.row0 * 2;
       w_col = t.col0 * 2;
@@ -337,7 +339,7 @@ struct MmCopies {
       t_base = (uint64_t)g.t + (long)t.row0 * t_pitch - kBias;
       t_len = uniform(t.rows * t_pitch + kBias);
       if constexpr (KIND == kRowsGrad) {
-        depth_left = g.n;
+        end_rows = g.n - (t.steps - 1) * 64;
         w_col = t.col0 * 2;
         w_base = (uint64_t)g.w + w_expert + w_col - kBias;
       } else {
@@ -360,46 +362,42 @@ struct MmCopies {
       }
       edge_w0 = t.col0 + at >= g.k ? kNowhere : 0;
       edge_w1 = t.col0 + at + 128 >= g.k ? kNowhere : 0;
-      lengths();
+      lengths(64);
     }
-    masks(left == 1);
+    now[0] = now[1] = 0;
+    if (left == 1) last();
   }
 
-  // Descriptors' lengths of transposed operands: the rows of this step that the sum has.
-  __device__ __forceinline__ void lengths() {
-    const int n = depth_left < 64 ? depth_left : 64;
-    if constexpr (kTT) t_len = n * t_pitch - t_col + kBias;
-    if constexpr (kWT) w_len = n * w_pitch - w_col + kBias;
+  // Descriptors' lengths of transposed operands, of which a step has `rows` rows.
+  __device__ __forceinline__ void lengths(int rows) {
+    if constexpr (kTT) t_len = uniform(rows * t_pitch - t_col + kBias);
+    if constexpr (kWT) w_len = uniform(rows * w_pitch - w_col + kBias);
   }
 
-  __device__ __forceinline__ void masks(bool last) {
-    now[0] = last ? tail[0] : 0;
-    now[1] = last ? tail[1] : 0;
+  // In front of a tile's last step, in which the sum may end.
+  __device__ __forceinline__ void last() {
+    if constexpr (kTT || kWT) lengths(end_rows);
+    now[0] = tail[0];
+    now[1] = tail[1];
   }
 
+  // The step after this one of the same tile.
   __device__ __forceinline__ void advance() {
-    if (--left == 0) {
-      next_tile();
-      return;
+    t_base += kTT ? 64 * (long)t_pitch : 128;
+    w_base += kWT ? 64 * (long)w_pitch : 128;
+    if constexpr (!kTT) t_len -= along;
+    if constexpr (!kWT) w_len -= along;
+    if constexpr (kSw) {
+      w1_base += 128;
+      w1_len -= along;
     }
-    if constexpr (kTT) t_base += 64 * (long)t_pitch;
-    else {
-      t_base += 128;
-      t_len -= along;
-    }
-    if constexpr (kWT) {
-      w_base += 64 * (long)w_pitch;
-      depth_left -= 64;
-      if (depth_left > 0) lengths();
-    } else {
-      w_base += 128;
-      w_len -= along;
-      if constexpr (kSw) {
-        w1_base += 128;
-        w1_len -= along;
-      }
-    }
-    if constexpr (!kTT || !kWT) masks(left == 1);
+  }
+  // Steps that may follow each other by `advance` alone; what there is to do behind n of them.
+  __device__ __forceinline__ int straight() const { return left > 1 ? left - 1 : left; }
+  __device__ __forceinline__ void passed(int n) {
+    left -= n;
+    if (left == 0) next_tile();
+    else if (left == 1) last();
   }
 
   __device__ __forceinline__ static v4i descriptor(uint64_t base, int len) {
@@ -489,7 +487,6 @@ template <int TYPE, int KIND>
 __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMmArgs g) {
   typedef typename MmAcc<TYPE>::T Acc;
   constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
-  constexpr int kStores = KIND == kSwiglu ? 8 : KIND == kSwigluSave ? 24 : 16;   // of a tile's epilogue, per wavefront
   __shared__ MmShared s;
   mm_schedule<KIND>(s, g);
   const MmTiles<TYPE, KIND> tiles(s, g);
@@ -504,11 +501,12 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   Acc acc[2][2][4][2];
 
   for (int i = 0; i < 2; i++) {
-    if (i) copies.advance();
     mm_copy(copies.template w_part<0>(i * kMmStage));
     mm_copy(copies.template t_part<0>(i * kMmStage));
     mm_copy(copies.template w_part<1>(i * kMmStage));
     mm_copy(copies.template t_part<1>(i * kMmStage));
+    copies.advance();
+    copies.passed(1);
   }
   mm_wait_copies<12>();
   mm_barrier();
@@ -517,7 +515,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   if (wm) mm_barrier();   // this group runs a barrier behind from here on
 
   uint32_t stage = 0;
-  bool stored = false;   // a tile's stores are younger than the copies that this step's waits are for
+  int stored = 0;   // this step's copies have been waited for in front of a tile's stores
   for (uint32_t round = 0, rounds = (tiles.total + gridDim.x - 1) / gridDim.x; round < rounds; round++) {
     const uint32_t p = tiles.position(round);
     if (p >= tiles.total) continue;
@@ -531,8 +529,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
 #pragma unroll
           for (int j = 0; j < 2; j++) acc[a][b][i][j] = Acc{0, 0, 0, 0};
     auto arrived = [&] {
-      if (stored) mm_wait_copies<8 + kStores>();
-      else mm_wait_copies<8>();
+      mm_wait_copies_unless<8>(stored);
       mm_barrier();
     };
     auto read = [&] {
@@ -544,41 +541,46 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
     const int rows = t.rows - wm * 16;
     auto multiply = [&](auto lower, Acc (&c)[4][2], const v4i (&w)[2][2], const MmCopy& copy, auto&& early) {
       constexpr int kFirst = decltype(lower)::value * 128;
-      eighth<TYPE, 0, true, kFirst>(c, w, tf, rows, copy);
+      eighth<TYPE, 0, kFirst>(c, w, tf, rows);
       __builtin_amdgcn_sched_barrier(0);
+      mm_copy(copy);
       early();
       __builtin_amdgcn_sched_barrier(0);
-      eighth<TYPE, 2, false, kFirst + 64>(c, w, tf, rows, copy);
-      mm_barrier();
+      eighth<TYPE, 2, kFirst + 64>(c, w, tf, rows);
+      __builtin_amdgcn_sched_barrier(0);
     };
     constexpr std::integral_constant<int, 0> upper;
     constexpr std::integral_constant<int, 1> lower;
-    for (int step = 0; step < t.steps; step++) {
-      t_at.template read<kT0, 2, 4>(stage, tf);
-      copies.advance();
-      const MmCopy w0 = copies.template w_part<0>(stage);
-      arrived();
-      multiply(upper, acc[0][0], wf0, w0, [] {});
+    for (int left = t.steps; left > 0; left--) {
+      {
+        t_at.template read<kT0, 2, 4>(stage, tf);
+        const MmCopy w0 = copies.template w_part<0>(stage);
+        arrived();
+        multiply(upper, acc[0][0], wf0, w0, [] {});
 
-      w_at.template read<kW1>(stage, wf1);
-      const MmCopy t0 = copies.template t_part<0>(stage);
-      read();
-      multiply(upper, acc[0][1], wf1, t0, [&] { t_at.template read<kT1, 0, 2>(stage, tf); });
+        w_at.template read<kW1>(stage, wf1);
+        const MmCopy t0 = copies.template t_part<0>(stage);
+        read();
+        multiply(upper, acc[0][1], wf1, t0, [&] { t_at.template read<kT1, 0, 2>(stage, tf); });
 
-      t_at.template read<kT1, 2, 4>(stage, tf);
-      const MmCopy w1 = copies.template w_part<1>(stage);
-      arrived();
-      multiply(lower, acc[1][0], wf0, w1, [] {});
+        t_at.template read<kT1, 2, 4>(stage, tf);
+        const MmCopy w1 = copies.template w_part<1>(stage);
+        arrived();
+        multiply(lower, acc[1][0], wf0, w1, [] {});
 
-      w_at.template read<kW0>(stage ^ kMmStage, wf0);
-      const MmCopy t1 = copies.template t_part<1>(stage);
-      read();
-      multiply(lower, acc[1][1], wf1, t1, [&] { t_at.template read<kT0, 0, 2>(stage ^ kMmStage, tf); });
-      stage ^= kMmStage;
-      stored = false;
+        w_at.template read<kW0>(stage ^ kMmStage, wf0);
+        const MmCopy t1 = copies.template t_part<1>(stage);
+        copies.advance();
+        read();
+        multiply(lower, acc[1][1], wf1, t1, [&] { t_at.template read<kT0, 0, 2>(stage ^ kMmStage, tf); });
+        stage ^= kMmStage;
+        stored = 0;
+      }
+      if (__builtin_expect(--copies.left <= 1, 0)) copies.passed(0);
     }
 
     mm_results();
+    mm_wait_copies<4>();   // what the next step waits for: behind the stores it would wait for these
     // a lane holds, of rows a * 128 + (2 i + wm) * 16 + l16, columns b * 128 + wn * 32 + j * 16 + 4 gq .. + 4
     const int room = tiles.cols - t.col0, col = wn * 32 + (gq & 1) * 16 + (gq >> 1) * 8;
     const long out_row0 = KIND == kWeightsGrad ? (long)t.expert * g.n + t.row0 : (long)t.row0;
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
         }
       }
     __builtin_amdgcn_sched_barrier(0);
-    stored = true;
+    stored = 1;
   }
   if (!wm) mm_barrier();
   mm_wait_copies<0>();   // (nothing may arrive in LDS that is another workgroup's by then)
