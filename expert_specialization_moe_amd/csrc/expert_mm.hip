@@ -12,18 +12,19 @@
 // copied from memory straight into LDS, in four parts of 16 KB (W0, T0, W1, T1: the halves of each operand), two steps deep.
 //
 // The step is four phases, a quarter of the tile each: (T0, W0), (T0, W1), (T1, W0), (T1, W1).  A phase is a memory half (fragments LDS ->
-// registers), a barrier, a matrix half (16 MFMAs a wavefront, a copy of one part of the step after next among them), and a barrier.  The
-// wavefronts form two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the
-// matrix cores the other moves data.  A phase's T fragments take the registers of those before as these are done with, so that every
-// memory half has four fragment reads (of sixteen rows x 64 bytes) a wavefront:
-//     phase                    0               1               2               3
-//     memory half reads        T0, 2nd half    W1              T1, 2nd half    W0 of the next step
-//     matrix half reads                        T1, 1st half                    T0 of the next step, 1st half
-//     matrix half copies       W0 of +2        T0 of +2        W1 of +2        T1 of +2
-// A part is copied into the place it had two steps before.  Its last reads were waited for in front of the barrier that ends a memory half, one
-// phase before the copy; the group behind has passed that barrier as well by then.  It is read again seven or eight phases on: in the memory
-// halves of phases 0 and 2 every wavefront waits until its own shares of what the next two phases read have arrived (the four younger copies
-// may be in flight), and the barriers between tell all others.
+// registers, the copy of a part of a coming step), a barrier, a matrix half (16 MFMAs a wavefront), and a barrier.  The wavefronts form
+// two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the matrix cores the
+// other moves data.  No memory half waits for fragments that it reads itself: a trip to LDS is longer than it.
+//     phase                      0                     1                  2                3
+//     memory half reads          W1, T0's 2nd half                        T1's 2nd half    W0 of the next step
+//     memory half copies         T1 of +1              W0 of +2           T0 of +2         W1 of +2
+//     memory half waits (copies) T1                                       W0, T0 of +1     W1 of +1
+//     matrix half reads                                T1's 1st half                       T0's 1st half of the next step
+// A second half of T is waited for behind the first products of its matrix half (and W1, read before it); its registers are those of the
+// half before, which the products are done with.  In half phases since the step's first, of the group that runs behind: W0 and T0's 1st
+// half are read and waited for at 2 (the end of phase 0's memory half), W1 and T0's 2nd half at 3, T1 at 7.  The group that runs ahead
+// copies into their places at 2 (W0), 4 (T0), 6 (W1) and 8 (T1).  And a part is read, by the group ahead, a barrier or more behind the memory
+// half in which the group behind waits for its own shares of it: then four younger copies, of two instructions, may be on their way.
 //
 // The copies run on across tiles: their state is ahead of the one that multiplies, so that a tile begins with its first steps in LDS.
 // They go through buffer descriptors: what lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
@@ -71,31 +72,33 @@ __device__ __forceinline__ void mm_copy(const MmCopy& p) {
                ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory");   // (the compiler keeps nothing in m0)
 }
 
-// An eighth of a step: c[i][j] += rows of t[i] x columns of w[j], i < 2, j < 2, both halves of the step; not where `rows` is at most LIMIT.  One
-// statement with its branches inside: around the compiler's own matrix instructions a condition makes it copy the accumulators.  Between
-// two products of one accumulator stand three others; whoever reads it next has to wait (mm_results).
-// The first eighth of a matrix half raises the wave's priority.  The second has the barrier that ends the matrix half, four products before its end:
-// the other group's first products queue up behind them (without: the matrix cores idle for some 60 cycles a half).
+// Products of a step: c[i][j] += rows of t[i] x columns of w[j], i = I, I + 1, j < 2; not where `rows` is at most LIMIT.  One statement with its branches
+// inside: around the compiler's own matrix instructions a condition makes it copy the accumulators.  Between two products of one
+// accumulator stand three others; whoever reads it next has to wait (mm_results).
+// A matrix half is kBegin for the first two i (both halves of the step; raises the wave's priority), then kNext and kEnd for the others (a half of the
+// step each).
+enum { kBegin, kNext, kEnd };
 #define ESMOE_MMA(op, i, j, ks) op " %[c" #i #j "], %[w" #j #ks "], %[t" #i #ks "], %[c" #i #j "]\n\t"
 #define ESMOE_MMA4(op, ks) ESMOE_MMA(op, 0, 0, ks) ESMOE_MMA(op, 0, 1, ks) ESMOE_MMA(op, 1, 0, ks) ESMOE_MMA(op, 1, 1, ks)
-#define ESMOE_MMA_IO                                                                                                                 \
-  [c00] "+v"(c[I][0]), [c01] "+v"(c[I][1]), [c10] "+v"(c[I + 1][0]), [c11] "+v"(c[I + 1][1])                                         \
-      : [w00] "v"(w[0][0]), [w01] "v"(w[0][1]), [w10] "v"(w[1][0]), [w11] "v"(w[1][1]), [t00] "v"(t[I][0]), [t01] "v"(t[I][1]),       \
-        [t10] "v"(t[I + 1][0]), [t11] "v"(t[I + 1][1]), [rows] "s"(rows), [limit] "n"(LIMIT)                                        \
-      : "scc", "memory"
-#define ESMOE_EIGHTH(op)                                                                                                              \
-  if constexpr (I == 0)                                                                                                               \
-    asm volatile("s_setprio 1\n\ts_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t" ESMOE_MMA4(op, 0) ESMOE_MMA4(op, 1) \
-                 ".Lesmoe_end%=:" : ESMOE_MMA_IO);                                                                                    \
+#define ESMOE_MMA_C [c00] "+v"(c[I][0]), [c01] "+v"(c[I][1]), [c10] "+v"(c[I + 1][0]), [c11] "+v"(c[I + 1][1])
+#define ESMOE_MMA_IN(ks) [w0##ks] "v"(w[0][ks]), [w1##ks] "v"(w[1][ks]), [t0##ks] "v"(t[I][ks]), [t1##ks] "v"(t[I + 1][ks])
+#define ESMOE_MMA_IF [rows] "s"(rows), [limit] "n"(LIMIT) : "scc", "memory"
+#define ESMOE_SKIP "s_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t"
+#define ESMOE_PRODUCTS(op)                                                                                                            \
+  if constexpr (PART == kBegin)                                                                                                       \
+    asm volatile("s_setprio 1\n\t" ESMOE_SKIP ESMOE_MMA4(op, 0) ESMOE_MMA4(op, 1) ".Lesmoe_end%=:"                                    \
+                 : ESMOE_MMA_C : ESMOE_MMA_IN(0), ESMOE_MMA_IN(1), ESMOE_MMA_IF);                                                     \
+  else if constexpr (PART == kNext)                                                                                                   \
+    asm volatile(ESMOE_SKIP ESMOE_MMA4(op, 0) ".Lesmoe_end%=:" : ESMOE_MMA_C : ESMOE_MMA_IN(0), ESMOE_MMA_IF);                        \
   else                                                                                                                                \
-    asm volatile("s_cmp_le_i32 %[rows], %[limit]\n\ts_cbranch_scc1 .Lesmoe_mid%=\n\t" ESMOE_MMA4(op, 0)                               \
-                 ".Lesmoe_mid%=:\n\ts_barrier\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t" ESMOE_MMA4(op, 1) ".Lesmoe_end%=:\n\ts_setprio 0"   \
-                 : ESMOE_MMA_IO)
-template <int TYPE, int I, int LIMIT>
-__device__ __forceinline__ void eighth(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows) {
-  if constexpr (TYPE == kMmInt8) { ESMOE_EIGHTH("v_mfma_i32_16x16x64_i8"); }
-  else if constexpr (TYPE == kMmFp16) { ESMOE_EIGHTH("v_mfma_f32_16x16x32_f16"); }
-  else { ESMOE_EIGHTH("v_mfma_f32_16x16x32_bf16"); }
+    asm volatile(ESMOE_SKIP ESMOE_MMA4(op, 1) ".Lesmoe_end%=:\n\ts_setprio 0" : ESMOE_MMA_C : ESMOE_MMA_IN(1), ESMOE_MMA_IF)
+template <int TYPE, int PART, int I, int LIMIT>
+__device__ __forceinline__ void products(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows) {
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (TYPE == kMmInt8) { ESMOE_PRODUCTS("v_mfma_i32_16x16x64_i8"); }
+  else if constexpr (TYPE == kMmFp16) { ESMOE_PRODUCTS("v_mfma_f32_16x16x32_f16"); }
+  else { ESMOE_PRODUCTS("v_mfma_f32_16x16x32_bf16"); }
+  __builtin_amdgcn_sched_barrier(0);
 }
 // In front of the first vector instruction that reads or writes an accumulator: the last product's result is there 7 issue slots on.
 __device__ __forceinline__ void mm_results() {
@@ -114,21 +117,21 @@ static_assert(sizeof(MmShared) <= 160 * 1024, "LDS");
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Until the wavefront's fragments are there and at most N of its copies and stores are not.
+// Until at most N of the wavefront's copies are on their way; MORE of its stores are younger than these where `stored` is set.
+template <int N, int MORE>
+__device__ __forceinline__ void mm_wait_copies(int stored) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_cmp_lg_u32 %2, 0\n\ts_cbranch_scc1 .Lesmoe_wait%=\n\ts_waitcnt vmcnt(%0) ; explicit\n.Lesmoe_wait%=:\n\ts_waitcnt vmcnt(%1) ; explicit"
+               ::"n"(N), "n"(N + MORE), "s"(uniform(stored)) : "memory", "scc");
+}
 template <int N>
 __device__ __forceinline__ void mm_wait_copies() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0) ; explicit" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) ; explicit" ::"n"(N) : "memory");
 }
 template <int N>
-__device__ __forceinline__ void mm_wait_copies_unless(int already) {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_cmp_lg_u32 %1, 0\n\ts_cbranch_scc1 .Lesmoe_wait%=\n\ts_waitcnt vmcnt(%0) ; explicit\n.Lesmoe_wait%=:\n\ts_waitcnt lgkmcnt(0)"
-               ::"n"(N), "s"(uniform(already)) : "memory", "scc");
-}
 __device__ __forceinline__ void mm_wait_fragments() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(N < 15 ? N : 15) : "memory");
 }
 __device__ __forceinline__ void mm_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -392,10 +395,8 @@ struct MmCopies {
       w1_len -= along;
     }
   }
-  // Steps that may follow each other by `advance` alone; what there is to do behind n of them.
-  __device__ __forceinline__ int straight() const { return left > 1 ? left - 1 : left; }
-  __device__ __forceinline__ void passed(int n) {
-    left -= n;
+  // What there is to do when one step or none is left.
+  __device__ __forceinline__ void passed() {
     if (left == 0) next_tile();
     else if (left == 1) last();
   }
@@ -487,6 +488,8 @@ template <int TYPE, int KIND>
 __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMmArgs g) {
   typedef typename MmAcc<TYPE>::T Acc;
   constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
+  constexpr int kStores = KIND == kSwiglu ? 8 : KIND == kSwigluSave ? 24 : 16;      // of a tile's epilogue, per wavefront
+  constexpr int kTReads = KIND == kWeightsGrad ? 8 : 4, kWReads = KIND >= kRowsGrad ? 8 : 4;   // LDS instructions of half a T, of a W
   __shared__ MmShared s;
   mm_schedule<KIND>(s, g);
   const MmTiles<TYPE, KIND> tiles(s, g);
@@ -500,22 +503,24 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   v4i tf[4][2], wf0[2][2], wf1[2][2];
   Acc acc[2][2][4][2];
 
-  for (int i = 0; i < 2; i++) {
-    mm_copy(copies.template w_part<0>(i * kMmStage));
-    mm_copy(copies.template t_part<0>(i * kMmStage));
-    mm_copy(copies.template w_part<1>(i * kMmStage));
-    mm_copy(copies.template t_part<1>(i * kMmStage));
-    copies.advance();
-    copies.passed(1);
-  }
-  mm_wait_copies<12>();
+  mm_copy(copies.template w_part<0>(0));
+  mm_copy(copies.template t_part<0>(0));
+  mm_copy(copies.template w_part<1>(0));
+  mm_copy(copies.template t_part<1>(0));
+  copies.advance();
+  copies.left--;
+  copies.passed();
+  mm_copy(copies.template w_part<0>(kMmStage));
+  mm_copy(copies.template t_part<0>(kMmStage));
+  mm_copy(copies.template w_part<1>(kMmStage));
+  mm_wait_copies<8>();
   mm_barrier();
   w_at.template read<kW0>(0, wf0);
   t_at.template read<kT0, 0, 2>(0, tf);
   if (wm) mm_barrier();   // this group runs a barrier behind from here on
 
   uint32_t stage = 0;
-  int stored = 0;   // this step's copies have been waited for in front of a tile's stores
+  int stored = 0;   // a tile's stores are younger than the copies that this step waits for
   for (uint32_t round = 0, rounds = (tiles.total + gridDim.x - 1) / gridDim.x; round < rounds; round++) {
     const uint32_t p = tiles.position(round);
     if (p >= tiles.total) continue;
@@ -528,59 +533,53 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
         for (int i = 0; i < 4; i++)
 #pragma unroll
           for (int j = 0; j < 2; j++) acc[a][b][i][j] = Acc{0, 0, 0, 0};
-    auto arrived = [&] {
-      mm_wait_copies_unless<8>(stored);
-      mm_barrier();
-    };
-    auto read = [&] {
-      mm_wait_fragments();
-      mm_barrier();
-    };
+    auto arrived = [&] { mm_wait_copies<8, kStores>(stored); };
     // A phase's matrix half, of the tile's upper or lower half of rows; behind its first products the first half of the next fragments of T, into
     // the registers that these leave.  A group whose sixteens have no rows has nothing to multiply.
     const int rows = t.rows - wm * 16;
-    auto multiply = [&](auto lower, Acc (&c)[4][2], const v4i (&w)[2][2], const MmCopy& copy, auto&& early) {
+    auto multiply = [&](auto lower, Acc (&c)[4][2], const v4i (&w)[2][2], auto&& early0, auto&& early1) {
       constexpr int kFirst = decltype(lower)::value * 128;
-      eighth<TYPE, 0, kFirst>(c, w, tf, rows);
-      __builtin_amdgcn_sched_barrier(0);
-      mm_copy(copy);
-      early();
-      __builtin_amdgcn_sched_barrier(0);
-      eighth<TYPE, 2, kFirst + 64>(c, w, tf, rows);
-      __builtin_amdgcn_sched_barrier(0);
+      products<TYPE, kBegin, 0, kFirst>(c, w, tf, rows);
+      early0();
+      products<TYPE, kNext, 2, kFirst + 64>(c, w, tf, rows);
+      early1();
+      products<TYPE, kEnd, 2, kFirst + 64>(c, w, tf, rows);
+      mm_barrier();
     };
     constexpr std::integral_constant<int, 0> upper;
     constexpr std::integral_constant<int, 1> lower;
+    const auto none = [] {};
     for (int left = t.steps; left > 0; left--) {
-      {
-        t_at.template read<kT0, 2, 4>(stage, tf);
-        const MmCopy w0 = copies.template w_part<0>(stage);
-        arrived();
-        multiply(upper, acc[0][0], wf0, w0, [] {});
+      w_at.template read<kW1>(stage, wf1);
+      t_at.template read<kT0, 2, 4>(stage, tf);
+      mm_copy(copies.template t_part<1>(stage ^ kMmStage));
+      copies.advance();
+      arrived();
+      mm_wait_fragments<kWReads + kTReads>();   // (all but the two just read)
+      mm_barrier();
+      multiply(upper, acc[0][0], wf0, none, none);
 
-        w_at.template read<kW1>(stage, wf1);
-        const MmCopy t0 = copies.template t_part<0>(stage);
-        read();
-        multiply(upper, acc[0][1], wf1, t0, [&] { t_at.template read<kT1, 0, 2>(stage, tf); });
+      if (__builtin_expect(--copies.left <= 1, 0)) copies.passed();
+      mm_copy(copies.template w_part<0>(stage));
+      mm_barrier();
+      multiply(upper, acc[0][1], wf1, [&] { t_at.template read<kT1, 0, 1>(stage, tf); }, [&] { t_at.template read<kT1, 1, 2>(stage, tf); });
 
-        t_at.template read<kT1, 2, 4>(stage, tf);
-        const MmCopy w1 = copies.template w_part<1>(stage);
-        arrived();
-        multiply(lower, acc[1][0], wf0, w1, [] {});
+      t_at.template read<kT1, 2, 4>(stage, tf);
+      mm_copy(copies.template t_part<0>(stage));
+      arrived();
+      mm_barrier();
+      multiply(lower, acc[1][0], wf0, none, none);
 
-        w_at.template read<kW0>(stage ^ kMmStage, wf0);
-        const MmCopy t1 = copies.template t_part<1>(stage);
-        copies.advance();
-        read();
-        multiply(lower, acc[1][1], wf1, t1, [&] { t_at.template read<kT0, 0, 2>(stage ^ kMmStage, tf); });
-        stage ^= kMmStage;
-        stored = 0;
-      }
-      if (__builtin_expect(--copies.left <= 1, 0)) copies.passed(0);
+      w_at.template read<kW0>(stage ^ kMmStage, wf0);
+      mm_copy(copies.template w_part<1>(stage));
+      arrived();
+      mm_barrier();
+      stage ^= kMmStage;
+      multiply(lower, acc[1][1], wf1, [&] { t_at.template read<kT0, 0, 1>(stage, tf); }, [&] { t_at.template read<kT0, 1, 2>(stage, tf); });
+      stored = 0;
     }
 
     mm_results();
-    mm_wait_copies<4>();   // what the next step waits for: behind the stores it would wait for these
     // a lane holds, of rows a * 128 + (2 i + wm) * 16 + l16, columns b * 128 + wn * 32 + j * 16 + 4 gq .. + 4
     const int room = tiles.cols - t.col0, col = wn * 32 + (gq & 1) * 16 + (gq >> 1) * 8;
     const long out_row0 = KIND == kWeightsGrad ? (long)t.expert * g.n + t.row0 : (long)t.row0;
