@@ -148,14 +148,18 @@ struct MmTile {
   int steps;
 };
 
-// Where a launch's tiles lie.  Full tiles (more than 128 rows) first, then the experts' short ends; the weights' gradient: by falling
-// number of rows.  Position p of the order belongs to round p / grid; odd rounds are dealt backwards, so that what a round is uneven in evens out.
+// Which tiles a workgroup multiplies, one a round.
+// Forward and the rows' gradient: an expert's full tiles (more than 128 rows) and its short end are worked on at the same time, so that its
+// weights come from memory once: a round is the next gridDim.x tiles by expert.  Its short tiles go to the next workgroups in turn and its
+// full ones to the others, so that everybody gets as many short ones.  (Full tiles of all experts first, then the short ones: the weights of
+// half of the experts were read twice, 32 experts x 512 rows, 4096 x 4096: 561 us.)
+// The weights' gradient: experts by falling number of rows, odd rounds dealt backwards, so that what a round is uneven in evens out.
 template <int TYPE, int KIND>
 struct MmTiles {
   const MmShared& s;
   const ExpertMmArgs& g;
   int cols, col_tiles, row_tiles;
-  uint32_t total, full_tiles;
+  uint32_t total, full_tiles, rounds, place;
 
   static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
   static constexpr int kWide = kSw ? 128 : 256;
@@ -171,13 +175,58 @@ struct MmTiles {
       full_tiles = (uint32_t)uniform((int)s.full) * col_tiles;
       total = full_tiles + (uint32_t)uniform((int)s.rest) * col_tiles;
     }
+    rounds = (total + gridDim.x - 1) / gridDim.x;
+    // (workgroups go to the eight XCDs in turn: neighbours in a round are on one)
+    place = gridDim.x % 8 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
   }
 
-  __device__ __forceinline__ uint32_t position(uint32_t round) const {
-    const uint32_t w = blockIdx.x, n = gridDim.x;
-    // (workgroups go to the eight XCDs in turn: a round's neighbours are dealt to one)
-    const uint32_t i = n % 8 ? w : (w & 7) * (n / 8) + (w >> 3);
-    return round * n + (round & 1 ? n - 1 - i : i);
+  // The first of the experts' running sums end(e) that is above u, and the sum before it.
+  template <typename F>
+  __device__ __forceinline__ int find(F&& end_of, uint32_t u, uint32_t& before) const {
+    const int lane = threadIdx.x & 63;
+    before = 0;
+    for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+      const uint32_t end = e0 + lane < g.num_experts ? end_of(e0 + lane) : 0xffffffffu;
+      const unsigned long long past = __ballot(end > u);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
+        return e0 + l < g.num_experts ? e0 + l : g.num_experts - 1;
+      }
+      before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+    }
+    return g.num_experts - 1;
+  }
+
+  // Of the first p tiles by expert: full ones; the others are short.
+  __device__ __forceinline__ uint32_t full_before(uint32_t p) const {
+    if (p >= total) return full_tiles;
+    const uint32_t unit = p / col_tiles, col = p - unit * col_tiles;
+    uint32_t before;
+    const int e = find([&](int i) { return sum_or_most(s.full_end[i], s.rest_end[i]); }, unit, before);
+    const uint32_t full0 = e ? (uint32_t)uniform((int)s.full_end[e - 1]) : 0, full = (uint32_t)uniform((int)s.full_end[e]) - full0;
+    const uint32_t inside = unit - before;   // units of the expert before this one
+    const uint32_t n = (full0 + (inside < full ? inside : full)) * col_tiles + (inside < full ? col : 0);
+    return n < full_tiles ? n : full_tiles;
+  }
+
+  // This workgroup's tile of a round; false where it has none.
+  __device__ __forceinline__ bool tile(uint32_t round, MmTile& t) const {
+    const uint32_t n = gridDim.x;
+    if constexpr (KIND == kWeightsGrad) {
+      const uint32_t p = round * n + (round & 1 ? n - 1 - place : place);
+      if (p >= total) return false;
+      t = at(p);
+    } else {
+      const uint32_t p = round * n, end = total - p < n ? total : p + n;
+      const uint32_t full = full_before(p), full_end = full_before(end), rest = p - full, rest_end = end - full_end;
+      // workgroups from `rest` on (round the whole grid) take the round's short tiles, those behind them the full ones
+      const uint32_t from = rest % n, i = place >= from ? place - from : place + n - from;
+      if (i < rest_end - rest) t = at(full_tiles + rest + i);
+      else if (i < end - p) t = at(full + i - (rest_end - rest));
+      else return false;
+    }
+    return true;
   }
 
   __device__ __forceinline__ MmTile at(uint32_t p) const {
@@ -204,22 +253,8 @@ struct MmTiles {
         unit = i / col_tiles;
         col = i - unit * col_tiles;
       }
-      const uint32_t* ends = full ? s.full_end : s.rest_end;
-      const int lane = threadIdx.x & 63;
-      int e = 0;
-      uint32_t before = 0;
-      for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
-        const uint32_t end = e0 + lane < g.num_experts ? ends[e0 + lane] : 0xffffffffu;
-        const unsigned long long past = __ballot(end > unit);
-        if (past) {
-          const int l = __builtin_ctzll(past);
-          e = e0 + l;
-          if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
-          break;
-        }
-        before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
-      }
-      e = e < g.num_experts ? e : g.num_experts - 1;
+      uint32_t before;
+      const int e = find([&](int i) { return full ? s.full_end[i] : s.rest_end[i]; }, unit, before);
       const int m = uniform(s.rows[e]), first = full ? (int)(unit - before) * 256 : m & ~255;
       t.expert = e;
       t.row0 = uniform(s.off[e]) + first;
@@ -316,18 +351,13 @@ struct MmCopies {
   __device__ __forceinline__ void next_tile() {
     const ExpertMmArgs& g = tiles.g;
     MmTile t;
-    do {   // (tiles without rows have nothing to copy; the weights' gradient alone has them, behind all others)
-      const uint32_t p = tiles.position(round++);
-      if (round > (tiles.total + gridDim.x - 1) / gridDim.x) {
+    do {   // (the weights' gradient has tiles without steps)
+      if (round == tiles.rounds) {
         left = 1 << 30;   // no more tiles: descriptors of nothing from here on
         t_len = w_len = w1_len = along = 0;
         return;
       }
-      if (p >= tiles.total) {
-        t.steps = 0;
-        continue;
-      }
-      t = tiles.at(p);
+      if (!tiles.tile(round++, t)) t.steps = 0;
     } while (t.steps == 0);
     left = t.steps;
     const long w_expert = (long)t.expert * g.n * g.k * kSize;
@@ -521,10 +551,9 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
 
   uint32_t stage = 0;
   int stored = 0;   // a tile's stores are younger than the copies that this step waits for
-  for (uint32_t round = 0, rounds = (tiles.total + gridDim.x - 1) / gridDim.x; round < rounds; round++) {
-    const uint32_t p = tiles.position(round);
-    if (p >= tiles.total) continue;
-    const MmTile t = tiles.at(p);
+  for (uint32_t round = 0; round < tiles.rounds; round++) {
+    MmTile t;
+    if (!tiles.tile(round, t)) continue;
 #pragma unroll
     for (int a = 0; a < 2; a++)
 #pragma unroll
