@@ -109,9 +109,8 @@ __device__ __forceinline__ void mm_results() {
 
 struct MmShared {
   uint8_t ring[2 * kMmStage];
-  int rows[kMmExperts], off[kMmExperts];
-  uint32_t full_end[kMmExperts], rest_end[kMmExperts];   // weights' gradient: full_end is the experts by falling rows
-  uint32_t full, rest;
+  int rows[kMmExperts], off[kMmExperts], order[kMmExperts];
+  uint32_t unit_end[kMmExperts], units;   // running sums, in order
 };
 static_assert(sizeof(MmShared) <= 160 * 1024, "LDS");
 
@@ -148,18 +147,22 @@ struct MmTile {
   int steps;
 };
 
-// Which tiles a workgroup multiplies, one a round.
-// Forward and the rows' gradient: an expert's full tiles (more than 128 rows) and its short end are worked on at the same time, so that its
-// weights come from memory once: a round is the next gridDim.x tiles by expert.  Its short tiles go to the next workgroups in turn and its
-// full ones to the others, so that everybody gets as many short ones.  (Full tiles of all experts first, then the short ones: the weights of
-// half of the experts were read twice, 32 experts x 512 rows, 4096 x 4096: 561 us.)
-// The weights' gradient: experts by falling number of rows, odd rounds dealt backwards, so that what a round is uneven in evens out.
+// The rows of an expert in units of at most 256, as equal as sixteens allow: a tile of few rows takes as long as its weights' way from memory,
+// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows ### us, twice 178 ### us).
+__device__ __forceinline__ uint32_t mm_units(int rows) { return ((uint32_t)rows + 255) / 256; }
+__device__ __forceinline__ int mm_unit_rows(int rows) {
+  const int units = (int)mm_units(rows);
+  return units ? ((rows + units - 1) / units + 15) & ~15 : 0;
+}
+
+// Which tiles a workgroup multiplies, one a round: experts by falling rows of a unit (the weights' gradient: rows), odd rounds dealt backwards, so that
+// what a round is uneven in evens out.
 template <int TYPE, int KIND>
 struct MmTiles {
   const MmShared& s;
   const ExpertMmArgs& g;
   int cols, col_tiles, row_tiles;
-  uint32_t total, full_tiles, rounds, place;
+  uint32_t total, rounds, place;
 
   static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
   static constexpr int kWide = kSw ? 128 : 256;
@@ -168,138 +171,90 @@ struct MmTiles {
     cols = kSw ? g.n / 2 : KIND >= kRowsGrad ? g.k : g.n;
     col_tiles = (cols + kWide - 1) / kWide;
     row_tiles = (g.n + 255) / 256;
-    if constexpr (KIND == kWeightsGrad) {
-      total = (uint32_t)g.num_experts * row_tiles * col_tiles;
-      full_tiles = 0;
-    } else {
-      full_tiles = (uint32_t)uniform((int)s.full) * col_tiles;
-      total = full_tiles + (uint32_t)uniform((int)s.rest) * col_tiles;
-    }
+    total = (KIND == kWeightsGrad ? (uint32_t)g.num_experts * row_tiles : (uint32_t)uniform((int)s.units)) * col_tiles;
     rounds = (total + gridDim.x - 1) / gridDim.x;
     // (workgroups go to the eight XCDs in turn: neighbours in a round are on one)
     place = gridDim.x % 8 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
   }
 
-  // The first of the experts' running sums end(e) that is above u, and the sum before it.
-  template <typename F>
-  __device__ __forceinline__ int find(F&& end_of, uint32_t u, uint32_t& before) const {
-    const int lane = threadIdx.x & 63;
-    before = 0;
-    for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
-      const uint32_t end = e0 + lane < g.num_experts ? end_of(e0 + lane) : 0xffffffffu;
-      const unsigned long long past = __ballot(end > u);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
-        return e0 + l < g.num_experts ? e0 + l : g.num_experts - 1;
-      }
-      before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
-    }
-    return g.num_experts - 1;
-  }
-
-  // Of the first p tiles by expert: full ones; the others are short.
-  __device__ __forceinline__ uint32_t full_before(uint32_t p) const {
-    if (p >= total) return full_tiles;
-    const uint32_t unit = p / col_tiles, col = p - unit * col_tiles;
-    uint32_t before;
-    const int e = find([&](int i) { return sum_or_most(s.full_end[i], s.rest_end[i]); }, unit, before);
-    const uint32_t full0 = e ? (uint32_t)uniform((int)s.full_end[e - 1]) : 0, full = (uint32_t)uniform((int)s.full_end[e]) - full0;
-    const uint32_t inside = unit - before;   // units of the expert before this one
-    const uint32_t n = (full0 + (inside < full ? inside : full)) * col_tiles + (inside < full ? col : 0);
-    return n < full_tiles ? n : full_tiles;
-  }
-
   // This workgroup's tile of a round; false where it has none.
   __device__ __forceinline__ bool tile(uint32_t round, MmTile& t) const {
-    const uint32_t n = gridDim.x;
-    if constexpr (KIND == kWeightsGrad) {
-      const uint32_t p = round * n + (round & 1 ? n - 1 - place : place);
-      if (p >= total) return false;
-      t = at(p);
-    } else {
-      const uint32_t p = round * n, end = total - p < n ? total : p + n;
-      const uint32_t full = full_before(p), full_end = full_before(end), rest = p - full, rest_end = end - full_end;
-      // workgroups from `rest` on (round the whole grid) take the round's short tiles, those behind them the full ones
-      const uint32_t from = rest % n, i = place >= from ? place - from : place + n - from;
-      if (i < rest_end - rest) t = at(full_tiles + rest + i);
-      else if (i < end - p) t = at(full + i - (rest_end - rest));
-      else return false;
-    }
-    return true;
-  }
-
-  __device__ __forceinline__ MmTile at(uint32_t p) const {
-    MmTile t;
+    const uint32_t p = round * gridDim.x + (round & 1 ? gridDim.x - 1 - place : place);
+    if (p >= total) return false;
+    uint32_t row, col;   // of the expert's tiles
     if constexpr (KIND == kWeightsGrad) {
       const uint32_t per = (uint32_t)row_tiles * col_tiles, rank = p / per, i = p - rank * per;
-      t.expert = uniform((int)s.full_end[rank]);
-      const int r = i / col_tiles;
-      t.row0 = r * 256;
+      t.expert = uniform(s.order[rank]);
+      row = i / col_tiles;
+      col = i - row * col_tiles;
+      t.row0 = row * 256;
       t.rows = g.n - t.row0 < 256 ? g.n - t.row0 : 256;
-      t.col0 = ((int)i - r * col_tiles) * 256;
       t.steps = (uniform(s.rows[t.expert]) + 63) >> 6;
-      return t;
     } else {
-      const bool full = p < full_tiles;
-      uint32_t unit, col;
-      if (full) {   // four units a group, a column's tiles together
-        const uint32_t group = p / (4 * col_tiles), i = p - group * 4 * col_tiles, have = full_tiles / col_tiles - 4 * group,
-                       wide = have < 4 ? have : 4;
-        col = i / wide;
-        unit = 4 * group + i - col * wide;
-      } else {
-        const uint32_t i = p - full_tiles;
-        unit = i / col_tiles;
-        col = i - unit * col_tiles;
+      // the expert whose units' running sum is the first above this unit
+      const uint32_t unit = p / col_tiles;
+      const int lane = threadIdx.x & 63;
+      int rank = g.num_experts - 1;
+      uint32_t before = 0;
+      for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+        const uint32_t end = e0 + lane < g.num_experts ? s.unit_end[e0 + lane] : 0xffffffffu;
+        const unsigned long long past = __ballot(end > unit);
+        if (past) {
+          const int l = __builtin_ctzll(past);
+          if (e0 + l < g.num_experts) rank = e0 + l;
+          if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
+          break;
+        }
+        before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
       }
-      uint32_t before;
-      const int e = find([&](int i) { return full ? s.full_end[i] : s.rest_end[i]; }, unit, before);
-      const int m = uniform(s.rows[e]), first = full ? (int)(unit - before) * 256 : m & ~255;
-      t.expert = e;
-      t.row0 = uniform(s.off[e]) + first;
-      t.rows = m - first < 256 ? m - first : 256;
-      t.col0 = (int)col * kWide;
+      t.expert = uniform(s.order[rank]);
+      const int m = uniform(s.rows[t.expert]), high = mm_unit_rows(m);
+      // four units a group, a column's tiles together
+      const uint32_t i = p - before * col_tiles, group = i / (4 * col_tiles), j = i - group * 4 * col_tiles, have = mm_units(m) - 4 * group,
+                     wide = have < 4 ? have : 4;
+      col = j / wide;
+      row = 4 * group + j - col * wide;
+      const int from = (int)row * high;   // (the last unit may be short of rows, or without any)
+      t.row0 = uniform(s.off[t.expert]) + from;
+      t.rows = m - from < high ? m - from : high;
+      if (t.rows <= 0) return false;
       t.steps = KIND == kRowsGrad ? (g.n + 63) >> 6 : TYPE == kMmInt8 ? (g.k + 127) >> 7 : (g.k + 63) >> 6;
-      return t;
     }
+    t.col0 = (int)col * kWide;
+    return true;
   }
 };
 
-// Reads the experts' rows and offsets, cut at the tensor's, and puts the tiles in order.
+// Reads the experts' rows and offsets, cut at the tensor's, and puts the experts in order.
 template <int KIND>
 __device__ __forceinline__ void mm_schedule(MmShared& s, const ExpertMmArgs& g) {
   const int tid = threadIdx.x;
+  auto height = [&](int e) { return KIND == kWeightsGrad ? s.rows[e] : mm_unit_rows(s.rows[e]); };
   for (int e = tid; e < g.num_experts; e += kMmThreads) {
     const int off = g.expert_offsets[e];
     s.rows[e] = fp4_rows(g.problem_sizes[e * 3], off, g.total_rows);
     s.off[e] = off;
+    s.unit_end[e] = (uint32_t)height(e);
   }
   __syncthreads();
-  if constexpr (KIND == kWeightsGrad) {
-    for (int e = tid; e < g.num_experts; e += kMmThreads) {
-      const int m = s.rows[e];
-      int rank = 0;
-      for (int j = 0; j < g.num_experts; j++) rank += s.rows[j] > m || (s.rows[j] == m && j < e);
-      s.full_end[rank] = (uint32_t)e;
-    }
-  } else if (tid < 64) {
-    uint32_t full = 0, rest = 0;
-    for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
-      const int e = e0 + tid, m = e < g.num_experts ? s.rows[e] : 0, end = m & 255;
-      const uint32_t f = sum_or_most(full, wave_inclusive_sum_or_most((uint32_t)(m >> 8) + (end > 128 ? 1u : 0u)));
-      const uint32_t r = sum_or_most(rest, wave_inclusive_sum_or_most(end && end <= 128 ? 1u : 0u));
-      if (e < g.num_experts) {
-        s.full_end[e] = f;
-        s.rest_end[e] = r;
-      }
-      full = (uint32_t)__builtin_amdgcn_readlane((int)f, 63);
-      rest = (uint32_t)__builtin_amdgcn_readlane((int)r, 63);
+  for (int e = tid; e < g.num_experts; e += kMmThreads) {
+    const uint32_t h = s.unit_end[e];
+    int rank = 0;
+    for (int j = 0; j < g.num_experts; j++) rank += s.unit_end[j] > h || (s.unit_end[j] == h && j < e);
+    s.order[rank] = e;
+  }
+  __syncthreads();
+  if (KIND != kWeightsGrad && tid < 64) {
+    uint32_t units = 0;
+    for (int p0 = 0; p0 < g.num_experts; p0 += 64) {
+      const int p = p0 + tid;
+      const uint32_t end = sum_or_most(units, wave_inclusive_sum_or_most(p < g.num_experts ? mm_units(s.rows[s.order[p]]) : 0));
+      if (p < g.num_experts) s.unit_end[p] = end;
+      units = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
     }
     if (tid == 0) {   // no more than experts with rows of their own can have
-      const uint32_t most_full = (uint32_t)(g.total_rows / 129), most_rest = (uint32_t)(g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
-      s.full = full < most_full ? full : most_full;
-      s.rest = rest < most_rest ? rest : most_rest;
+      const uint32_t most = (uint32_t)(g.total_rows / 256) + (uint32_t)(g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+      s.units = units < most ? units : most;
     }
   }
   __syncthreads();
@@ -351,7 +306,7 @@ struct MmCopies {
   __device__ __forceinline__ void next_tile() {
     const ExpertMmArgs& g = tiles.g;
     MmTile t;
-    do {   // (the weights' gradient has tiles without steps)
+    do {   // (there are tiles without rows or steps)
       if (round == tiles.rounds) {
         left = 1 << 30;   // no more tiles: descriptors of nothing from here on
         t_len = w_len = w1_len = along = 0;
@@ -682,7 +637,7 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   const ExpertMmArgs& g = *args;
   const long cols = kind >= 2 ? g.k : kind == 1 ? g.n / 2 : g.n, wide = kind == 1 ? 128 : 256, col_tiles = (cols + wide - 1) / wide;
   const long units = kind == 3 ? (long)g.num_experts * ((g.n + 255) / 256)
-                               : g.total_rows / 129 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+                               : g.total_rows / 256 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
   const long tiles = units * col_tiles, grid = tiles < cus ? tiles : cus;
   if (grid == 0) return 0;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
