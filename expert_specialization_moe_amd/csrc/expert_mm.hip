@@ -76,7 +76,8 @@ __device__ __forceinline__ void mm_copy(const MmCopy& p) {
 // inside: around the compiler's own matrix instructions a condition makes it copy the accumulators.  Between two products of one
 // accumulator stand three others; whoever reads it next has to wait (mm_results).
 // A matrix half is kBegin for the first two i (both halves of the step; raises the wave's priority), then kNext and kEnd for the others (a half of the
-// step each).
+// step each).  kEnd has the barrier that ends the matrix half in front of its last four products, at a priority above the other group's first
+// ones, which queue up behind them: without, the matrix cores idle from one group's last product until the other's first.
 enum { kBegin, kNext, kEnd };
 #define ESMOE_MMA(op, i, j, ks) op " %[c" #i #j "], %[w" #j #ks "], %[t" #i #ks "], %[c" #i #j "]\n\t"
 #define ESMOE_MMA4(op, ks) ESMOE_MMA(op, 0, 0, ks) ESMOE_MMA(op, 0, 1, ks) ESMOE_MMA(op, 1, 0, ks) ESMOE_MMA(op, 1, 1, ks)
@@ -91,7 +92,7 @@ enum { kBegin, kNext, kEnd };
   else if constexpr (PART == kNext)                                                                                                   \
     asm volatile(ESMOE_SKIP ESMOE_MMA4(op, 0) ".Lesmoe_end%=:" : ESMOE_MMA_C : ESMOE_MMA_IN(0), ESMOE_MMA_IF);                        \
   else                                                                                                                                \
-    asm volatile(ESMOE_SKIP ESMOE_MMA4(op, 1) ".Lesmoe_end%=:\n\ts_setprio 0" : ESMOE_MMA_C : ESMOE_MMA_IN(1), ESMOE_MMA_IF)
+    asm volatile("s_setprio 2\n\ts_cmp_le_i32 %[rows], %[limit]\n\ts_barrier\n\ts_cbranch_scc1 .Lesmoe_end%=\n\t" ESMOE_MMA4(op, 1) ".Lesmoe_end%=:\n\ts_setprio 0" : ESMOE_MMA_C : ESMOE_MMA_IN(1), ESMOE_MMA_IF)
 template <int TYPE, int PART, int I, int LIMIT>
 __device__ __forceinline__ void products(typename MmAcc<TYPE>::T (&c)[4][2], const v4i (&w)[2][2], const v4i (&t)[4][2], int rows) {
   __builtin_amdgcn_sched_barrier(0);
@@ -528,7 +529,6 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
       products<TYPE, kNext, 2, kFirst + 64>(c, w, tf, rows);
       early1();
       products<TYPE, kEnd, 2, kFirst + 64>(c, w, tf, rows);
-      mm_barrier();
     };
     constexpr std::integral_constant<int, 0> upper;
     constexpr std::integral_constant<int, 1> lower;
