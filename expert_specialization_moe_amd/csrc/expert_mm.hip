@@ -16,15 +16,15 @@
 // two groups of four, one wavefront of each per SIMD, and one group runs a barrier behind the other: while one feeds the matrix cores the
 // other moves data.  No memory half waits for fragments that it reads itself: a trip to LDS is longer than it.
 //     phase                      0                     1                  2                3
-//     memory half reads          W1, T0's 2nd half                        T1's 2nd half    W0 of the next step
+//     memory half reads          T0's 2nd half                            T1's 2nd half    W0 of the next step
 //     memory half copies         T1 of +1              W0 of +2           T0 of +2         W1 of +2
 //     memory half waits (copies) T1                                       W0, T0 of +1     W1 of +1
-//     matrix half reads                                T1's 1st half                       T0's 1st half of the next step
-// A second half of T is waited for behind the first products of its matrix half (and W1, read before it); its registers are those of the
-// half before, which the products are done with.  In half phases since the step's first, of the group that runs behind: W0 and T0's 1st
-// half are read and waited for at 2 (the end of phase 0's memory half), W1 and T0's 2nd half at 3, T1 at 7.  The group that runs ahead
-// copies into their places at 2 (W0), 4 (T0), 6 (W1) and 8 (T1).  And a part is read, by the group ahead, a barrier or more behind the memory
-// half in which the group behind waits for its own shares of it: then four younger copies, of two instructions, may be on their way.
+//     matrix half reads          W1                    T1's 1st half                       T0's 1st half of the next step
+// A second half of T is waited for behind the first products of its matrix half; its registers are those of the half before, which the products
+// are done with.  In half phases since the step's first, of the group that runs behind: W0 and T0's 1st half are read and waited for at 2
+// (the end of phase 0's memory half), T0's 2nd half at 3, W1 at 5, T1 at 7.  The group that runs ahead copies into their places at 2 (W0),
+// 4 (T0), 6 (W1) and 8 (T1).  And a part is read, by the group ahead, a barrier or more behind the memory half in which the group behind
+// waits for its own shares of it: then four younger copies, of two instructions, may be on their way.
 //
 // The copies run on across tiles: their state is ahead of the one that multiplies, so that a tile begins with its first steps in LDS.
 // They go through buffer descriptors: what lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   typedef typename MmAcc<TYPE>::T Acc;
   constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
   constexpr int kStores = KIND == kSwiglu ? 8 : KIND == kSwigluSave ? 24 : 16;      // of a tile's epilogue, per wavefront
-  constexpr int kTReads = KIND == kWeightsGrad ? 8 : 4, kWReads = KIND >= kRowsGrad ? 8 : 4;   // LDS instructions of half a T, of a W
+  constexpr int kTReads = KIND == kWeightsGrad ? 8 : 4;   // LDS instructions of half a T
   __shared__ MmShared s;
   mm_schedule<KIND>(s, g);
   const MmTiles<TYPE, KIND> tiles(s, g);
@@ -534,14 +534,13 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
     constexpr std::integral_constant<int, 1> lower;
     const auto none = [] {};
     for (int left = t.steps; left > 0; left--) {
-      w_at.template read<kW1>(stage, wf1);
       t_at.template read<kT0, 2, 4>(stage, tf);
       mm_copy(copies.template t_part<1>(stage ^ kMmStage));
       copies.advance();
       arrived();
-      mm_wait_fragments<kWReads + kTReads>();   // (all but the two just read)
+      mm_wait_fragments<kTReads>();   // (all but those just read)
       mm_barrier();
-      multiply(upper, acc[0][0], wf0, none, none);
+      multiply(upper, acc[0][0], wf0, [&] { w_at.template read<kW1, 0, 1>(stage, wf1); }, [&] { w_at.template read<kW1, 1, 2>(stage, wf1); });
 
       if (__builtin_expect(--copies.left <= 1, 0)) copies.passed();
       mm_copy(copies.template w_part<0>(stage));
