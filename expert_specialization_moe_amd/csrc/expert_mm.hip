@@ -67,7 +67,8 @@ struct MmCopy {
   uint32_t v0, v1;
 };
 __device__ __forceinline__ void mm_copy(const MmCopy& p) {
-  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 0\n\tbuffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
+  // (a scalar register that a vector instruction wrote is there for a memory instruction five slots on)
+  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 4\n\tbuffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
                "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024 lds"
                ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory");   // (the compiler keeps nothing in m0)
 }
