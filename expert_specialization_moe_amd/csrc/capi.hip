@@ -53,14 +53,6 @@ extern "C" int esmoe_launch_add_rms_norm_quant(const void* in, int in_dtype, con
 extern "C" int esmoe_launch_mxfp4_grouped_mm(const void* a, int dtype, const void* b, const uint8_t* sf, const int* problem_sizes,
                                              const int* expert_offsets, int num_experts, int total_rows, int n, int k, int swiglu,
                                              void* out, int cus, hipStream_t stream);
-extern "C" int esmoe_launch_expert_mm(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
-extern "C" int esmoe_launch_swiglu_grad(const void* grad_h, const void* gate_up, int fp16, long rows, int inter, void* grad, hipStream_t stream);
-extern "C" int esmoe_launch_int8_quant(const void* in, int fp16, long rows, int k, void* q, float* scales, hipStream_t stream);
-extern "C" int esmoe_launch_grad_squares(const esmoe::GradTable* t, int grid, double* partial, hipStream_t stream);
-extern "C" int esmoe_launch_grad_norm(const double* partial, int count, float* norm, hipStream_t stream);
-extern "C" int esmoe_launch_grad_clip(const esmoe::GradTable* t, int grid, const double* partial, int count, const float* given, double max_norm,
-                                      float eps, float* norm_out, hipStream_t stream);
-
 namespace {
 
 constexpr long kRouteChunk = 1024;   // fewest pairs of a chunk in routing.hip

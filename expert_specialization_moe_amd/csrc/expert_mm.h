@@ -1,5 +1,6 @@
-// What the entry points hand to the 16-bit and int8 grouped products (expert_mm.hip).
+// What the entry points hand to the 16-bit and int8 grouped products (expert_mm.hip) and to the kernels beside them.
 #pragma once
+#include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace esmoe {
@@ -23,3 +24,8 @@ struct ExpertMmArgs {
 };
 
 }  // namespace esmoe
+
+// kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 gradient of the weights
+extern "C" int esmoe_launch_expert_mm(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
+extern "C" int esmoe_launch_swiglu_grad(const void* grad_h, const void* gate_up, int fp16, long rows, int inter, void* grad, hipStream_t stream);
+extern "C" int esmoe_launch_int8_quant(const void* in, int fp16, long rows, int k, void* q, float* scales, hipStream_t stream);

@@ -632,7 +632,6 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
 
 using namespace esmoe;
 
-// kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 gradient of the weights
 extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cus, hipStream_t stream) {
   const ExpertMmArgs& g = *args;
   const long cols = kind >= 2 ? g.k : kind == 1 ? g.n / 2 : g.n, wide = kind == 1 ? 128 : 256, col_tiles = (cols + wide - 1) / wide;

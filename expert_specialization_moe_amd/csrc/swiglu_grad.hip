@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "expert_mm.h"
+
 namespace esmoe {
 
 typedef int v4i __attribute__((ext_vector_type(4)));

@@ -117,6 +117,12 @@ def test_zero_gradients(esmoe):
     assert float(esmoe.es_clip_grad_norm(e, 1.0)) == 0.0 and float(esmoe.es_grad_norm(e)) == 0.0
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-3, 25.0])
+def test_eps(esmoe, eps):
+    """Beside a norm of about its size."""
+    check(esmoe, make([((300,), F32), ((20, 17), BF)], 11), 10.0, eps)
+
+
 def test_a_given_norm(esmoe):
     """The norm over several ranks: the gradients of each are scaled by the same factor."""
     g = make([((100,), F32), ((50,), BF)], 7)
