@@ -902,7 +902,7 @@ int esmoe_grad_norm(const void* const* grads, const int* dtypes, const long* siz
     return esmoe_launch_grad_squares(&t, grid, (double*)workspace + before, (hipStream_t)stream);
   });
   if (rc) return rc;
-  rc = esmoe_launch_grad_norm((const double*)workspace, partials, norm, (hipStream_t)stream);
+  rc = esmoe_launch_grad_norm((const double*)workspace, partials, nullptr, norm, (hipStream_t)stream);
   if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
   return 0;
 }
@@ -925,11 +925,12 @@ int esmoe_clip_grad_norm(const void* const* grads, void* const* outputs, const i
       return esmoe_launch_grad_squares(&t, grid, (double*)workspace + before, (hipStream_t)stream);
     });
     if (rc) return rc;
-    if (partials == 0 && norm) {   // no elements at all: the norm is 0
-      rc = esmoe_launch_grad_norm((const double*)workspace, 0, norm, (hipStream_t)stream);
-      if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
-      return 0;
-    }
+  }
+  bool any = false;
+  for (int i = 0; i < count; i++) any |= sizes[i] > 0;
+  if (!any && norm) {   // nothing to scale, by whose launch it would be written: the given norm, or 0
+    rc = esmoe_launch_grad_norm((const double*)workspace, 0, given_norm, norm, (hipStream_t)stream);
+    if (rc) return fail(rc, "gradient norm launch failed: %s", hipGetErrorString((hipError_t)rc));
   }
   return for_grad_tables(grads, outputs, dtypes, sizes, count, [&](const esmoe::GradTable& t, int grid, int before) {
     return esmoe_launch_grad_clip(&t, grid, (const double*)workspace, partials, given_norm, max_norm, eps, before ? nullptr : norm,

@@ -23,6 +23,6 @@ static_assert(sizeof(GradTable) <= 3600, "kernel arguments");
 }  // namespace esmoe
 
 extern "C" int esmoe_launch_grad_squares(const esmoe::GradTable* t, int grid, double* partial, hipStream_t stream);
-extern "C" int esmoe_launch_grad_norm(const double* partial, int count, float* norm, hipStream_t stream);
+extern "C" int esmoe_launch_grad_norm(const double* partial, int count, const float* given, float* norm, hipStream_t stream);
 extern "C" int esmoe_launch_grad_clip(const esmoe::GradTable* t, int grid, const double* partial, int count, const float* given, double max_norm,
                                       double eps, float* norm_out, hipStream_t stream);

@@ -77,10 +77,11 @@ __device__ __forceinline__ double sum_partials(const double* __restrict__ partia
   return workgroup_sum(sum, s);
 }
 
-__global__ void __launch_bounds__(256) grad_norm_kernel(const double* __restrict__ partial, int count, float* __restrict__ norm) {
+__global__ void __launch_bounds__(256) grad_norm_kernel(const double* __restrict__ partial, int count, const float* __restrict__ given,
+                                                        float* __restrict__ norm) {
   __shared__ double s[256];
   const double sum = sum_partials(partial, count, s);
-  if (threadIdx.x == 0) *norm = (float)sqrt(sum);
+  if (threadIdx.x == 0) *norm = given ? *given : (float)sqrt(sum);
 }
 
 template <typename T>
@@ -117,8 +118,8 @@ extern "C" int esmoe_launch_grad_squares(const esmoe::GradTable* t, int grid, do
   hipLaunchKernelGGL(esmoe::grad_squares_kernel, dim3(grid), dim3(256), 0, stream, *t, partial);
   return (int)hipGetLastError();
 }
-extern "C" int esmoe_launch_grad_norm(const double* partial, int count, float* norm, hipStream_t stream) {
-  hipLaunchKernelGGL(esmoe::grad_norm_kernel, dim3(1), dim3(256), 0, stream, partial, count, norm);
+extern "C" int esmoe_launch_grad_norm(const double* partial, int count, const float* given, float* norm, hipStream_t stream) {
+  hipLaunchKernelGGL(esmoe::grad_norm_kernel, dim3(1), dim3(256), 0, stream, partial, count, given, norm);
   return (int)hipGetLastError();
 }
 extern "C" int esmoe_launch_grad_clip(const esmoe::GradTable* t, int grid, const double* partial, int count, const float* given, double max_norm,

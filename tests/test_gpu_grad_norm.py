@@ -132,6 +132,12 @@ def test_a_given_norm(esmoe):
     assert all(((x.float() - w).abs() <= O.out_bound(w.double(), 3 * 2.0 ** -24 * w.abs().double(), x.dtype)).all() for x, w in zip(g, want))
 
 
+def test_a_given_norm_of_nothing(esmoe):
+    total = torch.tensor(3.0, device="cuda")
+    for _ in range(3):
+        assert float(esmoe.es_clip_grad_norm([torch.zeros(0, device="cuda")], 1.0, norm=total)) == 3.0
+
+
 def test_one_by_one_or_together(esmoe):
     """Over a hundred tensors (several launches) against the same memory as one."""
     flat = torch.randn(300 * 64, device="cuda")
