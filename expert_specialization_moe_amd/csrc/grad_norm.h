@@ -15,7 +15,7 @@ struct GradTable {
   void* out[kGradTensors];             // clipping alone
   long size[kGradTensors];             // elements
   long end[kGradTensors];              // chunks up to and with the tensor's
-  uint8_t type[kGradTensors];
+  int type[kGradTensors];
   int count;
 };
 static_assert(sizeof(GradTable) <= 3600, "kernel arguments");
