@@ -25,7 +25,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["grouped_gemm.hip", "mxfp8_quant.hip", "fp8_quant.hip", "routing.hip", "gating.hip", "combine.hip",
-               "norm_quant.hip", "mxfp4_gemm.hip", "expert_mm.hip", "swiglu_grad.hip", "int8_quant.hip", "grad_norm.hip", "capi.hip"]
+               "norm_quant.hip", "mxfp4_gemm.hip", "expert_mm.hip", "expert_mm_few.hip", "swiglu_grad.hip", "int8_quant.hip", "grad_norm.hip", "capi.hip"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-mcode-object-version=5",
     # packed fp32 VALU ops are kept out of the device code

@@ -23,9 +23,21 @@ struct ExpertMmArgs {
   int out_fp16;               // int8: type of out
 };
 
+// A workgroup's place among those that share `total` items, round by round.  Workgroups go to the eight XCDs in turn: neighbours are on one, and where
+// there are fewer items than workgroups (the launch knows an upper bound alone) every XCD has as many.
+struct MmPlace {
+  uint32_t place, of;   // place >= total: nothing to do
+};
+__device__ __forceinline__ MmPlace mm_place(uint32_t total) {
+  if (gridDim.x % 8) return {blockIdx.x, gridDim.x};
+  const uint32_t each = (total < gridDim.x ? total + 7 : gridDim.x) / 8, at = blockIdx.x >> 3;
+  return {at < each ? (blockIdx.x & 7) * each + at : total, 8 * each};
+}
+
 }  // namespace esmoe
 
 // kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 gradient of the weights
 extern "C" int esmoe_launch_expert_mm(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
+extern "C" int esmoe_launch_expert_mm_few(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);   // kind 0 or 1
 extern "C" int esmoe_launch_swiglu_grad(const void* grad_h, const void* gate_up, int fp16, long rows, int inter, void* grad, hipStream_t stream);
 extern "C" int esmoe_launch_int8_quant(const void* in, int fp16, long rows, int k, void* q, float* scales, hipStream_t stream);

@@ -150,7 +150,7 @@ struct MmTile {
 };
 
 // The rows of an expert in units of at most 256, as equal as sixteens allow: a tile of few rows takes as long as its weights' way from memory,
-// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows ### us, twice 178 ### us).
+// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows 777 us, twice 178 730 us).
 __device__ __forceinline__ uint32_t mm_units(int rows) { return ((uint32_t)rows + 255) / 256; }
 __device__ __forceinline__ int mm_unit_rows(int rows) {
   const int units = (int)mm_units(rows);
@@ -164,7 +164,7 @@ struct MmTiles {
   const MmShared& s;
   const ExpertMmArgs& g;
   int cols, col_tiles, row_tiles;
-  uint32_t total, rounds, place;
+  uint32_t total, rounds, place, per_round;
 
   static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
   static constexpr int kWide = kSw ? 128 : 256;
@@ -174,14 +174,15 @@ struct MmTiles {
     col_tiles = (cols + kWide - 1) / kWide;
     row_tiles = (g.n + 255) / 256;
     total = (KIND == kWeightsGrad ? (uint32_t)g.num_experts * row_tiles : (uint32_t)uniform((int)s.units)) * col_tiles;
-    rounds = (total + gridDim.x - 1) / gridDim.x;
-    // (workgroups go to the eight XCDs in turn: neighbours in a round are on one)
-    place = gridDim.x % 8 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
+    const MmPlace at = mm_place(total);
+    place = at.place;
+    per_round = at.of;
+    rounds = place < total ? (total + per_round - 1) / per_round : 0;
   }
 
   // This workgroup's tile of a round; false where it has none.
   __device__ __forceinline__ bool tile(uint32_t round, MmTile& t) const {
-    const uint32_t p = round * gridDim.x + (round & 1 ? gridDim.x - 1 - place : place);
+    const uint32_t p = round * per_round + (round & 1 ? per_round - 1 - place : place);
     if (p >= total) return false;
     uint32_t row, col;   // of the expert's tiles
     if constexpr (KIND == kWeightsGrad) {
@@ -271,6 +272,7 @@ struct MmCopies {
   const MmTiles<TYPE, KIND>& tiles;
   uint32_t round, lds;
   int left, end_rows, along;   // steps; rows of a transposed operand in the last one; bytes of a step along rows
+  int steps, wrap;             // of the tile; those in front of its first one, which come last
   uint64_t t_base, w_base;
   uint64_t w1_base;            // SwiGLU: the up rows
   int t_len, w_len, w1_len, t_pitch, w_pitch, t_col, w_col;
@@ -300,7 +302,7 @@ struct MmCopies {
       }
     }
     round = 0;
-    left = 0;
+    left = wrap = 0;
     along = 128;
     next_tile();
   }
@@ -316,7 +318,7 @@ struct MmCopies {
       }
       if (!tiles.tile(round++, t)) t.steps = 0;
     } while (t.steps == 0);
-    left = t.steps;
+    left = steps = t.steps;
     const long w_expert = (long)t.expert * g.n * g.k * kSize;
     if constexpr (KIND == kWeightsGrad) {
       end_rows = uniform(tiles.s.rows[t.expert]) - (t.steps - 1) * 64;
@@ -355,7 +357,32 @@ struct MmCopies {
       lengths(64);
     }
     now[0] = now[1] = 0;
+    if constexpr (KIND < kRowsGrad) {
+      wrap = w_pitch % 4096 ? 0 : first_step(t);
+      left -= wrap;
+      forward(wrap);
+    }
     if (left == 1) last();
+  }
+
+  // Workgroups that begin together stay together, and where rows are whole 4096 bytes long what they read of a step is behind a few of the
+  // memory's channels.  There, tiles begin their sums at different steps (32 experts x 8 rows, 8192 x 2048: 188 us, all at the first 238; rows
+  // of 14336 bytes, with many rows an expert, lose 1 to 3% by it).  Not so the tiles that read the same rows, of eight columns of an expert;
+  // and by nothing but expert and column: the other rows of a call do not change a row's sum.
+  __device__ __forceinline__ int first_step(const MmTile& t) const {
+    const uint32_t group = (uint32_t)t.expert * ((tiles.col_tiles + 7) / 8) + (uint32_t)t.col0 / (8 * MmTiles<TYPE, KIND>::kWide);
+    return uniform((int)__umulhi(group * 2654435769u, (uint32_t)t.steps));   // (by the golden ratio: any number of them is spread evenly)
+  }
+  // Steps on along rows, or back.
+  __device__ __forceinline__ void forward(int n) {
+    t_base += n * 128;
+    w_base += n * 128;
+    t_len -= n * 128;
+    w_len -= n * 128;
+    if constexpr (kSw) {
+      w1_base += n * 128;
+      w1_len -= n * 128;
+    }
   }
 
   // Descriptors' lengths of transposed operands, of which a step has `rows` rows.
@@ -384,7 +411,11 @@ struct MmCopies {
   }
   // What there is to do when one step or none is left.
   __device__ __forceinline__ void passed() {
-    if (left == 0) next_tile();
+    if (KIND < kRowsGrad && left == 0 && wrap) {   // (rows of whole 4096 bytes: no step is short)
+      left = wrap;
+      wrap = 0;
+      forward(-steps);
+    } else if (left == 0) next_tile();
     else if (left == 1) last();
   }
 
@@ -480,7 +511,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   __shared__ MmShared s;
   mm_schedule<KIND>(s, g);
   const MmTiles<TYPE, KIND> tiles(s, g);
-  if (tiles.total == 0) return;   // (the whole launch)
+  if (tiles.rounds == 0) return;   // (the whole workgroup)
   const int wave = uniform(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
   const int lane = threadIdx.x & 63, l16 = lane & 15, gq = lane >> 4;
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s.ring;
@@ -637,6 +668,11 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   const long cols = kind >= 2 ? g.k : kind == 1 ? g.n / 2 : g.n, wide = kind == 1 ? 128 : 256, col_tiles = (cols + wide - 1) / wide;
   const long units = kind == 3 ? (long)g.num_experts * ((g.n + 255) / 256)
                                : g.total_rows / 256 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+  // A kernel of its own (expert_mm_few.hip) where there are not enough tiles for the CUs and few rows for the weights that it reads faster (us there and here,
+  // 4096 x 7168: 8 experts x 2 rows 83 / 110, x 32 rows 115 / 115, x 64 rows 189 / 122; one x 256 rows 77 / 136, x 512 rows 150 / 137; 2048 x 1024: 8
+  // experts x 64 rows 16 / 22, x 128 rows 26 / 25).  Tiles for all CUs (32 experts, 2048 x 4096: 103 / 95) are read at the memory's rate here.
+  if (kind <= 1 && (g.num_experts < g.total_rows ? g.num_experts : g.total_rows) * col_tiles < cus && g.total_rows * col_tiles <= 16 * cus)
+    return esmoe_launch_expert_mm_few(args, kind, cus, stream);
   const long tiles = units * col_tiles, grid = tiles < cus ? tiles : cus;
   if (grid == 0) return 0;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)

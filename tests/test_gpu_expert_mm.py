@@ -78,6 +78,30 @@ def test_forward(esmoe, rows, n, k, dtype):
     check_forward(esmoe, a, b, rows)
 
 
+def ragged(experts, most, seed):
+    """Rows of many experts, a third of them without any."""
+    g = np.random.default_rng(seed)
+    return [int(m) if g.random() < 0.67 else 0 for m in g.integers(1, most + 1, experts)]
+
+
+# Tiles for all CUs or many rows: the large kernel; long rows of whole 4096 bytes begin their sums at different steps there.
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,n,k", [(ragged(600, 3, 1), 16, 72), (ragged(1024, 5, 2), 24, 16), ([4100, 0, 70], 272, 136), ([3000, 1, 0, 1300], 48, 2048),
+                                      (ragged(300, 40, 3), 32, 2048), ([2, 700, 0, 513], 2320, 2048), ([1] * 40, 2048, 4096)], ids=range(7))
+def test_forward_of_many_tiles(esmoe, rows, n, k, dtype):
+    a, b, _ = operands(rows, n, k, dtype, n + k)
+    check_forward(esmoe, a, b, rows)
+
+
+# ... and few of both: one row tile or two, items of 16, 32 and 64 columns, units of an expert with more rows than one
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,n,k", [([16], 1000, 200), ([3, 0, 13], 264, 1032), ([1] * 9, 4096, 264), ([2] * 8, 2048, 520), ([17], 520, 264), ([33, 1, 0, 64], 4104, 136),
+                                      ([97, 0, 5], 2064, 2056), ([1], 8, 8), ([0, 0, 1], 16, 16384)], ids=range(9))
+def test_forward_of_few_rows(esmoe, rows, n, k, dtype):
+    a, b, _ = operands(rows, n, k, dtype, n + k)
+    check_forward(esmoe, a, b, rows)
+
+
 @pytest.mark.parametrize("n", [8, 24, 40, 264, 1000])
 def test_columns_that_fill_no_tile(esmoe, n):
     rows = [3, 130, 0, 260]

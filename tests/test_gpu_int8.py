@@ -58,6 +58,28 @@ def test_grouped_mm(esmoe, rows, n, k, dtype):
     check(run(esmoe, a, b, sa, sb, rows, offsets, True, dtype), h, 1.1 * eg * (u.abs() + eu) + (g.abs() + eg) * eu + 2.0 ** -20 * h.abs(), none, 55.0)
 
 
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("rows,n,k", [([4100, 0, 70], 272, 144), ([1, 0] * 300, 16, 48), ([2, 700, 0, 513], 2320, 4096), ([16], 1000, 208), ([2] * 8, 2048, 528),
+                                      ([33, 1, 0, 64], 4112, 144), ([97, 0, 5], 2064, 4112)], ids=range(7))
+def test_many_tiles_and_few_rows(esmoe, rows, n, k, swiglu):
+    """Each kernel and each of its shapes; sums are exact: the same bytes from all.  The scales' products are two roundings."""
+    a, b, sa, sb = operands(rows, n, k, n + k)
+    offsets = O.offsets_of(rows)
+    if swiglu and n % 16:
+        with pytest.raises(RuntimeError):
+            run(esmoe, a, b, sa, sb, rows, offsets, swiglu, BF)
+        return
+    got = run(esmoe, a, b, sa, sb, rows, offsets, swiglu, BF)
+    want = exact(a, b, sa, sb, rows, offsets)
+    none = want[:, 0].isnan()
+    err = 3 * 2.0 ** -24 * want.abs()
+    if swiglu:
+        (g, u), (eg, eu) = want.chunk(2, dim=1), err.chunk(2, dim=1)
+        want = O.swiglu(g, u)
+        err = 1.1 * eg * (u.abs() + eu) + (g.abs() + eg) * eu + 2.0 ** -20 * want.abs()
+    check(got, want, err, none, 55.0)
+
+
 def test_largest_sums(esmoe):
     """All values at their ends and the longest K: sums of 2^30, each exact."""
     k = 65536
