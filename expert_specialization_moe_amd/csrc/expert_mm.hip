@@ -184,14 +184,13 @@ struct MmTiles {
   __device__ __forceinline__ bool tile(uint32_t round, MmTile& t) const {
     const uint32_t p = round * per_round + (round & 1 ? per_round - 1 - place : place);
     if (p >= total) return false;
-    uint32_t row, col;   // of the expert's tiles
+    uint32_t first, units;   // of the expert's tiles; its rows' tiles
+    int high = 256, m = 0;
     if constexpr (KIND == kWeightsGrad) {
-      const uint32_t per = (uint32_t)row_tiles * col_tiles, rank = p / per, i = p - rank * per;
+      units = (uint32_t)row_tiles;
+      const uint32_t rank = p / (units * col_tiles);
+      first = rank * units * col_tiles;
       t.expert = uniform(s.order[rank]);
-      row = i / col_tiles;
-      col = i - row * col_tiles;
-      t.row0 = row * 256;
-      t.rows = g.n - t.row0 < 256 ? g.n - t.row0 : 256;
       t.steps = (uniform(s.rows[t.expert]) + 63) >> 6;
     } else {
       // the expert whose units' running sum is the first above this unit
@@ -211,17 +210,24 @@ struct MmTiles {
         before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
       }
       t.expert = uniform(s.order[rank]);
-      const int m = uniform(s.rows[t.expert]), high = mm_unit_rows(m);
-      // four units a group, a column's tiles together
-      const uint32_t i = p - before * col_tiles, group = i / (4 * col_tiles), j = i - group * 4 * col_tiles, have = mm_units(m) - 4 * group,
-                     wide = have < 4 ? have : 4;
-      col = j / wide;
-      row = 4 * group + j - col * wide;
-      const int from = (int)row * high;   // (the last unit may be short of rows, or without any)
+      m = uniform(s.rows[t.expert]);
+      high = mm_unit_rows(m);
+      units = mm_units(m);
+      first = before * col_tiles;
+      t.steps = KIND == kRowsGrad ? (g.n + 63) >> 6 : TYPE == kMmInt8 ? (g.k + 127) >> 7 : (g.k + 63) >> 6;
+    }
+    // four of the rows' tiles a group, a column's together: the 32 CUs of an XCD have four by eight tiles, which is the least to read (the weights'
+    // gradient, 2 x 16 tiles: 465 us, 4 x 8: 452; one expert 16384 x 4096 x 4096)
+    const uint32_t i = p - first, group = i / (4 * col_tiles), j = i - group * 4 * col_tiles, have = units - 4 * group, wide = have < 4 ? have : 4,
+                   col = j / wide, row = 4 * group + j - col * wide;
+    const int from = (int)row * high;
+    if constexpr (KIND == kWeightsGrad) {
+      t.row0 = from;
+      t.rows = g.n - from < 256 ? g.n - from : 256;
+    } else {   // (the last unit may be short of rows, or without any)
       t.row0 = uniform(s.off[t.expert]) + from;
       t.rows = m - from < high ? m - from : high;
       if (t.rows <= 0) return false;
-      t.steps = KIND == kRowsGrad ? (g.n + 63) >> 6 : TYPE == kMmInt8 ? (g.k + 127) >> 7 : (g.k + 63) >> 6;
     }
     t.col0 = (int)col * kWide;
     return true;
