@@ -263,12 +263,16 @@ namespace {
 // The call's tensors in launches of at most kGradTensors, empty ones left out; f(table, workgroups, partial sums before).
 template <typename F>
 int for_grad_tables(const void* const* grads, void* const* outputs, const int* dtypes, const long* sizes, int count, F&& f) {
-  long all = 0;
-  for (int i = 0; i < count; i++) all += (sizes[i] + esmoe::kGradChunk - 1) / esmoe::kGradChunk;
+  long all = 0, bytes = 0;
+  for (int i = 0; i < count; i++) {
+    all += (sizes[i] + esmoe::kGradChunk - 1) / esmoe::kGradChunk;
+    bytes += sizes[i] * (dtypes[i] == ESMOE_GRAD_FP32 ? 4 : 2);
+  }
   int before = 0;
   for (int i = 0; i < count;) {
     esmoe::GradTable t;
     t.count = 0;
+    t.stream = bytes > esmoe::kGradStream;
     long chunks = 0;
     for (; i < count && t.count < esmoe::kGradTensors; i++) {
       if (sizes[i] == 0) continue;
@@ -277,7 +281,7 @@ int for_grad_tables(const void* const* grads, void* const* outputs, const int* d
       t.out[t.count] = outputs ? outputs[i] : nullptr;
       t.size[t.count] = sizes[i];
       t.end[t.count] = chunks;
-      t.type[t.count++] = (uint8_t)dtypes[i];
+      t.type[t.count++] = dtypes[i];
     }
     if (t.count == 0) break;
     long grid = all <= esmoe::kGradWorkgroups ? chunks : (long)((double)esmoe::kGradWorkgroups * chunks / all) + 1;

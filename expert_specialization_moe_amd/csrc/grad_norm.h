@@ -10,6 +10,8 @@ constexpr int kGradTensors = 96;       // of a launch: the table has to fit in a
 constexpr long kGradChunk = 8192;      // elements
 constexpr int kGradWorkgroups = 2048;  // that a call's chunks are dealt to, and one more per launch at most
 
+constexpr long kGradStream = 512L << 20;
+
 struct GradTable {
   const void* in[kGradTensors];
   void* out[kGradTensors];             // clipping alone
@@ -17,6 +19,7 @@ struct GradTable {
   long end[kGradTensors];              // chunks up to and with the tensor's
   int type[kGradTensors];
   int count;
+  int stream;                          // all gradients of the call are more than kGradStream bytes
 };
 static_assert(sizeof(GradTable) <= 3600, "kernel arguments");
 

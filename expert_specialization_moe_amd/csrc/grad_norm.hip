@@ -5,9 +5,9 @@
 // A workgroup sums a contiguous share of all chunks into one partial sum; whoever needs the norm adds the partial sums in one fixed order,
 // so a call's result does not hang on which workgroup ends first and needs neither atomics nor cleared memory.
 // Bound by memory: every gradient is read for the norm, and read and written for the clipping.  3.2 GB of bf16 gradients: 476 us (6.8 TB/s)
-// and 1290 us (5.0 TB/s).  A chunk's loads are all under way before the first is used (one piece at a time: 762 and 1445 us), and neither
-// loads nor stores are to stay in the caches, which hold 256 MB (kept there: 568 us for the norm, which then waits for the last call's
-// outputs to leave).
+// and 1290 us (5.0 TB/s).  A chunk's loads are all under way before the first is used (one piece at a time: 762 and 1445 us).  What is
+// written is not kept in the caches, which hold 256 MB, and so is what is read of more than twice as much, whose second pass finds little of it
+// (us, read past the caches and kept there, both passes: 3.2 GB 1768 / 1830, 400 MB 223 / 220, 200 MB 112 / 95, 100 MB 58 / 52).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -55,17 +55,23 @@ struct Chunk {
   typedef typename Eight<T>::V V;
   V v[kPieces];
   T rest;
+  template <bool STREAM>
+  __device__ __forceinline__ static V piece(const V* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+  }
+  template <bool STREAM>
   __device__ __forceinline__ void read(const T* x, int n) {
     const int whole = n / 8;
     rest = (T)0.0f;
     if (n == kGradChunk) {   // (all loads under way at once)
 #pragma unroll
-      for (int i = 0; i < kPieces; i++) v[i] = __builtin_nontemporal_load((const V*)x + threadIdx.x + i * 256);
+      for (int i = 0; i < kPieces; i++) v[i] = piece<STREAM>((const V*)x + threadIdx.x + i * 256);
     } else {
 #pragma unroll
       for (int i = 0; i < kPieces; i++) {
         v[i] = V{};
-        if ((int)threadIdx.x + i * 256 < whole) v[i] = __builtin_nontemporal_load((const V*)x + threadIdx.x + i * 256);
+        if ((int)threadIdx.x + i * 256 < whole) v[i] = piece<STREAM>((const V*)x + threadIdx.x + i * 256);
       }
       if ((int)threadIdx.x < n - whole * 8) rest = x[whole * 8 + threadIdx.x];
     }
@@ -105,7 +111,8 @@ __global__ void __launch_bounds__(256) grad_squares_kernel(GradTable t, double* 
     auto add = [&](auto zero) {
       typedef decltype(zero) T;
       Chunk<T> chunk;
-      chunk.read((const T*)t.in[i] + first, n);
+      if (t.stream) chunk.template read<true>((const T*)t.in[i] + first, n);
+      else chunk.template read<false>((const T*)t.in[i] + first, n);
       sum += chunk.squares();
     };
     if (t.type[i] == kGradFp32) add(0.0f);
@@ -148,7 +155,7 @@ __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, const doubl
     auto clip = [&](auto zero) {
       typedef decltype(zero) T;
       Chunk<T> chunk;
-      chunk.read((const T*)t.in[i] + first, n);
+      chunk.template read<false>((const T*)t.in[i] + first, n);
       find();
       if (coef == 1.0f && t.in[i] == t.out[i]) return;
       chunk.scale(coef);
