@@ -360,7 +360,9 @@ int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, c
  *   a [total_rows, k], b [E, n, k], out: bf16 or fp16 (dtype), 16-byte aligned, sums in fp32.
  * n % 8 == 0 (% 16 with SwiGLU), k % 8 == 0, both up to 2^20; problem_sizes and expert_offsets as above, column 0 is used.  Rows of out
  * that belong to no expert are not written.  Counts and offsets are cut at total_rows; where experts claim the same rows, whose product
- * these get is open, and of more claims than an honest call can hold the last may not be served.
+ * these get is open, and of more claims than an honest call can hold the last may not be served.  The order of a sum goes by the sizes
+ * (num_experts, total_rows, n, k), the expert and the column: a call gives the same bytes every time, and a row the same whatever the others
+ * hold, but calls of other sizes may differ as another order of fp32 sums does.
  *
  * esmoe_grouped_mm_backward, from grad_out [total_rows, n]:
  *   grad_a[off_e + m, c] = cast( sum_j grad_out[off_e + m, j] * b[e, j, c] )    (rows that belong to no expert are not written)
