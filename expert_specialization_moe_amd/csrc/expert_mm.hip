@@ -145,7 +145,7 @@ __device__ __forceinline__ void mm_barrier() {
 struct MmTile {
   int expert;
   int row0, rows;   // of the tensor of rows (weights' gradient: of an expert's weights)
-  int col0;         // of the output
+  int col0, width;  // of the output
   int steps;
 };
 
@@ -164,7 +164,7 @@ struct MmTiles {
   const MmShared& s;
   const ExpertMmArgs& g;
   int cols, col_tiles, row_tiles;
-  uint32_t total, rounds, place, per_round;
+  uint32_t total, rounds, last, split, place, per_round;
 
   static constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
   static constexpr int kWide = kSw ? 128 : 256;
@@ -174,15 +174,22 @@ struct MmTiles {
     col_tiles = (cols + kWide - 1) / kWide;
     row_tiles = (g.n + 255) / 256;
     total = (KIND == kWeightsGrad ? (uint32_t)g.num_experts * row_tiles : (uint32_t)uniform((int)s.units)) * col_tiles;
-    const MmPlace at = mm_place(total);
+    // The last round's tiles in halves or quarters where there are workgroups for them (4096 x 7168, 4 experts x 128 rows: 124 us whole, 103; one
+    // x 512 rows 133, 115): by columns; with SwiGLU, whose gate and up columns no half of the products can leave out, by rows if more than 64.
+    const uint32_t grid = gridDim.x, over = total % grid;
+    split = over == 0 || over > grid / 2 ? 1 : over > grid / 4 ? 2 : 4;
+    const uint32_t all = total < grid ? total * split : total;
+    const MmPlace at = mm_place(all);
     place = at.place;
     per_round = at.of;
-    rounds = place < total ? (total + per_round - 1) / per_round : 0;
+    rounds = place < all ? (total < grid ? 1 : (total + grid - 1) / grid) : 0;
+    last = split > 1 ? (total < grid ? 0 : total / grid) : ~0u;   // the round of parts
   }
 
   // This workgroup's tile of a round; false where it has none.
   __device__ __forceinline__ bool tile(uint32_t round, MmTile& t) const {
-    const uint32_t p = round * per_round + (round & 1 ? per_round - 1 - place : place);
+    const uint32_t turn = round & 1 ? per_round - 1 - place : place, parts = round == last ? split : 1, q = turn / parts, part = turn - q * parts,
+                   p = round * per_round + q;
     if (p >= total) return false;
     uint32_t first, units;   // of the expert's tiles; its rows' tiles
     int high = 256, m = 0;
@@ -230,6 +237,19 @@ struct MmTiles {
       if (t.rows <= 0) return false;
     }
     t.col0 = (int)col * kWide;
+    t.width = kWide;
+    if (parts > 1) {
+      if (kSw && t.rows > 64) {
+        const int piece = ((t.rows + (int)parts - 1) / (int)parts + 15) & ~15, at = (int)part * piece;
+        t.row0 += at;
+        t.rows = t.rows - at < piece ? t.rows - at : piece;
+        if (t.rows <= 0) return false;
+      } else {
+        t.width = kWide / (int)parts;
+        t.col0 += (int)part * t.width;
+        if (t.col0 >= cols) return false;
+      }
+    }
     return true;
   }
 };
@@ -341,7 +361,7 @@ struct MmCopies {
         w_col = t.col0 * 2;
         w_base = (uint64_t)g.w + w_expert + w_col - kBias;
       } else {
-        const int left_rows = tiles.cols - t.col0, n = left_rows < (kSw ? 128 : 256) ? left_rows : (kSw ? 128 : 256);
+        const int left_rows = tiles.cols - t.col0, n = left_rows < t.width ? left_rows : t.width;
         w_base = (uint64_t)g.w + w_expert + (long)t.col0 * w_pitch - kBias;
         w_len = uniform(n * w_pitch + kBias);
         if constexpr (kSw) {
@@ -358,8 +378,8 @@ struct MmCopies {
         edge_t0 = t.row0 + at >= g.n ? kNowhere : 0;
         edge_t1 = t.row0 + at + 128 >= g.n ? kNowhere : 0;
       }
-      edge_w0 = t.col0 + at >= g.k ? kNowhere : 0;
-      edge_w1 = t.col0 + at + 128 >= g.k ? kNowhere : 0;
+      edge_w0 = at >= t.width || t.col0 + at >= g.k ? kNowhere : 0;
+      edge_w1 = at + 128 >= t.width || t.col0 + at + 128 >= g.k ? kNowhere : 0;
       lengths(64);
     }
     now[0] = now[1] = 0;
@@ -559,8 +579,8 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
     auto arrived = [&] { mm_wait_copies<8, kStores>(stored); };
     // A phase's matrix half, of the tile's upper or lower half of rows; behind its first products the first half of the next fragments of T, into
     // the registers that these leave.  A group whose sixteens have no rows has nothing to multiply.
-    const int rows = t.rows - wm * 16;
-    auto multiply = [&](auto lower, Acc (&c)[4][2], const v4i (&w)[2][2], auto&& early0, auto&& early1) {
+    const int rows0 = t.rows - wm * 16, rows1 = kSw || t.width > 128 ? rows0 : 0;   // for the first and second half of the columns
+    auto multiply = [&](auto lower, int rows, Acc (&c)[4][2], const v4i (&w)[2][2], auto&& early0, auto&& early1) {
       constexpr int kFirst = decltype(lower)::value * 128;
       products<TYPE, kBegin, 0, kFirst>(c, w, tf, rows);
       early0();
@@ -578,31 +598,31 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
       arrived();
       mm_wait_fragments<kTReads>();   // (all but those just read)
       mm_barrier();
-      multiply(upper, acc[0][0], wf0, [&] { w_at.template read<kW1, 0, 1>(stage, wf1); }, [&] { w_at.template read<kW1, 1, 2>(stage, wf1); });
+      multiply(upper, rows0, acc[0][0], wf0, [&] { w_at.template read<kW1, 0, 1>(stage, wf1); }, [&] { w_at.template read<kW1, 1, 2>(stage, wf1); });
 
       if (__builtin_expect(--copies.left <= 1, 0)) copies.passed();
       mm_copy(copies.template w_part<0>(stage));
       mm_barrier();
-      multiply(upper, acc[0][1], wf1, [&] { t_at.template read<kT1, 0, 1>(stage, tf); }, [&] { t_at.template read<kT1, 1, 2>(stage, tf); });
+      multiply(upper, rows1, acc[0][1], wf1, [&] { t_at.template read<kT1, 0, 1>(stage, tf); }, [&] { t_at.template read<kT1, 1, 2>(stage, tf); });
 
       t_at.template read<kT1, 2, 4>(stage, tf);
       mm_copy(copies.template t_part<0>(stage));
       arrived();
       mm_barrier();
-      multiply(lower, acc[1][0], wf0, none, none);
+      multiply(lower, rows0, acc[1][0], wf0, none, none);
 
       w_at.template read<kW0>(stage ^ kMmStage, wf0);
       mm_copy(copies.template w_part<1>(stage));
       arrived();
       mm_barrier();
       stage ^= kMmStage;
-      multiply(lower, acc[1][1], wf1, [&] { t_at.template read<kT0, 0, 1>(stage, tf); }, [&] { t_at.template read<kT0, 1, 2>(stage, tf); });
+      multiply(lower, rows1, acc[1][1], wf1, [&] { t_at.template read<kT0, 0, 1>(stage, tf); }, [&] { t_at.template read<kT0, 1, 2>(stage, tf); });
       stored = 0;
     }
 
     mm_results();
     // a lane holds, of rows a * 128 + (2 i + wm) * 16 + l16, columns b * 128 + wn * 32 + j * 16 + 4 gq .. + 4
-    const int room = tiles.cols - t.col0, col = wn * 32 + (gq & 1) * 16 + (gq >> 1) * 8;
+    const int room = tiles.cols - t.col0 < t.width ? tiles.cols - t.col0 : t.width, col = wn * 32 + (gq & 1) * 16 + (gq >> 1) * 8;
     const long out_row0 = KIND == kWeightsGrad ? (long)t.expert * g.n + t.row0 : (long)t.row0;
     const MmOut out(g.out, out_row0, t.rows, t.col0, tiles.cols);
     const bool fp16 = TYPE == kMmFp16 || (TYPE == kMmInt8 && g.out_fp16);
@@ -675,11 +695,11 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   const long units = kind == 3 ? (long)g.num_experts * ((g.n + 255) / 256)
                                : g.total_rows / 256 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
   // A kernel of its own (expert_mm_few.hip) where there are not enough tiles for the CUs and few rows for the weights that it reads faster (us there and here,
-  // 4096 x 7168: 8 experts x 2 rows 83 / 110, x 32 rows 115 / 115, x 64 rows 189 / 122; one x 256 rows 77 / 136, x 512 rows 150 / 137; 2048 x 1024: 8
-  // experts x 64 rows 16 / 22, x 128 rows 26 / 25).  Tiles for all CUs (32 experts, 2048 x 4096: 103 / 95) are read at the memory's rate here.
+  // 4096 x 7168: 8 experts x 2 rows 83 / 102, x 32 rows 115 / 106, x 64 rows 189 / 111; one x 256 rows 81 / 113, x 512 rows 150 / 115; 2048 x 1024: 8
+  // experts x 64 rows 16 / 21, x 128 rows 26 / 23).  Tiles for all CUs (32 experts, 2048 x 4096: 103 / 95) are read at the memory's rate here.
   if (kind <= 1 && (g.num_experts < g.total_rows ? g.num_experts : g.total_rows) * col_tiles < cus && g.total_rows * col_tiles <= 16 * cus)
     return esmoe_launch_expert_mm_few(args, kind, cus, stream);
-  const long tiles = units * col_tiles, grid = tiles < cus ? tiles : cus;
+  const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
 #define ESMOE_MM16(T)                                  \
