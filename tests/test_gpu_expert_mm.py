@@ -93,6 +93,21 @@ def test_forward_of_many_tiles(esmoe, rows, n, k, dtype):
     check_forward(esmoe, a, b, rows)
 
 
+# 300 tiles and 357 of 256 CUs: the last round's in quarters and in halves, by columns and (SwiGLU of more than 64 rows) by rows
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,n,k", [([2] * 100, 528, 72), ([2] * 119, 528, 72), ([100, 0, 66] * 50, 528, 136), ([70] * 119, 528, 64)], ids=range(4))
+def test_a_last_round_in_parts(esmoe, rows, n, k, dtype):
+    a, b, _ = operands(rows, n, k, dtype, n + k)
+    check_forward(esmoe, a, b, rows)
+    n, k = k, n
+    a, b, d = operands(rows, n, k, dtype, n + k)
+    offsets = O.offsets_of(rows)
+    ga_want, ga_mag, _, gb_want, gb_mag, _ = O.grouped_mm_grads(d, a, b, rows, offsets)
+    ga, gb = esmoe.es_grouped_mm_backward(d, a, b.transpose(1, 2), *meta(rows, offsets, n, k))
+    check(ga, ga_want, sum_error(n, ga_mag), ga_want[:, 0].isnan(), 0.0)
+    check(gb.transpose(1, 2), gb_want, sum_error(max(rows), gb_mag))
+
+
 # ... and few of both: one row tile or two, items of 16, 32 and 64 columns, units of an expert with more rows than one
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("rows,n,k", [([16], 1000, 200), ([3, 0, 13], 264, 1032), ([1] * 9, 4096, 264), ([2] * 8, 2048, 520), ([17], 520, 264), ([33, 1, 0, 64], 4104, 136),
