@@ -1,11 +1,13 @@
-// Grouped products of experts with few rows each (decode), 16 bits and int8: the sums of expert_mm.hip's forward forms.
+// Grouped products of experts with few rows each (decode, small steps), 16 bits and int8: the sums of expert_mm.hip's forward forms and rows' gradient.
 //
-// Bound by the weights' way from memory, and nothing is reused that would pay for LDS: an item is 16, 32 or 64 columns (SwiGLU: half of them gate
-// columns, half their up columns) of up to 16 or 32 rows of an expert, whose sum the four wavefronts of a workgroup split in steps of 128 bytes dealt
-// in turn.  Each loads weights and rows in the layout of the matrix instruction, several steps ahead in registers, across items; the four
-// sums are added in LDS, in one order.  An expert's items of the same columns are neighbours on one XCD: their weights come from memory once.
+// Bound by the weights' way from memory.  An item is 16 to 64 columns (SwiGLU: half of them gate columns, half their up columns) of up to 16 or 32 rows of
+// an expert, whose sum the four wavefronts of a workgroup split in steps of 128 bytes dealt in turn.  Weights and rows go from memory straight
+// into LDS, rows of 128 bytes whole: loads into registers in the layout of the matrix instruction touch half of sixteen lines each, and few
+// lines can be under way (8 experts x 32 rows, 4096 x 7168: 115 us so, 81).  A wavefront has a ring of steps of its own, as many as LDS holds,
+// whose copies run on across items; it waits for its own copies and reads, and no barrier stands in the way.  The four sums are added in
+// LDS, in one order for any number of rows.  An expert's items of the same columns are neighbours on one XCD: their weights come from memory once.
 // What lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
-// One row of each of 8 experts, 4096 x 7168 with SwiGLU, bf16: 79 us (5.9 TB/s of weights), int8 43 us.
+// One row of each of 8 experts, 4096 x 7168 with SwiGLU, bf16: 78 us (6.0 TB/s of weights), int8 41 us; 32 experts x 8 rows 299 us (6.3 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -20,13 +22,14 @@ namespace esmoe {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
-enum { kFewForward = 0, kFewSwiglu = 1, kFewSwigluSave = 2 };
+enum { kFewForward = 0, kFewSwiglu = 1, kFewSwigluSave = 2, kFewRowsGrad = 3 };
 
 constexpr int kFewWaves = 4, kFewThreads = 64 * kFewWaves;
 constexpr int kFewNowhere = (int)0x80000000u;   // an offset beyond every descriptor
@@ -42,161 +45,198 @@ __device__ __forceinline__ typename FewAcc<TYPE>::T few_product(v4i w, v4i t, ty
 }
 
 __device__ __forceinline__ int few_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t few_buffer(const void* p, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes > 0 ? bytes : 0, 0x00020000);
+__device__ __forceinline__ v4i few_descriptor(const void* p, int bytes) {
+  return v4i{few_uniform((int)(uint64_t)p), few_uniform((int)((uint64_t)p >> 32)), few_uniform(bytes > 0 ? bytes : 0), 0x00020000};
 }
-__device__ __forceinline__ v4i few_load(__amdgpu_buffer_rsrc_t rsrc, int at) {
-  return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+// 64 x 16 bytes into LDS (a scalar register that a vector instruction wrote is there for a memory instruction five slots on)
+__device__ __forceinline__ void few_copy(uint32_t lds, v4i rsrc, int at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(at), "s"(rsrc) : "memory");
 }
 __device__ __forceinline__ v2i few_half4(v4f v, bool fp16) {
   return fp16 ? __builtin_bit_cast(v2i, __builtin_convertvector(v, v4h)) : __builtin_bit_cast(v2i, __builtin_convertvector(v, v4bf));
 }
 
-template <int NT, int NC>
-struct FewShared {
-  v4f sums[kFewWaves][NT * NC][64];   // [row tile * NC + column tile][lane]
+// The experts' rows, cut at the tensor's, in units of ROWS.
+template <int ROWS>
+struct FewTable {
   int rows[kMmExperts], off[kMmExperts];
-  uint32_t unit_end[kMmExperts];   // running sums of the experts' units of NT * 16 rows
+  uint32_t unit_end[kMmExperts];   // running sums of units
   uint32_t units;
+
+  __device__ __forceinline__ void build(const ExpertMmArgs& g) {
+    const int lane = threadIdx.x;
+    if (lane < 64) {
+      uint32_t sum = 0;
+      for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+        const int e = e0 + lane, o = e < g.num_experts ? g.expert_offsets[e] : 0;
+        const int m = e < g.num_experts ? fp4_rows(g.problem_sizes[e * 3], o, g.total_rows) : 0;
+        const uint32_t end = sum_or_most(sum, wave_inclusive_sum_or_most(((uint32_t)m + ROWS - 1) / ROWS));
+        if (e < g.num_experts) {
+          rows[e] = m;
+          off[e] = o;
+          unit_end[e] = end;
+        }
+        sum = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+      }
+      if (lane == 0) {   // no more than experts with rows of their own can have
+        const uint32_t most = (uint32_t)(g.total_rows / ROWS) + (uint32_t)(g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
+        units = sum < most ? sum : most;
+      }
+    }
+    __syncthreads();
+  }
 };
 
+// Columns col0 .. + WIDE of up to ROWS rows of an expert; no rows where there is no such item.
 struct FewItem {
-  __amdgpu_buffer_rsrc_t t, w0, w1;
   int expert, rows, col0;
   long row0;
 };
-
-// NT row tiles x NC column tiles of sixteen; SwiGLU: the second half of the latter are the up columns.
-template <int TYPE, int KIND, int NT, int NC, int AHEAD>
-__global__ void __launch_bounds__(kFewThreads, 2) expert_mm_few_kernel(const ExpertMmArgs g) {
-  typedef typename FewAcc<TYPE>::T Acc;
-  constexpr bool kSw = KIND != kFewForward;
-  constexpr int kTiles = kSw ? NC / 2 : NC, kWide = kTiles * 16, kRows = NT * 16, kSize = TYPE == kMmInt8 ? 1 : 2;
-  __shared__ FewShared<NT, NC> s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = few_uniform(tid >> 6);
-  if (wave == 0) {
-    uint32_t units = 0;
-    for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
-      const int e = e0 + lane, off = e < g.num_experts ? g.expert_offsets[e] : 0;
-      const int rows = e < g.num_experts ? fp4_rows(g.problem_sizes[e * 3], off, g.total_rows) : 0;
-      const uint32_t end = sum_or_most(units, wave_inclusive_sum_or_most(((uint32_t)rows + kRows - 1) / kRows));
-      if (e < g.num_experts) {
-        s.rows[e] = rows;
-        s.off[e] = off;
-        s.unit_end[e] = end;
-      }
-      units = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+template <int ROWS, int WIDE>
+__device__ __forceinline__ FewItem few_item(const FewTable<ROWS>& s, const ExpertMmArgs& g, uint32_t p, uint32_t total, uint32_t col_items) {
+  FewItem t = {g.num_experts - 1, 0, 0, 0};
+  if (p >= total) return t;
+  // the expert whose units' running sum is the first above this unit
+  const uint32_t unit = p / col_items;
+  const int lane = threadIdx.x & 63;
+  uint32_t before = 0, behind = 0;
+  for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
+    const uint32_t end = e0 + lane < g.num_experts ? s.unit_end[e0 + lane] : 0xffffffffu;
+    const unsigned long long past = __ballot(end > unit);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      if (e0 + l < g.num_experts) t.expert = e0 + l;
+      if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
+      behind = (uint32_t)__builtin_amdgcn_readlane((int)end, l);
+      break;
     }
-    if (lane == 0) {   // no more than experts with rows of their own can have
-      const uint32_t most = (uint32_t)(g.total_rows / kRows) + (uint32_t)(g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
-      s.units = units < most ? units : most;
-    }
+    before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
   }
-  __syncthreads();
-  const int cols = kSw ? g.n / 2 : g.n, pitch = g.k * kSize;
-  const uint32_t col_items = (cols + kWide - 1) / kWide, total = (uint32_t)few_uniform((int)s.units) * col_items;
+  const uint32_t i = p - before * col_items, units = behind - before, col_item = i / units;
+  const int from = (int)(i - col_item * units) * ROWS, left = few_uniform(s.rows[t.expert]) - from;
+  t.rows = left < ROWS ? left : ROWS;
+  t.row0 = (long)few_uniform(s.off[t.expert]) + from;
+  t.col0 = (int)col_item * WIDE;
+  return t;
+}
 
-  auto item = [&](uint32_t p) {
-    FewItem t;
-    t.expert = g.num_experts - 1;
-    t.rows = t.col0 = 0;
-    t.row0 = 0;
-    if (p < total) {
-      // the expert whose units' running sum is the first above this unit
-      const uint32_t unit = p / col_items;
-      uint32_t before = 0, behind = 0;
-      for (int e0 = 0; e0 < g.num_experts; e0 += 64) {
-        const uint32_t end = e0 + lane < g.num_experts ? s.unit_end[e0 + lane] : 0xffffffffu;
-        const unsigned long long past = __ballot(end > unit);
-        if (past) {
-          const int l = __builtin_ctzll(past);
-          if (e0 + l < g.num_experts) t.expert = e0 + l;
-          if (l) before = (uint32_t)__builtin_amdgcn_readlane((int)end, l - 1);
-          behind = (uint32_t)__builtin_amdgcn_readlane((int)end, l);
-          break;
-        }
-        before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
-      }
-      const uint32_t i = p - before * col_items, units = behind - before, col_item = i / units;
-      const int from = (int)(i - col_item * units) * kRows, left = few_uniform(s.rows[t.expert]) - from;
-      t.rows = left < kRows ? left : kRows;
-      t.row0 = (long)few_uniform(s.off[t.expert]) + from;
-      t.col0 = (int)col_item * kWide;
-    }
-    const long w_row = (long)t.expert * g.n + t.col0;
-    const int wide = cols - t.col0 < kWide ? cols - t.col0 : kWide, w_len = t.rows ? wide * pitch : 0;
-    t.t = few_buffer((const char*)g.t + t.row0 * pitch, t.rows * pitch);
-    t.w0 = few_buffer((const char*)g.w + w_row * pitch, w_len);
-    t.w1 = few_buffer((const char*)g.w + (w_row + (kSw ? cols : 0)) * pitch, w_len);
-    return t;
-  };
+template <int NT, int NC, int DEPTH>
+struct FewShared {
+  static constexpr int kWeights = NC * 2048, kStep = kWeights + NT * 2048;
+  uint8_t ring[kFewWaves][DEPTH][kStep];   // a step: sixteen rows of 128 bytes a tile, the weights' tiles first
+  v4f sums[kFewWaves][NT * NC][64];        // [row tile * NC + column tile][lane]
+  FewTable<NT * 16> table;
+};
 
-  // A wavefront's steps, AHEAD of them on their way: lane l has 16 bytes along the sum of row (column) l % 16 at 16 * (l / 16), in each half of a
-  // step.  An item's last steps are followed by the first ones of the next item.
-  const int rounds = (pitch + kFewWaves * 128 - 1) / (kFewWaves * 128), row_at = (lane & 15) * pitch, along = wave * 128 + (lane >> 4) * 16;
-  v4i tf[AHEAD][NT][2], wf[AHEAD][NC][2];
-  Acc c[NT][NC];
-  auto load = [&](const FewItem& t, int step, int d) {
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      const int k = step * (kFewWaves * 128) + along + ks * 64, at = k < pitch ? row_at + k : kFewNowhere;
-#pragma unroll
-      for (int j = 0; j < NC; j++) wf[d][j][ks] = few_load(kSw && j >= kTiles ? t.w1 : t.w0, at + j % kTiles * 16 * pitch);
-#pragma unroll
-      for (int i = 0; i < NT; i++) tf[d][i][ks] = few_load(t.t, at + i * 16 * pitch);
-    }
-    __builtin_amdgcn_sched_barrier(0);   // (steps stay in their order: the compiler would put all loads together and wait for them together)
-  };
-  auto multiply = [&](int d) {
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int j = 0; j < NC; j++) c[i][j] = few_product<TYPE>(wf[d][j][ks], tf[d][i][ks], c[i][j]);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
+// NT row tiles x NC column tiles of sixteen (SwiGLU: the second half of the latter are the up columns), the sum over four wavefronts, DEPTH steps of each in LDS.
+template <int TYPE, int KIND, int NT, int NC, int DEPTH>
+__global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const ExpertMmArgs g) {
+  typedef typename FewAcc<TYPE>::T Acc;
+  typedef FewShared<NT, NC, DEPTH> Shared;
+  typedef __attribute__((address_space(3))) char* Lds;
+  constexpr bool kSw = KIND == kFewSwiglu || KIND == kFewSwigluSave, kGrad = KIND == kFewRowsGrad;
+  constexpr int kTiles = kSw ? NC / 2 : NC, kWide = kTiles * 16, kRows = NT * 16, kSize = TYPE == kMmInt8 ? 1 : 2, kCopies = Shared::kStep / 1024;
+  static_assert(sizeof(Shared) <= 160 * 1024, "LDS");
+  static_assert(!kGrad || NC == 4, "a weight row of a step is 128 bytes");
+  __shared__ Shared s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = few_uniform(tid >> 6), l16 = lane & 15, gq = lane >> 4;
+  s.table.build(g);
+  const int cols = kSw ? g.n / 2 : kGrad ? g.k : g.n, pitch = (kGrad ? g.n : g.k) * kSize, w_pitch = g.k * kSize;
+  const int rounds = (pitch + kFewWaves * 128 - 1) / (kFewWaves * 128);
+  const uint32_t col_items = (cols + kWide - 1) / kWide, total = (uint32_t)few_uniform((int)s.table.units) * col_items;
   const MmPlace at = mm_place(total);
-  uint32_t p = at.place;
-  FewItem next = item(p);
+  const uint32_t ring = (uint32_t)few_uniform((int)(uint32_t)(uintptr_t)(Lds)(char*)s.ring[wave][0]);
+
+  // A copy is eight rows of 128 bytes.  Rows along the sum: chunk x of row r in slot x ^ (r / 2 % 8), sixteen rows' reads of a chunk fall on different
+  // banks.  Weight rows across it (the gradient): pairs of chunks change places by the row's bits 1 and 3, which does the same for the transposing read.
+  const int row8 = lane >> 3;
+  int chunk[2], w_chunk[2];   // bytes along a row, of even and odd copies
 #pragma unroll
-  for (int d = 0; d < AHEAD; d++) load(next, d, d);
-  for (; p < total; p += at.of) {
-    const FewItem t = next;
-    next = item(p + at.of);
-    // Outputs: a unit is a tile's lane: row l % 16, columns 4 (l / 16) .. + 4.
-    constexpr int kUnits = NT * kTiles * 64, kEach = (kUnits + kFewThreads - 1) / kFewThreads;
-    // int8: scales, asked for ahead of the sums
-    float sa[kEach];
-    v4f sb[kEach][kSw ? 2 : 1];
-    if constexpr (TYPE == kMmInt8) {
-      const auto of_rows = few_buffer(g.sa + t.row0, t.rows * 4), of_cols = few_buffer(g.sb + (long)t.expert * g.n, g.n * 4);
+  for (int q = 0; q < 2; q++) {
+    const int row = q * 8 + row8, x = lane & 7;
+    chunk[q] = (x ^ (row >> 1 & 7)) * 16;
+    w_chunk[q] = kGrad ? ((x >> 1 ^ ((row >> 1 & 1) | (row >> 3 & 1) << 1)) << 1 | (x & 1)) * 16 : chunk[q];
+  }
+  // The copies' item and round, ahead of the products'.
+  uint32_t copy_p = at.place;
+  int copy_round = 0;
+  FewItem item = few_item<kRows, kWide>(s.table, g, copy_p, total, col_items);
+  auto copy = [&](uint32_t slot) {
+    const int step = copy_round * kFewWaves + wave, along = step * 128;
+    if constexpr (kGrad) {
+      const char* w = (const char*)g.w + ((long)item.expert * g.n + step * 64) * w_pitch + item.col0 * 2;
+      const int have = g.n - step * 64 < 64 ? g.n - step * 64 : 64;
+      const v4i wd = few_descriptor(w, item.rows && have > 0 ? have * w_pitch - item.col0 * 2 : 0);
 #pragma unroll
-      for (int u = 0; u < kEach; u++) {
-        const int tile = (tid + u * kFewThreads) >> 6, row = tile / kTiles * 16 + (lane & 15), col = tile % kTiles * 16 + (lane >> 4) * 4;
-        sa[u] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of_rows, row * 4, 0, 0));
+      for (int q = 0; q < NC * 2; q++) few_copy(few_uniform(ring + slot + q * 1024), wd, w_chunk[q & 1] + (q * 8 + row8) * w_pitch);
+    } else {
+      const char* w = (const char*)g.w + ((long)item.expert * g.n + item.col0) * w_pitch;
+      const int have = cols - item.col0 < kWide ? cols - item.col0 : kWide, len = item.rows ? have * w_pitch : 0;
 #pragma unroll
-        for (int h = 0; h < (kSw ? 2 : 1); h++) sb[u][h] = __builtin_bit_cast(v4f, few_load(of_cols, (h * cols + t.col0 + col) * 4));
+      for (int h = 0; h < (kSw ? 2 : 1); h++) {
+        const v4i wd = few_descriptor(w + h * (long)cols * w_pitch, len);
+#pragma unroll
+        for (int q = 0; q < kTiles * 2; q++) {
+          const int x = w_chunk[q & 1] + along;
+          few_copy(few_uniform(ring + slot + (h * kTiles * 2 + q) * 1024), wd, x < pitch ? (q * 8 + row8) * w_pitch + x : kFewNowhere);
+        }
       }
     }
-
+    const v4i td = few_descriptor((const char*)g.t + item.row0 * pitch, item.rows * pitch);
+#pragma unroll
+    for (int q = 0; q < NT * 2; q++) {
+      const int x = chunk[q & 1] + along;
+      few_copy(few_uniform(ring + slot + Shared::kWeights + q * 1024), td, x < pitch ? (q * 8 + row8) * pitch + x : kFewNowhere);
+    }
+    if (++copy_round == rounds) {
+      copy_round = 0;
+      copy_p = copy_p < total ? copy_p + at.of : copy_p;
+      item = few_item<kRows, kWide>(s.table, g, copy_p, total, col_items);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; d++) copy(d * Shared::kStep);
+  uint32_t slot = 0;
+  for (uint32_t p = at.place; p < total; p += at.of) {
+    const FewItem t = few_item<kRows, kWide>(s.table, g, p, total, col_items);
+    Acc c[NT][NC];
 #pragma unroll
     for (int i = 0; i < NT; i++)
 #pragma unroll
       for (int j = 0; j < NC; j++) c[i][j] = Acc{0, 0, 0, 0};
-    // (an item's steps are a multiple of AHEAD, the last ones of nothing: conditions among them would make the compiler move what is under way)
-    for (int r = AHEAD; r < rounds; r += AHEAD) {
+    for (int r = 0; r < rounds; r++) {
+      // (a wavefront reads, and copies into again, what is its own: it waits for its own copies and reads)
+      asm volatile("s_waitcnt vmcnt(%0) ; explicit" ::"n"((DEPTH - 1) * kCopies) : "memory");
+      v4i tf[NT][2], wf[NC][2];
+      const Lds step = (Lds)(uintptr_t)(ring + slot);
+      auto along = [&](int row, int ks) { return *(const __attribute__((address_space(3))) v4i*)(step + row * 128 + ((gq + ks * 4) ^ (l16 >> 1)) * 16); };
 #pragma unroll
-      for (int d = 0; d < AHEAD; d++) {
-        multiply(d);
-        load(t, r + d, d);
+      for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+        for (int i = 0; i < NT; i++) tf[i][ks] = along(NC * 16 + i * 16 + l16, ks);
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+          if constexpr (kGrad) {
+            // four lanes read 16 columns of a row, sixteen lanes of four rows, and the hardware hands lane i column i
+            typedef __attribute__((address_space(3))) v4s* Lds4;
+            const int row = ks * 32 + gq * 8 + (l16 >> 2), f = (row >> 1 & 1) | (row >> 3 & 1) << 1;
+            const Lds from = step + row * 128 + (j ^ f) * 32 + (l16 & 3) * 8;   // (row + 4: of the same bits 1 and 3)
+            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)from)),
+                      hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(from + 4 * 128)));
+            wf[j][ks] = v4i{lo[0], lo[1], hi[0], hi[1]};
+          } else wf[j][ks] = along(j * 16 + l16, ks);
+        }
       }
-    }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      copy(slot);
+      slot = slot == (DEPTH - 1) * Shared::kStep ? 0 : slot + Shared::kStep;
 #pragma unroll
-    for (int d = 0; d < AHEAD; d++) {
-      multiply(d);
-      load(next, d, d);
+      for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+          for (int j = 0; j < NC; j++) c[i][j] = few_product<TYPE>(wf[j][ks], tf[i][ks], c[i][j]);
     }
 
     __syncthreads();   // (the sums of the item before have been read)
@@ -205,24 +245,29 @@ __global__ void __launch_bounds__(kFewThreads, 2) expert_mm_few_kernel(const Exp
 #pragma unroll
       for (int j = 0; j < NC; j++) s.sums[wave][i * NC + j][lane] = __builtin_bit_cast(v4f, c[i][j]);
     __syncthreads();
+    // Outputs: a unit is a tile's lane: row l % 16, columns 4 (l / 16) .. + 4.
+    constexpr int kUnits = NT * kTiles;
     const bool fp16 = TYPE == kMmFp16 || (TYPE == kMmInt8 && g.out_fp16);
     auto put = [&](void* out, int width, v2i v, int row, int col) { *(v2i*)((char*)out + ((t.row0 + row) * width + col) * 2) = v; };
 #pragma unroll
-    for (int u = 0; u < kEach; u++) {
-      const int tile = (tid + u * kFewThreads) >> 6;
-      if (kUnits % kFewThreads && tile * 64 >= kUnits) break;
-      const int row = tile / kTiles * 16 + (lane & 15), col = t.col0 + tile % kTiles * 16 + (lane >> 4) * 4;
+    for (int u = 0; u < (kUnits + kFewWaves - 1) / kFewWaves; u++) {
+      const int tile = wave + u * kFewWaves, row = tile / kTiles * 16 + l16, col = t.col0 + tile % kTiles * 16 + gq * 4;
+      if (kUnits % kFewWaves && tile >= kUnits) break;
+      if (row >= t.rows || col >= cols) continue;
       v4f sum[kSw ? 2 : 1];
 #pragma unroll
       for (int h = 0; h < (kSw ? 2 : 1); h++) {
-        const int at = tile / kTiles * NC + h * kTiles + tile % kTiles;
-        Acc all = __builtin_bit_cast(Acc, s.sums[0][at][lane]);
+        const int part = tile / kTiles * NC + h * kTiles + tile % kTiles;
+        Acc all = __builtin_bit_cast(Acc, s.sums[0][part][lane]);
 #pragma unroll
-        for (int w = 1; w < kFewWaves; w++) all += __builtin_bit_cast(Acc, s.sums[w][at][lane]);
+        for (int w = 1; w < kFewWaves; w++) all += __builtin_bit_cast(Acc, s.sums[w][part][lane]);
+        if constexpr (TYPE == kMmInt8) {
+          const float sa = g.sa[t.row0 + row];
+          const v4f sb = *(const v4f*)(g.sb + (long)t.expert * g.n + h * cols + col);
 #pragma unroll
-        for (int x = 0; x < 4; x++) sum[h][x] = TYPE == kMmInt8 ? (float)all[x] * sa[u] * sb[u][h][x] : (float)all[x];
+          for (int x = 0; x < 4; x++) sum[h][x] = (float)all[x] * sa * sb[x];
+        } else sum[h] = all;
       }
-      if (row >= t.rows || col >= cols) continue;
       if constexpr (kSw) {
         v4f y;
 #pragma unroll
@@ -235,48 +280,51 @@ __global__ void __launch_bounds__(kFewThreads, 2) expert_mm_few_kernel(const Exp
       } else put(g.out, cols, few_half4(sum[0], fp16), row, col);
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (nothing may arrive in LDS that is another workgroup's by then)
+}
+
+template <int TYPE, int KIND, int NT, int NC, int DEPTH>
+int few_launch(const ExpertMmArgs& g, int cus, hipStream_t stream) {
+  const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
+  const int cols = KIND == kFewRowsGrad ? g.k : KIND == kFewForward ? g.n : g.n / 2, wide = KIND == kFewSwiglu || KIND == kFewSwigluSave ? NC * 8 : NC * 16;
+  const long items = (g.total_rows / (16 * NT) + experts) * ((cols + wide - 1) / wide);
+  const long most = (160 * 1024 / sizeof(FewShared<NT, NC, DEPTH>)) * (long)cus, grid = items < most ? items : most;
+  if (grid == 0) return 0;
+  hipLaunchKernelGGL((expert_mm_few_kernel<TYPE, KIND, NT, NC, DEPTH>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
+  return (int)hipGetLastError();
 }
 
 }  // namespace esmoe
 
 using namespace esmoe;
 
+// kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows
 extern "C" int esmoe_launch_expert_mm_few(const ExpertMmArgs* args, int kind, int cus, hipStream_t stream) {
   const ExpertMmArgs& g = *args;
   const long cols = kind == 1 ? g.n / 2 : g.n, experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
-  const int row_tiles = g.total_rows <= 16 ? 1 : 2;
-  auto col_items = [&](int col_tiles) {
-    const int wide = col_tiles * 16 / (kind == 1 ? 2 : 1);
-    return (cols + wide - 1) / wide;
+  // Half as wide an item where rows are few, or to leave no CU without (us, 32 and 64 columns, 4096 x 7168: 2 experts x 16 rows 23 / 30, 8 x 16 rows 79 / 80;
+  // 8 x 32 rows 90 / 81, one x 256 rows 46 / 35: the rows come from L2 once for each item).
+  const long units = experts > g.total_rows / 32 ? experts : g.total_rows / 32, wide = kind == 1 ? 16 : 32;   // of 32 rows, if they are spread evenly
+  const bool narrow = units * ((cols + wide - 1) / wide) <= cus || g.total_rows <= 16 * experts;
+  auto launch = [&](auto type, auto k) {
+    constexpr int TYPE = decltype(type)::value, KIND = decltype(k)::value;
+    if constexpr (KIND == kFewRowsGrad) {
+      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 4, 3>(g, cus, stream);
+    } else {
+      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 2, 4>(g, cus, stream);
+      if (narrow) return few_launch<TYPE, KIND, 2, 2, 3>(g, cus, stream);
+    }
+    return few_launch<TYPE, KIND, 2, 4, 2>(g, cus, stream);
   };
-  // As wide an item as leaves one for every CU: the rows come from L2 once for each (us, wide and narrow, 4096 x 7168: 4 experts x 16 rows 53 / 60, one
-  // x 256 rows 77 / 101; with half as many items as CUs, 2 x 16 rows 47 / 32).  16 rows at most are little beside 32 columns.
-  const long least = experts > g.total_rows / 32 ? experts : g.total_rows / 32;   // units, if rows are spread evenly
-  const int col_tiles = row_tiles == 1 ? (kind == 0 && experts * col_items(2) < cus ? 1 : 2) : least * col_items(4) < cus ? 2 : 4;
-  const long items = (g.total_rows / (16 * row_tiles) + experts) * col_items(col_tiles), grid = items < 2 * cus ? items : 2 * cus;
-  if (grid == 0) return 0;
-  // (as many steps ahead as let two workgroups live on a CU)
-#define ESMOE_FEW(T, K, NT, NC, AHEAD) \
-  hipLaunchKernelGGL((expert_mm_few_kernel<T, K, NT, NC, AHEAD>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g)
-#define ESMOE_FEW3(T, K)                                                              \
-  {                                                                                   \
-    if (row_tiles == 2 && col_tiles == 4) ESMOE_FEW(T, K, 2, 4, 2);                   \
-    else if (row_tiles == 2) ESMOE_FEW(T, K, 2, 2, 4);                                \
-    else if (K != kFewForward || col_tiles == 2) ESMOE_FEW(T, K, 1, 2, 4);            \
-    else ESMOE_FEW(T, K, 1, (K == kFewForward ? 1 : 2), 4);                           \
-  }
-#define ESMOE_FEW9(T)                                    \
-  {                                                      \
-    if (kind == 0) ESMOE_FEW3(T, kFewForward)            \
-    else if (g.gate_up) ESMOE_FEW3(T, kFewSwigluSave)    \
-    else ESMOE_FEW3(T, kFewSwiglu)                       \
-  }
-  if (g.type == kMmBf16) ESMOE_FEW9(kMmBf16)
-  else if (g.type == kMmFp16) ESMOE_FEW9(kMmFp16)
-  else if (kind == 0) ESMOE_FEW3(kMmInt8, kFewForward)
-  else ESMOE_FEW3(kMmInt8, kFewSwiglu)
-#undef ESMOE_FEW9
-#undef ESMOE_FEW3
-#undef ESMOE_FEW
-  return (int)hipGetLastError();
+  constexpr std::integral_constant<int, kFewForward> forward;
+  constexpr std::integral_constant<int, kFewSwiglu> swiglu;
+  constexpr std::integral_constant<int, kFewSwigluSave> save;
+  constexpr std::integral_constant<int, kFewRowsGrad> grad;
+  auto launch16 = [&](auto type) {
+    return kind == 2 ? launch(type, grad) : kind == 0 ? launch(type, forward) : g.gate_up ? launch(type, save) : launch(type, swiglu);
+  };
+  if (g.type == kMmBf16) return launch16(std::integral_constant<int, kMmBf16>());
+  if (g.type == kMmFp16) return launch16(std::integral_constant<int, kMmFp16>());
+  constexpr std::integral_constant<int, kMmInt8> int8;
+  return kind == 0 ? launch(int8, forward) : launch(int8, swiglu);
 }

@@ -4,7 +4,7 @@
 2. expert_mm.hip writes its matrix instructions, its copies into LDS and their waits in assembly, which the compiler does not look into: a copy's
    descriptor has to be there when it is read, nothing but matrix instructions may write an accumulator among them, and no wait of the
    compiler's own may stand between them.
-3. expert_mm_few.hip leaves all that to the compiler, which has to keep several steps of loads under way."""
+   So does expert_mm_few.hip with its copies and their waits."""
 import os
 import re
 import shutil
@@ -52,10 +52,11 @@ def registers(operand):
     return set(range(int(m.group(1)), int(m.group(2) or m.group(1)) + 1)) if m else set()
 
 
-def test_a_copys_descriptor_is_there_when_it_is_read(asm):
+@pytest.mark.parametrize("source", ["expert_mm", "expert_mm_few"])
+def test_a_copys_descriptor_is_there_when_it_is_read(asm, source):
     """A vector instruction's write of a scalar register takes five slots until a memory instruction may read it."""
     copies = 0
-    for name, lines in kernels(asm["expert_mm.hip"], "expert_mm_kernel").items():
+    for name, lines in kernels(asm[source + ".hip"], source + "_kernel").items():
         for at, line in enumerate(lines):
             m = re.match(r"buffer_load_dwordx4 v\d+, s\[(\d+):(\d+)\].* lds", line)
             if not m:
@@ -87,17 +88,17 @@ def test_nothing_stands_between_the_matrix_instructions(asm):
                 assert not registers(m.group(2)) & sums, (name, line)
 
 
-def test_few_rows_keep_their_loads_under_way(asm):
+def test_few_rows_keep_their_copies_under_way(asm):
+    """In the loop over steps: one wait for copies, which leaves all but the oldest step's under way, and none of the compiler's."""
     found = kernels(asm["expert_mm_few.hip"], "expert_mm_few_kernel")
-    assert len(found) == 8 * 3 + 3   # (16 columns a time: without SwiGLU)
+    assert len(found) == 2 * (3 * 3 + 2) + 2 * 3   # 16-bit: three shapes of three forward forms, two of the gradient; int8
     for name, lines in found.items():
-        ahead = int(re.search(r"Li(\d+)EEEvNS_12", name).group(1))
+        row_tiles, col_tiles, depth = map(int, re.search(r"Li(\d+)ELi(\d+)ELi(\d+)EEEvNS_12", name).groups())
+        matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
+        assert len(matrix) == 2 * row_tiles * col_tiles, name
         labels = {line.split(":")[0]: i for i, line in enumerate(lines) if re.match(r"\.LBB\w+:", line)}
-        loops = [lines[labels[m.group(1)]:i] for i, line in enumerate(lines) for m in [re.match(r"s_cbranch_\w+ (\.LBB\w+)", line)]
-                 if m and labels.get(m.group(1), i) < i]
-        loops = [b for b in loops if any("v_mfma" in line for line in b) and "s_barrier" not in b]
-        assert loops, name
-        inner = min(loops, key=len)
-        loads = sum(line.startswith("buffer_load") for line in inner)
-        waits = [int(n) for line in inner for n in re.findall(r"vmcnt\((\d+)\)", line)]
-        assert waits and min(waits) >= loads // ahead * (ahead - 1), (name, loads, waits)
+        back = [(labels[m.group(1)], i) for i, line in enumerate(lines) for m in [re.match(r"s_c?branch\w* (\.LBB\w+)", line)]
+                if m and labels.get(m.group(1), i) < matrix[0] and i > matrix[-1]]
+        begin, end = max(back)
+        waits = [line for line in lines[begin:end] if "vmcnt" in line]
+        assert [re.search(r"vmcnt\((\d+)\) ; explicit", w).group(1) for w in waits] == [str((depth - 1) * 2 * (row_tiles + col_tiles))], (name, waits)

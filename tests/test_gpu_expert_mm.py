@@ -93,9 +93,25 @@ def test_forward_of_many_tiles(esmoe, rows, n, k, dtype):
     check_forward(esmoe, a, b, rows)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,n,k", [(ragged(600, 40, 4), 528, 72), ([3000, 1, 0, 1300], 520, 2048), ([4100, 0, 70], 544, 200), ([1500, 0, 1700, 33], 784, 4096)], ids=range(4))
+def test_many_rows(esmoe, rows, n, k, dtype):
+    """More than the kernel of few rows takes, forward and gradients, with sums that end inside a step."""
+    a, b, d = operands(rows, n, k, dtype, n + k)
+    check_forward(esmoe, a, b, rows)
+    offsets = O.offsets_of(rows)
+    for d, a, b in ((d, a, b), (a, d, b.transpose(1, 2).contiguous())):   # (and the other way round)
+        n, k = b.shape[1:]
+        ga_want, ga_mag, _, gb_want, gb_mag, _ = O.grouped_mm_grads(d, a, b, rows, offsets)
+        ga, gb = esmoe.es_grouped_mm_backward(d, a, b.transpose(1, 2), *meta(rows, offsets, n, k))
+        check(ga, ga_want, sum_error(n, ga_mag), ga_want[:, 0].isnan(), 0.0)
+        check(gb.transpose(1, 2), gb_want, sum_error(max(rows), gb_mag))
+
+
 # 300 tiles and 357 of 256 CUs: the last round's in quarters and in halves, by columns and (SwiGLU of more than 64 rows) by rows
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("rows,n,k", [([2] * 100, 528, 72), ([2] * 119, 528, 72), ([100, 0, 66] * 50, 528, 136), ([70] * 119, 528, 64)], ids=range(4))
+@pytest.mark.parametrize("rows,n,k", [([2] * 100, 528, 72), ([2] * 119, 528, 72), ([100, 0, 66] * 50, 528, 136), ([70] * 119, 528, 64),
+                                      ([30] * 100, 528, 72), ([30] * 119, 528, 72)], ids=range(6))
 def test_a_last_round_in_parts(esmoe, rows, n, k, dtype):
     a, b, _ = operands(rows, n, k, dtype, n + k)
     check_forward(esmoe, a, b, rows)
