@@ -983,13 +983,18 @@ struct GradList {
 GradList grad_list(const char* op, at::TensorList grads) {
   TORCH_CHECK(!grads.empty(), op, ": no gradients given");
   GradList l;
+  l.in.reserve(grads.size());
+  l.dtypes.reserve(grads.size());
+  l.sizes.reserve(grads.size());
+  const c10::Device device = grads[0].defined() ? grads[0].device() : c10::Device(c10::kCPU);
   for (const torch::Tensor& g : grads) {
     TORCH_CHECK(g.defined() && g.layout() == torch::kStrided, op, ": gradients must be dense tensors");
-    TORCH_CHECK(is_half_type(g) || g.scalar_type() == torch::kFloat32, op, ": gradients must be float32, bfloat16 or half");
+    const torch::ScalarType type = g.scalar_type();
+    TORCH_CHECK(type == torch::kBFloat16 || type == torch::kHalf || type == torch::kFloat32, op, ": gradients must be float32, bfloat16 or half");
     TORCH_CHECK(g.is_non_overlapping_and_dense(), op, ": gradients must be dense in memory (their elements in any order, without gaps)");
-    TORCH_CHECK(g.device() == grads[0].device(), "all tensors must be on the same device");
+    TORCH_CHECK(g.device() == device, "all tensors must be on the same device");
     check_no_autograd(op, {&g});
-    l.dtypes.push_back(g.scalar_type() == torch::kFloat32 ? ESMOE_GRAD_FP32 : g.scalar_type() == torch::kHalf ? ESMOE_GRAD_FP16 : ESMOE_GRAD_BF16);
+    l.dtypes.push_back(type == torch::kFloat32 ? ESMOE_GRAD_FP32 : type == torch::kHalf ? ESMOE_GRAD_FP16 : ESMOE_GRAD_BF16);
     l.sizes.push_back((long)g.numel());
   }
   return l;
@@ -999,6 +1004,7 @@ GradList grad_list(const char* op, at::TensorList grads) {
 bool written_overlaps(at::TensorList grads, at::TensorList outputs, const torch::Tensor& norm) {
   struct Range { const char *from, *to; bool written; };
   std::vector<Range> ranges;
+  ranges.reserve(2 * grads.size() + 1);
   const auto add = [&](const torch::Tensor& t, bool written) {
     if (t.defined() && t.numel()) ranges.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes(), written});
   };
