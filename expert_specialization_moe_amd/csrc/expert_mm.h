@@ -23,6 +23,12 @@ struct ExpertMmArgs {
   int out_fp16;               // int8: type of out
 };
 
+// Whether weight rows are whole lines of 128 bytes and all of them more than the memory-side cache holds: a stream.
+inline bool expert_mm_whole_lines(const ExpertMmArgs& g) {
+  const long row = (long)g.k * (g.type == kMmInt8 ? 1 : 2);
+  return row % 128 == 0 && (uintptr_t)g.w % 128 == 0 && row * g.n * g.num_experts > (256L << 20);
+}
+
 // A workgroup's place among those that share `total` items, round by round.  Workgroups go to the eight XCDs in turn: neighbours are on one, and where
 // there are fewer items than workgroups (the launch knows an upper bound alone) every XCD has as many.
 struct MmPlace {

@@ -66,11 +66,17 @@ struct MmCopy {
   v4i rsrc;
   uint32_t v0, v1;
 };
+// STREAM: no cache is to keep it.
+template <bool STREAM = false>
 __device__ __forceinline__ void mm_copy(const MmCopy& p) {
   // (a scalar register that a vector instruction wrote is there for a memory instruction five slots on)
-  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 4\n\tbuffer_load_dwordx4 %[v0], %[rsrc], 0 offen lds\n\t"
-               "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024 lds"
-               ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory");   // (the compiler keeps nothing in m0)
+#define ESMOE_COPY(hint)                                                                                                            \
+  asm volatile("s_mov_b32 m0, %[lds]\n\ts_nop 4\n\tbuffer_load_dwordx4 %[v0], %[rsrc], 0 offen" hint " lds\n\t"                     \
+               "buffer_load_dwordx4 %[v1], %[rsrc], 0 offen offset:1024" hint " lds"                                                 \
+               ::[lds] "s"(p.lds), [v0] "v"(p.v0), [v1] "v"(p.v1), [rsrc] "s"(p.rsrc) : "memory")   // (the compiler keeps nothing in m0)
+  if constexpr (STREAM) ESMOE_COPY(" nt");
+  else ESMOE_COPY("");
+#undef ESMOE_COPY
 }
 
 // Products of a step: c[i][j] += rows of t[i] x columns of w[j], i = I, I + 1, j < 2; not where `rows` is at most LIMIT.  One statement with its branches
@@ -528,7 +534,7 @@ struct MmOut {
   }
 };
 
-template <int TYPE, int KIND>
+template <int TYPE, int KIND, bool STREAM>
 __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMmArgs g) {
   typedef typename MmAcc<TYPE>::T Acc;
   constexpr bool kSw = KIND == kSwiglu || KIND == kSwigluSave;
@@ -547,16 +553,16 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
   v4i tf[4][2], wf0[2][2], wf1[2][2];
   Acc acc[2][2][4][2];
 
-  mm_copy(copies.template w_part<0>(0));
+  mm_copy<STREAM>(copies.template w_part<0>(0));
   mm_copy(copies.template t_part<0>(0));
-  mm_copy(copies.template w_part<1>(0));
+  mm_copy<STREAM>(copies.template w_part<1>(0));
   mm_copy(copies.template t_part<1>(0));
   copies.advance();
   copies.left--;
   copies.passed();
-  mm_copy(copies.template w_part<0>(kMmStage));
+  mm_copy<STREAM>(copies.template w_part<0>(kMmStage));
   mm_copy(copies.template t_part<0>(kMmStage));
-  mm_copy(copies.template w_part<1>(kMmStage));
+  mm_copy<STREAM>(copies.template w_part<1>(kMmStage));
   mm_wait_copies<8>();
   mm_barrier();
   w_at.template read<kW0>(0, wf0);
@@ -601,7 +607,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
       multiply(upper, rows0, acc[0][0], wf0, [&] { w_at.template read<kW1, 0, 1>(stage, wf1); }, [&] { w_at.template read<kW1, 1, 2>(stage, wf1); });
 
       if (__builtin_expect(--copies.left <= 1, 0)) copies.passed();
-      mm_copy(copies.template w_part<0>(stage));
+      mm_copy<STREAM>(copies.template w_part<0>(stage));
       mm_barrier();
       multiply(upper, rows1, acc[0][1], wf1, [&] { t_at.template read<kT1, 0, 1>(stage, tf); }, [&] { t_at.template read<kT1, 1, 2>(stage, tf); });
 
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
       multiply(lower, rows0, acc[1][0], wf0, none, none);
 
       w_at.template read<kW0>(stage ^ kMmStage, wf0);
-      mm_copy(copies.template w_part<1>(stage));
+      mm_copy<STREAM>(copies.template w_part<1>(stage));
       arrived();
       mm_barrier();
       stage ^= kMmStage;
@@ -709,22 +715,31 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
     return esmoe_launch_expert_mm_few(args, kind, cus, stream);
   const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
-#define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
+  // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;
+  // 8192 rows by Zipf 563 / 535, one expert x 16384 rows, 4096 x 4096: 433 / 415)
+  const bool once = kind <= 1 && expert_mm_whole_lines(g) && g.total_rows <= 128 * experts;
+#define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K, false>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
+#define ESMOE_MM_ONCE(T, K)                                                                                                         \
+  {                                                                                                                                 \
+    if (once) hipLaunchKernelGGL((expert_mm_kernel<T, K, true>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g);               \
+    else ESMOE_MM(T, K);                                                                                                            \
+  }
 #define ESMOE_MM16(T)                                  \
   switch (kind) {                                      \
-    case 0: ESMOE_MM(T, kForward); break;              \
+    case 0: ESMOE_MM_ONCE(T, kForward) break;          \
     case 1:                                            \
-      if (g.gate_up) ESMOE_MM(T, kSwigluSave);         \
-      else ESMOE_MM(T, kSwiglu);                       \
+      if (g.gate_up) ESMOE_MM_ONCE(T, kSwigluSave)     \
+      else ESMOE_MM_ONCE(T, kSwiglu)                   \
       break;                                           \
     case 2: ESMOE_MM(T, kRowsGrad); break;             \
     default: ESMOE_MM(T, kWeightsGrad);                \
   }
   if (g.type == kMmBf16) { ESMOE_MM16(kMmBf16) }
   else if (g.type == kMmFp16) { ESMOE_MM16(kMmFp16) }
-  else if (kind == 0) ESMOE_MM(kMmInt8, kForward);
-  else ESMOE_MM(kMmInt8, kSwiglu);
+  else if (kind == 0) ESMOE_MM_ONCE(kMmInt8, kForward)
+  else ESMOE_MM_ONCE(kMmInt8, kSwiglu)
 #undef ESMOE_MM16
+#undef ESMOE_MM_ONCE
 #undef ESMOE_MM
   return (int)hipGetLastError();
 }

@@ -48,9 +48,12 @@ __device__ __forceinline__ int few_uniform(int v) { return __builtin_amdgcn_read
 __device__ __forceinline__ v4i few_descriptor(const void* p, int bytes) {
   return v4i{few_uniform((int)(uint64_t)p), few_uniform((int)((uint64_t)p >> 32)), few_uniform(bytes > 0 ? bytes : 0), 0x00020000};
 }
-// 64 x 16 bytes into LDS (a scalar register that a vector instruction wrote is there for a memory instruction five slots on)
+// 64 x 16 bytes into LDS (a scalar register that a vector instruction wrote is there for a memory instruction five slots on).  STREAM: no cache is to keep it
+template <bool STREAM>
 __device__ __forceinline__ void few_copy(uint32_t lds, v4i rsrc, int at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(at), "s"(rsrc) : "memory");
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(at), "s"(rsrc) : "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(at), "s"(rsrc) : "memory");
 }
 __device__ __forceinline__ v2i few_half4(v4f v, bool fp16) {
   return fp16 ? __builtin_bit_cast(v2i, __builtin_convertvector(v, v4h)) : __builtin_bit_cast(v2i, __builtin_convertvector(v, v4bf));
@@ -129,7 +132,7 @@ struct FewShared {
 };
 
 // NT row tiles x NC column tiles of sixteen (SwiGLU: the second half of the latter are the up columns), the sum over four wavefronts, DEPTH steps of each in LDS.
-template <int TYPE, int KIND, int NT, int NC, int DEPTH>
+template <int TYPE, int KIND, int NT, int NC, int DEPTH, bool STREAM>
 __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const ExpertMmArgs g) {
   typedef typename FewAcc<TYPE>::T Acc;
   typedef FewShared<NT, NC, DEPTH> Shared;
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const Expert
       const int have = g.n - step * 64 < 64 ? g.n - step * 64 : 64;
       const v4i wd = few_descriptor(w, item.rows && have > 0 ? have * w_pitch - item.col0 * 2 : 0);
 #pragma unroll
-      for (int q = 0; q < NC * 2; q++) few_copy(few_uniform(ring + slot + q * 1024), wd, w_chunk[q & 1] + (q * 8 + row8) * w_pitch);
+      for (int q = 0; q < NC * 2; q++) few_copy<STREAM>(few_uniform(ring + slot + q * 1024), wd, w_chunk[q & 1] + (q * 8 + row8) * w_pitch);
     } else {
       const char* w = (const char*)g.w + ((long)item.expert * g.n + item.col0) * w_pitch;
       const int have = cols - item.col0 < kWide ? cols - item.col0 : kWide, len = item.rows ? have * w_pitch : 0;
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const Expert
 #pragma unroll
         for (int q = 0; q < kTiles * 2; q++) {
           const int x = w_chunk[q & 1] + along;
-          few_copy(few_uniform(ring + slot + (h * kTiles * 2 + q) * 1024), wd, x < pitch ? (q * 8 + row8) * w_pitch + x : kFewNowhere);
+          few_copy<STREAM>(few_uniform(ring + slot + (h * kTiles * 2 + q) * 1024), wd, x < pitch ? (q * 8 + row8) * w_pitch + x : kFewNowhere);
         }
       }
     }
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const Expert
 #pragma unroll
     for (int q = 0; q < NT * 2; q++) {
       const int x = chunk[q & 1] + along;
-      few_copy(few_uniform(ring + slot + Shared::kWeights + q * 1024), td, x < pitch ? (q * 8 + row8) * pitch + x : kFewNowhere);
+      few_copy<false>(few_uniform(ring + slot + Shared::kWeights + q * 1024), td, x < pitch ? (q * 8 + row8) * pitch + x : kFewNowhere);
     }
     if (++copy_round == rounds) {
       copy_round = 0;
@@ -284,13 +287,14 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const Expert
 }
 
 template <int TYPE, int KIND, int NT, int NC, int DEPTH>
-int few_launch(const ExpertMmArgs& g, int cus, hipStream_t stream) {
+int few_launch(const ExpertMmArgs& g, int cus, bool stream_weights, hipStream_t stream) {
   const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
   const int cols = KIND == kFewRowsGrad ? g.k : KIND == kFewForward ? g.n : g.n / 2, wide = KIND == kFewSwiglu || KIND == kFewSwigluSave ? NC * 8 : NC * 16;
   const long items = (g.total_rows / (16 * NT) + experts) * ((cols + wide - 1) / wide);
   const long most = (160 * 1024 / sizeof(FewShared<NT, NC, DEPTH>)) * (long)cus, grid = items < most ? items : most;
   if (grid == 0) return 0;
-  hipLaunchKernelGGL((expert_mm_few_kernel<TYPE, KIND, NT, NC, DEPTH>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
+  if (stream_weights) hipLaunchKernelGGL((expert_mm_few_kernel<TYPE, KIND, NT, NC, DEPTH, true>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
+  else hipLaunchKernelGGL((expert_mm_few_kernel<TYPE, KIND, NT, NC, DEPTH, false>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
   return (int)hipGetLastError();
 }
 
@@ -306,15 +310,18 @@ extern "C" int esmoe_launch_expert_mm_few(const ExpertMmArgs* args, int kind, in
   // 8 x 32 rows 90 / 81, one x 256 rows 46 / 35: the rows come from L2 once for each item).
   const long units = experts > g.total_rows / 32 ? experts : g.total_rows / 32, wide = kind == 1 ? 16 : 32;   // of 32 rows, if they are spread evenly
   const bool narrow = units * ((cols + wide - 1) / wide) <= cus || g.total_rows <= 16 * experts;
+  // Rows of whole lines, of more weights than the caches hold, read once but for popular experts: past the caches (us so and through them: 32 experts x 8 rows,
+  // 4096 x 7168 268 / 297, 8 x 32 rows 74 / 82; but read twice or more, 4 experts x 128 rows, 130 / 96, and lines in two pieces, k = 7176, 384 / 338).
+  const bool once = expert_mm_whole_lines(g) && g.total_rows <= 32 * experts;
   auto launch = [&](auto type, auto k) {
     constexpr int TYPE = decltype(type)::value, KIND = decltype(k)::value;
     if constexpr (KIND == kFewRowsGrad) {
-      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 4, 3>(g, cus, stream);
+      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 4, 3>(g, cus, once, stream);
     } else {
-      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 2, 4>(g, cus, stream);
-      if (narrow) return few_launch<TYPE, KIND, 2, 2, 3>(g, cus, stream);
+      if (g.total_rows <= 16) return few_launch<TYPE, KIND, 1, 2, 4>(g, cus, once, stream);
+      if (narrow) return few_launch<TYPE, KIND, 2, 2, 3>(g, cus, once, stream);
     }
-    return few_launch<TYPE, KIND, 2, 4, 2>(g, cus, stream);
+    return few_launch<TYPE, KIND, 2, 4, 2>(g, cus, once, stream);
   };
   constexpr std::integral_constant<int, kFewForward> forward;
   constexpr std::integral_constant<int, kFewSwiglu> swiglu;

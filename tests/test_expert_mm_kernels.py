@@ -74,7 +74,8 @@ def test_a_copys_descriptor_is_there_when_it_is_read(asm, source):
 
 def test_nothing_stands_between_the_matrix_instructions(asm):
     found = kernels(asm["expert_mm.hip"], "expert_mm_kernel")
-    assert len(found) == 12   # two 16-bit types x (forward, SwiGLU with and without its projections, two gradients), int8 x 2
+    # two 16-bit types x (three forward forms, two ways to read the weights; two gradients), int8: two forms, two ways
+    assert len(found) == 2 * (3 * 2 + 2) + 2 * 2
     for name, lines in found.items():
         matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
         between = lines[matrix[0]:matrix[-1] + 1]
@@ -91,9 +92,10 @@ def test_nothing_stands_between_the_matrix_instructions(asm):
 def test_few_rows_keep_their_copies_under_way(asm):
     """In the loop over steps: one wait for copies, which leaves all but the oldest step's under way, and none of the compiler's."""
     found = kernels(asm["expert_mm_few.hip"], "expert_mm_few_kernel")
-    assert len(found) == 2 * (3 * 3 + 2) + 2 * 3   # 16-bit: three shapes of three forward forms, two of the gradient; int8
+    # 16-bit: three shapes of three forward forms, two of the gradient; int8; two ways to read the weights
+    assert len(found) == 2 * (2 * (3 * 3 + 2) + 2 * 3)
     for name, lines in found.items():
-        row_tiles, col_tiles, depth = map(int, re.search(r"Li(\d+)ELi(\d+)ELi(\d+)EEEvNS_12", name).groups())
+        row_tiles, col_tiles, depth = map(int, re.search(r"Li(\d+)ELi(\d+)ELi(\d+)ELb[01]EEEvNS_12", name).groups())
         matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
         assert len(matrix) == 2 * row_tiles * col_tiles, name
         labels = {line.split(":")[0]: i for i, line in enumerate(lines) if re.match(r"\.LBB\w+:", line)}
