@@ -704,15 +704,15 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   // 4096 x 7168: 8 experts x 2 rows 83 / 102, x 32 rows 115 / 106, x 64 rows 189 / 111; one x 256 rows 81 / 113, x 512 rows 150 / 115; 2048 x 1024: 8
   // experts x 64 rows 16 / 21, x 128 rows 26 / 23).  Tiles for all CUs (32 experts, 2048 x 4096: 103 / 95) are read at the memory's rate here.
   // A kernel of its own (expert_mm_few.hip) for few rows: it reads the weights at the memory's rate whatever their number (us there and here, 4096 x 7168, 8
-  // rows each of 8 / 32 experts: 79 / 103, 299 / 311; 7168 x 2048, 256 rows of 30: 155 / 171), but again for every 32 rows (32 experts x 64
-  // rows: 449 / 328), so up to eight an expert, which leaves popular ones room; or where there is not much to multiply for all CUs (8 x 32 rows
-  // 81 / 106, 8 x 64 rows 114 / 110, one x 512 66 / 114, one x 1024 145 / 122; 2048 x 1024, 8 x 128 rows 17 / 22, x 256 rows 31 / 25).
+  // rows each of 8 / 32 experts: 69 / 103, 267 / 283; 7168 x 2048, 256 rows of 30: 138 / 171), but again for every 32 rows (512 / 1024 rows by
+  // Zipf over 32 experts: 333 / 285, 396 / 302), so up to eight an expert, which leaves popular ones room; or where there is not much to
+  // multiply and less than two tiles a CU (8 x 32 rows 73 / 106, 8 x 64 rows 114 / 104, one x 512 66 / 112, one x 1024 145 / 122; 2048 x 1024, 8 x
+  // 128 rows 17 / 22, x 256 rows 31 / 25; 2304 x 4096, 512 rows by Zipf over 32 114 / 133).
   // The rows' gradient, whose weight rows it reads in pieces of 128 bytes: only that, and if tiles are not enough for the CUs (8 experts x 64
   // rows, 4096 x 2048: 30 / 65; one x 512 rows, 4096 x 4096: 46 / 72; 32 x 16 rows, 4096 x 2048, 256 tiles: 117 / 92).
   const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
-  const bool small = g.total_rows * col_tiles <= 32 * cus;
-  if (kind <= 1 ? small || g.total_rows <= 8 * experts : kind == 2 && small && experts * col_tiles < cus)
-    return esmoe_launch_expert_mm_few(args, kind, cus, stream);
+  const bool small = g.total_rows * col_tiles <= 32 * cus && experts * col_tiles < (kind <= 1 ? 2 : 1) * cus;
+  if (kind <= 1 ? small || g.total_rows <= 8 * experts : kind == 2 && small) return esmoe_launch_expert_mm_few(args, kind, cus, stream);
   const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
   // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;
