@@ -716,8 +716,9 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
   // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;
-  // 8192 rows by Zipf 563 / 535, one expert x 16384 rows, 4096 x 4096: 433 / 415)
-  const bool once = kind <= 1 && expert_mm_whole_lines(g) && g.total_rows <= 128 * experts;
+  // 8192 rows by Zipf 563 / 535, one expert x 16384 rows, 4096 x 4096: 433 / 415; the three products of a step of 32 experts x 16 / 64 / 128 rows, 4096 x
+  // 2048: 319 / 374, 361 / 394, 422 / 437)
+  const bool once = kind <= 2 && expert_mm_whole_lines(g) && g.total_rows <= 128 * experts;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K, false>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
 #define ESMOE_MM_ONCE(T, K)                                                                                                         \
   {                                                                                                                                 \
@@ -731,7 +732,7 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
       if (g.gate_up) ESMOE_MM_ONCE(T, kSwigluSave)     \
       else ESMOE_MM_ONCE(T, kSwiglu)                   \
       break;                                           \
-    case 2: ESMOE_MM(T, kRowsGrad); break;             \
+    case 2: ESMOE_MM_ONCE(T, kRowsGrad) break;         \
     default: ESMOE_MM(T, kWeightsGrad);                \
   }
   if (g.type == kMmBf16) { ESMOE_MM16(kMmBf16) }

@@ -74,8 +74,8 @@ def test_a_copys_descriptor_is_there_when_it_is_read(asm, source):
 
 def test_nothing_stands_between_the_matrix_instructions(asm):
     found = kernels(asm["expert_mm.hip"], "expert_mm_kernel")
-    # two 16-bit types x (three forward forms, two ways to read the weights; two gradients), int8: two forms, two ways
-    assert len(found) == 2 * (3 * 2 + 2) + 2 * 2
+    # two 16-bit types x (three forward forms and the rows' gradient, two ways to read the weights; the weights' gradient), int8: two forms, two ways
+    assert len(found) == 2 * (4 * 2 + 1) + 2 * 2
     for name, lines in found.items():
         matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
         between = lines[matrix[0]:matrix[-1] + 1]
