@@ -7,7 +7,7 @@
 // whose copies run on across items; it waits for its own copies and reads, and no barrier stands in the way.  The four sums are added in
 // LDS, in one order for any number of rows.  An expert's items of the same columns are neighbours on one XCD: their weights come from memory once.
 // What lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
-// One row of each of 8 experts, 4096 x 7168 with SwiGLU, bf16: 78 us (6.0 TB/s of weights), int8 41 us; 32 experts x 8 rows 299 us (6.3 TB/s).
+// One row of each of 8 experts, 4096 x 7168 with SwiGLU, bf16: 68 us (6.9 TB/s of weights), int8 36 us; 32 experts x 8 rows 267 us (7.0 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

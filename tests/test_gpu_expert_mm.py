@@ -108,6 +108,18 @@ def test_many_rows(esmoe, rows, n, k, dtype):
         check(gb.transpose(1, 2), gb_want, sum_error(max(rows), gb_mag))
 
 
+# Over 256 MB of weights in rows of whole lines, which are read past the caches: few rows (one tile of rows, two; half as wide items and whole ones) and many
+@pytest.mark.parametrize("rows,n,k,dtype", [([1] * 8 + [0] * 60, 2048, 1024, BF), ([2, 0, 3] * 11, 2048, 2048, HF), ([20, 31, 11] * 11, 2048, 2048, BF), ([40, 0, 77] * 11, 2048, 2048, HF),
+                                            ([1] * 10 + [0] * 7, 4096, 2048, HF), ([9, 40, 0] * 6, 4096, 2048, BF)], ids=range(6))
+def test_streamed_weights(esmoe, rows, n, k, dtype):
+    a, b, d = operands(rows, n, k, dtype, n + k)
+    offsets = O.offsets_of(rows)
+    check_forward(esmoe, a, b, rows)
+    ga_want, ga_mag, _, _, _, _ = O.grouped_mm_grads(d, a, b, rows, offsets)
+    ga, _ = esmoe.es_grouped_mm_backward(d, a, b.transpose(1, 2), *meta(rows, offsets, n, k), need_grad_b=False)
+    check(ga, ga_want, sum_error(n, ga_mag), ga_want[:, 0].isnan(), 0.0)
+
+
 # 300 tiles and 357 of 256 CUs: the last round's in quarters and in halves, by columns and (SwiGLU of more than 64 rows) by rows
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("rows,n,k", [([2] * 100, 528, 72), ([2] * 119, 528, 72), ([100, 0, 66] * 50, 528, 136), ([70] * 119, 528, 64),

@@ -60,7 +60,8 @@ def test_grouped_mm(esmoe, rows, n, k, dtype):
 
 @pytest.mark.parametrize("swiglu", [False, True])
 @pytest.mark.parametrize("rows,n,k", [([4100, 0, 70], 272, 144), ([1, 0] * 300, 16, 48), ([2, 700, 0, 513], 2320, 4096), ([16], 1000, 208), ([2] * 8, 2048, 528),
-                                      ([33, 1, 0, 64], 4112, 144), ([97, 0, 5], 2064, 4112), ([3000, 1, 0, 1300], 544, 4096), ([30, 0, 21] * 80, 528, 208)], ids=range(9))
+                                      ([33, 1, 0, 64], 4112, 144), ([97, 0, 5], 2064, 4112), ([3000, 1, 0, 1300], 544, 4096), ([30, 0, 21] * 80, 528, 208),
+                                      ([1] * 9 + [0] * 60, 4096, 1024), ([2, 0, 3] * 11, 4096, 2048), ([30, 0, 77] * 11, 4096, 2048)], ids=range(12))
 def test_many_tiles_and_few_rows(esmoe, rows, n, k, swiglu):
     """Each kernel and each of its shapes; sums are exact: the same bytes from all.  The scales' products are two roundings."""
     a, b, sa, sb = operands(rows, n, k, n + k)
