@@ -44,6 +44,6 @@ __device__ __forceinline__ MmPlace mm_place(uint32_t total) {
 
 // kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 gradient of the weights
 extern "C" int esmoe_launch_expert_mm(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
-extern "C" int esmoe_launch_expert_mm_few(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);   // kind 0 to 2
+extern "C" int esmoe_launch_expert_mm_few(const esmoe::ExpertMmArgs* args, int kind, int cus, hipStream_t stream);
 extern "C" int esmoe_launch_swiglu_grad(const void* grad_h, const void* gate_up, int fp16, long rows, int inter, void* grad, hipStream_t stream);
 extern "C" int esmoe_launch_int8_quant(const void* in, int fp16, long rows, int k, void* q, float* scales, hipStream_t stream);

@@ -712,7 +712,11 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   // rows, 4096 x 2048: 30 / 65; one x 512 rows, 4096 x 4096: 46 / 72; 32 x 16 rows, 4096 x 2048, 256 tiles: 117 / 92).
   const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
   const bool small = g.total_rows * col_tiles <= 32 * cus && experts * col_tiles < (kind <= 1 ? 2 : 1) * cus;
-  if (kind <= 1 ? small || g.total_rows <= 8 * experts : kind == 2 && small) return esmoe_launch_expert_mm_few(args, kind, cus, stream);
+  // The weights' gradient: where a tile for every second CU is all there is, or rows are few enough for the stores alone to count (8 experts x 50 rows, 720 x
+  // 520: 7 / 10; one x 4096 rows, 1024 x 1024: 70 / 75; 3 x 500 rows, 2048 x 2048, 192 tiles: 32 / 23; 32 experts, 4096 x 2048, x 1 row 106 / 123,
+  // x 16 rows 118 / 126, x 64 rows 157 / 134).
+  if (kind <= 1 ? small || g.total_rows <= 8 * experts : kind == 2 ? small : 2 * units * col_tiles <= cus || g.total_rows <= 16 * g.num_experts)
+    return esmoe_launch_expert_mm_few(args, kind, cus, stream);
   const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
   // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;

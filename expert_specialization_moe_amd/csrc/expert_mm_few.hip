@@ -1,4 +1,4 @@
-// Grouped products of experts with few rows each (decode, small steps), 16 bits and int8: the sums of expert_mm.hip's forward forms and rows' gradient.
+// Grouped products of experts with few rows each (decode, small steps), 16 bits and int8: the sums of expert_mm.hip.
 //
 // Bound by the weights' way from memory.  An item is 16 to 64 columns (SwiGLU: half of them gate columns, half their up columns) of up to 16 or 32 rows of
 // an expert, whose sum the four wavefronts of a workgroup split in steps of 128 bytes dealt in turn.  Weights and rows go from memory straight
@@ -286,6 +286,126 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_kernel(const Expert
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (nothing may arrive in LDS that is another workgroup's by then)
 }
 
+// The weights' gradient where there are few tiles for the large kernel, or next to no rows: out[j, c] = sum_m t[m, j] w[m, c] over an expert's rows.  Bound by the
+// stores.  A wavefront has 64 x 64 outputs and a ring of its own, two steps of 32 rows of 64 columns of either operand, as above; both are read
+// transposed.  An expert without rows gets zeros.
+constexpr int kOuterRows = 32, kOuterStep = 2 * kOuterRows * 128, kOuterCopies = kOuterStep / 1024, kOuterStores = 8;
+struct FewOuterShared {
+  uint8_t ring[kFewWaves][2][kOuterStep];
+  FewTable<kOuterRows> table;
+};
+
+// Odd groups of sixteen lanes give their part of x for the even neighbour's of y: eight columns a lane of one of two tiles instead of four of both.
+__device__ __forceinline__ v4i few_pair(v2i x, v2i y) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
+  return v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kFewThreads) expert_mm_few_outer_kernel(const ExpertMmArgs g) {
+  typedef __attribute__((address_space(3))) char* Lds;
+  typedef __attribute__((address_space(3))) v4s* Lds4;
+  __shared__ FewOuterShared s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = few_uniform(tid >> 6), l16 = lane & 15, gq = lane >> 4;
+  s.table.build(g);
+  const int pitch = g.n * 2, w_pitch = g.k * 2;
+  const uint32_t col_tiles = (g.k + 63) / 64, tiles = (uint32_t)((g.n + 63) / 64) * col_tiles, total = (uint32_t)g.num_experts * tiles;
+  const MmPlace at = mm_place((total + kFewWaves - 1) / kFewWaves);
+  const uint32_t ring = (uint32_t)few_uniform((int)(uint32_t)(uintptr_t)(Lds)(char*)s.ring[wave][0]);
+  const int row8 = lane >> 3, x = lane & 7;
+  int chunk[2];
+#pragma unroll
+  for (int q = 0; q < 2; q++) chunk[q] = ((x >> 1 ^ ((row8 >> 1 & 1) | q << 1)) << 1 | (x & 1)) * 16;
+
+  // The copies' item (of those with rows) and step, ahead of the products'.
+  const uint32_t first = at.place * kFewWaves + wave, stride = at.of * kFewWaves;
+  uint32_t copy_p = first;
+  int copy_step = 0, copy_rows = 0;
+  auto find = [&] {   // from copy_p on
+    while (copy_p < total && (copy_rows = few_uniform(s.table.rows[copy_p / tiles])) == 0) copy_p += stride;
+  };
+  auto copy = [&](uint32_t slot) {
+    const bool any = copy_p < total;
+    const uint32_t expert = any ? copy_p / tiles : 0, i = any ? copy_p - expert * tiles : 0, row = i / col_tiles, col = i - row * col_tiles;
+    const int m0 = copy_step * kOuterRows, have = !any ? 0 : copy_rows - m0 < kOuterRows ? copy_rows - m0 : kOuterRows;
+    const long from = (long)few_uniform(s.table.off[expert]) + m0;
+    const v4i td = few_descriptor((const char*)g.t + from * pitch + row * 128, have * pitch - (int)row * 128),
+              wd = few_descriptor((const char*)g.w + from * w_pitch + col * 128, have * w_pitch - (int)col * 128);
+#pragma unroll
+    for (int q = 0; q < 4; q++) few_copy<false>(few_uniform(ring + slot + q * 1024), td, chunk[q & 1] + (q * 8 + row8) * pitch);
+#pragma unroll
+    for (int q = 0; q < 4; q++) few_copy<false>(few_uniform(ring + slot + kOuterStep / 2 + q * 1024), wd, chunk[q & 1] + (q * 8 + row8) * w_pitch);
+    if (any && ++copy_step * kOuterRows >= copy_rows) {
+      copy_step = 0;
+      copy_p += stride;
+      find();
+    }
+  };
+  find();
+  copy(0);
+  copy(kOuterStep);
+  uint32_t slot = 0;
+  int stored = 0;   // an item's stores are younger than the copies that this step waits for
+  for (uint32_t p = first; p < total; p += stride) {
+    const uint32_t expert = p / tiles, i0 = p - expert * tiles, tile = i0 / col_tiles;
+    const int row0 = (int)tile * 64, col0 = (int)(i0 - tile * col_tiles) * 64, rows = few_uniform(s.table.rows[expert]);
+    v4f c[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) c[i][j] = v4f{0, 0, 0, 0};
+    for (int m = 0; m < rows; m += kOuterRows) {
+      asm volatile("s_cmp_lg_u32 %2, 0\n\ts_cbranch_scc1 .Lesmoe_wait%=\n\ts_waitcnt vmcnt(%0) ; explicit\n.Lesmoe_wait%=:\n\ts_waitcnt vmcnt(%1) ; explicit"
+                   ::"n"(kOuterCopies), "n"(kOuterCopies + kOuterStores), "s"(few_uniform(stored)) : "memory", "scc");
+      const Lds step = (Lds)(uintptr_t)(ring + slot);
+      // four lanes read 16 columns of a row, sixteen lanes of four rows, and the hardware hands lane i column i
+      auto read = [&](int part, int i) {
+        const int row = gq * 8 + (l16 >> 2), f = (row >> 1 & 1) | (row >> 3 & 1) << 1;
+        const Lds from = step + part + row * 128 + (i ^ f) * 32 + (l16 & 3) * 8;   // (row + 4: of the same bits 1 and 3)
+        const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)from)),
+                  hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(from + 4 * 128)));
+        return v4i{lo[0], lo[1], hi[0], hi[1]};
+      };
+      v4i tf[4], wf[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        tf[i] = read(0, i);
+        wf[i] = read(kOuterStep / 2, i);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) c[i][j] = few_product<TYPE>(wf[j], tf[i], c[i][j]);
+      if (m + kOuterRows < rows) {
+        copy(slot);
+        slot ^= kOuterStep;
+        stored = 0;
+      }
+    }
+    // A lane has row i * 16 + l % 16, after the exchange eight columns of one of two tiles: stored in front of the copies into the last step's place.
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((char*)g.out + (((long)expert * g.n + row0) * g.k + col0) * 2, 0,
+                                                        (g.n - row0 < 64 ? g.n - row0 : 64) * w_pitch - col0 * 2, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const int col = j * 16 + (gq & 1) * 16 + (gq >> 1) * 8;
+        __builtin_amdgcn_raw_buffer_store_b128(few_pair(few_half4(c[i][j], TYPE == kMmFp16), few_half4(c[i][j + 1], TYPE == kMmFp16)), rsrc,
+                                               col0 + col < g.k ? (i * 16 + l16) * w_pitch + col * 2 : kFewNowhere, 0, 0);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (rows > 0) {
+      copy(slot);
+      slot ^= kOuterStep;
+      stored = 1;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (nothing may arrive in LDS that is another workgroup's by then)
+}
+
 template <int TYPE, int KIND, int NT, int NC, int DEPTH>
 int few_launch(const ExpertMmArgs& g, int cus, bool stream_weights, hipStream_t stream) {
   const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
@@ -302,9 +422,15 @@ int few_launch(const ExpertMmArgs& g, int cus, bool stream_weights, hipStream_t 
 
 using namespace esmoe;
 
-// kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows
+// kind: 0 forward, 1 forward with SwiGLU, 2 gradient of the rows, 3 of the weights
 extern "C" int esmoe_launch_expert_mm_few(const ExpertMmArgs* args, int kind, int cus, hipStream_t stream) {
   const ExpertMmArgs& g = *args;
+  if (kind == 3) {
+    const long items = ((long)g.num_experts * ((g.n + 63) / 64) * ((g.k + 63) / 64) + kFewWaves - 1) / kFewWaves, grid = items < 2 * cus ? items : 2 * cus;
+    if (g.type == kMmBf16) hipLaunchKernelGGL((expert_mm_few_outer_kernel<kMmBf16>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
+    else hipLaunchKernelGGL((expert_mm_few_outer_kernel<kMmFp16>), dim3((unsigned)grid), dim3(kFewThreads), 0, stream, g);
+    return (int)hipGetLastError();
+  }
   const long cols = kind == 1 ? g.n / 2 : g.n, experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
   // Half as wide an item where rows are few, or to leave no CU without (us, 32 and 64 columns, 4096 x 7168: 2 experts x 16 rows 23 / 30, 8 x 16 rows 79 / 80;
   // 8 x 32 rows 90 / 81, one x 256 rows 46 / 35: the rows come from L2 once for each item).

@@ -89,18 +89,25 @@ def test_nothing_stands_between_the_matrix_instructions(asm):
                 assert not registers(m.group(2)) & sums, (name, line)
 
 
+def loop_waits(lines):
+    """Waits for memory in the innermost loop around all of a kernel's matrix instructions."""
+    matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
+    labels = {line.split(":")[0]: i for i, line in enumerate(lines) if re.match(r"\.LBB\w+:", line)}
+    back = [(labels[m.group(1)], i) for i, line in enumerate(lines) for m in [re.match(r"s_c?branch\w* (\.LBB\w+)", line)]
+            if m and labels.get(m.group(1), i) < matrix[0] and i > matrix[-1]]
+    begin, end = max(back)
+    waits = [re.search(r"vmcnt\((\d+)\)( ; explicit)?", line) for line in lines[begin:end] if "vmcnt" in line]
+    assert all(w.group(2) for w in waits)
+    return len(matrix), [int(w.group(1)) for w in waits]
+
+
 def test_few_rows_keep_their_copies_under_way(asm):
-    """In the loop over steps: one wait for copies, which leaves all but the oldest step's under way, and none of the compiler's."""
+    """In the loop over steps: a wait for copies that leaves all but the oldest step's under way (and stores that are younger), and none of the compiler's."""
     found = kernels(asm["expert_mm_few.hip"], "expert_mm_few_kernel")
     # 16-bit: three shapes of three forward forms, two of the gradient; int8; two ways to read the weights
     assert len(found) == 2 * (2 * (3 * 3 + 2) + 2 * 3)
     for name, lines in found.items():
         row_tiles, col_tiles, depth = map(int, re.search(r"Li(\d+)ELi(\d+)ELi(\d+)ELb[01]EEEvNS_12", name).groups())
-        matrix = [i for i, line in enumerate(lines) if line.startswith("v_mfma")]
-        assert len(matrix) == 2 * row_tiles * col_tiles, name
-        labels = {line.split(":")[0]: i for i, line in enumerate(lines) if re.match(r"\.LBB\w+:", line)}
-        back = [(labels[m.group(1)], i) for i, line in enumerate(lines) for m in [re.match(r"s_c?branch\w* (\.LBB\w+)", line)]
-                if m and labels.get(m.group(1), i) < matrix[0] and i > matrix[-1]]
-        begin, end = max(back)
-        waits = [line for line in lines[begin:end] if "vmcnt" in line]
-        assert [re.search(r"vmcnt\((\d+)\) ; explicit", w).group(1) for w in waits] == [str((depth - 1) * 2 * (row_tiles + col_tiles))], (name, waits)
+        assert loop_waits(lines) == (2 * row_tiles * col_tiles, [(depth - 1) * 2 * (row_tiles + col_tiles)]), name
+    found = kernels(asm["expert_mm_few.hip"], "expert_mm_few_outer_kernel")
+    assert len(found) == 2 and all(loop_waits(lines) == (16, [8, 16]) for lines in found.values())
