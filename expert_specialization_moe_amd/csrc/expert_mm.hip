@@ -643,15 +643,21 @@ __global__ void __launch_bounds__(kMmThreads, 2) expert_mm_kernel(const ExpertMm
           sb[b][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (first + wn * 32 + j * 16 + gq * 4) * 4, 0, 0));
       }
     }
+    // (a row's scale is asked for a row ahead: the loads come behind all copies under way, together once instead of each)
+    auto row_scale = [&](int row) {
+      if constexpr (TYPE == kMmInt8)
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mm_buffer(g.sa + t.row0, t.rows * 4), row * 4, 0, 0));
+      else return 1.0f;
+    };
+    float next_sa = row_scale(wm * 16 + l16);
 #pragma unroll
     for (int a = 0; a < 2; a++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         __builtin_amdgcn_sched_barrier(0);   // (a row's values at a time: all at once are more than the registers)
         const int row = a * 128 + (2 * i + wm) * 16 + l16;
-        float sa = 1.0f;
-        if constexpr (TYPE == kMmInt8)
-          sa = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mm_buffer(g.sa + t.row0, t.rows * 4), row * 4, 0, 0));
+        const float sa = next_sa;
+        if (a * 4 + i < 7) next_sa = row_scale(((i + 1) / 4 + a) * 128 + (2 * ((i + 1) & 3) + wm) * 16 + l16);
         auto value = [&](int b, int j) {
           const Acc sum = acc[a][b][i][j];
           if constexpr (TYPE == kMmInt8) {
