@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "expert_mm.h"
+#include "expert_mm_units.h"
 #include "mxfp4_units.h"
 #include "swiglu.h"
 #include "wave_scan.h"
@@ -155,14 +156,6 @@ struct MmTile {
   int steps;
 };
 
-// The rows of an expert in units of at most 256, as equal as sixteens allow: a tile of few rows takes as long as its weights' way from memory,
-// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows 777 us, twice 178 730 us).
-__device__ __forceinline__ uint32_t mm_units(int rows) { return ((uint32_t)rows + 255) / 256; }
-__device__ __forceinline__ int mm_unit_rows(int rows) {
-  const int units = (int)mm_units(rows);
-  return units ? ((rows + units - 1) / units + 15) & ~15 : 0;
-}
-
 // Which tiles a workgroup multiplies, one a round: experts by falling rows of a unit (the weights' gradient: rows), odd rounds dealt backwards, so that
 // what a round is uneven in evens out.
 template <int TYPE, int KIND>
@@ -204,7 +197,7 @@ struct MmTiles {
       const uint32_t rank = p / (units * col_tiles);
       first = rank * units * col_tiles;
       t.expert = uniform(s.order[rank]);
-      t.steps = (uniform(s.rows[t.expert]) + 63) >> 6;
+      t.steps = mm_steps(uniform(s.rows[t.expert]), 64);
     } else {
       // the expert whose units' running sum is the first above this unit
       const uint32_t unit = p / col_tiles;
