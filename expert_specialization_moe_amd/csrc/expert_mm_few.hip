@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "expert_mm.h"
+#include "expert_mm_units.h"
 #include "mxfp4_units.h"
 #include "swiglu.h"
 #include "wave_scan.h"
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_outer_kernel(const 
   // The copies' item (of those with rows) and step, ahead of the products'.
   const uint32_t first = at.place * kFewWaves + wave, stride = at.of * kFewWaves;
   uint32_t copy_p = first;
-  int copy_step = 0, copy_rows = 0;
+  int copy_step = 0, copy_rows = 0;   // (counted in steps: one behind the last row may pass 31 bits)
   auto find = [&] {   // from copy_p on
     while (copy_p < total && (copy_rows = few_uniform(s.table.rows[copy_p / tiles])) == 0) copy_p += stride;
   };
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_outer_kernel(const 
     for (int q = 0; q < 4; q++) few_copy<false>(few_uniform(ring + slot + q * 1024), td, chunk[q & 1] + (q * 8 + row8) * pitch);
 #pragma unroll
     for (int q = 0; q < 4; q++) few_copy<false>(few_uniform(ring + slot + kOuterStep / 2 + q * 1024), wd, chunk[q & 1] + (q * 8 + row8) * w_pitch);
-    if (any && ++copy_step * kOuterRows >= copy_rows) {
+    if (any && ++copy_step == mm_steps(copy_rows, kOuterRows)) {
       copy_step = 0;
       copy_p += stride;
       find();
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_outer_kernel(const 
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) c[i][j] = v4f{0, 0, 0, 0};
-    for (int m = 0; m < rows; m += kOuterRows) {
+    for (int left = mm_steps(rows, kOuterRows); left > 0; left--) {
       asm volatile("s_cmp_lg_u32 %2, 0\n\ts_cbranch_scc1 .Lesmoe_wait%=\n\ts_waitcnt vmcnt(%0) ; explicit\n.Lesmoe_wait%=:\n\ts_waitcnt vmcnt(%1) ; explicit"
                    ::"n"(kOuterCopies), "n"(kOuterCopies + kOuterStores), "s"(few_uniform(stored)) : "memory", "scc");
       const Lds step = (Lds)(uintptr_t)(ring + slot);
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kFewThreads) expert_mm_few_outer_kernel(const 
       for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) c[i][j] = few_product<TYPE>(wf[j], tf[i], c[i][j]);
-      if (m + kOuterRows < rows) {
+      if (left > 1) {
         copy(slot);
         slot ^= kOuterStep;
         stored = 0;

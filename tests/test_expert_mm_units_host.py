@@ -52,3 +52,13 @@ def test_units_hold_every_row_once(host, lengths):
 def test_steps_hold_every_row_once(host, lengths, each):
     for rows in lengths:
         assert host.steps(rows, each) == -(-rows // each)
+
+
+# The walk of the weights' gradient for few tiles: a step's copies begin at row 32 * step, and the last step is the one that the next would be
+# behind all rows of.  `step * 32 >= rows` instead, in 31 bits, never says so of the longest experts.
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 64, 65, (1 << 30) - 31, MOST - 32, MOST - 31, MOST - 30, MOST - 1, MOST])
+def test_a_step_of_32_rows_begins_at_an_int(host, rows):
+    last = host.steps(rows, 32) - 1
+    assert 0 <= last * 32 < rows <= MOST and rows - last * 32 <= 32
+    wraps = ctypes.c_int32((last + 1) * 32).value < rows
+    assert wraps == (rows > MOST - 31)
