@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "expert_mm.h"
 
 namespace esmoe {
@@ -32,23 +34,36 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const uint16_t* __rest
   const v4i d4 = *(const v4i*)(grad_h + row * inter + col);
   const v4i g4 = *(const v4i*)(gate_up + row * 2 * inter + col), u4 = *(const v4i*)(gate_up + (row * 2 + 1) * inter + col);
   v4i og, ou;
+  float far = 0;   // the largest |d * u|
+  auto each = [&](auto wide) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    uint32_t a[2], b[2];
+    for (int i = 0; i < 4; i++) {
+      uint32_t a[2], b[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const float d = grad_in<FP16>((uint32_t)d4[i] >> (16 * j) & 0xffffu), g = grad_in<FP16>((uint32_t)g4[i] >> (16 * j) & 0xffffu),
-                  u = grad_in<FP16>((uint32_t)u4[i] >> (16 * j) & 0xffffu);
-      // (1 - s as a sigmoid of its own: the difference cancels)
-      const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);   // exp(-g), up to infinity
-      const float s = __builtin_amdgcn_rcpf(1.0f + e);
-      const float rest = e < __builtin_inff() ? e * s : 1.0f;
-      a[j] = grad_out<FP16>(d * u * (s * __builtin_fmaf(g, rest, 1.0f)));
-      b[j] = grad_out<FP16>(d * (g * s));
+      for (int j = 0; j < 2; j++) {
+        const float d = grad_in<FP16>((uint32_t)d4[i] >> (16 * j) & 0xffffu), g = grad_in<FP16>((uint32_t)g4[i] >> (16 * j) & 0xffffu),
+                    u = grad_in<FP16>((uint32_t)u4[i] >> (16 * j) & 0xffffu);
+        // (1 - s as a sigmoid of its own: the difference cancels)
+        const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);   // exp(-g), up to infinity
+        const float s = __builtin_amdgcn_rcpf(1.0f + e);
+        const float rest = e < __builtin_inff() ? e * s : 1.0f;
+        const float slope = s * __builtin_fmaf(g, rest, 1.0f);
+        if constexpr (decltype(wide)::value) {
+          a[j] = grad_out<FP16>((float)((double)d * (double)u * (double)slope));
+        } else {
+          const float du = d * u;
+          far = __builtin_fmaxf(far, __builtin_fabsf(du));
+          a[j] = grad_out<FP16>(du * slope);
+        }
+        b[j] = grad_out<FP16>(d * (g * s));
+      }
+      og[i] = (int)(a[0] | a[1] << 16);
+      ou[i] = (int)(b[0] | b[1] << 16);
     }
-    og[i] = (int)(a[0] | a[1] << 16);
-    ou[i] = (int)(b[0] | b[1] << 16);
-  }
+  };
+  each(std::false_type());
+  // In bf16 d * u may leave fp32 next to a slope that brings it back: such a thread does its eight again in 64 bits.
+  if (!FP16 && far == __builtin_inff()) each(std::true_type());
   *(v4i*)(grad + row * 2 * inter + col) = og;
   *(v4i*)(grad + (row * 2 + 1) * inter + col) = ou;
 }
