@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "expert_mm.h"
+#include "expert_mm_rule.h"
 #include "expert_mm_units.h"
 #include "mxfp4_units.h"
 #include "swiglu.h"
@@ -696,31 +697,14 @@ using namespace esmoe;
 
 extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cus, hipStream_t stream) {
   const ExpertMmArgs& g = *args;
-  const long cols = kind >= 2 ? g.k : kind == 1 ? g.n / 2 : g.n, wide = kind == 1 ? 128 : 256, col_tiles = (cols + wide - 1) / wide;
-  const long units = kind == 3 ? (long)g.num_experts * ((g.n + 255) / 256)
-                               : g.total_rows / 256 + (g.num_experts < g.total_rows ? g.num_experts : g.total_rows);
-  // A kernel of its own (expert_mm_few.hip) where there are not enough tiles for the CUs and few rows for the weights that it reads faster (us there and here,
-  // 4096 x 7168: 8 experts x 2 rows 83 / 102, x 32 rows 115 / 106, x 64 rows 189 / 111; one x 256 rows 81 / 113, x 512 rows 150 / 115; 2048 x 1024: 8
-  // experts x 64 rows 16 / 21, x 128 rows 26 / 23).  Tiles for all CUs (32 experts, 2048 x 4096: 103 / 95) are read at the memory's rate here.
-  // A kernel of its own (expert_mm_few.hip) for few rows: it reads the weights at the memory's rate whatever their number (us there and here, 4096 x 7168, 8
-  // rows each of 8 / 32 experts: 69 / 103, 267 / 283; 7168 x 2048, 256 rows of 30: 138 / 171), but again for every 32 rows (512 / 1024 rows by
-  // Zipf over 32 experts: 333 / 285, 396 / 302), so up to eight an expert, which leaves popular ones room; or where there is not much to
-  // multiply and less than two tiles a CU (8 x 32 rows 73 / 106, 8 x 64 rows 114 / 104, one x 512 66 / 112, one x 1024 145 / 122; 2048 x 1024, 8 x
-  // 128 rows 17 / 22, x 256 rows 31 / 25; 2304 x 4096, 512 rows by Zipf over 32 114 / 133).
-  // The rows' gradient, whose weight rows it reads in pieces of 128 bytes: only that, and if tiles are not enough for the CUs (8 experts x 64
-  // rows, 4096 x 2048: 30 / 65; one x 512 rows, 4096 x 4096: 46 / 72; 32 x 16 rows, 4096 x 2048, 256 tiles: 117 / 92).
-  const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
-  const bool small = g.total_rows * col_tiles <= 32 * cus && experts * col_tiles < (kind <= 1 ? 2 : 1) * cus;
-  // The weights' gradient: where a tile for every second CU is all there is, or rows are few enough for the stores alone to count (8 experts x 50 rows, 720 x
-  // 520: 7 / 10; one x 4096 rows, 1024 x 1024: 70 / 75; 3 x 500 rows, 2048 x 2048, 192 tiles: 32 / 23; 32 experts, 4096 x 2048, x 1 row 106 / 123,
-  // x 16 rows 118 / 126, x 64 rows 157 / 134).
-  if (kind <= 1 ? small || g.total_rows <= 8 * experts : kind == 2 ? small : 2 * units * col_tiles <= cus || g.total_rows <= 16 * g.num_experts)
-    return esmoe_launch_expert_mm_few(args, kind, cus, stream);
-  const long tiles = units * col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
+  if (expert_mm_takes_few(kind, g.num_experts, g.total_rows, g.n, g.k, cus)) return esmoe_launch_expert_mm_few(args, kind, cus, stream);
+  const MmTileCount count = expert_mm_tiles(kind, g.num_experts, g.total_rows, g.n, g.k);
+  const long tiles = count.units * count.col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
   // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;
   // 8192 rows by Zipf 563 / 535, one expert x 16384 rows, 4096 x 4096: 433 / 415; the three products of a step of 32 experts x 16 / 64 / 128 rows, 4096 x
   // 2048: 319 / 374, 361 / 394, 422 / 437)
+  const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
   const bool once = kind <= 2 && expert_mm_whole_lines(g) && g.total_rows <= 128 * experts;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K, false>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)
 #define ESMOE_MM_ONCE(T, K)                                                                                                         \
