@@ -1,7 +1,9 @@
 // Gradient of silu(gate) * up with respect to both, elementwise:
 //   s = sigmoid(g):   grad_gate = d * u * s * (1 + g * (1 - s)),   grad_up = d * g * s
-// from the two projections as the forward pass stored them, in fp32, rounded once to the tensors' type (the two products behind it take
-// their operands in that type).  Bound by memory: 10 bytes an element of the output.
+// in fp32.  Two roundings to the tensors' type are choices: the projections as the forward pass stored them (in 32 bits they would be twice the
+// memory that a training step keeps, 4 bytes more an element written there and read here), and the gradient itself, whose two products take their
+// operands in that type (as two parts of 16 bits it would double them).  They cost a gradient's norm 3.0e-3 instead of 1.7e-3 in bf16, 3.7e-4 instead of
+// 2.1e-4 in fp16.  Bound by memory: 10 bytes an element of the output.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -246,7 +246,8 @@ def es_grouped_mm_backward(grad_output, a, b, problem_sizes, expert_offsets, gra
 def es_grouped_mm_swiglu_backward(grad_output, a, b, gate_up, problem_sizes, expert_offsets, grad_a=None, grad_b=None, need_grad_a=True,
                                   need_grad_b=True):
     """Gradients of es_grouped_mm_swiglu from grad_output [M, I] and the gate_up that it wrote: (grad_a, grad_b) as es_grouped_mm_backward's.
-    The gradient of gate_up is rounded to its type on the way, into a buffer of the call's own."""
+    The gradient of gate_up is rounded to its type on the way, into a buffer of the call's own: in fp16 one from 65520 on is infinite and one below
+    2^-25 zero.  Gradients are linear in grad_output: scale it by a power of two where they are such, and the results back."""
     grad_a, grad_b = _product_grads(a, b, grad_a, grad_b, need_grad_a, need_grad_b)
     _ns.es_grouped_mm_swiglu_backward.default(grad_output, a, b, gate_up, problem_sizes, expert_offsets, grad_a, grad_b)
     return grad_a, grad_b

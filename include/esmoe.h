@@ -371,7 +371,9 @@ int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, c
  *
  * esmoe_swiglu_backward: from grad_out [total_rows, inter] of silu(gate) * up and gate_up [total_rows, 2 * inter] the gradient
  *   grad_gate_up = cast( grad_out * up * s * (1 + gate * (1 - s)) | grad_out * gate * s ), s = sigmoid(gate), in fp32; inter % 8 == 0.
- *   grad_gate_up may be gate_up itself.  It is the grad_out that esmoe_grouped_mm_backward takes for a product with swiglu.
+ *   grad_gate_up may be gate_up itself.  It is the grad_out that esmoe_grouped_mm_backward takes for a product with swiglu.  The cast is to dtype:
+ *   in fp16 a gradient from 65520 on is infinite, one below 2^-14 loses bits and one below 2^-25 is zero.  All gradients are linear in grad_out,
+ *   so a caller whose gradients are such scales grad_out by a power of two, and the results back.
  * No counterpart in the reference, which is forward only and 8-bit.
  */
 int esmoe_grouped_mm(void* out, int dtype, const void* a, const void* b, const int32_t* problem_sizes, const int32_t* expert_offsets,
@@ -383,7 +385,8 @@ int esmoe_swiglu_backward(const void* grad_out, const void* gate_up, int dtype, 
 
 /*
  * Grouped product in 8-bit integers, a scale per row of a (token) and per row of b (channel):
- *   out[off_e + m, j] = cast( sa[off_e + m] * sb[e, j] * sum_c a[off_e + m, c] * b[e, j, c] ), the sum in int32 and exact
+ *   out[off_e + m, j] = cast( sa[off_e + m] * sb[e, j] * sum_c a[off_e + m, c] * b[e, j, c] ), the sum in int32 and exact, then in fp32 the
+ *     sum, times sa, times sb, each rounded (sum * sa has to stay below 3.4e38, too)
  *   swiglu != 0, n = 2 * inter, gate rows first: out[off_e + m, i] = cast( silu(gate) * up ) of the two scaled sums
  *   a [total_rows, k], b [E, n, k] int8; sa [total_rows], sb [E, n] fp32; out bf16 or fp16 (out_dtype)
  * k % 16 == 0 up to 65536; the rest as esmoe_grouped_mm.  esmoe_int8_quant makes rows (of a, or of weights) so:

@@ -260,6 +260,19 @@ def test_a_training_step(esmoe, dtype):
         assert float((g.double() - w).norm()) <= 8 * half * float(w.norm()), name
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,k", [(8, 136), (24, 776), (264, 8), (520, 264), (784, 520)])
+def test_weights_gradient_of_many_experts(esmoe, n, k, dtype):
+    """Sums of every length in steps of 64, from none on, columns and rows that end inside a tile's sixteens."""
+    rows = ([0, 1, 7, 63, 64, 65, 127, 128, 129, 200] * 30)[:300 if n * k < 100000 else 60]
+    a, b, d = operands(rows, n, k, dtype, n + k + 3)
+    assert only_large(len(rows), a.size(0), n, k, (WEIGHTS,))
+    _, _, _, want, mag, _ = O.grouped_mm_grads(d, a, b, rows, O.offsets_of(rows))
+    gb = torch.full_like(b, 55.0)
+    backward(esmoe, a, b, d, rows, O.offsets_of(rows), grad_b=gb.transpose(1, 2), need_grad_a=False)
+    check(gb, want, sum_error(200, mag))
+
+
 # ---------------------------------------------------------------------------- 8-bit integers
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("rows,n,k", [WHOLE, RAGGED[:2] + (1040,)], ids=IDS)

@@ -37,3 +37,39 @@ def test_factors_whose_product_leaves_fp32(esmoe):
              (2.0 ** 126, 2.0 ** 60, -80.0), (1.5, -2.25, 7.0), (2.0 ** -90, 2.0 ** 100, -30.0), (2.0 ** -70, 2.0 ** -50, 9.0)]
     d, up, gate = (torch.tensor(x, device="cuda").to(BF)[None].contiguous() for x in zip(*cases))
     check_gradient(gradient(esmoe, d, gate, up), d, gate, up)
+
+
+def test_what_fp16_holds(esmoe):
+    """The gradient of gate_up is rounded to the tensors' type in front of its products: from 65520 on it is infinite in fp16, below 2^-25 zero, and
+    between, down from 2^-14, it has steps of 2^-24."""
+    gate = torch.full((6, 8), 32.0, device="cuda").to(HF)   # (its sigmoid is 1 in fp32: grad_up = 32 d; grad_gate = d u)
+    gate[3:] = -14.0                                        # (sigmoid 8.3e-7: grad_up = -1.16e-5 d, grad_gate = -1.08e-5 d u)
+    d, up = torch.ones_like(gate), torch.ones_like(gate)
+    d[0], d[1], d[2] = 2047.0, 2048.0, -4096.0
+    d[3], d[4], d[5] = 2.0 ** -10, 0.5, 2.0 ** -2
+    up[4:] = 3.0
+    g, u = gradient(esmoe, d, gate, up)
+    assert (u[0] == 65504).all() and (g[0] == 2047).all()
+    assert not u[1:3].isfinite().any()
+    assert (u[3] == 0).all() and (g[3] == 0).all()
+    check_gradient((g[4:], u[4:]), d[4:], gate[4:], up[4:])
+    assert (u[4] == round(-14 * 0.5 / (1 + 2.718281828459045 ** 14) * 2 ** 24) * 2.0 ** -24).all()
+
+
+def test_grad_output_chooses_the_range(esmoe):
+    """Gradients are linear in grad_output: one times 2^12 gives them times 2^12, where fp16 holds them, with the bits that it would have lost."""
+    rows, n, k = [130, 0, 70], 64, 48
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, generator=gen, device="cuda")
+    a, b, gate_up = rand(200, k).to(HF), (0.1 * rand(3, n, k)).to(HF), rand(200, n).to(HF)
+    small = (rand(200, n // 2) * 2.0 ** -17).to(HF)
+    offsets = O.offsets_of(rows)
+    m = meta(rows, offsets, n, k)
+    dgu = O.swiglu_grad(small, gate_up)
+    want_a, _, _, want_b, _, _ = O.grouped_mm_grads(dgu, a, b, rows, offsets)
+    scale = 2.0 ** 12
+    ga, gb = esmoe.es_grouped_mm_swiglu_backward(small * scale, a, b.transpose(1, 2), gate_up, *m)
+    for got, want in ((ga, want_a), (gb.transpose(1, 2), want_b)):
+        got = (got.double() / scale)[~want.isnan()], want[~want.isnan()]
+        # two roundings, of the gradient of gate_up and of the result, half a step each of values that agree at worst
+        assert float((got[0] - got[1]).norm()) <= 2 * 2.0 ** -11 * 1.01 * float(got[1].norm())
