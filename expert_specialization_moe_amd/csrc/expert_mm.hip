@@ -701,9 +701,9 @@ extern "C" int esmoe_launch_expert_mm(const ExpertMmArgs* args, int kind, int cu
   const MmTileCount count = expert_mm_tiles(kind, g.num_experts, g.total_rows, g.n, g.k);
   const long tiles = count.units * count.col_tiles, grid = 4 * tiles < cus ? 4 * tiles : cus;   // (a tile may be four workgroups' work)
   if (grid == 0) return 0;
-  // (rows' tiles that are few enough read their weights past the caches: 32 experts x 64 rows, 4096 x 7168: 304 us, through them 326; x 256 rows 265 / 268;
-  // 8192 rows by Zipf 563 / 535, one expert x 16384 rows, 4096 x 4096: 433 / 415; the three products of a step of 32 experts x 16 / 64 / 128 rows, 4096 x
-  // 2048: 319 / 374, 361 / 394, 422 / 437)
+  // (rows' tiles that are few enough read their weights past the caches, us so and through them: 32 experts x 64 rows, 4096 x 7168: 301 / 325; x 256 rows
+  // 440 / 436, 8192 rows by Zipf 533 / 518, one expert x 16384 rows, 4096 x 4096: 430 / 411; 4096 x 2048, 32 experts x 16 / 64 / 128 rows: forward 86 / 97,
+  // 98 / 105, 108 / 116, rows' gradient 86 / 99, 89 / 102, 98 / 105)
   const long experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
   const bool once = kind <= 2 && expert_mm_whole_lines(g) && g.total_rows <= 128 * experts;
 #define ESMOE_MM(T, K) hipLaunchKernelGGL((expert_mm_kernel<T, K, false>), dim3((unsigned)grid), dim3(kMmThreads), 0, stream, g)

@@ -3,9 +3,10 @@
 // Bound by the weights' way from memory.  An item is 16 to 64 columns (SwiGLU: half of them gate columns, half their up columns) of up to 16 or 32 rows of
 // an expert, whose sum the four wavefronts of a workgroup split in steps of 128 bytes dealt in turn.  Weights and rows go from memory straight
 // into LDS, rows of 128 bytes whole: loads into registers in the layout of the matrix instruction touch half of sixteen lines each, and few
-// lines can be under way (8 experts x 32 rows, 4096 x 7168: 115 us so, 81).  A wavefront has a ring of steps of its own, as many as LDS holds,
-// whose copies run on across items; it waits for its own copies and reads, and no barrier stands in the way.  The four sums are added in
-// LDS, in one order for any number of rows.  An expert's items of the same columns are neighbours on one XCD: their weights come from memory once.
+// lines can be under way (8 experts x 32 rows, 4096 x 7168: 115 us so, 82 through LDS and the caches, 73 past the caches).  A wavefront has a ring
+// of steps of its own, as many as LDS holds, whose copies run on across items; it waits for its own copies and reads, and no barrier stands in
+// the way.  The four sums are added in LDS, in one order for any number of rows.  An expert's items of the same columns are neighbours on one XCD:
+// their weights come from memory once.
 // What lies beyond an expert's rows, the columns or the sum's length arrives as zeros without a load.
 // One row of each of 8 experts, 4096 x 7168 with SwiGLU, bf16: 68 us (6.9 TB/s of weights), int8 36 us; 32 experts x 8 rows 267 us (7.0 TB/s).
 #include <hip/hip_runtime.h>
@@ -433,12 +434,12 @@ extern "C" int esmoe_launch_expert_mm_few(const ExpertMmArgs* args, int kind, in
     return (int)hipGetLastError();
   }
   const long cols = kind == 1 ? g.n / 2 : g.n, experts = g.num_experts < g.total_rows ? g.num_experts : g.total_rows;
-  // Half as wide an item where rows are few, or to leave no CU without (us, 32 and 64 columns, 4096 x 7168: 2 experts x 16 rows 23 / 30, 8 x 16 rows 79 / 80;
-  // 8 x 32 rows 90 / 81, one x 256 rows 46 / 35: the rows come from L2 once for each item).
+  // Half as wide an item where rows are few, or to leave no CU without (us, 32 and 64 columns, 4096 x 7168: 2 experts x 16 rows 23 / 30, 8 x 16 rows 72 / 70;
+  // 8 x 32 rows 86 / 73, one x 256 rows 61 / 46: the rows come from L2 once for each item).
   const long units = experts > g.total_rows / 32 ? experts : g.total_rows / 32, wide = kind == 1 ? 16 : 32;   // of 32 rows, if they are spread evenly
   const bool narrow = units * ((cols + wide - 1) / wide) <= cus || g.total_rows <= 16 * experts;
   // Rows of whole lines, of more weights than the caches hold, read once but for popular experts: past the caches (us so and through them: 32 experts x 8 rows,
-  // 4096 x 7168 268 / 297, 8 x 32 rows 74 / 82; but read twice or more, 4 experts x 128 rows, 130 / 96, and lines in two pieces, k = 7176, 384 / 338).
+  // 4096 x 7168 267 / 298, 8 x 32 rows 74 / 82; but read twice or more, 4 experts x 128 rows, 108 / 95, and lines in two pieces, k = 7176, 373 / 339).
   const bool once = expert_mm_whole_lines(g) && g.total_rows <= 32 * experts;
   auto launch = [&](auto type, auto k) {
     constexpr int TYPE = decltype(type)::value, KIND = decltype(k)::value;
