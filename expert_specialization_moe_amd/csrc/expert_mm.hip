@@ -174,8 +174,8 @@ struct MmTiles {
     col_tiles = (cols + kWide - 1) / kWide;
     row_tiles = (g.n + 255) / 256;
     total = (KIND == kWeightsGrad ? (uint32_t)g.num_experts * row_tiles : (uint32_t)uniform((int)s.units)) * col_tiles;
-    // The last round's tiles in halves or quarters where there are workgroups for them (4096 x 7168, 4 experts x 128 rows: 124 us whole, 103; one
-    // x 512 rows 133, 115): by columns; with SwiGLU, whose gate and up columns no half of the products can leave out, by rows if more than 64.
+    // The last round's tiles in halves or quarters where there are workgroups for them (us whole and so: one expert x 1024 rows, 4096 x 7168, 142 / 126, with
+    // SwiGLU 138 / 113; 9 x 300 rows, 4096 x 4096, 161 / 146, either way): by columns; with SwiGLU, whose gate and up columns no half of the products can leave out, by rows if more than 64.
     const uint32_t grid = gridDim.x, over = total % grid;
     split = over == 0 || over > grid / 2 ? 1 : over > grid / 4 ? 2 : 4;
     const uint32_t all = total < grid ? total * split : total;
@@ -223,8 +223,8 @@ struct MmTiles {
       first = before * col_tiles;
       t.steps = KIND == kRowsGrad ? (g.n + 63) >> 6 : TYPE == kMmInt8 ? (g.k + 127) >> 7 : (g.k + 63) >> 6;
     }
-    // four of the rows' tiles a group, a column's together: the 32 CUs of an XCD have four by eight tiles, which is the least to read (the weights'
-    // gradient, 2 x 16 tiles: 465 us, 4 x 8: 452; one expert 16384 x 4096 x 4096)
+    // four of the rows' tiles a group, a column's together: the 32 CUs of an XCD have four by eight tiles, which is the least to read (one expert
+    // 16384 x 4096 x 4096, us with 2 x 16 tiles and 4 x 8: forward 417 / 407, the weights' gradient 425 / 418)
     const uint32_t i = p - first, group = i / (4 * col_tiles), j = i - group * 4 * col_tiles, have = units - 4 * group, wide = have < 4 ? have : 4,
                    col = j / wide, row = 4 * group + j - col * wide;
     const int from = (int)row * high;
@@ -392,8 +392,8 @@ struct MmCopies {
   }
 
   // Workgroups that begin together stay together, and where rows are whole 4096 bytes long what they read of a step is behind a few of the
-  // memory's channels.  There, tiles begin their sums at different steps (32 experts x 8 rows, 8192 x 2048: 188 us, all at the first 238; rows
-  // of 14336 bytes, with many rows an expert, lose 1 to 3% by it).  Not so the tiles that read the same rows, of eight columns of an expert;
+  // memory's channels.  There, tiles begin their sums at different steps (32 experts x 64 rows, 8192 x 2048: 191 us, all at the first 247; x 512
+  // rows, 4096 x 2048: 238, 240; rows of 14336 bytes, with many rows an expert, lose 1 to 3% by it).  Not so the tiles that read the same rows, of eight columns of an expert;
   // and by nothing but expert and column: the other rows of a call do not change a row's sum.
   __device__ __forceinline__ int first_step(const MmTile& t) const {
     const uint32_t group = (uint32_t)t.expert * ((tiles.col_tiles + 7) / 8) + (uint32_t)t.col0 / (8 * MmTiles<TYPE, KIND>::kWide);

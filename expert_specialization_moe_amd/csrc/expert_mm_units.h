@@ -16,7 +16,7 @@ namespace esmoe {
 ESMOE_MM_UNITS_HD int mm_steps(int length, int each) { return (int)(((uint32_t)length + (uint32_t)(each - 1)) / (uint32_t)each); }
 
 // The rows of an expert in units of at most 256, as equal as sixteens allow: a tile of few rows takes as long as its weights' way from memory,
-// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows 777 us, twice 178 730 us).
+// a full one hardly longer (32 experts x 356 rows, 4096 x 7168: 256 and 100 rows 667 us, twice 178 650 us).
 ESMOE_MM_UNITS_HD uint32_t mm_units(int rows) { return ((uint32_t)rows + 255) / 256; }
 ESMOE_MM_UNITS_HD int mm_unit_rows(int rows) {
   const uint32_t units = mm_units(rows);

@@ -4,8 +4,8 @@
 // Squares are formed and added in 64 bits: no gradient is too large or too small for its square, and the order of the sum does not show.
 // A workgroup sums a contiguous share of all chunks into one partial sum; whoever needs the norm adds the partial sums in one fixed order,
 // so a call's result does not hang on which workgroup ends first and needs neither atomics nor cleared memory.
-// Bound by memory: every gradient is read for the norm, and read and written for the clipping.  3.2 GB of bf16 gradients: 476 us (6.8 TB/s)
-// and 1290 us (5.0 TB/s).  A chunk's loads are all under way before the first is used (one piece at a time: 762 and 1445 us).  What is
+// Bound by memory: every gradient is read for the norm, and read and written for the clipping.  3.2 GB of bf16 gradients: 478 us (6.7 TB/s)
+// and 1297 us (5.0 TB/s).  A chunk's loads are all under way before the first is used (one piece at a time: 762 and 1445 us).  What is
 // written is not kept in the caches, which hold 256 MB, and so is what is read of more than twice as much, whose second pass finds little of it
 // (us, read past the caches and kept there, both passes: 3.2 GB 1768 / 1830, 400 MB 223 / 220, 200 MB 112 / 95, 100 MB 58 / 52).
 #include <hip/hip_runtime.h>
