@@ -36,25 +36,31 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const uint16_t* __rest
   const v4i d4 = *(const v4i*)(grad_h + row * inter + col);
   const v4i g4 = *(const v4i*)(gate_up + row * 2 * inter + col), u4 = *(const v4i*)(gate_up + (row * 2 + 1) * inter + col);
   v4i og, ou;
-  float far = 0;   // the largest |d * u|
+  // Rare values that a thread does its eight again for, in 64 bits: in bf16 a product d * u that leaves fp32 next to a slope that brings it back; in fp16
+  // a projection that was stored as infinite, a finite sum beyond 65504.  It counts as the largest number: what is not zero beside it gets infinite,
+  // but zeros stay zeros.
+  float far = 0;
   auto each = [&](auto wide) {
+    constexpr bool kWide = decltype(wide)::value;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       uint32_t a[2], b[2];
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        const float d = grad_in<FP16>((uint32_t)d4[i] >> (16 * j) & 0xffffu), g = grad_in<FP16>((uint32_t)g4[i] >> (16 * j) & 0xffffu),
-                    u = grad_in<FP16>((uint32_t)u4[i] >> (16 * j) & 0xffffu);
+        const float d = grad_in<FP16>((uint32_t)d4[i] >> (16 * j) & 0xffffu), g0 = grad_in<FP16>((uint32_t)g4[i] >> (16 * j) & 0xffffu),
+                    u0 = grad_in<FP16>((uint32_t)u4[i] >> (16 * j) & 0xffffu);
+        auto held = [](float v) { return FP16 && kWide && __builtin_fabsf(v) == __builtin_inff() ? __builtin_copysignf(0x1.fffffep127f, v) : v; };
+        const float g = held(g0), u = held(u0);
         // (1 - s as a sigmoid of its own: the difference cancels)
         const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);   // exp(-g), up to infinity
         const float s = __builtin_amdgcn_rcpf(1.0f + e);
         const float rest = e < __builtin_inff() ? e * s : 1.0f;
         const float slope = s * __builtin_fmaf(g, rest, 1.0f);
-        if constexpr (decltype(wide)::value) {
+        if constexpr (kWide) {
           a[j] = grad_out<FP16>((float)((double)d * (double)u * (double)slope));
         } else {
           const float du = d * u;
-          far = __builtin_fmaxf(far, __builtin_fabsf(du));
+          far = __builtin_fmaxf(far, FP16 ? __builtin_fmaxf(__builtin_fabsf(g), __builtin_fabsf(u)) : __builtin_fabsf(du));
           a[j] = grad_out<FP16>(du * slope);
         }
         b[j] = grad_out<FP16>(d * (g * s));
@@ -64,8 +70,7 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const uint16_t* __rest
     }
   };
   each(std::false_type());
-  // In bf16 d * u may leave fp32 next to a slope that brings it back: such a thread does its eight again in 64 bits.
-  if (!FP16 && far == __builtin_inff()) each(std::true_type());
+  if (far == __builtin_inff()) each(std::true_type());
   *(v4i*)(grad + row * 2 * inter + col) = og;
   *(v4i*)(grad + (row * 2 + 1) * inter + col) = ou;
 }

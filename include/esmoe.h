@@ -373,7 +373,8 @@ int esmoe_mxfp4_grouped_mm(void* out, int dtype, const void* a, const void* b, c
  *   grad_gate_up = cast( grad_out * up * s * (1 + gate * (1 - s)) | grad_out * gate * s ), s = sigmoid(gate), in fp32; inter % 8 == 0.
  *   grad_gate_up may be gate_up itself.  It is the grad_out that esmoe_grouped_mm_backward takes for a product with swiglu.  The cast is to dtype:
  *   in fp16 a gradient from 65520 on is infinite, one below 2^-14 loses bits and one below 2^-25 is zero.  All gradients are linear in grad_out,
- *   so a caller whose gradients are such scales grad_out by a power of two, and the results back.
+ *   so a caller whose gradients are such scales grad_out by a power of two, and the results back.  An infinity of an fp16 gate_up counts as the finite
+ *   sum beyond 65504 that it was: with a gate far below zero, or where grad_out is zero, the gradients are zero and not NaN.
  * No counterpart in the reference, which is forward only and 8-bit.
  */
 int esmoe_grouped_mm(void* out, int dtype, const void* a, const void* b, const int32_t* problem_sizes, const int32_t* expert_offsets,

@@ -73,3 +73,29 @@ def test_grad_output_chooses_the_range(esmoe):
         got = (got.double() / scale)[~want.isnan()], want[~want.isnan()]
         # two roundings, of the gradient of gate_up and of the result, half a step each of values that agree at worst
         assert float((got[0] - got[1]).norm()) <= 2 * 2.0 ** -11 * 1.01 * float(got[1].norm())
+
+
+def test_projections_that_fp16_does_not_hold(esmoe):
+    """A stored infinity is a finite sum beyond 65504.  Far below zero silu and its slope are zero, and a row without a gradient has none whatever
+    its projections: no NaN comes of either.  Forward and backward in one."""
+    k = 16
+    a = torch.ones((4, k), device="cuda").to(HF)
+    w = torch.zeros((1, 32, k), device="cuda").to(HF)
+    w[0, :8], w[0, 16:24] = -4400.0, 0.0625         # gate -70400, up 1
+    w[0, 8:16], w[0, 24:] = 4400.0, 4400.0          # gate and up 70400
+    a[2:] = 2.0 ** -8                               # gates of -275 and 275, up 2^-8 and 275: all held
+    m = meta([4], [0], 32, k)
+    h, gate_up = torch.empty((4, 16), dtype=HF, device="cuda"), torch.empty((4, 32), dtype=HF, device="cuda")
+    esmoe.es_grouped_mm_swiglu(h, a, w.transpose(1, 2), *m, gate_up=gate_up)
+    assert gate_up[:2, :8].isinf().all() and gate_up[:2, 8:16].isinf().all() and (h[:, :8] == 0).all()
+    d = torch.zeros_like(h)
+    d[0, :8], d[2, :8], d[3, 8:] = 1.0, 1.0, 2.0 ** -8
+    ga, gb = esmoe.es_grouped_mm_swiglu_backward(d, a, w.transpose(1, 2), gate_up, *m)
+    # rows 0 and 2: sigmoid(-275) and less; row 1: no gradient; row 3: grad_gate = 275 / 256, grad_up = 275 / 256, times weights of 4400
+    assert (ga[:3] == 0).all()
+    want = torch.full((k,), 8 * 2 * 275 / 256 * 4400, dtype=torch.float64, device="cuda")
+    assert want[0] > 65520 and ga[3].isinf().all()
+    gb = gb.transpose(1, 2)[0]
+    assert (gb[:8] == 0).all() and (gb[16:24] == 0).all()
+    one = 275 / 256 * 2.0 ** -8
+    assert ((gb[8:16].double() - one).abs() <= 2 * 2.0 ** -11 * one).all() and ((gb[24:].double() - one).abs() <= 2 * 2.0 ** -11 * one).all()
